@@ -217,6 +217,112 @@ int ms_matmul_f32(float *d_c, const float *d_a, const float *d_b, int M, int K, 
 int ms_q4_quantize(uint8_t *d_packed, float *h_scale, const void *d_w, int dtype, int n_out,
                    int n_in, int block_size);
 
+/* ---- paged KV cache: ragged batches of new rows --------------------------- */
+/* No reference counterpart (the reference keeps one contiguous cache per
+ * sequence).  For serving many sequences of changing length: the cache is a
+ * pool of pages of `page_size` positions each, and a sequence's position p lives
+ * in slot p % page_size of page table[p / page_size].  One step of a batch is
+ *   ms_paged_batch_set       lengths and page tables, once a step
+ *   ms_paged_append          per layer: q and k rotated, k and v into the pages
+ *   ms_paged_attention       per layer: the new rows over the pages
+ * and, behind the head, ms_logits_process before ms_sample.
+ * These calls check their arguments before they look for ms_init, so every
+ * refusal holds without a GPU.  They are asynchronous on the library's stream. */
+#define MS_KV_F32 0  /* element type of the pools */
+#define MS_KV_BF16 1
+#define MS_KV_F16 2
+
+/* One layer's heads and its pools.  Element (page p, slot s, kv head h, dim d)
+ * of a pool is at ((p * page_rows + s) * n_kv_heads + h) * head_dim + d. */
+typedef struct {
+  int n_heads, n_kv_heads; /* n_heads a multiple of n_kv_heads */
+  int head_dim;            /* 64, 128, 256 or 512 */
+  int rot_dim;             /* ms_paged_append: rotated dims per head, even; 0: none */
+  int window;              /* ms_paged_attention: a row attends to its own position and the
+                              window - 1 before it; 0: to all */
+  int dtype;               /* MS_KV_* */
+  int page_rows;           /* rows from a page's start to the next page's; 0: page_size (pages
+                              back to back), more where pools lie interleaved (K and V of a
+                              page side by side, several layers in one allocation) */
+  float scale;             /* of the scores; 0: 1 / sqrt(head_dim) */
+  void *k, *v;             /* device pools, 16-byte aligned */
+} ms_paged_layer;
+
+typedef struct ms_paged_batch ms_paged_batch;
+/* A batch of at most max_seqs sequences with at most max_rows new rows together
+ * and max_pages pages each, over pools of n_pages pages.  Holds the device
+ * copies of the tables; serves any number of layers. */
+int ms_paged_batch_create(int page_size, int n_pages, int max_seqs, int max_rows, int max_pages,
+                          ms_paged_batch **out);
+int ms_paged_batch_destroy(ms_paged_batch *b);
+/* The step's sequences: h_new[s] new rows (0: none) of h_len[s] positions in
+ * all, the new ones last (positions h_len - h_new .. h_len - 1); h_pages
+ * [n_seqs][max_pages].  The rows of all calls that take the batch lie sequence after
+ * sequence.  Refused, with the batch left as it was: lengths out of range, more
+ * rows than max_rows, a page id outside the pool below a sequence's length, and
+ * a page that two sequences (or two places of one) would write.  A leading run of
+ * pages may be -1: freed behind a sliding window; a call that needs one is
+ * refused.  Reading a page from several sequences (a shared prefix) is fine.
+ * The host arrays may be reused on return. */
+int ms_paged_batch_set(ms_paged_batch *b, int n_seqs, const int32_t *h_new,
+                       const int32_t *h_len, const int32_t *h_pages);
+/* cos and sin [n_pos][rot_dim/2] of positions pos0.. for ms_paged_append.
+ * wide = 0: the reference's fp32 angles (kernels.mojo:563-577), the values
+ * ms_rope and the model use; wide = 1: angles pos * theta^(-2i/rot_dim) in 64
+ * bits, rounded once: at position 100000 the fp32 angles are off by up to 0.05. */
+int ms_rope_table(float *d_cos, float *d_sin, int rot_dim, float theta, int pos0, int n_pos,
+                  int wide);
+/* The rows' k (rotated) and v into their pages, and q (rotated) to d_q_out.  Row
+ * r of k and v: n_kv_heads * head_dim floats at d_k + r * kv_stride and
+ * d_v + r * kv_stride; of q: n_heads * head_dim at d_q + r * q_stride and
+ * d_q_out + r * q_out_stride (strides in floats, multiples of 4; pointers 16-byte
+ * aligned).  d_q_out may be d_q with the same stride, else the two must not
+ * overlap; d_q NULL: k and v only.  Dim i and i + rot_dim/2 of a head turn by
+ * the angle of d_cos / d_sin [position][i] (n_pos rows, all positions of the
+ * batch's new rows below it; unused where rot_dim is 0).  Computed in fp32; the
+ * pools' values are rounded once, to nearest even (fp16: infinity past 65519). */
+int ms_paged_append(const ms_paged_layer *layer, const ms_paged_batch *b, const float *d_k,
+                    const float *d_v, size_t kv_stride, const float *d_q, size_t q_stride,
+                    float *d_q_out, size_t q_out_stride, const float *d_cos,
+                    const float *d_sin, int n_pos);
+/* Causal GQA attention of the batch's rows over the pages (the rows' own keys
+ * among them: append first), d_q and d_out rows as in ms_paged_append, which must
+ * not overlap.  The row at position p attends to positions max(0, p - window +
+ * 1) .. p.  Products take q, the probabilities and the pools' values with all
+ * their bits, sums are fp32.  Slots outside the attended positions are never
+ * used, whatever they hold; a value that is not finite reaches only the rows
+ * that attend to it.  Rows behind the last sequence's are left as they were. */
+int ms_paged_attention(const ms_paged_layer *layer, ms_paged_batch *b, const float *d_q,
+                       size_t q_stride, float *d_out, size_t out_stride);
+
+/* ---- logits: penalties, biases, grammar masks ------------------------------- */
+/* One row of ms_logits_process. */
+typedef struct {
+  float repetition;            /* > 0; 1: none */
+  float frequency, presence;   /* 0: none */
+  int32_t n_prompt, n_generated; /* ids of the row's history: the prompt's, then the generated */
+  int64_t history;             /* its first id in d_history */
+  int64_t bias;                /* the row's first entry in d_bias_ids / d_bias */
+  int32_t n_bias;
+  int32_t mask;                /* row of d_masks; -1: everything is allowed */
+} ms_logits_row;
+/* Beside ms_sample's penalty (the reference's, once per occurrence, one row):
+ * a batch of rows, each with its own settings, in this order, per id i:
+ *   seen (in the prompt or generated): x > 0 ? x / repetition : x * repetition
+ *   generated c > 0 times:             x - frequency * c - presence
+ *   every bias entry of id i:          + bias (several add up, in their order)
+ *   bit i of the mask row is 0:        -infinity, whatever x was
+ * d_logits rows of in_stride floats to d_out rows of out_stride; d_out may be
+ * d_logits with the same stride, else the two must not overlap.  Mask rows have
+ * (vocab + 31) / 32 words, id i in bit i % 32 of word i / 32.  Ids outside
+ * [0, vocab) are passed over.  A mask that allows nothing leaves a row of
+ * -infinity.  h_rows is read before the call returns.  n_history, n_bias and n_masks
+ * are the sizes of the device arrays; a row that reaches past them is refused. */
+int ms_logits_process(const float *d_logits, size_t in_stride, float *d_out, size_t out_stride,
+                      int rows, int vocab, const ms_logits_row *h_rows,
+                      const int32_t *d_history, size_t n_history, const int32_t *d_bias_ids,
+                      const float *d_bias, size_t n_bias, const uint32_t *d_masks, int n_masks);
+
 /* ---- tokenizers (host only, no device use) ----------------------------------
  * Strings are byte strings: the reference builds its text from chr(byte), so
  * each byte is one code point 0..255.  Text outputs take (out, cap) and set *len

@@ -21,6 +21,9 @@ LIB_PATH = os.path.join(_HERE, "libms_gpu.so")
 
 MS_CACHE_LINEAR = 0
 MS_CACHE_CIRCULAR = 1
+MS_KV_F32 = 0
+MS_KV_BF16 = 1
+MS_KV_F16 = 2
 MAT_NAMES = ("Q", "K", "V", "O", "Gate", "Up", "Down")
 
 
@@ -86,6 +89,26 @@ class FileLayer(C.Structure):
                 ("kv_dim", C.c_int)]
 
 
+class PagedLayer(C.Structure):
+    """ms_paged_layer: a layer's heads and the page pools of its cache."""
+    _fields_ = [("n_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("rot_dim", C.c_int), ("window", C.c_int), ("dtype", C.c_int),
+                ("page_rows", C.c_int), ("scale", C.c_float), ("k", C.c_void_p),
+                ("v", C.c_void_p)]
+
+
+class LogitsRow(C.Structure):
+    """ms_logits_row: one row's penalties, history, biases and mask."""
+    _fields_ = [("repetition", C.c_float), ("frequency", C.c_float), ("presence", C.c_float),
+                ("n_prompt", C.c_int32), ("n_generated", C.c_int32), ("history", C.c_int64),
+                ("bias", C.c_int64), ("n_bias", C.c_int32), ("mask", C.c_int32)]
+
+    def __init__(self, repetition=1.0, frequency=0.0, presence=0.0, n_prompt=0, n_generated=0,
+                 history=0, bias=0, n_bias=0, mask=-1):
+        super().__init__(repetition, frequency, presence, n_prompt, n_generated, history, bias,
+                         n_bias, mask)
+
+
 _P = C.c_void_p
 _I = C.c_int
 _SZ = C.c_size_t
@@ -114,6 +137,14 @@ _SIGS = {
     "ms_lm_head_argmax": [_P, _I, _I, _P, _I, _F, _P, _P],
     "ms_sample": [_P, _I, _F, _P, _I, _F, _U64, _P],
     "ms_embed_q4": [_P, _I, _I, _F, _P, _I, _P],
+    "ms_paged_batch_create": [_I, _I, _I, _I, _I, C.POINTER(C.c_void_p)],
+    "ms_paged_batch_destroy": [_P],
+    "ms_paged_batch_set": [_P, _I, _P, _P, _P],
+    "ms_rope_table": [_P, _P, _I, _F, _I, _I, _I],
+    "ms_paged_append": [C.POINTER(PagedLayer), _P, _P, _P, _SZ, _P, _SZ, _P, _SZ, _P, _P, _I],
+    "ms_paged_attention": [C.POINTER(PagedLayer), _P, _P, _SZ, _P, _SZ],
+    "ms_logits_process": [_P, _SZ, _P, _SZ, _I, _I, C.POINTER(LogitsRow), _P, _SZ, _P, _P, _SZ,
+                          _P, _I],
     "ms_model_create": [C.POINTER(ModelDesc), C.POINTER(LayerDesc), C.POINTER(C.c_void_p)],
     "ms_model_destroy": [_P],
     "ms_model_set_matrix": [_P, _I, _I, _P, _I, _F],
@@ -315,6 +346,85 @@ class DeviceBuffer:
                 _lib.ms_free(self.ptr)
         except Exception:
             pass
+
+
+# ---- paged KV cache and logits of a serving batch ----------------------------------
+def _ptr(b):
+    return b.ptr if b is not None else None
+
+
+class PagedBatch:
+    """Owner of an ms_paged_batch handle: a step's sequences and their page tables, for
+    every layer's paged_append and paged_attention."""
+
+    def __init__(self, page_size: int, n_pages: int, max_seqs: int, max_rows: int,
+                 max_pages: int):
+        self.h = None
+        self.max_pages = int(max_pages)
+        h = C.c_void_p()
+        check(_lib.ms_paged_batch_create(page_size, n_pages, max_seqs, max_rows, max_pages,
+                                         C.byref(h)))
+        self.h = h.value
+
+    def set(self, new: Sequence[int], length: Sequence[int], pages) -> None:
+        """new[s] new rows of length[s] positions in all; pages [n_seqs][at most max_pages]
+        (-1: no page)."""
+        n = np.ascontiguousarray(new, dtype=np.int32)
+        l = np.ascontiguousarray(length, dtype=np.int32)
+        p = np.asarray(pages, dtype=np.int32)
+        if n.ndim != 1 or l.shape != n.shape or p.ndim != 2 or p.shape[0] != n.size or \
+                p.shape[1] > self.max_pages:
+            raise MSError("PagedBatch.set: shapes do not fit")
+        if p.shape[1] < self.max_pages:
+            p = np.pad(p, ((0, 0), (0, self.max_pages - p.shape[1])), constant_values=-1)
+        p = np.ascontiguousarray(p)
+        check(_lib.ms_paged_batch_set(self.h, n.size, n.ctypes.data, l.ctypes.data,
+                                      p.ctypes.data))
+
+    def close(self) -> None:
+        if self.h:
+            check(_lib.ms_paged_batch_destroy(self.h))
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def rope_table(rot_dim: int, theta: float, n_pos: int, pos0: int = 0, wide: bool = False):
+    """Device buffers of cos and sin [n_pos][rot_dim/2] for paged_append: the reference's
+    fp32 angles, or 64-bit ones (wide)."""
+    c, s = (DeviceBuffer(n_pos * (rot_dim // 2) * 4) for _ in range(2))
+    check(_lib.ms_rope_table(c.ptr, s.ptr, rot_dim, float(theta), pos0, n_pos, int(wide)))
+    return c, s
+
+
+def paged_append(layer: PagedLayer, batch: PagedBatch, k, v, kv_stride: int, q=None,
+                 q_stride: int = 0, q_out=None, q_out_stride: int = 0, cos=None, sin=None,
+                 n_pos: int = 0) -> None:
+    """The batch's new k (rotated) and v rows into their pages, q rotated to q_out
+    (ms_paged_append; buffers are objects with a device address `ptr`)."""
+    check(_lib.ms_paged_append(C.byref(layer), batch.h, _ptr(k), _ptr(v), kv_stride, _ptr(q),
+                               q_stride, _ptr(q_out), q_out_stride, _ptr(cos), _ptr(sin), n_pos))
+
+
+def paged_attention(layer: PagedLayer, batch: PagedBatch, q, q_stride: int, out,
+                    out_stride: int) -> None:
+    """Causal attention of the batch's rows over the pages (ms_paged_attention)."""
+    check(_lib.ms_paged_attention(C.byref(layer), batch.h, _ptr(q), q_stride, _ptr(out),
+                                  out_stride))
+
+
+def logits_process(logits, in_stride: int, out, out_stride: int, vocab: int,
+                   rows: Sequence[LogitsRow], history=None, n_history: int = 0, bias_ids=None,
+                   bias=None, n_bias: int = 0, masks=None, n_masks: int = 0) -> None:
+    """Penalties, biases and grammar masks of a batch of logits rows (ms_logits_process)."""
+    arr = (LogitsRow * max(len(rows), 1))(*rows)
+    check(_lib.ms_logits_process(_ptr(logits), in_stride, _ptr(out), out_stride, len(rows), vocab,
+                                 arr, _ptr(history), n_history, _ptr(bias_ids), _ptr(bias),
+                                 n_bias, _ptr(masks), n_masks))
 
 
 # ---- architecture presets -------------------------------------------------------
