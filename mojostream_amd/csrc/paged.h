@@ -56,6 +56,7 @@ struct PagedPlan {
   int G = 0, nq = 0, n_kv = 0, window = 0;
   bool valid = false;
   int n_items = 0, n_merge = 0, n_parts = 0;
+  int most = 0;  // (row, head) pairs of the longest chunk
   size_t merge_at = 0;  // byte offset of the merge list
   Upload up;
 };
