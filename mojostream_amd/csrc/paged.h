@@ -38,8 +38,8 @@ struct PagedRow {
   int32_t pos, page, slot, seq;
 };
 
-// One block's part of the attention (per kv head): rows r0 .. r0 + 16 NQ - 1 of the
-// sequence's new * G (row, query head) pairs, numbered row * G + head, over the
+// One block's part of the attention (per kv head): pairs from r0 on (the plan's rows of them) of
+// the sequence's new * G (row, query head) pairs, numbered row * G + head, over the
 // keys k0 .. k1 - 1.
 struct PagedItem {
   int32_t row, n_new, len, seq;  // the sequence: first row, new rows, positions
@@ -53,10 +53,10 @@ struct PagedMerge {
 
 // A split of the batch's work, for layers of the same shape.
 struct PagedPlan {
-  int G = 0, nq = 0, n_kv = 0, window = 0;
+  int G = 0, rows = 0, n_kv = 0, window = 0, blocks = 0;
   bool valid = false;
   int n_items = 0, n_merge = 0, n_parts = 0;
-  int most = 0;  // (row, head) pairs of the longest chunk
+  int most = 0;  // (row, head) pairs of the longest item
   size_t merge_at = 0;  // byte offset of the merge list
   Upload up;
 };

@@ -22,7 +22,8 @@ struct PagedAttnArgs {
   int n_kv, G, window, page_size, page_rows;
   FastDiv by_page, by_g;  // n / page_size, n / G
   float scale;            // of the scores, log2(e) in it
-  float *part_o, *part_ml;  // [part][kv head][16 nq][head dim], [part][kv head][16 nq][2]
+  float *part_o, *part_ml;  // [part][kv head][part_rows][head dim], [part][kv head][part_rows][2]
+  int part_rows;          // (row, head) pairs of the longest item
 };
 
 template <int DT>
@@ -114,22 +115,22 @@ __device__ inline float sum_groups(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The item's rows one after the other, key by key, with 256 threads: a key that a row does
-// not attend to is not multiplied by anything.  Parts lie 16 NQS rows apart.
-template <int HD, int DT, int NQ, int NQS>
+// The item's rows one after the other, key by key, with NT threads: a key that a row does
+// not attend to is not multiplied by anything.
+template <int HD, int DT, int NT>
 __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedItem &it, int kvh,
-                                         float *lds) {
-  constexpr int ND = (HD + 255) / 256;
-  float *p_of = lds, *red = lds + 256;  // probabilities of 256 keys (-1: not attended); 8
+                                         int most, float *lds) {
+  constexpr int ND = (HD + NT - 1) / NT, NW = NT / 64;
+  float *p_of = lds, *red = lds + NT;  // probabilities of NT keys (-1: not attended); 2 NW
   const int tid = threadIdx.x;
-  const int nrows = min(16 * NQ, it.n_new * a.G - it.r0);
+  const int nrows = min(most, it.n_new * a.G - it.r0);
   for (int r = 0; r < nrows; ++r) {
     const int t = (it.r0 + r) / a.G, h = (it.r0 + r) % a.G;
     const int pos = it.len - it.n_new + t;
     const int lo = a.window && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
     const float *q = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD;
     float m = -INFINITY, l = 0.f, o[ND] = {};
-    for (int k0 = it.k0; k0 < it.k1; k0 += 256) {
+    for (int k0 = it.k0; k0 < it.k1; k0 += NT) {
       const int key = k0 + tid;
       const bool on = key < it.k1 && key >= lo && key <= pos;
       float s = 0.f;
@@ -144,21 +145,23 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
       for (int off = 1; off < 64; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
       if ((tid & 63) == 0) red[tid >> 6] = mx;
       __syncthreads();
-      mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+      mx = red[0];
+      for (int w = 1; w < NW; ++w) mx = fmaxf(mx, red[w]);
       const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;
       // (lifted like the tiles' probabilities: parts of both kinds are merged)
       const float p = on ? __builtin_amdgcn_exp2f(Form<DT>::F16 ? s - base + kLift : s - base) : 0.f;
       p_of[tid] = on ? p : -1.f;
       float sum = p;
       for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
-      if ((tid & 63) == 0) red[4 + (tid >> 6)] = sum;
+      if ((tid & 63) == 0) red[NW + (tid >> 6)] = sum;
       __syncthreads();
       const float al = __builtin_amdgcn_exp2f(m - base);
-      l = l * al + (red[4] + red[5]) + (red[6] + red[7]);
+      l *= al;
+      for (int w = 0; w < NW; ++w) l += red[NW + w];
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[i] *= al;
       m = mn;
-      for (int j = 0; j < 256 && k0 + j < it.k1; ++j) {
+      for (int j = 0; j < NT && k0 + j < it.k1; ++j) {
         const float pj = p_of[j];
         if (pj == -1.f) continue;
         const uint32_t pg = div_by(k0 + j, a.by_page);
@@ -167,18 +170,18 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
         const size_t at = (row * a.n_kv + kvh) * HD;
 #pragma unroll
         for (int i = 0; i < ND; ++i)
-          if (tid + 256 * i < HD) o[i] += pj * load_kv<DT>(a.v, at + tid + 256 * i);
+          if (tid + NT * i < HD) o[i] += pj * load_kv<DT>(a.v, at + tid + NT * i);
       }
       __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
-      const int d = tid + 256 * i;
+      const int d = tid + NT * i;
       if (d >= HD) continue;
       if (it.part < 0) {
         a.out[(size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD + d] = o[i] / l;
       } else {
-        const size_t pr = ((size_t)it.part * a.n_kv + kvh) * (16 * NQS) + r;
+        const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
         a.part_o[pr * HD + d] = o[i];
         if (d == 0) {
           a.part_ml[pr * 2] = m;
@@ -187,6 +190,83 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
       }
     }
   }
+}
+
+// A tile's probabilities as the operand of the second product, from its scores: t = s sc - m,
+// m the running maximum, in log2; p = 2^t.  `edge`: some row does not attend to some key.
+// m serves all of a query's keys and may lag behind by kLag, so that a tile needs neither a
+// cross-lane maximum nor a rescaling of the sums, unless a score exceeds it.
+// span(n, &low, &high): the keys that the lane's query of query tile n attends to.
+template <int DT, int NQ, int ND, class Span>
+__device__ __forceinline__ void probabilities(const f4 (&s)[2][NQ], int kb, bool edge,
+                                              const float (&sc)[NQ], const Span &span,
+                                              float (&m)[NQ], float (&l)[NQ], f4 (&o)[NQ][ND],
+                                              uint32_t (&pf)[NQ][Form<DT>::QP][4]) {
+  constexpr bool F16 = Form<DT>::F16;
+  const int g = (threadIdx.x & 63) >> 4;
+  float t[NQ][8], top = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[n][j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], -m[n]);
+  if (edge) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      int low, high;
+      span(n, &low, &high);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
+        if (key > high || key < low) t[n][j] = -INFINITY;
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, t[n][j]);
+  if (__any(top > kLag)) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      // (from the scores: beside kLow they are lost in t)
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        mx = fmaxf(mx, t[n][j] == -INFINITY ? -INFINITY : s[j >> 2][n][j & 3] * sc[n]);
+      const float mn = fmaxf(m[n], max_groups(mx)), al = __builtin_amdgcn_exp2f(m[n] - mn);
+      m[n] = mn;
+      l[n] *= al;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[n][d] *= al;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (t[n][j] != -INFINITY) t[n][j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], -mn);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    float *p = t[n];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(F16 ? p[j] + kLift : p[j]);
+    l[n] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      split2<F16, Form<DT>::QP>(p[2 * j], p[2 * j + 1], &pf[n][0][j], 4);
+  }
+}
+
+// 2^k that brings the largest of fp16 queries' values below 2^15, and its inverse.
+__device__ inline void lift_of(float big, float *up, float *down) {
+  int e = big > 0.f && big < INFINITY ? 14 + 127 - (int)((__float_as_uint(big) >> 23) & 255) : 0;
+  e = max(-100, min(100, e));
+  *up = __uint_as_float((uint32_t)(127 + e) << 23);
+  *down = __uint_as_float((uint32_t)(127 - e) << 23);
+}
+
+// Dims of a value row that a lane of item_by_tile loads at once: 16 bytes, 8 at head dim 64.
+template <int HD, int DT>
+__host__ __device__ constexpr int v_dims() {
+  return DT == MS_KV_F32 || HD == 64 ? 4 : 8;
 }
 
 // The attention of one item: 16 NQ (row, head) pairs, the block's four waves taking its
@@ -203,37 +283,31 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
 //                   4 (l / 16) + j - 4 of the second.  A: lane l loads VD dims of its eight keys
 //                   and turns them in its registers: MFMA t of a chunk of 16 VD dims takes
 //                   dim VD (l % 16) + t.  D: dims VD (4 (l / 16) + e) + t of query l % 16.
-// A maximum per query serves all its keys and may lag behind by kLag, so that a tile needs
-// neither a cross-lane maximum nor a rescaling of the sums, unless a score exceeds it.
-//
 // A value that is not finite makes the sums it is multiplied into not finite, with the
 // zeros of masked keys too; where the end finds such a sum the item is done again key by
 // key.
-template <int HD, int DT, int NQ, int NQS>
+template <int HD, int DT, int NQ, int W>
 __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const PagedItem &it, int kvh,
                                              char *lds) {
   using F = Form<DT>;
   constexpr bool F16 = F::F16;
   constexpr int QP = F::QP, KP = F::KP, KS = HD / 32, ES = DT == MS_KV_F32 ? 4 : 2;
-  constexpr int VD = HD >= 128 ? 8 : HD / 16, CD = 16 * VD, NC = HD / CD;
+  constexpr int VD = v_dims<HD, DT>(), CD = 16 * VD, NC = HD / CD;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
   const int nrows = min(16 * NQ, it.n_new * a.G - it.r0), base = it.len - it.n_new;
 
   // ---- q: parts in LDS in fragment order; per query its position and scale
   u4 *qf = reinterpret_cast<u4 *>(lds);  // [nq][s][part][64]
   float sc[NQ];
-  int lim[NQ], low[NQ];
   const int t_first = it.r0 / a.G, t_last = (it.r0 + nrows - 1) / a.G;
   const int low_key = a.window ? max(it.k0, base + t_first - a.window + 1) : it.k0;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int r = 16 * n + c16, t = (it.r0 + r) / a.G, h = (it.r0 + r) - t * a.G;
     const bool real = r < nrows;
-    lim[n] = real ? min(it.k1 - 1, base + t) : it.k1 - 1;
-    low[n] = real && a.window ? max(low_key, base + t - a.window + 1) : low_key;
     const float *q = a.q + (size_t)(it.row + (real ? t : t_first)) * a.q_ld +
                      (size_t)(kvh * a.G + (real ? h : 0)) * HD + 8 * g;
-    float x[(KS + 3) / 4][8];
+    float x[(KS + W - 1) / W][8];
     float big = 0.f;
     if constexpr (F16) {
       // (every wave needs the whole row's largest value)
@@ -244,14 +318,12 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
       }
       big = max_groups(big);
     }
-    // 2^(14 - exponent of the largest); 1 where there is none
-    const int ex = big > 0.f && big < INFINITY ? 14 - (int)((__float_as_uint(big) >> 23) & 255) + 127 : 0;
-    const int exc = max(-100, min(100, ex));
-    const float up = F16 ? __uint_as_float((uint32_t)(exc + 127) << 23) : 1.f;
-    sc[n] = F16 ? a.scale * __uint_as_float((uint32_t)(127 - exc) << 23) : a.scale;
+    float up = 1.f, down = 1.f;
+    if constexpr (F16) lift_of(big, &up, &down);
+    sc[n] = a.scale * down;
 #pragma unroll
-    for (int si = 0; si < (KS + 3) / 4; ++si) {
-      const int s = wave + 4 * si;
+    for (int si = 0; si < (KS + W - 1) / W; ++si) {
+      const int s = wave + W * si;
       if (s < KS) {
         const f4 u = ldg<f4>(q + 32 * s), v = ldg<f4>(q + 32 * s + 4);
 #pragma unroll
@@ -267,6 +339,11 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   }
   __syncthreads();
 
+  auto span = [&](int n, int *low, int *high) {
+    const int r = min(16 * n + c16, nrows - 1), pos = base + (int)div_by(it.r0 + r, a.by_g);
+    *high = min(it.k1 - 1, pos);
+    *low = a.window ? max(low_key, pos - a.window + 1) : low_key;
+  };
   f4 o[NQ][NC * VD] = {};
   float m[NQ], l[NQ];
 #pragma unroll
@@ -291,8 +368,11 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   };
   int page = 0, slot = 0;
   if (wave < n_tiles) find(wave, &page, &slot);
-  for (int tile = wave; tile < n_tiles; tile += 4) {
+  for (int tile = wave; tile < n_tiles; tile += W) {
     const int kb = it.k0 + tile * kTile;
+    // (the fragments of q are read anew for every tile, not kept)
+    int at = lane;
+    asm volatile("" : "+v"(at));
     const int row = page * a.page_rows + slot;
     const char *kp[2], *vp[8];
 #pragma unroll
@@ -301,7 +381,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       vp[j] = vb0 + (uint64_t)(uint32_t)__shfl(row, 16 * (j >> 2) + 4 * g + (j & 3), 64) * row_bytes;
-    if (tile + 4 < n_tiles) find(tile + 4, &page, &slot);
+    if (tile + W < n_tiles) find(tile + W, &page, &slot);
 
     // ---- scores
     // (the products of the leading parts have a sum of their own: a running sum that takes
@@ -328,7 +408,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int pa = QP - 1; pa >= 0; --pa) {
-          const u4 q = qf[((n * KS + ks) * QP + pa) * 64 + lane];
+          const u4 q = qf[((n * KS + ks) * QP + pa) * 64 + at];
 #pragma unroll
           for (int pb = KP - 1; pb >= 0; --pb) {
             if (pa + pb >= F::TERMS) continue;
@@ -345,45 +425,8 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
 #pragma unroll
       for (int i = 0; i < 2; ++i) s[i][n] += s_low[i][n];
 
-    // ---- probabilities
-    const bool whole = kb >= all_lo && kb + kTile - 1 <= all_hi;
     uint32_t pf[NQ][QP][4];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float t[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], -m[n]);
-      if (!whole) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
-          if (key > lim[n] || key < low[n]) t[j] = -INFINITY;
-        }
-      }
-      float mx = t[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, t[j]);
-      if (__any(mx > kLag)) {
-        // (t is a score less the old maximum; taken anew from the scores, which near kLow
-        // are lost in it)
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, t[j] == -INFINITY ? -INFINITY : s[j >> 2][n][j & 3] * sc[n]);
-        const float mn = fmaxf(m[n], max_groups(top)), al = __builtin_amdgcn_exp2f(m[n] - mn);
-        m[n] = mn;
-        l[n] *= al;
-#pragma unroll
-        for (int d = 0; d < NC * VD; ++d) o[n][d] *= al;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (t[j] != -INFINITY) t[j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], -mn);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = __builtin_amdgcn_exp2f(F16 ? t[j] + kLift : t[j]);
-      l[n] += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) split2<F16, QP>(t[2 * j], t[2 * j + 1], &pf[n][0][j], 4);
-    }
+    probabilities<DT, NQ>(s, kb, kb < all_lo || kb + kTile - 1 > all_hi, sc, span, m, l, o, pf);
 
     // ---- values
 #pragma unroll
@@ -453,24 +496,25 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   }
   // (also: every wave is done with q)
   if (__syncthreads_or(bad)) {
-    item_by_key<HD, DT, NQ, NQS>(a, it, kvh, reinterpret_cast<float *>(lds));
+    item_by_key<HD, DT, 64 * W>(a, it, kvh, 16 * NQ, reinterpret_cast<float *>(lds));
     return;
   }
   float *ml = reinterpret_cast<float *>(lds);  // [2][wave][16 NQ]
-  constexpr int LD = CD + 4;
-  float *os = ml + 2 * 4 * 16 * NQ;            // [wave][16][LD]
+  constexpr int LD = CD + 4, ROWS = 16 * NQ;
+  float *os = ml + 2 * W * ROWS;               // [wave][16][LD]
   if (g == 0)
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      ml[wave * 16 * NQ + 16 * n + c16] = m[n];
-      ml[(4 + wave) * 16 * NQ + 16 * n + c16] = l[n];
+      ml[wave * ROWS + 16 * n + c16] = m[n];
+      ml[(W + wave) * ROWS + 16 * n + c16] = l[n];
     }
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const float *mw = ml + 16 * n + c16;
-    const float top = fmaxf(fmaxf(mw[0], mw[16 * NQ]), fmaxf(mw[32 * NQ], mw[48 * NQ]));
-    const float w = __builtin_amdgcn_exp2f(m[n] - top);
+    float top = kLow;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, ml[w * ROWS + 16 * n + c16]);
+    const float f = __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       __syncthreads();
@@ -480,28 +524,28 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
         for (int t = 0; t < VD; t += 4) {
           f4 x;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) x[u] = o[n][c * VD + t + u][e] * w;
+          for (int u = 0; u < 4; ++u) x[u] = o[n][c * VD + t + u][e] * f;
           *reinterpret_cast<f4 *>(os + (wave * 16 + c16) * LD + VD * (4 * g + e) + t) = x;
         }
       __syncthreads();
-      for (int i = tid; i < 4 * CD; i += 256) {
+      for (int i = tid; i < 4 * CD; i += 64 * W) {
         const int r16 = i / (CD / 4), d = i % (CD / 4) * 4, r = 16 * n + r16;
         if (r >= nrows) continue;
-        const float *mr = ml + r;
-        const float m0 = mr[0], m1 = mr[16 * NQ], m2 = mr[32 * NQ], m3 = mr[48 * NQ];
-        const float mt = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-        const float *lr = mr + 64 * NQ;
-        const float ls = (lr[0] * __builtin_amdgcn_exp2f(m0 - mt) + lr[16 * NQ] * __builtin_amdgcn_exp2f(m1 - mt)) +
-                         (lr[32 * NQ] * __builtin_amdgcn_exp2f(m2 - mt) + lr[48 * NQ] * __builtin_amdgcn_exp2f(m3 - mt));
-        const float *p = os + r16 * LD + d;
-        const f4 x = (*reinterpret_cast<const f4 *>(p) + *reinterpret_cast<const f4 *>(p + 16 * LD)) +
-                     (*reinterpret_cast<const f4 *>(p + 32 * LD) + *reinterpret_cast<const f4 *>(p + 48 * LD));
+        float mt = kLow, ls = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) mt = fmaxf(mt, ml[w * ROWS + r]);
+        f4 x = {};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          ls += ml[(W + w) * ROWS + r] * __builtin_amdgcn_exp2f(ml[w * ROWS + r] - mt);
+          x += *reinterpret_cast<const f4 *>(os + (w * 16 + r16) * LD + d);
+        }
         if (it.part < 0) {
           const int t = (it.r0 + r) / a.G, h = (it.r0 + r) - t * a.G;
           *reinterpret_cast<f4 *>(a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD +
                                   c * CD + d) = x / ls;
         } else {
-          const size_t pr = ((size_t)it.part * a.n_kv + kvh) * (16 * NQS) + r;
+          const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
           *reinterpret_cast<f4 *>(a.part_o + pr * HD + c * CD + d) = x;
           if (c == 0 && d == 0) {
             a.part_ml[pr * 2] = mt;
@@ -513,30 +557,351 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   }
 }
 
-template <int HD, int DT, int NQ>
-constexpr int attn_lds() {
-  constexpr int q = Form<DT>::QP * NQ * HD * 32, vd = HD >= 128 ? 8 : HD / 16;
-  constexpr int e = (128 * NQ + 64 * (16 * vd + 4)) * 4;
+// How a block of item_by_block divides an item: W waves in groups of SP, a group having 16 NQ
+// (row, head) pairs, each of its waves HD / SP dims of them.  A wave's share of q in parts and of
+// the sums then stays in its registers (two waves a SIMD).
+template <int HD, int DT>
+struct Shape {
+  // (two query tiles a wave where the registers hold them: a fragment then serves six products)
+  static constexpr int NQ = HD == 64 || (HD == 128 && DT != MS_KV_F32) ? 2 : 1;
+  static constexpr int W = NQ == 2 ? 4 : 8, SP = HD == 512 ? 2 : 1;
+  static constexpr int PAIRS = 16 * NQ * W / SP;
+  static constexpr int FRAG = kTile * HD * 2 * Form<DT>::KP;  // bytes of K's or V's fragments
+  static constexpr int XS = SP > 1 ? W * NQ * 2 * 64 * 16 : 0;
+  static constexpr int LDS = 2 * FRAG + XS + 2 * kTile * 4;
+  // (fragments of fp32 pools of 512 dims take more LDS than there is; in turns in one buffer the
+  // waves ran out of registers: 1.0 to 1.2 ms where item_by_tile takes 0.61 ms, 1024 rows over 4096
+  // keys, 8 heads)
+  static constexpr bool FITS = LDS <= 160 * 1024;
+};
+
+// The attention of one item of a longer chunk.  The waves go over the item's 32-key tiles
+// together: a tile's keys and values are loaded once for the block, in whole rows, and put
+// into LDS as MFMA fragments (those of fp32 pools in parts): K as the rows lie, V turned in
+// registers; the waves read both without bank conflicts.  (item_by_tile's loads of K take 16
+// bytes of 16 rows a quarter wave, sixteen cache accesses where a row's take one or two; with
+// many queries these accesses bound it.)  The loads of V run beside the first product, those of
+// the next K beside the second.  Where a group has several waves each computes the scores over
+// its dims, and all take the sum, in the same order.
+template <int HD, int DT>
+__device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const PagedItem &it, int kvh,
+                                              char *lds) {
+  using F = Form<DT>;
+  using B = Shape<HD, DT>;
+  constexpr bool F16 = F::F16;
+  constexpr int NQ = B::NQ, W = B::W, SP = B::SP;
+  constexpr int QP = F::QP, KP = F::KP, KS = HD / 32, ES = DT == MS_KV_F32 ? 4 : 2;
+  constexpr int VD = HD / (16 * W) < 2 ? 2 : HD / (16 * W), CD = 16 * VD, NC = HD / CD;
+  constexpr int KW = KS / SP, CW = NC / SP;  // a wave's 32-dim steps and chunks of CD dims
+  constexpr int D8 = HD / 8, UK = kTile * D8 / (64 * W);  // K units of 8 dims a thread
+  constexpr bool STRICT = KW * KP >= 8;
+  constexpr int RING = 4;
+  static_assert(CW >= 1 && UK >= 1 && 64 * W / D8 * UK == kTile, "shape");
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
+  const int grp = wave / SP, part = wave % SP;
+  const int nrows = min(B::PAIRS, it.n_new * a.G - it.r0), base = it.len - it.n_new;
+  u4 *kf = reinterpret_cast<u4 *>(lds);                        // [half][ks][part][64], slots turned by (ks, g)
+  u4 *vf = kf + B::FRAG / 16;                                  // [c][t][part][64]
+  f4 *xs = reinterpret_cast<f4 *>(lds + 2 * B::FRAG);           // [wave][nq][half][64]
+  uint32_t *rows = reinterpret_cast<uint32_t *>(lds + B::LDS - 2 * kTile * 4);  // [2][32]
+
+  // ---- q
+  u4 q[NQ][KW][QP];
+  float sc[NQ], m[NQ], l[NQ];
+  const int t_first = it.r0 / a.G, r_wave = 16 * NQ * grp;
+  const int low_key = a.window ? max(it.k0, base + t_first - a.window + 1) : it.k0;
+  const bool busy = r_wave < nrows;
+  // the keys that all of this wave's rows attend to, and that any of them does
+  const int tw0 = (it.r0 + r_wave) / a.G, tw1 = (it.r0 + min(nrows, r_wave + 16 * NQ) - 1) / a.G;
+  const int all_lo = a.window ? max(low_key, base + tw1 - a.window + 1) : low_key;
+  const int all_hi = min(it.k1 - 1, base + tw0), any_hi = min(it.k1 - 1, base + tw1);
+  const int any_lo = a.window ? max(low_key, base + tw0 - a.window + 1) : low_key;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = r_wave + 16 * n + c16;
+    const bool real = r < nrows;
+    const int t = real ? (it.r0 + r) / a.G : t_first, h = real ? (it.r0 + r) - t * a.G : 0;
+    m[n] = kLow;
+    l[n] = 0.f;
+    const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
+    float up = 1.f, down = 1.f;
+    if constexpr (F16) {
+      float big = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const f4 u = ldg<f4>(qp + 32 * ks), v = ldg<f4>(qp + 32 * ks + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) big = fmaxf(big, fmaxf(fabsf(u[j]), fabsf(v[j])));
+      }
+      lift_of(max_groups(big), &up, &down);
+    }
+    sc[n] = a.scale * down;
+    qp += 32 * KW * part;
+#pragma unroll
+    for (int ks = 0; ks < KW; ++ks) {
+      const f4 u = ldg<f4>(qp + 32 * ks), v = ldg<f4>(qp + 32 * ks + 4);
+      uint32_t p[QP][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        split2<F16, QP>(real ? u[2 * j] * up : 0.f, real ? u[2 * j + 1] * up : 0.f, &p[0][j], 4);
+        split2<F16, QP>(real ? v[2 * j] * up : 0.f, real ? v[2 * j + 1] * up : 0.f, &p[0][2 + j], 4);
+      }
+#pragma unroll
+      for (int i = 0; i < QP; ++i) q[n][ks][i] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  f4 o[NQ][CW * VD] = {};
+  const int n_tiles = (it.k1 - it.k0 + kTile - 1) / kTile;
+  auto span = [&](int n, int *low, int *high) {
+    const int r = min(r_wave + 16 * n + c16, nrows - 1), pos = base + (int)div_by(it.r0 + r, a.by_g);
+    *high = min(it.k1 - 1, pos);
+    *low = a.window ? max(low_key, pos - a.window + 1) : low_key;
+  };
+  const uint32_t row_bytes = (uint32_t)a.n_kv * HD * ES;
+  const char *kb0 = static_cast<const char *>(a.k) + ((size_t)kvh * HD + 8 * (tid % D8)) * ES;
+  const char *vb0 = static_cast<const char *>(a.v) + ((size_t)kvh * HD + wave * CD + VD * c16) * ES;
+  // Pool row of a tile's key `tid`, never one outside the attended keys; two tiles' rows in LDS.
+  // Those of the next are written between the two barriers of a tile, in place of the last's,
+  // whose readers are past the first of them.
+  auto find = [&](int tile) {
+    const int key = min(max(it.k0 + tile * kTile + tid, low_key), it.k1 - 1);
+    const int pg = (int)div_by((uint32_t)key, a.by_page);
+    return ldg<int32_t>(a.pages + (size_t)it.seq * a.stride + pg) * a.page_rows + key - pg * a.page_size;
+  };
+  uint32_t kr[UK][ES * 2];      // 8 dims of a key
+  uint32_t vr[8][VD * ES / 4];  // VD dims of eight keys
+  auto load_k = [&](int tile) {
+    const uint32_t *row = rows + (tile & 1) * kTile + tid / D8;
+#pragma unroll
+    for (int u = 0; u < UK; ++u) {
+      const char *p = kb0 + (uint64_t)row[64 * W / D8 * u] * row_bytes;
+#pragma unroll
+      for (int j = 0; j < ES / 2; ++j) {
+        const u4 x = ldg<u4>(p + 16 * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kr[u][4 * j + e] = x[e];
+      }
+    }
+  };
+  auto load_v = [&](int tile) {
+    const u4 *row = reinterpret_cast<const u4 *>(rows + (tile & 1) * kTile) + g;
+    const u4 r0 = row[0], r1 = row[4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const char *p = vb0 + (uint64_t)(j < 4 ? r0[j & 3] : r1[j & 3]) * row_bytes;
+      if constexpr (VD * ES == 4) {
+        vr[j][0] = ldg<uint32_t>(p);
+      } else if constexpr (VD * ES == 8) {
+        const u2 x = ldg<u2>(p);
+        vr[j][0] = x[0];
+        vr[j][1] = x[1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < VD * ES / 16; ++i) {
+          const u4 x = ldg<u4>(p + 16 * i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vr[j][4 * i + e] = x[e];
+        }
+      }
+    }
+  };
+  const bool v_busy = wave < NC;
+  if (tid < kTile) rows[tid] = find(0);
+  __syncthreads();
+  load_k(0);
+  for (int tile = 0; tile < n_tiles; ++tile) {
+    const int kb = it.k0 + tile * kTile;
+#pragma unroll
+    for (int u = 0; u < UK; ++u) {
+      const int key = (tid + 64 * W * u) / D8, d8 = tid % D8;
+      u4 *dst = kf + (((key >> 4) * KS + (d8 >> 2)) * KP) * 64 + (d8 & 3) * 16 + ((key ^ d8) & 15);
+      if constexpr (ES == 2) {
+        dst[0] = u4{kr[u][0], kr[u][1], kr[u][2], kr[u][3]};
+      } else {
+        uint32_t p[KP][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          split2<false, KP>(__uint_as_float(kr[u][2 * j]), __uint_as_float(kr[u][2 * j + 1]), &p[0][j], 4);
+#pragma unroll
+        for (int i = 0; i < KP; ++i) dst[64 * i] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __syncthreads();
+    if (v_busy) load_v(tile);
+    int next = 0;
+    if (tid < kTile) next = find(min(tile + 1, n_tiles - 1));
+    uint32_t pf[NQ][QP][4];
+    f4 s[2][NQ] = {};
+    const bool work = busy && kb <= any_hi && kb + kTile - 1 >= any_lo;
+    const bool edge = kb < all_lo || kb + kTile - 1 > all_hi;
+    if (work) {
+      // (fragment by fragment, read RING - 1 ahead: over many of them the compiler, left to
+      // itself, reads as far ahead as it can and runs out of registers)
+      f4 s_low[NQ] = {};
+      u4 x[RING];
+      auto read = [&](int f) {
+        const int i = f / (KW * KP), ks = KW * part + f / KP % KW, pb = KP - 1 - f % KP;
+        x[f % RING] = kf[((i * KS + ks) * KP + pb) * 64 + g * 16 + ((c16 ^ (4 * ks + g)) & 15)];
+      };
+#pragma unroll
+      for (int f = 0; f < RING - 1; ++f) read(f);
+#pragma unroll
+      for (int f = 0; f < 2 * KW * KP; ++f) {
+        const int i = f / (KW * KP), ks = f / KP % KW, pb = KP - 1 - f % KP;
+        if (f + RING - 1 < 2 * KW * KP) read(f + RING - 1);
+#pragma unroll
+        for (int pa = QP - 1; pa >= 0; --pa) {
+          if (pa + pb >= F::TERMS) continue;
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            f4 &d = pa + pb ? s_low[n] : s[i][n];
+            d = mfma<F16>(x[f % RING], q[n][ks][pa], d);
+          }
+        }
+        if (ks == KW - 1 && pb == 0) {
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            s[i][n] += s_low[n];
+            s_low[n] = f4{};
+            if constexpr (SP > 1) xs[((wave * NQ + n) * 2 + i) * 64 + lane] = s[i][n];
+          }
+        }
+        if constexpr (STRICT) __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (SP == 1) probabilities<DT, NQ>(s, kb, edge, sc, span, m, l, o, pf);
+    }
+    if (tid < kTile) rows[((tile + 1) & 1) * kTile + tid] = next;
+    if (v_busy) {
+#pragma unroll
+      for (int t = 0; t < VD; ++t) {
+        uint32_t p[KP][4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          if constexpr (ES == 2)
+            p[0][d] = __builtin_amdgcn_perm(vr[2 * d + 1][t / 2], vr[2 * d][t / 2],
+                                            t & 1 ? 0x07060302u : 0x05040100u);
+          else
+            split2<false, KP>(__uint_as_float(vr[2 * d][t]), __uint_as_float(vr[2 * d + 1][t]), &p[0][d], 4);
+        }
+#pragma unroll
+        for (int i = 0; i < KP; ++i)
+          vf[((wave * VD + t) * KP + i) * 64 + lane] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
+        if constexpr (ES == 4) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __syncthreads();
+    if (tile + 1 < n_tiles) load_k(tile + 1);
+    if (work) {
+      if constexpr (SP > 1) {
+#pragma unroll
+        for (int w = 0; w < SP; ++w) {
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const f4 x = xs[(((grp * SP + w) * NQ + n) * 2 + i) * 64 + lane];
+              s[i][n] = w ? s[i][n] + x : x;
+            }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        probabilities<DT, NQ>(s, kb, edge, sc, span, m, l, o, pf);
+      }
+      u4 x[RING];
+      auto read = [&](int f) {
+        x[f % RING] = vf[((CW * VD * part + f / KP) * KP + KP - 1 - f % KP) * 64 + lane];
+      };
+#pragma unroll
+      for (int f = 0; f < RING - 1; ++f) read(f);
+#pragma unroll
+      for (int f = 0; f < CW * VD * KP; ++f) {
+        const int d = f / KP, pb = KP - 1 - f % KP;
+        if (f + RING - 1 < CW * VD * KP) read(f + RING - 1);
+#pragma unroll
+        for (int pa = QP - 1; pa >= 0; --pa) {
+          if (pa + pb >= F::TERMS) continue;
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+            o[n][d] = mfma<F16>(x[f % RING], u4{pf[n][pa][0], pf[n][pa][1], pf[n][pa][2], pf[n][pa][3]}, o[n][d]);
+        }
+        if constexpr (STRICT) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  // ---- every wave has its rows' sums
+  int bad = 0;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    l[n] = sum_groups(l[n]);
+    bad |= !(fabsf(l[n]) < INFINITY);
+#pragma unroll
+    for (int d = 0; d < CW * VD; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[n][d][e]) < INFINITY);
+  }
+  if (__syncthreads_or(bad)) {
+    item_by_key<HD, DT, 64 * W>(a, it, kvh, B::PAIRS, reinterpret_cast<float *>(lds));
+    return;
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = r_wave + 16 * n + c16;
+    if (r >= nrows) continue;
+    const int t = (it.r0 + r) / a.G, h = (it.r0 + r) - t * a.G;
+    const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
+    float *dst = (it.part < 0 ? a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD
+                              : a.part_o + pr * HD) + CW * CD * part;
+    const float f = it.part < 0 ? l[n] : 1.f;
+#pragma unroll
+    for (int c = 0; c < CW; ++c)
+#pragma unroll
+      for (int e = 0; e < 4 * VD; e += 4) {  // dims VD (4 g + e / VD) + e % VD of the chunk
+        f4 x;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = o[n][c * VD + (e + u) % VD][(e + u) / VD] / f;
+        *reinterpret_cast<f4 *>(dst + c * CD + 4 * VD * g + e) = x;
+      }
+    if (it.part >= 0 && g == 0 && part == 0) {
+      a.part_ml[pr * 2] = m[n];
+      a.part_ml[pr * 2 + 1] = l[n];
+    }
+  }
+}
+
+template <int HD, int DT, int NQ, int W>
+constexpr int tile_lds() {
+  constexpr int q = Form<DT>::QP * NQ * HD * 32;
+  constexpr int e = W * (32 * NQ + 16 * (16 * v_dims<HD, DT>() + 4)) * 4;
   return q > e ? q : e;
 }
 
-// At most 16 NQ pairs an item; items of at most 16 (single tokens in a call that has longer
-// chunks too) take one query tile instead of NQ.
-template <int HD, int DT, int NQ>
-__global__ __launch_bounds__(256, HD * NQ >= 512 ? 1 : 2) void k_paged_attn(PagedAttnArgs a) {
-  __shared__ __align__(16) char lds[attn_lds<HD, DT, NQ>()];
-  const int kvh = blockIdx.x % a.n_kv;
+
+// Items of at most 16 pairs: single tokens.
+template <int HD, int DT>
+__global__ __launch_bounds__(256, 2) void k_paged_tile(PagedAttnArgs a) {
+  __shared__ __align__(16) char lds[tile_lds<HD, DT, 1, 4>()];
+  item_by_tile<HD, DT, 1, 4>(a, a.items[blockIdx.x / a.n_kv], blockIdx.x % a.n_kv, lds);
+}
+
+// Items of longer chunks, and single tokens beside them.
+template <int HD, int DT, int NT = 64 * Shape<HD, DT>::W>
+__global__ __launch_bounds__(NT, 2) void k_paged_block(PagedAttnArgs a) {
+  constexpr int A = tile_lds<HD, DT, 1, Shape<HD, DT>::W>(), B = Shape<HD, DT>::LDS;
+  __shared__ __align__(16) char lds[A > B ? A : B];
   const PagedItem it = a.items[blockIdx.x / a.n_kv];
-  if constexpr (NQ > 1) {
-    if (it.n_new * a.G - it.r0 <= 16) return item_by_tile<HD, DT, 1, NQ>(a, it, kvh, lds);
-  }
-  item_by_tile<HD, DT, NQ, NQ>(a, it, kvh, lds);
+  if (it.n_new * a.G - it.r0 <= 16)
+    item_by_tile<HD, DT, 1, Shape<HD, DT>::W>(a, it, blockIdx.x % a.n_kv, lds);
+  else
+    item_by_block<HD, DT>(a, it, blockIdx.x % a.n_kv, lds);
 }
 
 // The parts of one result, weighted by e^(their maximum - the largest): a block per (row,
 // head), its threads HD / 4 columns by 1024 / HD groups of parts.
 constexpr int kMaxParts = 1024;
-template <int HD, int NQ>
+template <int HD>
 __global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a, const PagedMerge *merge) {
   constexpr int COLS = HD / 4, GRP = 256 / COLS;
   __shared__ float w[kMaxParts], red[8];
@@ -544,7 +909,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a, const Page
   const int tid = threadIdx.x, kvh = blockIdx.x % a.n_kv, r = blockIdx.y;
   const PagedMerge g = merge[blockIdx.x / a.n_kv];
   if (r >= g.n_new * a.G - g.r0) return;
-  const size_t pr = ((size_t)g.part * a.n_kv + kvh) * (16 * NQ) + r, step = (size_t)a.n_kv * 16 * NQ;
+  const size_t pr = ((size_t)g.part * a.n_kv + kvh) * a.part_rows + r, step = (size_t)a.n_kv * a.part_rows;
   const int col = tid % COLS, grp = tid / COLS;
   float top = -INFINITY;
   for (int p = tid; p < g.n; p += 256) {
@@ -578,47 +943,66 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a, const Page
       o / ((red[4] + red[5]) + (red[6] + red[7]));
 }
 
-// Blocks of 16 nq (row, head) pairs and spans of keys.  The spans are cut so that about
-// `blocks` blocks have the same number of tiles each; the longest come first.
+// Items of p->rows (row, head) pairs, their keys cut into spans so that the work fits
+// `blocks` blocks at a time; the longest come first.
 int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
-  const int rows_of = 16 * p->nq;
+  struct Span {
+    int seq, r0, k0, k1, tiles, cost;  // cost: of a tile, in tiles of one wave
+  };
+  std::vector<Span> spans;
+  int64_t work = 0;
+  int most = 0, longest = 0;
+  for (int s = 0; s < b->n_seqs; ++s) {
+    const int pairs = b->n_new[s] * p->G, base = b->len[s] - b->n_new[s];
+    most = std::max(most, std::min(pairs, p->rows));
+    for (int r0 = 0; r0 < pairs; r0 += p->rows) {
+      const int t0 = r0 / p->G, t1 = std::min((r0 + p->rows - 1) / p->G, b->n_new[s] - 1);
+      const int lo = p->window ? std::max(0, base + t0 - p->window + 1) : 0;
+      const int k0 = lo / kTile * kTile, k1 = base + t1 + 1, n = (k1 - k0 + kTile - 1) / kTile;
+      // (an item of at most 16 pairs spreads four tiles over its waves)
+      spans.push_back({s, r0, k0, k1, n, p->rows > 16 && pairs - r0 > 16 ? 4 : 1});
+      work += (int64_t)n * spans.back().cost;
+      longest = std::max(longest, n * spans.back().cost);
+    }
+  }
+  // The longest part a block gets, `per`: at least a tile for each of four waves, and no more
+  // parts than a merge takes; from an even share up, where its end is soonest: all blocks at once
+  // are done with the longest, more of them after about half of one more.
+  auto cuts_of = [](const Span &x, int per) { return (x.tiles * x.cost + per - 1) / per; };
+  const int64_t fill = std::max((work * p->n_kv + blocks - 1) / blocks,
+                                ((int64_t)b->max_pos / kTile * 4 + kMaxParts) / kMaxParts);
+  int per = (int)((fill + 3) / 4 * 4);
+  int64_t best = INT64_MAX;
+  for (int64_t c = per;; c += std::max<int64_t>(4, c / 8 / 4 * 4)) {
+    int64_t n = 0, top = 0;
+    for (const Span &x : spans) {
+      const int cuts = cuts_of(x, (int)c);
+      n += cuts;
+      top = std::max<int64_t>(top, (x.tiles + cuts - 1) / cuts * x.cost);
+    }
+    n *= p->n_kv;
+    const int64_t end = n <= blocks ? top : std::max(top, work * p->n_kv / blocks) + top / 2;
+    if (end < best) {
+      best = end;
+      per = (int)c;
+    }
+    if (c >= longest || c > 4 * fill + 64) break;
+  }
   std::vector<PagedItem> items;
   std::vector<PagedMerge> merge;
-  auto spans = [&](int s, int r0, int *k0, int *k1) {
-    const int t0 = r0 / p->G, t1 = std::min((r0 + rows_of - 1) / p->G, b->n_new[s] - 1);
-    const int base = b->len[s] - b->n_new[s];
-    const int lo = p->window ? std::max(0, base + t0 - p->window + 1) : 0;
-    *k0 = lo / kTile * kTile;
-    *k1 = base + t1 + 1;
-  };
-  int64_t tiles = 0;
-  for (int s = 0; s < b->n_seqs; ++s)
-    for (int r0 = 0; r0 < b->n_new[s] * p->G; r0 += rows_of) {
-      int k0, k1;
-      spans(s, r0, &k0, &k1);
-      tiles += (k1 - k0 + kTile - 1) / kTile;
+  std::vector<std::pair<int, int>> order;
+  int parts = 0;
+  for (const Span &x : spans) {
+    const int cuts = cuts_of(x, per), s = x.seq;
+    if (cuts > 1) merge.push_back({b->first[s], b->n_new[s], x.r0, parts, cuts});
+    for (int c = 0; c < cuts; ++c) {
+      const int i0 = (int)((int64_t)x.tiles * c / cuts), i1 = (int)((int64_t)x.tiles * (c + 1) / cuts);
+      order.push_back({-(i1 - i0) * x.cost, (int)items.size()});
+      items.push_back({b->first[s], b->n_new[s], b->len[s], s, x.r0, x.k0 + i0 * kTile,
+                       std::min(x.k1, x.k0 + i1 * kTile), cuts > 1 ? parts++ : -1});
     }
-  // (a multiple of four, a tile for every wave; no more parts than a merge takes)
-  const int64_t fill = std::max((tiles * p->n_kv + blocks - 1) / blocks,
-                                ((int64_t)b->max_pos / kTile + kMaxParts) / kMaxParts);
-  const int per = (int)((fill + 3) / 4 * 4);
-  int parts = 0, most = 0;
-  for (int s = 0; s < b->n_seqs; ++s)
-    for (int r0 = 0; r0 < b->n_new[s] * p->G; r0 += rows_of) {
-      int k0, k1;
-      spans(s, r0, &k0, &k1);
-      const int n = (k1 - k0 + kTile - 1) / kTile, cuts = (n + per - 1) / per;
-      most = std::max(most, b->n_new[s] * p->G);
-      if (cuts > 1) merge.push_back({b->first[s], b->n_new[s], r0, parts, cuts});
-      for (int c = 0; c < cuts; ++c)
-        items.push_back({b->first[s], b->n_new[s], b->len[s], s, r0,
-                         k0 + (int)((int64_t)n * c / cuts) * kTile,
-                         std::min(k1, k0 + (int)((int64_t)n * (c + 1) / cuts) * kTile),
-                         cuts > 1 ? parts++ : -1});
-    }
-  std::stable_sort(items.begin(), items.end(), [](const PagedItem &x, const PagedItem &y) {
-    return x.k1 - x.k0 > y.k1 - y.k0;
-  });
+  }
+  std::sort(order.begin(), order.end());
   p->n_items = (int)items.size();
   p->n_merge = (int)merge.size();
   p->n_parts = parts;
@@ -626,17 +1010,18 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
   p->merge_at = items.size() * sizeof(PagedItem);
   const size_t bytes = p->merge_at + merge.size() * sizeof(PagedMerge);
   if (int rc = p->up.reserve(bytes)) return rc;
-  std::copy(items.begin(), items.end(), reinterpret_cast<PagedItem *>(p->up.h));
+  for (size_t i = 0; i < items.size(); ++i)
+    reinterpret_cast<PagedItem *>(p->up.h)[i] = items[order[i].second];
   std::copy(merge.begin(), merge.end(), reinterpret_cast<PagedMerge *>(p->up.h + p->merge_at));
   if (int rc = p->up.send(bytes)) return rc;
   p->valid = true;
   return MS_OK;
 }
 
-int plan_for(ms_paged_batch *b, int G, int nq, int n_kv, int window, PagedPlan **out) {
+int plan_for(ms_paged_batch *b, int G, int rows, int n_kv, int window, int blocks, PagedPlan **out) {
   PagedPlan *p = nullptr;
   for (PagedPlan *x : b->plans)
-    if (x->G == G && x->nq == nq && x->n_kv == n_kv && x->window == window) p = x;
+    if (x->G == G && x->rows == rows && x->n_kv == n_kv && x->window == window && x->blocks == blocks) p = x;
   if (!p) {
     // (a model has a few shapes of layers; more than that reuse the oldest place)
     if (b->plans.size() < 8) {
@@ -648,38 +1033,46 @@ int plan_for(ms_paged_batch *b, int G, int nq, int n_kv, int window, PagedPlan *
     p = b->plans.back();
     p->valid = false;
     p->G = G;
-    p->nq = nq;
+    p->rows = rows;
+    p->blocks = blocks;
     p->n_kv = n_kv;
     p->window = window;
   }
   *out = p;
-  return p->valid ? MS_OK : make_plan(b, p, 2 * ctx().n_cu);
+  return p->valid ? MS_OK : make_plan(b, p, blocks);
 }
 
-template <int HD, int DT, int NQ>
-void launch(const PagedAttnArgs &a, const PagedPlan &p, hipStream_t st) {
-  hipLaunchKernelGGL((k_paged_attn<HD, DT, NQ>), dim3(p.n_items * a.n_kv), dim3(256), 0, st, a);
-  if (p.n_merge)
-    hipLaunchKernelGGL((k_paged_merge<HD, NQ>), dim3(p.n_merge * a.n_kv, std::min(16 * NQ, p.most)), dim3(256), 0, st,
-                       a,
-                       reinterpret_cast<const PagedMerge *>(p.up.d + p.merge_at));
-}
 template <int HD, int DT>
-void launch_nq(const PagedAttnArgs &a, const PagedPlan &p, hipStream_t st) {
-  constexpr int MAXQ = HD >= 512 ? 1 : HD == 256 ? 2 : 4;
-  if constexpr (MAXQ > 1) {
-    if (p.nq > 1) return launch<HD, DT, MAXQ>(a, p, st);
+int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
+  using B = Shape<HD, DT>;
+  const int rows = most > 16 && B::FITS ? B::PAIRS : 16;
+  PagedPlan *p = nullptr;
+  if (int rc = plan_for(b, a.G, rows, a.n_kv, a.window, (rows > 16 ? 8 / B::W : 2) * ctx().n_cu, &p))
+    return rc;
+  a.part_rows = p->most;
+  if (const size_t n = (size_t)p->n_parts * a.n_kv * a.part_rows) {
+    void *buf = nullptr;
+    if (int rc = scratch(n * (HD + 2) * 4, &buf)) return rc;
+    a.part_o = static_cast<float *>(buf);
+    a.part_ml = a.part_o + n * HD;
   }
-  launch<HD, DT, 1>(a, p, st);
+  a.items = reinterpret_cast<const PagedItem *>(p->up.d);
+  const dim3 grid(p->n_items * a.n_kv);
+  if (rows == 16)
+    hipLaunchKernelGGL((k_paged_tile<HD, DT>), grid, dim3(256), 0, st, a);
+  else if constexpr (B::FITS)
+    hipLaunchKernelGGL((k_paged_block<HD, DT>), grid, dim3(64 * B::W), 0, st, a);
+  if (p->n_merge)
+    hipLaunchKernelGGL(k_paged_merge<HD>, dim3(p->n_merge * a.n_kv, p->most), dim3(256), 0, st, a,
+                       reinterpret_cast<const PagedMerge *>(p->up.d + p->merge_at));
+  MS_HIP_TRY(hipGetLastError());
+  return MS_OK;
 }
 template <int HD>
-void launch_dt(const PagedAttnArgs &a, const PagedPlan &p, int dtype, hipStream_t st) {
-  if (dtype == MS_KV_F32)
-    launch_nq<HD, MS_KV_F32>(a, p, st);
-  else if (dtype == MS_KV_BF16)
-    launch_nq<HD, MS_KV_BF16>(a, p, st);
-  else
-    launch_nq<HD, MS_KV_F16>(a, p, st);
+int launch_type(PagedAttnArgs &a, ms_paged_batch *b, int dtype, int most, hipStream_t st) {
+  if (dtype == MS_KV_F32) return launch<HD, MS_KV_F32>(a, b, most, st);
+  if (dtype == MS_KV_BF16) return launch<HD, MS_KV_BF16>(a, b, most, st);
+  return launch<HD, MS_KV_F16>(a, b, most, st);
 }
 
 }  // namespace
@@ -714,21 +1107,7 @@ extern "C" int ms_paged_attention(const ms_paged_layer *L, ms_paged_batch *b, co
   if (int rc = require_init()) return rc;
   OnDevice on;
   hipStream_t st = ctx().stream;
-  const int nq = most <= 16 ? 1 : hd >= 512 ? 1 : hd == 256 ? 2 : 4;
-  PagedPlan *p = nullptr;
-  try {
-    if (int rc = plan_for(b, G, nq, L->n_kv_heads, L->window, &p)) return rc;
-  } catch (const std::exception &e) {
-    return fail(MS_E_NOMEM, std::string("paged_attention: ") + e.what());
-  }
   PagedAttnArgs a{};
-  const size_t rows = (size_t)p->n_parts * L->n_kv_heads * 16 * nq;
-  if (rows) {
-    void *buf = nullptr;
-    if (int rc = scratch(rows * (hd + 2) * 4, &buf)) return rc;
-    a.part_o = static_cast<float *>(buf);
-    a.part_ml = a.part_o + rows * hd;
-  }
   a.q = d_q;
   a.out = d_out;
   a.q_ld = q_stride;
@@ -737,7 +1116,6 @@ extern "C" int ms_paged_attention(const ms_paged_layer *L, ms_paged_batch *b, co
   a.v = L->v;
   a.pages = b->d_pages();
   a.stride = b->stride;
-  a.items = reinterpret_cast<const PagedItem *>(p->up.d);
   a.n_kv = L->n_kv_heads;
   a.G = G;
   a.window = L->window;
@@ -746,12 +1124,14 @@ extern "C" int ms_paged_attention(const ms_paged_layer *L, ms_paged_batch *b, co
   a.by_page = fast_div(b->page_size);
   a.by_g = fast_div(G);
   a.scale = (float)((L->scale == 0.f ? 1.0 / std::sqrt((double)hd) : L->scale) * 1.4426950408889634);
-  switch (hd) {
-    case 64: launch_dt<64>(a, *p, L->dtype, st); break;
-    case 128: launch_dt<128>(a, *p, L->dtype, st); break;
-    case 256: launch_dt<256>(a, *p, L->dtype, st); break;
-    default: launch_dt<512>(a, *p, L->dtype, st); break;
+  try {
+    switch (hd) {
+      case 64: return launch_type<64>(a, b, L->dtype, most, st);
+      case 128: return launch_type<128>(a, b, L->dtype, most, st);
+      case 256: return launch_type<256>(a, b, L->dtype, most, st);
+      default: return launch_type<512>(a, b, L->dtype, most, st);
+    }
+  } catch (const std::exception &e) {
+    return fail(MS_E_NOMEM, std::string("paged_attention: ") + e.what());
   }
-  MS_HIP_TRY(hipGetLastError());
-  return MS_OK;
 }
