@@ -53,10 +53,10 @@ struct PagedMerge {
 
 // A split of the batch's work, for layers of the same shape.
 struct PagedPlan {
-  int G = 0, rows = 0, n_kv = 0, window = 0, blocks = 0;
+  int G = 0, rows = 0, n_kv = 0, window = 0, blocks = 0, tile_cost = 0;
   bool valid = false;
   int n_items = 0, n_merge = 0, n_parts = 0;
-  int most = 0;  // (row, head) pairs of the longest item
+  int most = 0, most_parts = 0;  // (row, head) pairs of the longest item; parts of one result
   size_t merge_at = 0;  // byte offset of the merge list
   Upload up;
 };

@@ -263,16 +263,22 @@ __device__ inline void lift_of(float big, float *up, float *down) {
   *down = __uint_as_float((uint32_t)(127 - e) << 23);
 }
 
+// Waves that share a tile in item_by_tile: 128 dims each at most, so that a wave's whole tile is
+// in flight at once.
+template <int HD>
+constexpr int tile_split() {
+  return HD <= 128 ? 1 : HD / 128;
+}
 // Dims of a value row that a lane of item_by_tile loads at once: 16 bytes, 8 at head dim 64.
 template <int HD, int DT>
 __host__ __device__ constexpr int v_dims() {
   return DT == MS_KV_F32 || HD == 64 ? 4 : 8;
 }
 
-// The attention of one item: 16 NQ (row, head) pairs, the block's four waves taking its
-// 32-key tiles in turn, each with sums of its own that are joined at the end.  No LDS and
-// no barrier in the loop over the keys: K and V come from the pages straight into the
-// registers that the MFMAs take them from.
+// The attention of one item of at most 16 (row, head) pairs: the block's W waves, in groups of
+// SP that divide the head's dims, take its 32-key tiles in turn, each with sums of its own that are
+// joined at the end.  K and V come from the pages straight into the registers that the
+// MFMAs take them from; LDS carries only the groups' scores.
 //
 // v_mfma_f32_16x16x32: lane l holds A[l % 16][8 (l / 16) + j], B[8 (l / 16) + j][l % 16] and
 // D[4 (l / 16) + e][l % 16].
@@ -286,187 +292,177 @@ __host__ __device__ constexpr int v_dims() {
 // A value that is not finite makes the sums it is multiplied into not finite, with the
 // zeros of masked keys too; where the end finds such a sum the item is done again key by
 // key.
-template <int HD, int DT, int NQ, int W>
+template <int HD, int DT, int W>
 __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const PagedItem &it, int kvh,
                                              char *lds) {
   using F = Form<DT>;
   constexpr bool F16 = F::F16;
-  constexpr int QP = F::QP, KP = F::KP, KS = HD / 32, ES = DT == MS_KV_F32 ? 4 : 2;
-  constexpr int VD = v_dims<HD, DT>(), CD = 16 * VD, NC = HD / CD;
+  constexpr int SP = tile_split<HD>(), NG = W / SP, HW = HD / SP;
+  constexpr int QP = F::QP, KP = F::KP, KS = HW / 32, ES = DT == MS_KV_F32 ? 4 : 2;
+  constexpr int VD = v_dims<HD, DT>(), CD = 16 * VD, NC = HW / CD;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
-  const int nrows = min(16 * NQ, it.n_new * a.G - it.r0), base = it.len - it.n_new;
-
-  // ---- q: parts in LDS in fragment order; per query its position and scale
-  u4 *qf = reinterpret_cast<u4 *>(lds);  // [nq][s][part][64]
-  float sc[NQ];
-  const int t_first = it.r0 / a.G, t_last = (it.r0 + nrows - 1) / a.G;
+  const int grp = wave / SP, part = wave % SP;
+  const int nrows = min(16, it.n_new * a.G - it.r0), base = it.len - it.n_new;
+  const int t_first = (int)div_by(it.r0, a.by_g), t_last = (int)div_by(it.r0 + nrows - 1, a.by_g);
   const int low_key = a.window ? max(it.k0, base + t_first - a.window + 1) : it.k0;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = 16 * n + c16, t = (it.r0 + r) / a.G, h = (it.r0 + r) - t * a.G;
-    const bool real = r < nrows;
-    const float *q = a.q + (size_t)(it.row + (real ? t : t_first)) * a.q_ld +
-                     (size_t)(kvh * a.G + (real ? h : 0)) * HD + 8 * g;
-    float x[(KS + W - 1) / W][8];
-    float big = 0.f;
-    if constexpr (F16) {
-      // (every wave needs the whole row's largest value)
-      for (int s = 0; s < KS; ++s) {
-        const f4 u = ldg<f4>(q + 32 * s), v = ldg<f4>(q + 32 * s + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) big = fmaxf(big, fmaxf(fabsf(u[j]), fabsf(v[j])));
-      }
-      big = max_groups(big);
-    }
-    float up = 1.f, down = 1.f;
-    if constexpr (F16) lift_of(big, &up, &down);
-    sc[n] = a.scale * down;
-#pragma unroll
-    for (int si = 0; si < (KS + W - 1) / W; ++si) {
-      const int s = wave + W * si;
-      if (s < KS) {
-        const f4 u = ldg<f4>(q + 32 * s), v = ldg<f4>(q + 32 * s + 4);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[si][j] = real ? (j < 4 ? u[j] : v[j - 4]) * up : 0.f;
-        uint32_t p[QP][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) split2<F16, QP>(x[si][2 * j], x[si][2 * j + 1], &p[0][j], 4);
-#pragma unroll
-        for (int i = 0; i < QP; ++i)
-          qf[((n * KS + s) * QP + i) * 64 + lane] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
-      }
-    }
-  }
-  __syncthreads();
-
-  auto span = [&](int n, int *low, int *high) {
-    const int r = min(16 * n + c16, nrows - 1), pos = base + (int)div_by(it.r0 + r, a.by_g);
-    *high = min(it.k1 - 1, pos);
-    *low = a.window ? max(low_key, pos - a.window + 1) : low_key;
-  };
-  f4 o[NQ][NC * VD] = {};
-  float m[NQ], l[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    m[n] = kLow;
-    l[n] = 0.f;
-  }
   const int n_tiles = (it.k1 - it.k0 + kTile - 1) / kTile;
-  // keys that every row attends to
-  const int all_lo = a.window ? max(low_key, base + t_last - a.window + 1) : low_key;
-  const int all_hi = min(it.k1 - 1, base + t_first);
-  const int32_t *pages = a.pages + (size_t)it.seq * a.stride;
-  const uint32_t row_bytes = (uint32_t)a.n_kv * HD * ES;
-  const char *kb0 = static_cast<const char *>(a.k) + ((size_t)kvh * HD + 8 * g) * ES;
-  const char *vb0 = static_cast<const char *>(a.v) + ((size_t)kvh * HD + VD * c16) * ES;
+
   // row of key kb + (lane & 31), never one outside the attended keys
+  const int32_t *pages = a.pages + (size_t)it.seq * a.stride;
   auto find = [&](int tile, int *page, int *slot) {
-    const int key = min(max(it.k0 + tile * kTile + (lane & 31), low_key), it.k1 - 1);
+    const int key = min(max(it.k0 + min(tile, n_tiles - 1) * kTile + (lane & 31), low_key), it.k1 - 1);
     const int pg = (int)div_by((uint32_t)key, a.by_page);
     *slot = key - pg * a.page_size;
     *page = ldg<int32_t>(pages + pg);
   };
-  int page = 0, slot = 0;
-  if (wave < n_tiles) find(wave, &page, &slot);
-  for (int tile = wave; tile < n_tiles; tile += W) {
-    const int kb = it.k0 + tile * kTile;
-    // (the fragments of q are read anew for every tile, not kept)
-    int at = lane;
-    asm volatile("" : "+v"(at));
-    const int row = page * a.page_rows + slot;
-    const char *kp[2], *vp[8];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      kp[i] = kb0 + (uint64_t)(uint32_t)__shfl(row, 16 * i + c16, 64) * row_bytes;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      vp[j] = vb0 + (uint64_t)(uint32_t)__shfl(row, 16 * (j >> 2) + 4 * g + (j & 3), 64) * row_bytes;
-    if (tile + W < n_tiles) find(tile + W, &page, &slot);
+  int page, slot;
+  find(grp, &page, &slot);
+  const uint32_t row_bytes = (uint32_t)a.n_kv * HD * ES;
+  const char *kb0 = static_cast<const char *>(a.k) + ((size_t)kvh * HD + HW * part + 8 * g) * ES;
+  const char *vb0 = static_cast<const char *>(a.v) + ((size_t)kvh * HD + HW * part + VD * c16) * ES;
 
-    // ---- scores
-    // (the products of the leading parts have a sum of their own: a running sum that takes
-    // the small ones too rounds six times as often)
-    f4 s[2][NQ] = {}, s_low[2][NQ] = {};
+  // ---- q
+  float sc[1];
+  u4 q[KS][QP];
+  {
+    const bool real = c16 < nrows;
+    const int t = real ? (int)div_by(it.r0 + c16, a.by_g) : t_first, h = real ? it.r0 + c16 - t * a.G : 0;
+    const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
+    float up = 1.f, down = 1.f;
+    if constexpr (F16) {
+      // (the whole row's largest value)
+      float big = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      uint32_t kf[2][KP][4];
+      for (int s = 0; s < HD / 32; ++s) {
+        const f4 u = ldg<f4>(qp + 32 * s), v = ldg<f4>(qp + 32 * s + 4);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if constexpr (ES == 2) {
-          const u4 x = ldg<u4>(kp[i] + ks * 64);
+        for (int j = 0; j < 4; ++j) big = fmaxf(big, fmaxf(fabsf(u[j]), fabsf(v[j])));
+      }
+      lift_of(max_groups(big), &up, &down);
+    }
+    sc[0] = a.scale * down;
+    qp += HW * part;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) kf[i][0][j] = x[j];
-        } else {
-          const f4 x = ldg<f4>(kp[i] + ks * 128), y = ldg<f4>(kp[i] + ks * 128 + 16);
-          split2<false, KP>(x[0], x[1], &kf[i][0][0], 4);
-          split2<false, KP>(x[2], x[3], &kf[i][0][1], 4);
-          split2<false, KP>(y[0], y[1], &kf[i][0][2], 4);
-          split2<false, KP>(y[2], y[3], &kf[i][0][3], 4);
-        }
+    for (int s = 0; s < KS; ++s) {
+      const f4 u = ldg<f4>(qp + 32 * s), v = ldg<f4>(qp + 32 * s + 4);
+      uint32_t p[QP][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        split2<F16, QP>(real ? u[2 * j] * up : 0.f, real ? u[2 * j + 1] * up : 0.f, &p[0][j], 4);
+        split2<F16, QP>(real ? v[2 * j] * up : 0.f, real ? v[2 * j + 1] * up : 0.f, &p[0][2 + j], 4);
       }
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+      for (int i = 0; i < QP; ++i) q[s][i] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
+    }
+  }
+
+  f4 o[1][NC * VD] = {};
+  float m[1] = {kLow}, l[1] = {0.f};
+  auto span = [&](int, int *low, int *high) {
+    const int pos = base + (int)div_by(it.r0 + min(c16, nrows - 1), a.by_g);
+    *high = min(it.k1 - 1, pos);
+    *low = a.window ? max(low_key, pos - a.window + 1) : low_key;
+  };
+  // keys that every row attends to
+  const int all_lo = a.window ? max(low_key, base + t_last - a.window + 1) : low_key;
+  const int all_hi = min(it.k1 - 1, base + t_first);
+  f4 *xs = reinterpret_cast<f4 *>(lds);  // [2][wave][half][64]
+  for (int step = 0; step * NG < n_tiles; ++step) {
+    const int tile = step * NG + grp, kb = it.k0 + tile * kTile;
+    const bool work = SP == 1 || tile < n_tiles;
+    if (SP == 1 && tile >= n_tiles) break;
+    f4 s[2][1] = {};
+    const char *vp[8];
+    u4 vr[8][NC];
+    if (work) {
+      const int row = page * a.page_rows + slot;
+      u4 kr[2][KS][ES / 2];
 #pragma unroll
-        for (int pa = QP - 1; pa >= 0; --pa) {
-          const u4 q = qf[((n * KS + ks) * QP + pa) * 64 + at];
+      for (int i = 0; i < 2; ++i) {
+        const char *p = kb0 + (uint64_t)(uint32_t)__shfl(row, 16 * i + c16, 64) * row_bytes;
 #pragma unroll
-          for (int pb = KP - 1; pb >= 0; --pb) {
-            if (pa + pb >= F::TERMS) continue;
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              (pa + pb ? s_low : s)[i][n] =
-                  mfma<F16>(u4{kf[i][pb][0], kf[i][pb][1], kf[i][pb][2], kf[i][pb][3]}, q,
-                            (pa + pb ? s_low : s)[i][n]);
+          for (int j = 0; j < ES / 2; ++j) kr[i][ks][j] = ldg<u4>(p + ks * 32 * ES + 16 * j);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        vp[j] = vb0 + (uint64_t)(uint32_t)__shfl(row, 16 * (j >> 2) + 4 * g + (j & 3), 64) * row_bytes;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          if constexpr (VD * ES == 16) {
+            vr[j][c] = ldg<u4>(vp[j] + c * CD * ES);
+          } else {
+            const u2 y = ldg<u2>(vp[j]);
+            vr[j][0] = u4{y[0], y[1], 0, 0};
           }
         }
-    }
-#pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) s[i][n] += s_low[i][n];
+      }
+      find(tile + NG, &page, &slot);
 
-    uint32_t pf[NQ][QP][4];
-    probabilities<DT, NQ>(s, kb, kb < all_lo || kb + kTile - 1 > all_hi, sc, span, m, l, o, pf);
+      // ---- scores (the products of the leading parts have a sum of their own: a running sum
+      // that takes the small ones too rounds as often as there are products)
+      f4 s_low[2] = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t kf[KP][4];
+          if constexpr (ES == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kf[0][j] = kr[i][ks][0][j];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              split2<false, KP>(__uint_as_float(kr[i][ks][j / 2][2 * (j & 1)]),
+                                __uint_as_float(kr[i][ks][j / 2][2 * (j & 1) + 1]), &kf[0][j], 4);
+          }
+#pragma unroll
+          for (int pb = KP - 1; pb >= 0; --pb)
+#pragma unroll
+            for (int pa = QP - 1; pa >= 0; --pa) {
+              if (pa + pb >= F::TERMS) continue;
+              f4 &d = pa + pb ? s_low[i] : s[i][0];
+              d = mfma<F16>(u4{kf[pb][0], kf[pb][1], kf[pb][2], kf[pb][3]}, q[ks][pa], d);
+            }
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i][0] += s_low[i];
+    }
+    if constexpr (SP > 1) {
+      // (two buffers: the next step's scores do not wait for this one's readers)
+      f4 *x = xs + (step & 1) * W * 2 * 64;
+      if (work)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[(wave * 2 + i) * 64 + lane] = s[i][0];
+      __syncthreads();
+      if (work)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[i][0] = x[(grp * SP * 2 + i) * 64 + lane];
+#pragma unroll
+          for (int w = 1; w < SP; ++w) s[i][0] += x[((grp * SP + w) * 2 + i) * 64 + lane];
+        }
+    }
+    if (!work) continue;
+    uint32_t pf[1][QP][4];
+    probabilities<DT, 1>(s, kb, kb < all_lo || kb + kTile - 1 > all_hi, sc, span, m, l, o, pf);
 
     // ---- values
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       uint32_t vf[VD][KP][4];
-      if constexpr (ES == 2) {
-        uint32_t x[8][VD / 2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if constexpr (VD == 8) {
-            const u4 y = ldg<u4>(vp[j] + c * CD * ES);
+      for (int t = 0; t < VD; ++t)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) x[j][d] = y[d];
-          } else {
-            const u2 y = ldg<u2>(vp[j] + c * CD * ES);
-            x[j][0] = y[0];
-            x[j][1] = y[1];
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < VD; ++t)
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            vf[t][0][d] = __builtin_amdgcn_perm(x[2 * d + 1][t / 2], x[2 * d][t / 2],
+        for (int d = 0; d < 4; ++d) {
+          if constexpr (ES == 2)
+            vf[t][0][d] = __builtin_amdgcn_perm(vr[2 * d + 1][c][t / 2], vr[2 * d][c][t / 2],
                                                 t & 1 ? 0x07060302u : 0x05040100u);
-      } else {
-        float x[8][VD];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int d = 0; d < VD / 4; ++d) {
-            const f4 y = ldg<f4>(vp[j] + c * CD * ES + 16 * d);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[j][4 * d + e] = y[e];
-          }
-#pragma unroll
-        for (int t = 0; t < VD; ++t)
-#pragma unroll
-          for (int d = 0; d < 4; ++d) split2<false, KP>(x[2 * d][t], x[2 * d + 1][t], &vf[t][0][d], 4);
-      }
+          else
+            split2<false, KP>(__uint_as_float(vr[2 * d][c][t]), __uint_as_float(vr[2 * d + 1][c][t]),
+                              &vf[t][0][d], 4);
+        }
 #pragma unroll
       for (int pa = QP - 1; pa >= 0; --pa)
 #pragma unroll
@@ -474,83 +470,73 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
           if (pa + pb >= F::TERMS) continue;
 #pragma unroll
           for (int t = 0; t < VD; ++t)
-#pragma unroll
-            for (int n = 0; n < NQ; ++n)
-              o[n][c * VD + t] = mfma<F16>(u4{vf[t][pb][0], vf[t][pb][1], vf[t][pb][2], vf[t][pb][3]},
-                                           u4{pf[n][pa][0], pf[n][pa][1], pf[n][pa][2], pf[n][pa][3]},
-                                           o[n][c * VD + t]);
+            o[0][c * VD + t] = mfma<F16>(u4{vf[t][pb][0], vf[t][pb][1], vf[t][pb][2], vf[t][pb][3]},
+                                         u4{pf[0][pa][0], pf[0][pa][1], pf[0][pa][2], pf[0][pa][3]},
+                                         o[0][c * VD + t]);
         }
     }
   }
 
-  // ---- the waves' sums joined
-  int bad = 0;
+  // ---- the groups' sums joined
+  l[0] = sum_groups(l[0]);
+  int bad = !(fabsf(l[0]) < INFINITY);
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    l[n] = sum_groups(l[n]);
-    bad |= !(fabsf(l[n]) < INFINITY);
+  for (int d = 0; d < NC * VD; ++d)
 #pragma unroll
-    for (int d = 0; d < NC * VD; ++d)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[n][d][e]) < INFINITY);
-  }
-  // (also: every wave is done with q)
+    for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[0][d][e]) < INFINITY);
+  // (also: every wave is done with xs)
   if (__syncthreads_or(bad)) {
-    item_by_key<HD, DT, 64 * W>(a, it, kvh, 16 * NQ, reinterpret_cast<float *>(lds));
+    item_by_key<HD, DT, 64 * W>(a, it, kvh, 16, reinterpret_cast<float *>(lds));
     return;
   }
-  float *ml = reinterpret_cast<float *>(lds);  // [2][wave][16 NQ]
-  constexpr int LD = CD + 4, ROWS = 16 * NQ;
-  float *os = ml + 2 * W * ROWS;               // [wave][16][LD]
-  if (g == 0)
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      ml[wave * ROWS + 16 * n + c16] = m[n];
-      ml[(W + wave) * ROWS + 16 * n + c16] = l[n];
-    }
+  float *ml = reinterpret_cast<float *>(lds);  // [2][group][16]
+  constexpr int LD = CD + 4;
+  float *os = ml + 2 * NG * 16;                // [wave][16][LD]
+  if (g == 0 && part == 0) {
+    ml[grp * 16 + c16] = m[0];
+    ml[(NG + grp) * 16 + c16] = l[0];
+  }
   __syncthreads();
+  float top = kLow;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    float top = kLow;
+  for (int w = 0; w < NG; ++w) top = fmaxf(top, ml[w * 16 + c16]);
+  const float f = __builtin_amdgcn_exp2f(m[0] - top);
 #pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, ml[w * ROWS + 16 * n + c16]);
-    const float f = __builtin_amdgcn_exp2f(m[n] - top);
+  for (int c = 0; c < NC; ++c) {
+    if (c) __syncthreads();
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      __syncthreads();
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int t = 0; t < VD; t += 4) {
+        f4 x;
 #pragma unroll
-        for (int t = 0; t < VD; t += 4) {
-          f4 x;
+        for (int u = 0; u < 4; ++u) x[u] = o[0][c * VD + t + u][e] * f;
+        *reinterpret_cast<f4 *>(os + (wave * 16 + c16) * LD + VD * (4 * g + e) + t) = x;
+      }
+    __syncthreads();
+    for (int i = tid; i < 16 * SP * (CD / 4); i += 64 * W) {
+      const int d = i % (CD / 4) * 4, pt = i / (CD / 4) % SP, r = i / (CD / 4 * SP);
+      if (r >= nrows) break;
+      float mt = kLow, ls = 0.f;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) x[u] = o[n][c * VD + t + u][e] * f;
-          *reinterpret_cast<f4 *>(os + (wave * 16 + c16) * LD + VD * (4 * g + e) + t) = x;
-        }
-      __syncthreads();
-      for (int i = tid; i < 4 * CD; i += 64 * W) {
-        const int r16 = i / (CD / 4), d = i % (CD / 4) * 4, r = 16 * n + r16;
-        if (r >= nrows) continue;
-        float mt = kLow, ls = 0.f;
+      for (int w = 0; w < NG; ++w) mt = fmaxf(mt, ml[w * 16 + r]);
+      f4 x = {};
 #pragma unroll
-        for (int w = 0; w < W; ++w) mt = fmaxf(mt, ml[w * ROWS + r]);
-        f4 x = {};
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          ls += ml[(W + w) * ROWS + r] * __builtin_amdgcn_exp2f(ml[w * ROWS + r] - mt);
-          x += *reinterpret_cast<const f4 *>(os + (w * 16 + r16) * LD + d);
-        }
-        if (it.part < 0) {
-          const int t = (it.r0 + r) / a.G, h = (it.r0 + r) - t * a.G;
-          *reinterpret_cast<f4 *>(a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD +
-                                  c * CD + d) = x / ls;
-        } else {
-          const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
-          *reinterpret_cast<f4 *>(a.part_o + pr * HD + c * CD + d) = x;
-          if (c == 0 && d == 0) {
-            a.part_ml[pr * 2] = mt;
-            a.part_ml[pr * 2 + 1] = ls;
-          }
+      for (int w = 0; w < NG; ++w) {
+        ls += ml[(NG + w) * 16 + r] * __builtin_amdgcn_exp2f(ml[w * 16 + r] - mt);
+        x += *reinterpret_cast<const f4 *>(os + ((w * SP + pt) * 16 + r) * LD + d);
+      }
+      const int dim = pt * HW + c * CD + d;
+      if (it.part < 0) {
+        const int t = (int)div_by(it.r0 + r, a.by_g), h = it.r0 + r - t * a.G;
+        *reinterpret_cast<f4 *>(a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD + dim) =
+            x / ls;
+      } else {
+        const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
+        *reinterpret_cast<f4 *>(a.part_o + pr * HD + dim) = x;
+        if (dim == 0) {
+          a.part_ml[pr * 2] = mt;
+          a.part_ml[pr * 2 + 1] = ls;
         }
       }
     }
@@ -871,83 +857,86 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   }
 }
 
-template <int HD, int DT, int NQ, int W>
+template <int HD, int DT, int W>
 constexpr int tile_lds() {
-  constexpr int q = Form<DT>::QP * NQ * HD * 32;
-  constexpr int e = W * (32 * NQ + 16 * (16 * v_dims<HD, DT>() + 4)) * 4;
-  return q > e ? q : e;
+  constexpr int x = tile_split<HD>() > 1 ? 2 * W * 2 * 64 * 16 : 0;
+  constexpr int e = (32 * (W / tile_split<HD>()) + W * 16 * (16 * v_dims<HD, DT>() + 4)) * 4;
+  return x > e ? x : e;
 }
-
 
 // Items of at most 16 pairs: single tokens.
 template <int HD, int DT>
 __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedAttnArgs a) {
-  __shared__ __align__(16) char lds[tile_lds<HD, DT, 1, 4>()];
-  item_by_tile<HD, DT, 1, 4>(a, a.items[blockIdx.x / a.n_kv], blockIdx.x % a.n_kv, lds);
+  __shared__ __align__(16) char lds[tile_lds<HD, DT, 4>()];
+  item_by_tile<HD, DT, 4>(a, a.items[blockIdx.x / a.n_kv], blockIdx.x % a.n_kv, lds);
 }
 
 // Items of longer chunks, and single tokens beside them.
 template <int HD, int DT, int NT = 64 * Shape<HD, DT>::W>
 __global__ __launch_bounds__(NT, 2) void k_paged_block(PagedAttnArgs a) {
-  constexpr int A = tile_lds<HD, DT, 1, Shape<HD, DT>::W>(), B = Shape<HD, DT>::LDS;
+  constexpr int A = tile_lds<HD, DT, Shape<HD, DT>::W>(), B = Shape<HD, DT>::LDS;
   __shared__ __align__(16) char lds[A > B ? A : B];
   const PagedItem it = a.items[blockIdx.x / a.n_kv];
   if (it.n_new * a.G - it.r0 <= 16)
-    item_by_tile<HD, DT, 1, Shape<HD, DT>::W>(a, it, blockIdx.x % a.n_kv, lds);
+    item_by_tile<HD, DT, Shape<HD, DT>::W>(a, it, blockIdx.x % a.n_kv, lds);
   else
     item_by_block<HD, DT>(a, it, blockIdx.x % a.n_kv, lds);
 }
 
-// The parts of one result, weighted by e^(their maximum - the largest): a block per (row,
-// head), its threads HD / 4 columns by 1024 / HD groups of parts.
+// The parts of one result, weighted by e^(their maximum - the largest).  A block takes RPB rows,
+// its 256 threads being HD / 4 columns of RPB rows by GRP groups of parts: many rows of a few parts
+// (chunks) or one row of many (a single token over a long context).
 constexpr int kMaxParts = 1024;
 template <int HD>
-__global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a, const PagedMerge *merge) {
-  constexpr int COLS = HD / 4, GRP = 256 / COLS;
-  __shared__ float w[kMaxParts], red[8];
-  __shared__ f4 os[GRP][COLS];
-  const int tid = threadIdx.x, kvh = blockIdx.x % a.n_kv, r = blockIdx.y;
+__global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a, const PagedMerge *merge, int rpb) {
+  constexpr int COLS = HD / 4, ALL = 256 / COLS;
+  __shared__ f4 os[ALL][COLS];
+  __shared__ float ls[ALL];
+  const int tid = threadIdx.x, kvh = blockIdx.x % a.n_kv, col = tid % COLS, at = tid / COLS;
+  const int gpr = ALL / rpb, row = at / gpr, grp = at % gpr, r = blockIdx.y * rpb + row;
   const PagedMerge g = merge[blockIdx.x / a.n_kv];
-  if (r >= g.n_new * a.G - g.r0) return;
-  const size_t pr = ((size_t)g.part * a.n_kv + kvh) * a.part_rows + r, step = (size_t)a.n_kv * a.part_rows;
-  const int col = tid % COLS, grp = tid / COLS;
-  float top = -INFINITY;
-  for (int p = tid; p < g.n; p += 256) {
-    w[p] = ldg<float>(a.part_ml + (pr + p * step) * 2);
-    top = fmaxf(top, w[p]);
+  const bool real = r < g.n_new * a.G - g.r0 && r < a.part_rows;
+  const size_t step = (size_t)a.n_kv * a.part_rows;
+  const size_t pr = ((size_t)g.part * a.n_kv + kvh) * a.part_rows + (real ? r : 0);
+  const int n = real ? g.n : 0;
+  float top = kLow;
+  if (COLS * gpr >= 64) {  // the wave is one row's
+    for (int p = tid & 63; p < n; p += 64) top = fmaxf(top, ldg<float>(a.part_ml + (pr + p * step) * 2));
+    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  } else {
+    for (int p = 0; p < n; ++p) top = fmaxf(top, ldg<float>(a.part_ml + (pr + p * step) * 2));
   }
-  for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  if ((tid & 63) == 0) red[tid >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  if (top == -INFINITY) top = 0.f;
   float l = 0.f;
-  for (int p = tid; p < g.n; p += 256) {
-    w[p] = __builtin_amdgcn_exp2f(w[p] - top);
-    l += w[p] * ldg<float>(a.part_ml + (pr + p * step) * 2 + 1);
-  }
-  for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off, 64);
-  if ((tid & 63) == 0) red[4 + (tid >> 6)] = l;
-  __syncthreads();
   f4 o = {};
   const float *po = a.part_o + pr * HD + 4 * col;
-#pragma unroll 4
-  for (int p = grp; p < g.n; p += GRP) o += w[p] * ldg<f4>(po + p * step * HD);
-  os[grp][col] = o;
-  __syncthreads();
-  if (tid >= COLS) return;
-#pragma unroll
-  for (int i = 1; i < GRP; ++i) o += os[i][col];
-  const int t = (g.r0 + r) / a.G, h = (g.r0 + r) - t * a.G;
+#pragma unroll 8
+  for (int p = grp; p < n; p += gpr) {
+    const float *ml = a.part_ml + (pr + p * step) * 2;
+    const float w = __builtin_amdgcn_exp2f(ldg<float>(ml) - top);
+    l += w * ldg<float>(ml + 1);
+    o += w * ldg<f4>(po + p * step * HD);
+  }
+  if (gpr > 1) {
+    os[at][col] = o;
+    if (col == 0) ls[at] = l;
+    __syncthreads();
+    if (grp) return;
+    for (int i = 1; i < gpr; ++i) {
+      o += os[at + i][col];
+      l += ls[at + i];
+    }
+  }
+  if (!real) return;
+  const int t = (int)div_by(g.r0 + r, a.by_g), h = g.r0 + r - t * a.G;
   *reinterpret_cast<f4 *>(a.out + (size_t)(g.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD + 4 * col) =
-      o / ((red[4] + red[5]) + (red[6] + red[7]));
+      o / l;
 }
 
 // Items of p->rows (row, head) pairs, their keys cut into spans so that the work fits
 // `blocks` blocks at a time; the longest come first.
 int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
   struct Span {
-    int seq, r0, k0, k1, tiles, cost;  // cost: of a tile, in tiles of one wave
+    int seq, r0, k0, k1, tiles, cost;  // cost: of a tile, in quarters of a block's step
   };
   std::vector<Span> spans;
   int64_t work = 0;
@@ -959,14 +948,12 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
       const int t0 = r0 / p->G, t1 = std::min((r0 + p->rows - 1) / p->G, b->n_new[s] - 1);
       const int lo = p->window ? std::max(0, base + t0 - p->window + 1) : 0;
       const int k0 = lo / kTile * kTile, k1 = base + t1 + 1, n = (k1 - k0 + kTile - 1) / kTile;
-      // (an item of at most 16 pairs spreads four tiles over its waves)
-      spans.push_back({s, r0, k0, k1, n, p->rows > 16 && pairs - r0 > 16 ? 4 : 1});
+      spans.push_back({s, r0, k0, k1, n, p->rows > 16 && pairs - r0 > 16 ? 4 : p->tile_cost});
       work += (int64_t)n * spans.back().cost;
       longest = std::max(longest, n * spans.back().cost);
     }
   }
-  // The longest part a block gets, `per`: at least a tile for each of four waves, and no more
-  // parts than a merge takes; from an even share up, where its end is soonest: all blocks at once
+  // The longest part a block gets, `per`: at least a step, and no more parts than a merge takes; from an even share up, where its end is soonest: all blocks at once
   // are done with the longest, more of them after about half of one more.
   auto cuts_of = [](const Span &x, int per) { return (x.tiles * x.cost + per - 1) / per; };
   const int64_t fill = std::max((work * p->n_kv + blocks - 1) / blocks,
@@ -991,9 +978,10 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
   std::vector<PagedItem> items;
   std::vector<PagedMerge> merge;
   std::vector<std::pair<int, int>> order;
-  int parts = 0;
+  int parts = 0, most_parts = 0;
   for (const Span &x : spans) {
     const int cuts = cuts_of(x, per), s = x.seq;
+    most_parts = std::max(most_parts, cuts);
     if (cuts > 1) merge.push_back({b->first[s], b->n_new[s], x.r0, parts, cuts});
     for (int c = 0; c < cuts; ++c) {
       const int i0 = (int)((int64_t)x.tiles * c / cuts), i1 = (int)((int64_t)x.tiles * (c + 1) / cuts);
@@ -1007,6 +995,7 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
   p->n_merge = (int)merge.size();
   p->n_parts = parts;
   p->most = most;
+  p->most_parts = most_parts;
   p->merge_at = items.size() * sizeof(PagedItem);
   const size_t bytes = p->merge_at + merge.size() * sizeof(PagedMerge);
   if (int rc = p->up.reserve(bytes)) return rc;
@@ -1018,10 +1007,13 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
   return MS_OK;
 }
 
-int plan_for(ms_paged_batch *b, int G, int rows, int n_kv, int window, int blocks, PagedPlan **out) {
+int plan_for(ms_paged_batch *b, int G, int rows, int n_kv, int window, int blocks, int tile_cost,
+             PagedPlan **out) {
   PagedPlan *p = nullptr;
   for (PagedPlan *x : b->plans)
-    if (x->G == G && x->rows == rows && x->n_kv == n_kv && x->window == window && x->blocks == blocks) p = x;
+    if (x->G == G && x->rows == rows && x->n_kv == n_kv && x->window == window && x->blocks == blocks &&
+        x->tile_cost == tile_cost)
+      p = x;
   if (!p) {
     // (a model has a few shapes of layers; more than that reuse the oldest place)
     if (b->plans.size() < 8) {
@@ -1035,6 +1027,7 @@ int plan_for(ms_paged_batch *b, int G, int rows, int n_kv, int window, int block
     p->G = G;
     p->rows = rows;
     p->blocks = blocks;
+    p->tile_cost = tile_cost;
     p->n_kv = n_kv;
     p->window = window;
   }
@@ -1047,8 +1040,9 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   using B = Shape<HD, DT>;
   const int rows = most > 16 && B::FITS ? B::PAIRS : 16;
   PagedPlan *p = nullptr;
-  if (int rc = plan_for(b, a.G, rows, a.n_kv, a.window, (rows > 16 ? 8 / B::W : 2) * ctx().n_cu, &p))
-    return rc;
+  // blocks that run at once; a step of single tokens takes a tile for every group of waves
+  const int w = rows > 16 ? B::W : 4, cost = std::max(1, 4 * tile_split<HD>() / w);
+  if (int rc = plan_for(b, a.G, rows, a.n_kv, a.window, 8 / w * ctx().n_cu, cost, &p)) return rc;
   a.part_rows = p->most;
   if (const size_t n = (size_t)p->n_parts * a.n_kv * a.part_rows) {
     void *buf = nullptr;
@@ -1062,9 +1056,13 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
     hipLaunchKernelGGL((k_paged_tile<HD, DT>), grid, dim3(256), 0, st, a);
   else if constexpr (B::FITS)
     hipLaunchKernelGGL((k_paged_block<HD, DT>), grid, dim3(64 * B::W), 0, st, a);
-  if (p->n_merge)
-    hipLaunchKernelGGL(k_paged_merge<HD>, dim3(p->n_merge * a.n_kv, p->most), dim3(256), 0, st, a,
-                       reinterpret_cast<const PagedMerge *>(p->up.d + p->merge_at));
+  if (p->n_merge) {
+    // about four parts a thread
+    int rpb = 1024 / HD;
+    while (rpb > 1 && 1024 / HD / rpb * 4 < p->most_parts) rpb /= 2;
+    hipLaunchKernelGGL(k_paged_merge<HD>, dim3(p->n_merge * a.n_kv, cdiv(p->most, rpb)), dim3(256), 0, st, a,
+                       reinterpret_cast<const PagedMerge *>(p->up.d + p->merge_at), rpb);
+  }
   MS_HIP_TRY(hipGetLastError());
   return MS_OK;
 }
