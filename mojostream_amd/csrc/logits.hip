@@ -7,83 +7,166 @@
 namespace ms {
 namespace {
 
-constexpr int kLogTile = 4096;  // logits of a block
 constexpr int kLogRows = 64;    // rows of a launch: their settings are kernel arguments
-constexpr int kLogNT = 256;
+constexpr int kOwners = 1024;   // a power of two
 
 struct LogitsArgs {
   const float *x;
   float *y;
   size_t x_ld, y_ld;
-  int vocab, words;
+  int vocab, words, in_place;
   const int32_t *hist, *bias_ids;
   const float *bias;
   const uint32_t *masks;
   ms_logits_row rows[kLogRows];
 };
 
-// A block has kLogTile ids of one row: it counts the history's ids among them and adds
-// up their biases in LDS, then goes over its logits once.
-__global__ __launch_bounds__(kLogNT) void k_logits(LogitsArgs a) {
-  __shared__ uint32_t cnt[kLogTile];  // bit 31: seen; below: times generated
-  __shared__ float add[kLogTile];
-  __shared__ int owner[kLogTile];
-  const int tid = threadIdx.x, t0 = blockIdx.x * kLogTile;
+// What a block knows of an id: seen, has a bias, times generated.
+constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kMade = 0x3FFFFFFFu;
+
+// A block has 4 PER NT ids of one row.  It loads its logits (only those that the mask
+// allows), counts the history's ids among them and adds up their biases in LDS meanwhile, and
+// goes over them once.  VEC: four ids side by side a thread, where rows are 16-byte aligned.  In
+// place, four logits that nothing changes are neither loaded nor stored.
+template <int NT, int PER, bool VEC>
+__global__ __launch_bounds__(NT) void k_logits(LogitsArgs a) {
+  constexpr int TILE = 4 * PER * NT;
+  __shared__ uint32_t cnt[TILE];
+  __shared__ float add[TILE];
+  __shared__ int owner[kOwners];
+  const int tid = threadIdx.x, t0 = blockIdx.x * TILE;
   const ms_logits_row &w = a.rows[blockIdx.y];
-  const int nt = min(kLogTile, a.vocab - t0);
-  for (int i = tid; i < nt; i += kLogNT) {
-    cnt[i] = 0;
-    add[i] = 0.f;
-    owner[i] = kLogNT;
-  }
-  __syncthreads();
-  for (int i = tid; i < w.n_prompt + w.n_generated; i += kLogNT) {
-    const uint32_t at = (uint32_t)a.hist[w.history + i] - (uint32_t)t0;
-    if (at >= (uint32_t)nt) continue;
-    if (i < w.n_prompt)
-      atomicOr(&cnt[at], 0x80000000u);
-    else
-      atomicAdd(&cnt[at], 1u);
-  }
-  // Entries of one id add up in their order: of the threads that hold one, the lowest
-  // goes first.
-  for (int i0 = 0; i0 < w.n_bias; i0 += kLogNT) {
-    uint32_t at = 0;
-    float v = 0.f;
-    bool wait = false;
-    if (i0 + tid < w.n_bias) {
-      at = (uint32_t)a.bias_ids[w.bias + i0 + tid] - (uint32_t)t0;
-      wait = at < (uint32_t)nt;
-      if (wait) v = a.bias[w.bias + i0 + tid];
+  const int nt = min(TILE, a.vocab - t0), nh = w.n_prompt + w.n_generated, nb = w.n_bias;
+  const float *x = a.x + blockIdx.y * a.x_ld + t0;
+  float *y = a.y + blockIdx.y * a.y_ld + t0;
+  auto id = [&](int j, int e) { return VEC ? (j * NT + tid) * 4 + e : (j * 4 + e) * NT + tid; };
+  auto load = [&](int j, uint32_t ok) {
+    float4_t v = {};
+    if (VEC && id(j, 3) < nt) {
+      if (ok) v = ldg<float4_t>(x + id(j, 0));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (ok >> e & 1) v[e] = ldg<float>(x + id(j, e));
     }
-    while (__syncthreads_or(wait)) {
-      if (wait) atomicMin(&owner[at], tid);
-      __syncthreads();
-      const bool mine = wait && owner[at] == tid;
-      __syncthreads();
-      if (mine) {
-        add[at] += v;
-        owner[at] = kLogNT;
-        wait = false;
+    return v;
+  };
+
+  // ---- what the mask allows of this thread's ids (those past the row: nothing), their logits
+  uint32_t ok[PER];
+  float4_t v[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    ok[j] = 0;
+    if (VEC) {
+      const int i = id(j, 0);
+      if (i < nt) {
+        ok[j] = w.mask < 0 ? 15u : ldg<uint32_t>(a.masks + (size_t)w.mask * a.words + ((t0 + i) >> 5)) >> ((t0 + i) & 31) & 15u;
+        if (i + 3 >= nt) ok[j] &= (1u << (nt - i)) - 1;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = id(j, e);
+        if (i < nt)
+          ok[j] |= (w.mask < 0 ? 1u : ldg<uint32_t>(a.masks + (size_t)w.mask * a.words + ((t0 + i) >> 5)) >> ((t0 + i) & 31) & 1u) << e;
       }
     }
   }
-  __syncthreads();
-  const float *x = a.x + blockIdx.y * a.x_ld + t0;
-  float *y = a.y + blockIdx.y * a.y_ld + t0;
-  for (int i = tid; i < nt; i += kLogNT) {
-    const bool ok = w.mask < 0 ||
-                    (a.masks[(size_t)w.mask * a.words + ((t0 + i) >> 5)] >> ((t0 + i) & 31) & 1);
-    float v = -INFINITY;
-    if (ok) {
-      v = x[i];
-      const uint32_t c = cnt[i], made = c & 0x7FFFFFFFu;
-      if (c) v = v > 0.f ? v / w.repetition : v * w.repetition;
-      if (made) v = v - w.frequency * (float)made - w.presence;
-      v += add[i];
+  if (!a.in_place)
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v[j] = load(j, ok[j]);
+
+  // ---- history and biases
+  if (nh + nb > 0) {
+    for (int i = tid; i < TILE; i += NT) cnt[i] = 0;
+    if (nb > 0) {
+      for (int i = tid; i < TILE; i += NT) add[i] = 0.f;
+      for (int i = tid; i < kOwners; i += NT) owner[i] = NT;
     }
-    y[i] = v;
+    __syncthreads();
+    const int32_t *h = a.hist + w.history;
+    for (int i0 = tid; i0 < nh; i0 += 4 * NT) {
+      uint32_t at[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) at[u] = (uint32_t)ldg<int32_t>(h + min(i0 + u * NT, nh - 1)) - (uint32_t)t0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * NT;
+        if (i >= nh || at[u] >= (uint32_t)nt) continue;
+        if (i < w.n_prompt)
+          atomicOr(&cnt[at[u]], kSeen);
+        else
+          atomicAdd(&cnt[at[u]], 1u);
+      }
+    }
+    // Entries of one id add up in their order: of the threads that hold one, the lowest goes first.
+    // (Threads whose ids share a place among the owners take turns too.)
+    for (int i0 = 0; i0 < nb; i0 += NT) {
+      uint32_t at = 0;
+      float b = 0.f;
+      bool wait = false;
+      if (i0 + tid < nb) {
+        at = (uint32_t)ldg<int32_t>(a.bias_ids + w.bias + i0 + tid) - (uint32_t)t0;
+        wait = at < (uint32_t)nt;
+        if (wait) b = ldg<float>(a.bias + w.bias + i0 + tid);
+      }
+      while (__syncthreads_or(wait)) {
+        if (wait) atomicMin(&owner[at & (kOwners - 1)], tid);
+        __syncthreads();
+        const bool mine = wait && owner[at & (kOwners - 1)] == tid;
+        __syncthreads();
+        if (mine) {
+          add[at] += b;
+          atomicOr(&cnt[at], kBiased);
+          owner[at & (kOwners - 1)] = NT;
+          wait = false;
+        }
+      }
+    }
+    __syncthreads();
   }
+
+  // ---- once over the logits
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    uint32_t c[4] = {};
+    if (nh + nb > 0)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (ok[j] >> e & 1) c[e] = cnt[id(j, e)];
+    if (a.in_place) {
+      if (ok[j] == 15 && !(c[0] | c[1] | c[2] | c[3])) continue;
+      v[j] = load(j, ok[j]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float z = v[j][e];
+      if (c[e]) {
+        const uint32_t made = c[e] & kMade;
+        if (c[e] & (kSeen | kMade)) z = z > 0.f ? z / w.repetition : z * w.repetition;
+        if (made) z = z - w.frequency * (float)made - w.presence;
+        if (c[e] & kBiased) z += add[id(j, e)];
+      }
+      v[j][e] = ok[j] >> e & 1 ? z : -INFINITY;
+    }
+    if (VEC && id(j, 3) < nt) {
+      *reinterpret_cast<float4_t *>(y + id(j, 0)) = v[j];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (id(j, e) < nt) y[id(j, e)] = v[j][e];
+    }
+  }
+}
+
+template <int NT, int PER>
+void launch_tiles(const LogitsArgs &a, int rows, bool vec, hipStream_t st) {
+  const dim3 grid(cdiv(a.vocab, 4 * PER * NT), rows);
+  if (vec)
+    hipLaunchKernelGGL((k_logits<NT, PER, true>), grid, dim3(NT), 0, st, a);
+  else
+    hipLaunchKernelGGL((k_logits<NT, PER, false>), grid, dim3(NT), 0, st, a);
 }
 
 }  // namespace
@@ -115,7 +198,7 @@ extern "C" int ms_logits_process(const float *d_logits, size_t in_stride, float 
                  at + "a penalty is not a finite number");
     MS_CHECK_ARG(w.n_prompt >= 0 && w.n_generated >= 0 && w.n_bias >= 0, at + "negative count");
     const int64_t h = (int64_t)w.n_prompt + w.n_generated;
-    MS_CHECK_ARG(h <= (1 << 30) && w.history >= 0 && (uint64_t)w.history <= n_history &&
+    MS_CHECK_ARG(h < (1 << 30) && w.history >= 0 && (uint64_t)w.history <= n_history &&
                      (uint64_t)h <= n_history - (uint64_t)w.history && (h == 0 || d_history),
                  at + "the history reaches past d_history");
     MS_CHECK_ARG(w.bias >= 0 && (uint64_t)w.bias <= n_bias &&
@@ -136,12 +219,19 @@ extern "C" int ms_logits_process(const float *d_logits, size_t in_stride, float 
   a.bias_ids = d_bias_ids;
   a.bias = d_bias;
   a.masks = d_masks;
+  a.in_place = d_logits == d_out;
+  const bool vec = aligned16(d_logits) && aligned16(d_out) && in_stride % 4 == 0 && out_stride % 4 == 0;
   for (int r0 = 0; r0 < rows; r0 += kLogRows) {
     const int n = rows - r0 < kLogRows ? rows - r0 : kLogRows;
     a.x = d_logits + (size_t)r0 * in_stride;
     a.y = d_out + (size_t)r0 * out_stride;
     for (int r = 0; r < kLogRows; ++r) a.rows[r] = h_rows[r0 + (r < n ? r : 0)];
-    hipLaunchKernelGGL(k_logits, dim3(cdiv(vocab, kLogTile), n), dim3(kLogNT), 0, ctx().stream, a);
+    // Every block reads its row's whole history: blocks of 8192 ids, smaller ones only where those
+    // would leave compute units idle.
+    if ((long)n * cdiv(vocab, 8192) >= ctx().n_cu)
+      launch_tiles<512, 4>(a, n, vec, ctx().stream);
+    else
+      launch_tiles<256, 1>(a, n, vec, ctx().stream);
     MS_HIP_TRY(hipGetLastError());
   }
   return MS_OK;

@@ -3,6 +3,7 @@
 #include <cstring>
 #include <exception>
 #include <new>
+#include <type_traits>
 
 #include "devutil.h"
 #include "paged.h"
@@ -102,52 +103,76 @@ struct AppendArgs {
   void *kp, *vp;
   size_t q_ld, kv_ld, q_out_ld;
   int n_heads, n_kv, hd, rot, page_rows;
-  int per_row;  // threads of a row
+  int log_units;  // log2 of a head's threads
+  int per_row;    // threads of a row
   long total;
   FastDiv by_row;  // total < 2^31
 };
 
-template <int DT>
-__device__ inline void store_kv(void *pool, size_t at, float x) {
+typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+
+// One or four values of a pool, rounded to nearest even.
+template <int DT, class V>
+__device__ inline void store_kv(void *pool, size_t at, V x) {
+  constexpr bool ONE = sizeof(V) == 4;
   if constexpr (DT == MS_KV_F32)
-    static_cast<float *>(pool)[at] = x;
-  else if constexpr (DT == MS_KV_BF16)
+    *reinterpret_cast<V *>(static_cast<float *>(pool) + at) = x;
+  else if constexpr (DT == MS_KV_BF16 && ONE)
     static_cast<__bf16 *>(pool)[at] = (__bf16)x;
-  else
+  else if constexpr (DT == MS_KV_BF16)
+    *reinterpret_cast<bf4 *>(static_cast<__bf16 *>(pool) + at) = __builtin_convertvector(x, bf4);
+  else if constexpr (ONE)
     static_cast<_Float16 *>(pool)[at] = (_Float16)x;
+  else
+    *reinterpret_cast<half4_t *>(static_cast<_Float16 *>(pool) + at) = __builtin_convertvector(x, half4_t);
 }
 
-// One thread per pair of values.
-template <int DT>
+// A thread takes N values and the N that turn with them (or 2 N side by side that do not turn) of
+// one head of a row: q heads, k heads, v heads.  Bound by memory: 3001 rows of 40 + 8 + 8
+// heads of 128 dims into bf16 pools, 161 MB.
+template <int DT, int N>
 __global__ void k_paged_append(AppendArgs a) {
+  typedef float V __attribute__((ext_vector_type(N)));
+  using T = std::conditional_t<N == 1, float, V>;
   const long i = (long)blockIdx.x * kBlock + threadIdx.x;
   if (i >= a.total) return;
   const int r = (int)div_by((uint32_t)i, a.by_row), u = (int)(i - (long)r * a.per_row);
-  const int pairs = a.hd >> 1, half = a.rot >> 1;
-  const int hh = u / pairs, p = u % pairs;  // q heads, k heads, v heads
+  const int hh = u >> a.log_units, p = (u & ((1 << a.log_units) - 1)) * N, half = a.rot >> 1;
   const PagedRow w = a.rows[r];
   const int nq = a.q ? a.n_heads : 0;
   const int what = hh < nq ? 0 : hh < nq + a.n_kv ? 1 : 2;
   const int h = what == 0 ? hh : what == 1 ? hh - nq : hh - nq - a.n_kv;
   const bool turn = what < 2 && p < half;
-  const int d0 = what == 2 ? 2 * p : turn ? p : a.rot + 2 * (p - half), d1 = turn ? p + half : d0 + 1;
+  const int d0 = what == 2 ? 2 * p : turn ? p : a.rot + 2 * (p - half), d1 = turn ? p + half : d0 + N;
   const float *src = (what == 0 ? a.q + r * a.q_ld : (what == 1 ? a.k : a.v) + r * a.kv_ld) + h * a.hd;
-  float x = src[d0], y = src[d1];
+  T x = ldg<T>(src + d0), y = ldg<T>(src + d1);
   if (turn) {
     const size_t t = (size_t)w.pos * half + p;
-    const float c = a.cos_t[t], s = a.sin_t[t], x0 = x;
+    const T c = ldg<T>(a.cos_t + t), s = ldg<T>(a.sin_t + t), x0 = x;
     x = x0 * c - y * s;
     y = x0 * s + y * c;
   }
   if (what == 0) {
     float *o = a.q_out + r * a.q_out_ld + h * a.hd;
-    o[d0] = x;
-    o[d1] = y;
+    *reinterpret_cast<T *>(o + d0) = x;
+    *reinterpret_cast<T *>(o + d1) = y;
   } else {
     const size_t at = (((size_t)w.page * a.page_rows + w.slot) * a.n_kv + h) * a.hd;
     store_kv<DT>(what == 1 ? a.kp : a.vp, at + d0, x);
     store_kv<DT>(what == 1 ? a.kp : a.vp, at + d1, y);
   }
+}
+
+template <int N>
+void launch_append(const AppendArgs &a, int dtype, hipStream_t st) {
+  const dim3 grid(cdiv(a.total, kBlock)), blk(kBlock);
+  if (dtype == MS_KV_F32)
+    hipLaunchKernelGGL((k_paged_append<MS_KV_F32, N>), grid, blk, 0, st, a);
+  else if (dtype == MS_KV_BF16)
+    hipLaunchKernelGGL((k_paged_append<MS_KV_BF16, N>), grid, blk, 0, st, a);
+  else
+    hipLaunchKernelGGL((k_paged_append<MS_KV_F16, N>), grid, blk, 0, st, a);
 }
 
 }  // namespace
@@ -347,20 +372,20 @@ extern "C" int ms_paged_append(const ms_paged_layer *L, const ms_paged_batch *b,
   a.hd = L->head_dim;
   a.rot = L->rot_dim;
   a.page_rows = page_rows(L, b);
-  a.per_row = ((d_q ? L->n_heads : 0) + 2 * L->n_kv_heads) * (L->head_dim / 2);
+  // four pairs a thread where they and their table entries are whole 16-byte words
+  const bool four = L->rot_dim % 8 == 0 && (L->rot_dim == 0 || (aligned16(d_cos) && aligned16(d_sin)));
+  const int units = L->head_dim / (four ? 8 : 2);
+  while ((1 << a.log_units) < units) ++a.log_units;
+  a.per_row = ((d_q ? L->n_heads : 0) + 2 * L->n_kv_heads) * units;
   a.total = (long)a.per_row * b->rows;
   a.by_row = fast_div(a.per_row);
   MS_CHECK_ARG(a.total < ((long)1 << 31), "paged_append: too many rows for one call");
   if (int rc = require_init()) return rc;
   OnDevice on;
-  const dim3 grid(cdiv(a.total, kBlock)), blk(kBlock);
-  hipStream_t st = ctx().stream;
-  if (L->dtype == MS_KV_F32)
-    hipLaunchKernelGGL(k_paged_append<MS_KV_F32>, grid, blk, 0, st, a);
-  else if (L->dtype == MS_KV_BF16)
-    hipLaunchKernelGGL(k_paged_append<MS_KV_BF16>, grid, blk, 0, st, a);
+  if (four)
+    launch_append<4>(a, L->dtype, ctx().stream);
   else
-    hipLaunchKernelGGL(k_paged_append<MS_KV_F16>, grid, blk, 0, st, a);
+    launch_append<1>(a, L->dtype, ctx().stream);
   MS_HIP_TRY(hipGetLastError());
   return MS_OK;
 }

@@ -884,14 +884,15 @@ __global__ __launch_bounds__(NT, 2) void k_paged_block(PagedAttnArgs a) {
 }
 
 // The parts of one result, weighted by e^(their maximum - the largest).  A block takes RPB rows,
-// its 256 threads being HD / 4 columns of RPB rows by GRP groups of parts: many rows of a few parts
+// its NT threads being HD / 4 columns of RPB rows by GRP groups of parts: many rows of a few parts
 // (chunks) or one row of many (a single token over a long context).
 constexpr int kMaxParts = 1024;
-template <int HD>
-__global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a, const PagedMerge *merge, int rpb) {
-  constexpr int COLS = HD / 4, ALL = 256 / COLS;
+template <int HD, int NT>
+__global__ __launch_bounds__(NT) void k_paged_merge(PagedAttnArgs a, const PagedMerge *merge, int rpb) {
+  constexpr int COLS = HD / 4, ALL = NT / COLS;
+  constexpr int AHEAD = 4;
   __shared__ f4 os[ALL][COLS];
-  __shared__ float ls[ALL];
+  __shared__ f2 ls[ALL];
   const int tid = threadIdx.x, kvh = blockIdx.x % a.n_kv, col = tid % COLS, at = tid / COLS;
   const int gpr = ALL / rpb, row = at / gpr, grp = at % gpr, r = blockIdx.y * rpb + row;
   const PagedMerge g = merge[blockIdx.x / a.n_kv];
@@ -899,31 +900,49 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedAttnArgs a, const Page
   const size_t step = (size_t)a.n_kv * a.part_rows;
   const size_t pr = ((size_t)g.part * a.n_kv + kvh) * a.part_rows + (real ? r : 0);
   const int n = real ? g.n : 0;
-  float top = kLow;
-  if (COLS * gpr >= 64) {  // the wave is one row's
-    for (int p = tid & 63; p < n; p += 64) top = fmaxf(top, ldg<float>(a.part_ml + (pr + p * step) * 2));
-    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  } else {
-    for (int p = 0; p < n; ++p) top = fmaxf(top, ldg<float>(a.part_ml + (pr + p * step) * 2));
-  }
-  float l = 0.f;
+  // (maxima and sums come in the same round of loads: both are written by other dies)
+  float m = kLow, l = 0.f;
   f4 o = {};
   const float *po = a.part_o + pr * HD + 4 * col;
-#pragma unroll 8
-  for (int p = grp; p < n; p += gpr) {
-    const float *ml = a.part_ml + (pr + p * step) * 2;
-    const float w = __builtin_amdgcn_exp2f(ldg<float>(ml) - top);
-    l += w * ldg<float>(ml + 1);
-    o += w * ldg<f4>(po + p * step * HD);
+  for (int p0 = grp; p0 < n; p0 += AHEAD * gpr) {
+    f2 ml[AHEAD];
+    f4 x[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int p = min(p0 + i * gpr, n - 1);
+      ml[i] = ldg<f2>(a.part_ml + (pr + p * step) * 2);
+      x[i] = ldg<f4>(po + p * step * HD);
+      if (p0 + i * gpr >= n) ml[i].x = -INFINITY;
+    }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) mn = fmaxf(mn, ml[i].x);
+    const float f = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= f;
+    o *= f;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (p0 + i * gpr >= n) continue;
+      const float w = __builtin_amdgcn_exp2f(ml[i].x - mn);
+      l += w * ml[i].y;
+      o += w * x[i];
+    }
   }
   if (gpr > 1) {
     os[at][col] = o;
-    if (col == 0) ls[at] = l;
+    if (col == 0) ls[at] = f2{m, l};
     __syncthreads();
     if (grp) return;
+    float top = m;
+    for (int i = 1; i < gpr; ++i) top = fmaxf(top, ls[at + i].x);
+    const float f = __builtin_amdgcn_exp2f(m - top);
+    l *= f;
+    o *= f;
     for (int i = 1; i < gpr; ++i) {
-      o += os[at + i][col];
-      l += ls[at + i];
+      const float w = __builtin_amdgcn_exp2f(ls[at + i].x - top);
+      l += w * ls[at + i].y;
+      o += w * os[at + i][col];
     }
   }
   if (!real) return;
@@ -1057,11 +1076,15 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   else if constexpr (B::FITS)
     hipLaunchKernelGGL((k_paged_block<HD, DT>), grid, dim3(64 * B::W), 0, st, a);
   if (p->n_merge) {
-    // about four parts a thread
+    // about four parts a thread, more of them in a larger block
+    const PagedMerge *merge = reinterpret_cast<const PagedMerge *>(p->up.d + p->merge_at);
     int rpb = 1024 / HD;
     while (rpb > 1 && 1024 / HD / rpb * 4 < p->most_parts) rpb /= 2;
-    hipLaunchKernelGGL(k_paged_merge<HD>, dim3(p->n_merge * a.n_kv, cdiv(p->most, rpb)), dim3(256), 0, st, a,
-                       reinterpret_cast<const PagedMerge *>(p->up.d + p->merge_at), rpb);
+    const dim3 mg(p->n_merge * a.n_kv, cdiv(p->most, rpb));
+    if (1024 / HD * 4 < p->most_parts)
+      hipLaunchKernelGGL((k_paged_merge<HD, 1024>), mg, dim3(1024), 0, st, a, merge, rpb);
+    else
+      hipLaunchKernelGGL((k_paged_merge<HD, 256>), mg, dim3(256), 0, st, a, merge, rpb);
   }
   MS_HIP_TRY(hipGetLastError());
   return MS_OK;
