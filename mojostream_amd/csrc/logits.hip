@@ -52,6 +52,21 @@ __global__ __launch_bounds__(NT) void k_logits(LogitsArgs a) {
     return v;
   };
 
+  // ---- the first of the history and of the biases, on their way beside the mask's words
+  const int32_t *h = a.hist + w.history;
+  int32_t h_id[4] = {}, b_id = 0;
+  float b_val = 0.f;
+  auto load_h = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) h_id[u] = ldg<int32_t>(h + min(i0 + u * NT, nh - 1));
+  };
+  auto load_b = [&](int i) {
+    b_id = ldg<int32_t>(a.bias_ids + w.bias + min(i, nb - 1));
+    b_val = ldg<float>(a.bias + w.bias + min(i, nb - 1));
+  };
+  if (nh > 0) load_h(tid);
+  if (nb > 0) load_b(tid);
+
   // ---- what the mask allows of this thread's ids (those past the row: nothing), their logits
   uint32_t ok[PER];
   float4_t v[PER];
@@ -85,39 +100,32 @@ __global__ __launch_bounds__(NT) void k_logits(LogitsArgs a) {
       for (int i = tid; i < kOwners; i += NT) owner[i] = NT;
     }
     __syncthreads();
-    const int32_t *h = a.hist + w.history;
     for (int i0 = tid; i0 < nh; i0 += 4 * NT) {
-      uint32_t at[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) at[u] = (uint32_t)ldg<int32_t>(h + min(i0 + u * NT, nh - 1)) - (uint32_t)t0;
+      if (i0 > tid) load_h(i0);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + u * NT;
-        if (i >= nh || at[u] >= (uint32_t)nt) continue;
+        const uint32_t at = (uint32_t)h_id[u] - (uint32_t)t0;
+        if (i >= nh || at >= (uint32_t)nt) continue;
         if (i < w.n_prompt)
-          atomicOr(&cnt[at[u]], kSeen);
+          atomicOr(&cnt[at], kSeen);
         else
-          atomicAdd(&cnt[at[u]], 1u);
+          atomicAdd(&cnt[at], 1u);
       }
     }
     // Entries of one id add up in their order: of the threads that hold one, the lowest goes first.
     // (Threads whose ids share a place among the owners take turns too.)
     for (int i0 = 0; i0 < nb; i0 += NT) {
-      uint32_t at = 0;
-      float b = 0.f;
-      bool wait = false;
-      if (i0 + tid < nb) {
-        at = (uint32_t)ldg<int32_t>(a.bias_ids + w.bias + i0 + tid) - (uint32_t)t0;
-        wait = at < (uint32_t)nt;
-        if (wait) b = ldg<float>(a.bias + w.bias + i0 + tid);
-      }
+      if (i0) load_b(i0 + tid);
+      const uint32_t at = (uint32_t)b_id - (uint32_t)t0;
+      bool wait = i0 + tid < nb && at < (uint32_t)nt;
       while (__syncthreads_or(wait)) {
         if (wait) atomicMin(&owner[at & (kOwners - 1)], tid);
         __syncthreads();
         const bool mine = wait && owner[at & (kOwners - 1)] == tid;
         __syncthreads();
         if (mine) {
-          add[at] += b;
+          add[at] += b_val;
           atomicOr(&cnt[at], kBiased);
           owner[at & (kOwners - 1)] = NT;
           wait = false;
@@ -229,7 +237,7 @@ extern "C" int ms_logits_process(const float *d_logits, size_t in_stride, float 
     // Every block reads its row's whole history: blocks of 8192 ids, smaller ones only where those
     // would leave compute units idle.
     if ((long)n * cdiv(vocab, 8192) >= ctx().n_cu)
-      launch_tiles<512, 4>(a, n, vec, ctx().stream);
+      launch_tiles<1024, 2>(a, n, vec, ctx().stream);
     else
       launch_tiles<256, 1>(a, n, vec, ctx().stream);
     MS_HIP_TRY(hipGetLastError());
