@@ -697,6 +697,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   if (tid < kTile) rows[tid] = find(0);
   __syncthreads();
   load_k(0);
+  if (v_busy) load_v(0);
   for (int tile = 0; tile < n_tiles; ++tile) {
     const int kb = it.k0 + tile * kTile;
 #pragma unroll
@@ -716,7 +717,6 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
       }
     }
     __syncthreads();
-    if (v_busy) load_v(tile);
     int next = 0;
     if (tid < kTile) next = find(min(tile + 1, n_tiles - 1));
     uint32_t pf[NQ][QP][4];
@@ -779,7 +779,10 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
       }
     }
     __syncthreads();
-    if (tile + 1 < n_tiles) load_k(tile + 1);
+    if (tile + 1 < n_tiles) {
+      load_k(tile + 1);
+      if (v_busy) load_v(tile + 1);
+    }
     if (work) {
       if constexpr (SP > 1) {
 #pragma unroll
