@@ -275,7 +275,7 @@ __host__ __device__ constexpr int v_dims() {
   return DT == MS_KV_F32 || HD == 64 ? 4 : 8;
 }
 
-// The attention of one item of at most 16 (row, head) pairs: the block's W waves, in groups of
+// The attention of one item of at most 16 NQ (row, head) pairs: the block's W waves, in groups of
 // SP that divide the head's dims, take its 32-key tiles in turn, each with sums of its own that are
 // joined at the end.  K and V come from the pages straight into the registers that the
 // MFMAs take them from; LDS carries only the groups' scores.
@@ -292,7 +292,7 @@ __host__ __device__ constexpr int v_dims() {
 // A value that is not finite makes the sums it is multiplied into not finite, with the
 // zeros of masked keys too; where the end finds such a sum the item is done again key by
 // key.
-template <int HD, int DT, int W>
+template <int HD, int DT, int NQ, int W>
 __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const PagedItem &it, int kvh,
                                              char *lds) {
   using F = Form<DT>;
@@ -302,7 +302,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   constexpr int VD = v_dims<HD, DT>(), CD = 16 * VD, NC = HW / CD;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
   const int grp = wave / SP, part = wave % SP;
-  const int nrows = min(16, it.n_new * a.G - it.r0), base = it.len - it.n_new;
+  const int nrows = min(16 * NQ, it.n_new * a.G - it.r0), base = it.len - it.n_new;
   const int t_first = (int)div_by(it.r0, a.by_g), t_last = (int)div_by(it.r0 + nrows - 1, a.by_g);
   const int low_key = a.window ? max(it.k0, base + t_first - a.window + 1) : it.k0;
   const int n_tiles = (it.k1 - it.k0 + kTile - 1) / kTile;
@@ -322,11 +322,13 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   const char *vb0 = static_cast<const char *>(a.v) + ((size_t)kvh * HD + HW * part + VD * c16) * ES;
 
   // ---- q
-  float sc[1];
-  u4 q[KS][QP];
-  {
-    const bool real = c16 < nrows;
-    const int t = real ? (int)div_by(it.r0 + c16, a.by_g) : t_first, h = real ? it.r0 + c16 - t * a.G : 0;
+  float sc[NQ];
+  u4 q[NQ][KS][QP];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = 16 * n + c16;
+    const bool real = r < nrows;
+    const int t = real ? (int)div_by(it.r0 + r, a.by_g) : t_first, h = real ? it.r0 + r - t * a.G : 0;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
     float up = 1.f, down = 1.f;
     if constexpr (F16) {
@@ -340,7 +342,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
       }
       lift_of(max_groups(big), &up, &down);
     }
-    sc[0] = a.scale * down;
+    sc[n] = a.scale * down;
     qp += HW * part;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -352,26 +354,31 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
         split2<F16, QP>(real ? v[2 * j] * up : 0.f, real ? v[2 * j + 1] * up : 0.f, &p[0][2 + j], 4);
       }
 #pragma unroll
-      for (int i = 0; i < QP; ++i) q[s][i] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
+      for (int i = 0; i < QP; ++i) q[n][s][i] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
     }
   }
 
-  f4 o[1][NC * VD] = {};
-  float m[1] = {kLow}, l[1] = {0.f};
-  auto span = [&](int, int *low, int *high) {
-    const int pos = base + (int)div_by(it.r0 + min(c16, nrows - 1), a.by_g);
+  f4 o[NQ][NC * VD] = {};
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    m[n] = kLow;
+    l[n] = 0.f;
+  }
+  auto span = [&](int n, int *low, int *high) {
+    const int pos = base + (int)div_by(it.r0 + min(16 * n + c16, nrows - 1), a.by_g);
     *high = min(it.k1 - 1, pos);
     *low = a.window ? max(low_key, pos - a.window + 1) : low_key;
   };
   // keys that every row attends to
   const int all_lo = a.window ? max(low_key, base + t_last - a.window + 1) : low_key;
   const int all_hi = min(it.k1 - 1, base + t_first);
-  f4 *xs = reinterpret_cast<f4 *>(lds);  // [2][wave][half][64]
+  f4 *xs = reinterpret_cast<f4 *>(lds);  // [2][wave][half][nq][64]
   for (int step = 0; step * NG < n_tiles; ++step) {
     const int tile = step * NG + grp, kb = it.k0 + tile * kTile;
     const bool work = SP == 1 || tile < n_tiles;
     if (SP == 1 && tile >= n_tiles) break;
-    f4 s[2][1] = {};
+    f4 s[2][NQ] = {};
     const char *vp[8];
     u4 vr[8][NC];
     if (work) {
@@ -402,7 +409,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
 
       // ---- scores (the products of the leading parts have a sum of their own: a running sum
       // that takes the small ones too rounds as often as there are products)
-      f4 s_low[2] = {};
+      f4 s_low[2][NQ] = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -422,31 +429,37 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
 #pragma unroll
             for (int pa = QP - 1; pa >= 0; --pa) {
               if (pa + pb >= F::TERMS) continue;
-              f4 &d = pa + pb ? s_low[i] : s[i][0];
-              d = mfma<F16>(u4{kf[pb][0], kf[pb][1], kf[pb][2], kf[pb][3]}, q[ks][pa], d);
+#pragma unroll
+              for (int n = 0; n < NQ; ++n) {
+                f4 &d = (pa + pb ? s_low : s)[i][n];
+                d = mfma<F16>(u4{kf[pb][0], kf[pb][1], kf[pb][2], kf[pb][3]}, q[n][ks][pa], d);
+              }
             }
         }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[i][0] += s_low[i];
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[i][n] += s_low[i][n];
     }
     if constexpr (SP > 1) {
       // (two buffers: the next step's scores do not wait for this one's readers)
-      f4 *x = xs + (step & 1) * W * 2 * 64;
+      f4 *x = xs + (step & 1) * W * 2 * NQ * 64 + lane;
       if (work)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) x[(wave * 2 + i) * 64 + lane] = s[i][0];
+        for (int i = 0; i < 2 * NQ; ++i) x[(wave * 2 * NQ + i) * 64] = s[i / NQ][i % NQ];
       __syncthreads();
       if (work)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          s[i][0] = x[(grp * SP * 2 + i) * 64 + lane];
+        for (int i = 0; i < 2 * NQ; ++i) {
+          f4 z = x[(grp * SP * 2 * NQ + i) * 64];
 #pragma unroll
-          for (int w = 1; w < SP; ++w) s[i][0] += x[((grp * SP + w) * 2 + i) * 64 + lane];
+          for (int w = 1; w < SP; ++w) z += x[((grp * SP + w) * 2 * NQ + i) * 64];
+          s[i / NQ][i % NQ] = z;
         }
     }
     if (!work) continue;
-    uint32_t pf[1][QP][4];
-    probabilities<DT, 1>(s, kb, kb < all_lo || kb + kTile - 1 > all_hi, sc, span, m, l, o, pf);
+    uint32_t pf[NQ][QP][4];
+    probabilities<DT, NQ>(s, kb, kb < all_lo || kb + kTile - 1 > all_hi, sc, span, m, l, o, pf);
 
     // ---- values
 #pragma unroll
@@ -470,73 +483,85 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
           if (pa + pb >= F::TERMS) continue;
 #pragma unroll
           for (int t = 0; t < VD; ++t)
-            o[0][c * VD + t] = mfma<F16>(u4{vf[t][pb][0], vf[t][pb][1], vf[t][pb][2], vf[t][pb][3]},
-                                         u4{pf[0][pa][0], pf[0][pa][1], pf[0][pa][2], pf[0][pa][3]},
-                                         o[0][c * VD + t]);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+              o[n][c * VD + t] = mfma<F16>(u4{vf[t][pb][0], vf[t][pb][1], vf[t][pb][2], vf[t][pb][3]},
+                                           u4{pf[n][pa][0], pf[n][pa][1], pf[n][pa][2], pf[n][pa][3]},
+                                           o[n][c * VD + t]);
         }
     }
   }
 
   // ---- the groups' sums joined
-  l[0] = sum_groups(l[0]);
-  int bad = !(fabsf(l[0]) < INFINITY);
+  int bad = 0;
 #pragma unroll
-  for (int d = 0; d < NC * VD; ++d)
+  for (int n = 0; n < NQ; ++n) {
+    l[n] = sum_groups(l[n]);
+    bad |= !(fabsf(l[n]) < INFINITY);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[0][d][e]) < INFINITY);
+    for (int d = 0; d < NC * VD; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[n][d][e]) < INFINITY);
+  }
   // (also: every wave is done with xs)
   if (__syncthreads_or(bad)) {
-    item_by_key<HD, DT, 64 * W>(a, it, kvh, 16, reinterpret_cast<float *>(lds));
+    item_by_key<HD, DT, 64 * W>(a, it, kvh, 16 * NQ, reinterpret_cast<float *>(lds));
     return;
   }
-  float *ml = reinterpret_cast<float *>(lds);  // [2][group][16]
-  constexpr int LD = CD + 4;
-  float *os = ml + 2 * NG * 16;                // [wave][16][LD]
-  if (g == 0 && part == 0) {
-    ml[grp * 16 + c16] = m[0];
-    ml[(NG + grp) * 16 + c16] = l[0];
-  }
+  float *ml = reinterpret_cast<float *>(lds);  // [2][group][16 NQ]
+  constexpr int LD = CD + 4, ROWS = 16 * NQ;
+  float *os = ml + 2 * NG * ROWS;              // [wave][16][LD]
+  if (g == 0 && part == 0)
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      ml[grp * ROWS + 16 * n + c16] = m[n];
+      ml[(NG + grp) * ROWS + 16 * n + c16] = l[n];
+    }
   __syncthreads();
-  float top = kLow;
 #pragma unroll
-  for (int w = 0; w < NG; ++w) top = fmaxf(top, ml[w * 16 + c16]);
-  const float f = __builtin_amdgcn_exp2f(m[0] - top);
+  for (int n = 0; n < NQ; ++n) {
+    if (16 * n >= nrows) break;
+    float top = kLow;
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (c) __syncthreads();
+    for (int w = 0; w < NG; ++w) top = fmaxf(top, ml[w * ROWS + 16 * n + c16]);
+    const float f = __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int c = 0; c < NC; ++c) {
+      if (n + c) __syncthreads();
 #pragma unroll
-      for (int t = 0; t < VD; t += 4) {
-        f4 x;
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = o[0][c * VD + t + u][e] * f;
-        *reinterpret_cast<f4 *>(os + (wave * 16 + c16) * LD + VD * (4 * g + e) + t) = x;
-      }
-    __syncthreads();
-    for (int i = tid; i < 16 * SP * (CD / 4); i += 64 * W) {
-      const int d = i % (CD / 4) * 4, pt = i / (CD / 4) % SP, r = i / (CD / 4 * SP);
-      if (r >= nrows) break;
-      float mt = kLow, ls = 0.f;
+        for (int t = 0; t < VD; t += 4) {
+          f4 x;
 #pragma unroll
-      for (int w = 0; w < NG; ++w) mt = fmaxf(mt, ml[w * 16 + r]);
-      f4 x = {};
+          for (int u = 0; u < 4; ++u) x[u] = o[n][c * VD + t + u][e] * f;
+          *reinterpret_cast<f4 *>(os + (wave * 16 + c16) * LD + VD * (4 * g + e) + t) = x;
+        }
+      __syncthreads();
+      for (int i = tid; i < 16 * SP * (CD / 4); i += 64 * W) {
+        const int d = i % (CD / 4) * 4, pt = i / (CD / 4) % SP, r16 = i / (CD / 4 * SP), r = 16 * n + r16;
+        if (r >= nrows) break;
+        float mt = kLow, ls = 0.f;
 #pragma unroll
-      for (int w = 0; w < NG; ++w) {
-        ls += ml[(NG + w) * 16 + r] * __builtin_amdgcn_exp2f(ml[w * 16 + r] - mt);
-        x += *reinterpret_cast<const f4 *>(os + ((w * SP + pt) * 16 + r) * LD + d);
-      }
-      const int dim = pt * HW + c * CD + d;
-      if (it.part < 0) {
-        const int t = (int)div_by(it.r0 + r, a.by_g), h = it.r0 + r - t * a.G;
-        *reinterpret_cast<f4 *>(a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD + dim) =
-            x / ls;
-      } else {
-        const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
-        *reinterpret_cast<f4 *>(a.part_o + pr * HD + dim) = x;
-        if (dim == 0) {
-          a.part_ml[pr * 2] = mt;
-          a.part_ml[pr * 2 + 1] = ls;
+        for (int w = 0; w < NG; ++w) mt = fmaxf(mt, ml[w * ROWS + r]);
+        f4 x = {};
+#pragma unroll
+        for (int w = 0; w < NG; ++w) {
+          ls += ml[(NG + w) * ROWS + r] * __builtin_amdgcn_exp2f(ml[w * ROWS + r] - mt);
+          x += *reinterpret_cast<const f4 *>(os + ((w * SP + pt) * 16 + r16) * LD + d);
+        }
+        const int dim = pt * HW + c * CD + d;
+        if (it.part < 0) {
+          const int t = (int)div_by(it.r0 + r, a.by_g), h = it.r0 + r - t * a.G;
+          *reinterpret_cast<f4 *>(a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD + dim) =
+              x / ls;
+        } else {
+          const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
+          *reinterpret_cast<f4 *>(a.part_o + pr * HD + dim) = x;
+          if (dim == 0) {
+            a.part_ml[pr * 2] = mt;
+            a.part_ml[pr * 2 + 1] = ls;
+          }
         }
       }
     }
@@ -860,28 +885,29 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   }
 }
 
-template <int HD, int DT, int W>
+template <int HD, int DT, int NQ, int W>
 constexpr int tile_lds() {
-  constexpr int x = tile_split<HD>() > 1 ? 2 * W * 2 * 64 * 16 : 0;
-  constexpr int e = (32 * (W / tile_split<HD>()) + W * 16 * (16 * v_dims<HD, DT>() + 4)) * 4;
+  constexpr int x = tile_split<HD>() > 1 ? 2 * W * 2 * NQ * 64 * 16 : 0;
+  constexpr int e = (32 * NQ * (W / tile_split<HD>()) + W * 16 * (16 * v_dims<HD, DT>() + 4)) * 4;
   return x > e ? x : e;
 }
 
-// Items of at most 16 pairs: single tokens.
-template <int HD, int DT>
-__global__ __launch_bounds__(256, 2) void k_paged_tile(PagedAttnArgs a) {
-  __shared__ __align__(16) char lds[tile_lds<HD, DT, 4>()];
-  item_by_tile<HD, DT, 4>(a, a.items[blockIdx.x / a.n_kv], blockIdx.x % a.n_kv, lds);
+// Items of at most 16 NQ pairs: single tokens, or a few of them.  (Two query tiles of three parts do
+// not fit the registers of two waves a SIMD: with spills 110 us where one wave takes 72 us.)
+template <int HD, int DT, int NQ>
+__global__ __launch_bounds__(256, NQ == 2 && DT != MS_KV_F16 ? 1 : 2) void k_paged_tile(PagedAttnArgs a) {
+  __shared__ __align__(16) char lds[tile_lds<HD, DT, NQ, 4>()];
+  item_by_tile<HD, DT, NQ, 4>(a, a.items[blockIdx.x / a.n_kv], blockIdx.x % a.n_kv, lds);
 }
 
 // Items of longer chunks, and single tokens beside them.
 template <int HD, int DT, int NT = 64 * Shape<HD, DT>::W>
 __global__ __launch_bounds__(NT, 2) void k_paged_block(PagedAttnArgs a) {
-  constexpr int A = tile_lds<HD, DT, Shape<HD, DT>::W>(), B = Shape<HD, DT>::LDS;
+  constexpr int A = tile_lds<HD, DT, 1, Shape<HD, DT>::W>(), B = Shape<HD, DT>::LDS;
   __shared__ __align__(16) char lds[A > B ? A : B];
   const PagedItem it = a.items[blockIdx.x / a.n_kv];
   if (it.n_new * a.G - it.r0 <= 16)
-    item_by_tile<HD, DT, Shape<HD, DT>::W>(a, it, blockIdx.x % a.n_kv, lds);
+    item_by_tile<HD, DT, 1, Shape<HD, DT>::W>(a, it, blockIdx.x % a.n_kv, lds);
   else
     item_by_block<HD, DT>(a, it, blockIdx.x % a.n_kv, lds);
 }
@@ -970,7 +996,7 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
       const int t0 = r0 / p->G, t1 = std::min((r0 + p->rows - 1) / p->G, b->n_new[s] - 1);
       const int lo = p->window ? std::max(0, base + t0 - p->window + 1) : 0;
       const int k0 = lo / kTile * kTile, k1 = base + t1 + 1, n = (k1 - k0 + kTile - 1) / kTile;
-      spans.push_back({s, r0, k0, k1, n, p->rows > 16 && pairs - r0 > 16 ? 4 : p->tile_cost});
+      spans.push_back({s, r0, k0, k1, n, p->rows > 32 && pairs - r0 > 16 ? 4 : p->tile_cost});
       work += (int64_t)n * spans.back().cost;
       longest = std::max(longest, n * spans.back().cost);
     }
@@ -1060,10 +1086,15 @@ int plan_for(ms_paged_batch *b, int G, int rows, int n_kv, int window, int block
 template <int HD, int DT>
 int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   using B = Shape<HD, DT>;
-  const int rows = most > 16 && B::FITS ? B::PAIRS : 16;
+  // Few pairs: tiles by a wave each, two query tiles of them to head dim 128 (32 sequences of 8 rows x
+  // 4 heads over 4096 keys, bf16: 72 us against 104 us of the block's 128 pairs), 16 pairs an item
+  // at larger ones, whose second item finds its keys in the caches (head dim 256: 44 us, 52 us with two
+  // query tiles, 64 us by blocks).
+  constexpr bool TWO = HD <= 128;
+  const int rows = most <= 16 ? 16 : most <= 32 ? (TWO ? 32 : 16) : B::FITS ? B::PAIRS : 16;
   PagedPlan *p = nullptr;
   // blocks that run at once; a step of single tokens takes a tile for every group of waves
-  const int w = rows > 16 ? B::W : 4, cost = std::max(1, 4 * tile_split<HD>() / w);
+  const int w = rows > 32 ? B::W : 4, cost = std::max(1, 4 * tile_split<HD>() / w);
   if (int rc = plan_for(b, a.G, rows, a.n_kv, a.window, 8 / w * ctx().n_cu, cost, &p)) return rc;
   a.part_rows = p->most;
   if (const size_t n = (size_t)p->n_parts * a.n_kv * a.part_rows) {
@@ -1075,7 +1106,10 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   a.items = reinterpret_cast<const PagedItem *>(p->up.d);
   const dim3 grid(p->n_items * a.n_kv);
   if (rows == 16)
-    hipLaunchKernelGGL((k_paged_tile<HD, DT>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_paged_tile<HD, DT, 1>), grid, dim3(256), 0, st, a);
+  else if (rows == 32) {
+    if constexpr (TWO) hipLaunchKernelGGL((k_paged_tile<HD, DT, 2>), grid, dim3(256), 0, st, a);
+  }
   else if constexpr (B::FITS)
     hipLaunchKernelGGL((k_paged_block<HD, DT>), grid, dim3(64 * B::W), 0, st, a);
   if (p->n_merge) {
