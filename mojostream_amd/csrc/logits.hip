@@ -199,22 +199,22 @@ extern "C" int ms_logits_process(const float *d_logits, size_t in_stride, float 
                "logits_process: d_logits and d_out overlap");
   for (int r = 0; r < rows; ++r) {
     const ms_logits_row &w = h_rows[r];
-    const std::string at = "logits_process: row " + std::to_string(r) + ": ";
+    auto at = [r](const char *msg) { return "logits_process: row " + std::to_string(r) + ": " + msg; };
     MS_CHECK_ARG(w.repetition > 0.f && w.repetition < INFINITY,
-                 at + "the repetition penalty must be positive and finite");
+                 at("the repetition penalty must be positive and finite"));
     MS_CHECK_ARG(std::fabs(w.frequency) < INFINITY && std::fabs(w.presence) < INFINITY,
-                 at + "a penalty is not a finite number");
-    MS_CHECK_ARG(w.n_prompt >= 0 && w.n_generated >= 0 && w.n_bias >= 0, at + "negative count");
+                 at("a penalty is not a finite number"));
+    MS_CHECK_ARG(w.n_prompt >= 0 && w.n_generated >= 0 && w.n_bias >= 0, at("negative count"));
     const int64_t h = (int64_t)w.n_prompt + w.n_generated;
     MS_CHECK_ARG(h < (1 << 30) && w.history >= 0 && (uint64_t)w.history <= n_history &&
                      (uint64_t)h <= n_history - (uint64_t)w.history && (h == 0 || d_history),
-                 at + "the history reaches past d_history");
+                 at("the history reaches past d_history"));
     MS_CHECK_ARG(w.bias >= 0 && (uint64_t)w.bias <= n_bias &&
                      (uint64_t)w.n_bias <= n_bias - (uint64_t)w.bias &&
                      (w.n_bias == 0 || (d_bias_ids && d_bias)),
-                 at + "the biases reach past d_bias");
+                 at("the biases reach past d_bias"));
     MS_CHECK_ARG(w.mask >= -1 && w.mask < n_masks && (w.mask < 0 || d_masks),
-                 at + "no such mask");
+                 at("no such mask"));
   }
   if (int rc = require_init()) return rc;
   OnDevice on;

@@ -11,6 +11,7 @@ namespace ms {
 class OnDevice {
  public:
   OnDevice() {
+    if (ctx().device < 0) return;
     if (hipGetDevice(&was_) != hipSuccess) was_ = -1;
     if (was_ != ctx().device) (void)hipSetDevice(ctx().device);
   }

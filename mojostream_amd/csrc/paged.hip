@@ -47,25 +47,25 @@ void Upload::release() {
 }
 
 int paged_check(const char *what, const ms_paged_layer *L, const ms_paged_batch *b) {
-  const std::string w(what);
-  MS_CHECK_ARG(L && b, w + ": null layer or batch");
+  auto w = [what](const char *msg) { return std::string(what) + msg; };
+  MS_CHECK_ARG(L && b, w(": null layer or batch"));
   MS_CHECK_ARG(L->n_kv_heads >= 1 && L->n_heads >= 1 && L->n_heads % L->n_kv_heads == 0,
-               w + ": n_heads must be a multiple of n_kv_heads");
-  MS_CHECK_ARG(L->n_heads <= 1024, w + ": at most 1024 query heads");
+               w(": n_heads must be a multiple of n_kv_heads"));
+  MS_CHECK_ARG(L->n_heads <= 1024, w(": at most 1024 query heads"));
   MS_CHECK_ARG(L->head_dim == 64 || L->head_dim == 128 || L->head_dim == 256 ||
                    L->head_dim == 512,
-               w + ": head_dim must be 64, 128, 256 or 512");
+               w(": head_dim must be 64, 128, 256 or 512"));
   MS_CHECK_ARG(L->dtype == MS_KV_F32 || L->dtype == MS_KV_BF16 || L->dtype == MS_KV_F16,
-               w + ": unknown pool type");
-  MS_CHECK_ARG(L->window >= 0, w + ": negative window");
+               w(": unknown pool type"));
+  MS_CHECK_ARG(L->window >= 0, w(": negative window"));
   MS_CHECK_ARG(L->page_rows == 0 || L->page_rows >= b->page_size,
-               w + ": page_rows is less than the page size");
+               w(": page_rows is less than the page size"));
   MS_CHECK_ARG((int64_t)page_rows(L, b) * b->n_pages < ((int64_t)1 << 31),
-               w + ": a pool has fewer than 2^31 rows");
-  MS_CHECK_ARG(L->k && L->v, w + ": null pool");
+               w(": a pool has fewer than 2^31 rows"));
+  MS_CHECK_ARG(L->k && L->v, w(": null pool"));
   MS_CHECK_ARG(((reinterpret_cast<uintptr_t>(L->k) | reinterpret_cast<uintptr_t>(L->v)) & 15) == 0,
-               w + ": the pools must be 16-byte aligned");
-  MS_CHECK_ARG(b->set, w + ": the batch was not set");
+               w(": the pools must be 16-byte aligned"));
+  MS_CHECK_ARG(b->set, w(": the batch was not set"));
   return MS_OK;
 }
 
@@ -187,8 +187,8 @@ extern "C" int ms_paged_batch_create(int page_size, int n_pages, int max_seqs, i
   MS_CHECK_ARG(page_size >= 1 && n_pages >= 1 && max_seqs >= 1 && max_rows >= 1 && max_pages >= 1,
                "paged_batch_create: sizes must be positive");
   MS_CHECK_ARG((int64_t)page_size * n_pages < ((int64_t)1 << 31) &&
-                   (int64_t)page_size * max_pages < ((int64_t)1 << 31),
-               "paged_batch_create: fewer than 2^31 positions");
+                   (int64_t)page_size * max_pages <= ((int64_t)1 << 30),
+               "paged_batch_create: fewer than 2^31 slots, at most 2^30 positions a sequence");
   MS_CHECK_ARG((int64_t)max_seqs * max_pages < ((int64_t)1 << 28) && max_seqs <= (1 << 20) &&
                    max_rows <= (1 << 24),
                "paged_batch_create: too many sequences, rows or pages");
@@ -211,13 +211,15 @@ extern "C" int ms_paged_batch_create(int page_size, int n_pages, int max_seqs, i
 
 extern "C" int ms_paged_batch_destroy(ms_paged_batch *b) {
   if (!b) return MS_OK;
-  if (ctx().device >= 0) {
+  {
     OnDevice on;
-    (void)hipStreamSynchronize(ctx().stream);
+    if (ctx().device >= 0) (void)hipStreamSynchronize(ctx().stream);
     b->up.release();
-    for (PagedPlan *p : b->plans) p->up.release();
+    for (PagedPlan *p : b->plans) {
+      p->up.release();
+      delete p;
+    }
   }
-  for (PagedPlan *p : b->plans) delete p;
   delete b;
   return MS_OK;
 }
@@ -234,21 +236,21 @@ extern "C" int ms_paged_batch_set(ms_paged_batch *b, int n_seqs, const int32_t *
     int stride = 0, max_pos = 0;
     const int64_t stamp = ++b->n_set;
     for (int s = 0; s < n_seqs; ++s) {
-      const std::string w = "paged_batch_set: sequence " + std::to_string(s) + ": ";
+      auto w = [&](const std::string &msg) { return "paged_batch_set: sequence " + std::to_string(s) + ": " + msg; };
       const int n = h_new[s], l = h_len[s];
-      MS_CHECK_ARG(n >= 0 && l >= n, w + "the length is less than its new rows");
-      MS_CHECK_ARG((int64_t)l <= (int64_t)P * b->max_pages, w + "more positions than its pages hold");
+      MS_CHECK_ARG(n >= 0 && l >= n, w("the length is less than its new rows"));
+      MS_CHECK_ARG((int64_t)l <= (int64_t)P * b->max_pages, w("more positions than its pages hold"));
       const int used = l == 0 ? 0 : (l - 1) / P + 1;
       const int32_t *pg = h_pages + (size_t)s * b->max_pages;
       int gone = 0;
       while (gone < used && pg[gone] == -1) ++gone;
       for (int i = gone; i < used; ++i)
         MS_CHECK_ARG(pg[i] >= 0 && pg[i] < b->n_pages,
-                     w + "page " + std::to_string(i) + " is " + std::to_string(pg[i]));
-      MS_CHECK_ARG(n == 0 || (l - n) / P >= gone, w + "a new row's page is missing");
+                     w("page " + std::to_string(i) + " is " + std::to_string(pg[i])));
+      MS_CHECK_ARG(n == 0 || (l - n) / P >= gone, w("a new row's page is missing"));
       for (int i = n ? (l - n) / P : used; i < used; ++i) {
         MS_CHECK_ARG(b->writer[pg[i]] != stamp,
-                     w + "page " + std::to_string(pg[i]) + " would be written twice");
+                     w("page " + std::to_string(pg[i]) + " would be written twice"));
         b->writer[pg[i]] = stamp;
       }
       first[s] = (int)rows;
@@ -256,7 +258,7 @@ extern "C" int ms_paged_batch_set(ms_paged_batch *b, int n_seqs, const int32_t *
       len[s] = l;
       held[s] = gone * P;
       rows += n;
-      MS_CHECK_ARG(rows <= b->max_rows, w + "more rows than the batch holds");
+      MS_CHECK_ARG(rows <= b->max_rows, w("more rows than the batch holds"));
       stride = used > stride ? used : stride;
       if (n && l > max_pos) max_pos = l;
     }

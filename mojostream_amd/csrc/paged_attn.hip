@@ -10,6 +10,7 @@ namespace ms {
 namespace {
 
 constexpr int kTile = 32;  // keys of a tile
+constexpr int kMaxParts = 1024;  // about the most parts of one result
 
 struct PagedAttnArgs {
   const float *q;
@@ -43,7 +44,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLow = -3.0e38f;  // running maximum before the first key
+constexpr float kLow = -0x1.fffffep+127f;  // running maximum before the first key
 // The maximum that scores are taken against may lag behind by this much (log2): a
 // probability is at most 2^kLag.
 constexpr float kLag = 8.0f;
@@ -258,7 +259,7 @@ __device__ __forceinline__ void probabilities(const f4 (&s)[2][NQ], int kb, bool
 // 2^k that brings the largest of fp16 queries' values below 2^15, and its inverse.
 __device__ inline void lift_of(float big, float *up, float *down) {
   int e = big > 0.f && big < INFINITY ? 14 + 127 - (int)((__float_as_uint(big) >> 23) & 255) : 0;
-  e = max(-100, min(100, e));
+  e = max(-126, min(126, e));
   *up = __uint_as_float((uint32_t)(127 + e) << 23);
   *down = __uint_as_float((uint32_t)(127 - e) << 23);
 }
@@ -591,8 +592,8 @@ struct Shape {
 // into LDS as MFMA fragments (those of fp32 pools in parts): K as the rows lie, V turned in
 // registers; the waves read both without bank conflicts.  (item_by_tile's loads of K take 16
 // bytes of 16 rows a quarter wave, sixteen cache accesses where a row's take one or two; with
-// many queries these accesses bound it.)  The loads of V run beside the first product, those of
-// the next K beside the second.  Where a group has several waves each computes the scores over
+// many queries these accesses bound it.)  The next tile's rows are loaded beside the second
+// product of this one and wait in registers.  Where a group has several waves each computes the scores over
 // its dims, and all take the sum, in the same order.
 template <int HD, int DT>
 __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const PagedItem &it, int kvh,
@@ -915,7 +916,6 @@ __global__ __launch_bounds__(NT, 2) void k_paged_block(PagedAttnArgs a) {
 // The parts of one result, weighted by e^(their maximum - the largest).  A block takes RPB rows,
 // its NT threads being HD / 4 columns of RPB rows by GRP groups of parts: many rows of a few parts
 // (chunks) or one row of many (a single token over a long context).
-constexpr int kMaxParts = 1024;
 template <int HD, int NT>
 __global__ __launch_bounds__(NT) void k_paged_merge(PagedAttnArgs a, const PagedMerge *merge, int rpb) {
   constexpr int COLS = HD / 4, ALL = NT / COLS;
@@ -1001,7 +1001,7 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
       longest = std::max(longest, n * spans.back().cost);
     }
   }
-  // The longest part a block gets, `per`: at least a step, and no more parts than a merge takes; from an even share up, where its end is soonest: all blocks at once
+  // The longest part a block gets, `per`: at least a step, and no more than kMaxParts of them; from an even share up, where its end is soonest: all blocks at once
   // are done with the longest, more of them after about half of one more.
   auto cuts_of = [](const Span &x, int per) { return (x.tiles * x.cost + per - 1) / per; };
   const int64_t fill = std::max((work * p->n_kv + blocks - 1) / blocks,
@@ -1150,10 +1150,10 @@ extern "C" int ms_paged_attention(const ms_paged_layer *L, ms_paged_batch *b, co
     const int lo = L->window ? std::max(0, b->len[s] - b->n_new[s] - L->window + 1) : 0;
     MS_CHECK_ARG(lo >= b->held[s], "paged_attention: sequence " + std::to_string(s) +
                                        " attends to a position whose page is -1");
-    MS_CHECK_ARG((int64_t)b->n_new[s] * G < ((int64_t)1 << 30),
-                 "paged_attention: too many rows for one call");
     most = std::max(most, b->n_new[s] * G);
   }
+  MS_CHECK_ARG((int64_t)b->rows * L->n_heads < ((int64_t)1 << 30),
+               "paged_attention: too many rows for one call");
   if (b->rows == 0) return require_init();
   MS_CHECK_ARG(d_q && d_out && aligned16(d_q) && aligned16(d_out) && q_stride % 4 == 0 &&
                    out_stride % 4 == 0 && q_stride >= (size_t)q_dim &&

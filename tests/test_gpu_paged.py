@@ -168,6 +168,15 @@ ATTENDS = [
     ([(4, 1500)], 4, 1, 128, 16, 0, 0),                                  # exactly 16 (row, head) pairs
     ([(9, 1111)], 8, 1, 64, 16, 0, 0),
     ([(250, 250)], 3, 3, 64, 32, 0, 100),
+    ([(5, 300), (8, 8), (1, 40)], 8, 2, 256, 16, 0, 0),                  # 17 to 32 pairs
+    ([(5, 300), (8, 8)], 8, 2, 128, 16, 0, 33),
+    ([(7, 500), (1, 77)], 4, 1, 64, 32, 0, 0),
+    ([(4, 90)], 16, 2, 512, 16, 0, 0),
+    ([(1, 9000)], 4, 1, 128, 64, 0, 0),                                  # many parts of one result
+    ([(40, 3000)], 8, 1, 512, 16, 0, 0),                                 # chunks over split keys
+    ([(200, 4100)], 4, 1, 128, 16, 0, 0),
+    ([(90, 400), (33, 33)], 4, 2, 128, 16, 0, 70),
+    ([(129, 129)], 1, 1, 256, 16, 0, 0),                                 # one pair past a block's
 ]
 
 
@@ -194,6 +203,34 @@ def test_attention_scale(gpu):
     st.pool["v"][s[1::3], o[1::3]] *= 1e-6
     st.upload()
     st.check_attention()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("new,hd", [(1, 128), (7, 64), (50, 128), (20, 256)])
+def test_attention_sizes_of_q(gpu, dtype, new, hd):
+    """Queries of very different size: between rows, and between the dims of one."""
+    ms = gpu
+    say(f"attention, sizes of q: {dtype} new={new} hd={hd}")
+    st = Setup(ms, [(new, 150)], 4, 2, hd, dtype, 16, seed=13)
+    q = f32(new, 4, hd, seed=14)
+    q[:, 0] *= 1e-30
+    q[:, 1] *= 1e-4
+    q[:, 2, ::2] *= 1e-6
+    q[:, 3] = 0
+    q = q.reshape(new, -1)
+    want, tol = st.attend(q)
+    got = st.run_attention(q)
+    assert np.all(np.abs(got - want) <= tol)
+    # far beyond fp16, the best key takes all: a finite result, that key's values
+    g = st.slots(0, 0, 150)
+    k, v = decode(st.pool["k"][g], dtype), decode(st.pool["v"][g], dtype)
+    q = f32(new, 4, hd, seed=15)
+    big = (q * np.float32(1e30)).reshape(new, -1)
+    got = st.run_attention(big).reshape(new, 4, hd)
+    for r in range(new):
+        for h in range(4):
+            best = np.argmax(k[:150 - new + r + 1, h // 2] @ q[r, h].astype(np.float64))
+            assert np.array_equal(got[r, h], v[best, h // 2].astype(np.float32))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
