@@ -264,6 +264,42 @@ __device__ inline void lift_of(float big, float *up, float *down) {
   *down = __uint_as_float((uint32_t)(127 - e) << 23);
 }
 
+// KS 32-dim steps of a query's dims from qp on (that lane's eight of each) in parts, as the first
+// product's operand; 0 where the query is not real.  What their product has to be multiplied by: *down.
+template <int DT, int KS>
+__device__ __forceinline__ void load_q(const float *qp, bool real, u4 (&q)[KS][Form<DT>::QP],
+                                       float *down) {
+  constexpr bool F16 = Form<DT>::F16;
+  constexpr int QP = Form<DT>::QP;
+  f4 x[KS][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    x[ks][0] = ldg<f4>(qp + 32 * ks);
+    x[ks][1] = ldg<f4>(qp + 32 * ks + 4);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  float up = 1.f;
+  *down = 1.f;
+  if constexpr (F16) {
+    float big = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[ks][j >> 2][j & 3]));
+    lift_of(max_groups(big), &up, down);
+  }
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    uint32_t p[QP][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      split2<F16, QP>(real ? x[ks][j >> 1][2 * (j & 1)] * up : 0.f,
+                      real ? x[ks][j >> 1][2 * (j & 1) + 1] * up : 0.f, &p[0][j], 4);
+#pragma unroll
+    for (int i = 0; i < QP; ++i) q[ks][i] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
+  }
+}
+
 // Waves that share a tile in item_by_tile: 128 dims each at most, so that a wave's whole tile is
 // in flight at once.
 template <int HD>
@@ -321,9 +357,51 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   const uint32_t row_bytes = (uint32_t)a.n_kv * HD * ES;
   const char *kb0 = static_cast<const char *>(a.k) + ((size_t)kvh * HD + HW * part + 8 * g) * ES;
   const char *vb0 = static_cast<const char *>(a.v) + ((size_t)kvh * HD + HW * part + VD * c16) * ES;
+  // The next tile's keys are loaded once this one's are multiplied, its values once these are, where
+  // there are registers for it (not for fp32 pools and one query tile: 160 us with spills, 126 us with
+  // both loaded as the tile begins; 32 tokens over 4096 keys, 8 kv heads of 128 dims).
+  constexpr bool AHEAD = F16 ? NQ == 1 : ES == 2 || NQ == 2;
+  u4 kr[2][KS][ES / 2], vr[8][NC];
+  auto load_k = [&](int row) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const char *p = kb0 + (uint64_t)(uint32_t)__shfl(row, 16 * i + c16, 64) * row_bytes;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < ES / 2; ++j) kr[i][ks][j] = ldg<u4>(p + ks * 32 * ES + 16 * j);
+    }
+  };
+  auto load_v = [&](int row) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const char *p = vb0 + (uint64_t)(uint32_t)__shfl(row, 16 * (j >> 2) + 4 * g + (j & 3), 64) * row_bytes;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if constexpr (VD * ES == 16) {
+          vr[j][c] = ldg<u4>(p + c * CD * ES);
+        } else {
+          const u2 y = ldg<u2>(p);
+          vr[j][0] = u4{y[0], y[1], 0, 0};
+        }
+      }
+    }
+  };
+  int ahead = grp;
+  auto next = [&]() {  // pool row of the lane's key of the next tile
+    const int row = page * a.page_rows + slot;
+    find(ahead += NG, &page, &slot);
+    return row;
+  };
+  int row;
+  if (AHEAD && grp < n_tiles) {
+    row = next();
+    load_k(row);
+    load_v(row);
+  }
 
   // ---- q
-  float sc[NQ];
+  float sc[NQ], down[NQ];
   u4 q[NQ][KS][QP];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -331,32 +409,8 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
     const bool real = r < nrows;
     const int t = real ? (int)div_by(it.r0 + r, a.by_g) : t_first, h = real ? it.r0 + r - t * a.G : 0;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
-    float up = 1.f, down = 1.f;
-    if constexpr (F16) {
-      // (the whole row's largest value)
-      float big = 0.f;
-#pragma unroll
-      for (int s = 0; s < HD / 32; ++s) {
-        const f4 u = ldg<f4>(qp + 32 * s), v = ldg<f4>(qp + 32 * s + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) big = fmaxf(big, fmaxf(fabsf(u[j]), fabsf(v[j])));
-      }
-      lift_of(max_groups(big), &up, &down);
-    }
-    sc[n] = a.scale * down;
-    qp += HW * part;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const f4 u = ldg<f4>(qp + 32 * s), v = ldg<f4>(qp + 32 * s + 4);
-      uint32_t p[QP][4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        split2<F16, QP>(real ? u[2 * j] * up : 0.f, real ? u[2 * j + 1] * up : 0.f, &p[0][j], 4);
-        split2<F16, QP>(real ? v[2 * j] * up : 0.f, real ? v[2 * j + 1] * up : 0.f, &p[0][2 + j], 4);
-      }
-#pragma unroll
-      for (int i = 0; i < QP; ++i) q[n][s][i] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
-    }
+    load_q<DT, KS>(qp + HW * part, real, q[n], &down[n]);
+    sc[n] = SP == 1 ? a.scale * down[n] : a.scale;
   }
 
   f4 o[NQ][NC * VD] = {};
@@ -377,37 +431,15 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   f4 *xs = reinterpret_cast<f4 *>(lds);  // [2][wave][half][nq][64]
   for (int step = 0; step * NG < n_tiles; ++step) {
     const int tile = step * NG + grp, kb = it.k0 + tile * kTile;
-    const bool work = SP == 1 || tile < n_tiles;
+    const bool work = SP == 1 || tile < n_tiles, more = tile + NG < n_tiles;
     if (SP == 1 && tile >= n_tiles) break;
     f4 s[2][NQ] = {};
-    const char *vp[8];
-    u4 vr[8][NC];
     if (work) {
-      const int row = page * a.page_rows + slot;
-      u4 kr[2][KS][ES / 2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const char *p = kb0 + (uint64_t)(uint32_t)__shfl(row, 16 * i + c16, 64) * row_bytes;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int j = 0; j < ES / 2; ++j) kr[i][ks][j] = ldg<u4>(p + ks * 32 * ES + 16 * j);
+      if (!AHEAD) {
+        row = next();
+        load_k(row);
+        load_v(row);
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        vp[j] = vb0 + (uint64_t)(uint32_t)__shfl(row, 16 * (j >> 2) + 4 * g + (j & 3), 64) * row_bytes;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          if constexpr (VD * ES == 16) {
-            vr[j][c] = ldg<u4>(vp[j] + c * CD * ES);
-          } else {
-            const u2 y = ldg<u2>(vp[j]);
-            vr[j][0] = u4{y[0], y[1], 0, 0};
-          }
-        }
-      }
-      find(tile + NG, &page, &slot);
-
       // ---- scores (the products of the leading parts have a sum of their own: a running sum
       // that takes the small ones too rounds as often as there are products)
       f4 s_low[2][NQ] = {};
@@ -441,13 +473,17 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int n = 0; n < NQ; ++n) s[i][n] += s_low[i][n];
+      if (AHEAD && more) {
+        row = next();
+        load_k(row);
+      }
     }
     if constexpr (SP > 1) {
       // (two buffers: the next step's scores do not wait for this one's readers)
       f4 *x = xs + (step & 1) * W * 2 * NQ * 64 + lane;
       if (work)
 #pragma unroll
-        for (int i = 0; i < 2 * NQ; ++i) x[(wave * 2 * NQ + i) * 64] = s[i / NQ][i % NQ];
+        for (int i = 0; i < 2 * NQ; ++i) x[(wave * 2 * NQ + i) * 64] = s[i / NQ][i % NQ] * down[i % NQ];
       __syncthreads();
       if (work)
 #pragma unroll
@@ -491,6 +527,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
                                            o[n][c * VD + t]);
         }
     }
+    if (AHEAD && more) load_v(row);
   }
 
   // ---- the groups' sums joined
@@ -617,54 +654,16 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   f4 *xs = reinterpret_cast<f4 *>(lds + 2 * B::FRAG);           // [wave][nq][half][64]
   uint32_t *rows = reinterpret_cast<uint32_t *>(lds + B::LDS - 2 * kTile * 4);  // [2][32]
 
-  // ---- q
-  u4 q[NQ][KW][QP];
-  float sc[NQ], m[NQ], l[NQ];
-  const int t_first = it.r0 / a.G, r_wave = 16 * NQ * grp;
+  float sc[NQ], down[NQ], m[NQ], l[NQ];
+  const int t_first = (int)div_by(it.r0, a.by_g), r_wave = 16 * NQ * grp;
   const int low_key = a.window ? max(it.k0, base + t_first - a.window + 1) : it.k0;
   const bool busy = r_wave < nrows;
   // the keys that all of this wave's rows attend to, and that any of them does
-  const int tw0 = (it.r0 + r_wave) / a.G, tw1 = (it.r0 + min(nrows, r_wave + 16 * NQ) - 1) / a.G;
+  const int tw0 = (int)div_by(it.r0 + r_wave, a.by_g);
+  const int tw1 = (int)div_by(it.r0 + min(nrows, r_wave + 16 * NQ) - 1, a.by_g);
   const int all_lo = a.window ? max(low_key, base + tw1 - a.window + 1) : low_key;
   const int all_hi = min(it.k1 - 1, base + tw0), any_hi = min(it.k1 - 1, base + tw1);
   const int any_lo = a.window ? max(low_key, base + tw0 - a.window + 1) : low_key;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = r_wave + 16 * n + c16;
-    const bool real = r < nrows;
-    const int t = real ? (it.r0 + r) / a.G : t_first, h = real ? (it.r0 + r) - t * a.G : 0;
-    m[n] = kLow;
-    l[n] = 0.f;
-    const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
-    float up = 1.f, down = 1.f;
-    if constexpr (F16) {
-      float big = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const f4 u = ldg<f4>(qp + 32 * ks), v = ldg<f4>(qp + 32 * ks + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) big = fmaxf(big, fmaxf(fabsf(u[j]), fabsf(v[j])));
-      }
-      lift_of(max_groups(big), &up, &down);
-    }
-    sc[n] = a.scale * down;
-    qp += 32 * KW * part;
-#pragma unroll
-    for (int ks = 0; ks < KW; ++ks) {
-      const f4 u = ldg<f4>(qp + 32 * ks), v = ldg<f4>(qp + 32 * ks + 4);
-      uint32_t p[QP][4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        split2<F16, QP>(real ? u[2 * j] * up : 0.f, real ? u[2 * j + 1] * up : 0.f, &p[0][j], 4);
-        split2<F16, QP>(real ? v[2 * j] * up : 0.f, real ? v[2 * j + 1] * up : 0.f, &p[0][2 + j], 4);
-      }
-#pragma unroll
-      for (int i = 0; i < QP; ++i) q[n][ks][i] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-
-  f4 o[NQ][CW * VD] = {};
   const int n_tiles = (it.k1 - it.k0 + kTile - 1) / kTile;
   auto span = [&](int n, int *low, int *high) {
     const int r = min(r_wave + 16 * n + c16, nrows - 1), pos = base + (int)div_by(it.r0 + r, a.by_g);
@@ -724,6 +723,21 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   __syncthreads();
   load_k(0);
   if (v_busy) load_v(0);
+
+  // ---- q, beside the first tile's loads
+  u4 q[NQ][KW][QP];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = r_wave + 16 * n + c16;
+    const bool real = r < nrows;
+    const int t = real ? (int)div_by(it.r0 + r, a.by_g) : t_first, h = real ? (it.r0 + r) - t * a.G : 0;
+    m[n] = kLow;
+    l[n] = 0.f;
+    const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
+    load_q<DT, KW>(qp + 32 * KW * part, real, q[n], &down[n]);
+    sc[n] = SP == 1 ? a.scale * down[n] : a.scale;
+  }
+  f4 o[NQ][CW * VD] = {};
   for (int tile = 0; tile < n_tiles; ++tile) {
     const int kb = it.k0 + tile * kTile;
 #pragma unroll
@@ -778,7 +792,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
           for (int n = 0; n < NQ; ++n) {
             s[i][n] += s_low[n];
             s_low[n] = f4{};
-            if constexpr (SP > 1) xs[((wave * NQ + n) * 2 + i) * 64 + lane] = s[i][n];
+            if constexpr (SP > 1) xs[((wave * NQ + n) * 2 + i) * 64 + lane] = s[i][n] * down[n];
           }
         }
         if constexpr (STRICT) __builtin_amdgcn_sched_barrier(0);
@@ -865,18 +879,18 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   for (int n = 0; n < NQ; ++n) {
     const int r = r_wave + 16 * n + c16;
     if (r >= nrows) continue;
-    const int t = (it.r0 + r) / a.G, h = (it.r0 + r) - t * a.G;
+    const int t = (int)div_by(it.r0 + r, a.by_g), h = (it.r0 + r) - t * a.G;
     const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
     float *dst = (it.part < 0 ? a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD
                               : a.part_o + pr * HD) + CW * CD * part;
-    const float f = it.part < 0 ? l[n] : 1.f;
+    const float f = it.part < 0 ? 1.f / l[n] : 1.f;
 #pragma unroll
     for (int c = 0; c < CW; ++c)
 #pragma unroll
       for (int e = 0; e < 4 * VD; e += 4) {  // dims VD (4 g + e / VD) + e % VD of the chunk
         f4 x;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = o[n][c * VD + (e + u) % VD][(e + u) / VD] / f;
+        for (int u = 0; u < 4; ++u) x[u] = o[n][c * VD + (e + u) % VD][(e + u) / VD] * f;
         *reinterpret_cast<f4 *>(dst + c * CD + 4 * VD * g + e) = x;
       }
     if (it.part >= 0 && g == 0 && part == 0) {
