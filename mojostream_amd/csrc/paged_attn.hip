@@ -617,7 +617,9 @@ struct Shape {
   static constexpr int PAIRS = 16 * NQ * W / SP;
   static constexpr int FRAG = kTile * HD * 2 * Form<DT>::KP;  // bytes of K's or V's fragments
   static constexpr int XS = SP > 1 ? W * NQ * 2 * 64 * 16 : 0;
-  static constexpr int LDS = 2 * FRAG + XS + 2 * kTile * 4;
+  static constexpr int VD = HD / (16 * W) < 2 ? 2 : HD / (16 * W);  // dims of a value row a lane loads
+  static constexpr int USED = 2 * FRAG + XS + 2 * kTile * 4, OUT = W * 16 * (16 * VD + 4) * 4;
+  static constexpr int LDS = USED > OUT ? USED : OUT;
   // (fragments of fp32 pools of 512 dims take more LDS than there is; in turns in one buffer the
   // waves ran out of registers: 1.0 to 1.2 ms where item_by_tile takes 0.61 ms, 1024 rows over 4096
   // keys, 8 heads)
@@ -640,11 +642,11 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   constexpr bool F16 = F::F16;
   constexpr int NQ = B::NQ, W = B::W, SP = B::SP;
   constexpr int QP = F::QP, KP = F::KP, KS = HD / 32, ES = DT == MS_KV_F32 ? 4 : 2;
-  constexpr int VD = HD / (16 * W) < 2 ? 2 : HD / (16 * W), CD = 16 * VD, NC = HD / CD;
+  constexpr int VD = B::VD, CD = 16 * VD, NC = HD / CD;
   constexpr int KW = KS / SP, CW = NC / SP;  // a wave's 32-dim steps and chunks of CD dims
   constexpr int D8 = HD / 8, UK = kTile * D8 / (64 * W);  // K units of 8 dims a thread
   constexpr bool STRICT = KW * KP >= 8;
-  constexpr int RING = 4;
+  constexpr int RING = 3;
   static_assert(CW >= 1 && UK >= 1 && 64 * W / D8 * UK == kTile, "shape");
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
   const int grp = wave / SP, part = wave % SP;
@@ -875,25 +877,41 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     item_by_key<HD, DT, 64 * W>(a, it, kvh, B::PAIRS, reinterpret_cast<float *>(lds));
     return;
   }
+  // Through LDS, a wave's own part of it, so that rows are stored whole: a lane's dims are 16 bytes of
+  // sixteen rows a quarter wave.
+  constexpr int LD = CD + 4, C4 = CD / 4;
+  static_assert(W * 16 * LD * 4 <= B::LDS, "LDS");
+  int ln = lane;  // (an opaque copy: the addresses below are not made ahead of the loop)
+  asm volatile("" : "+v"(ln));
+  float *own = reinterpret_cast<float *>(lds) + wave * 16 * LD;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const int r = r_wave + 16 * n + c16;
-    if (r >= nrows) continue;
-    const int t = (int)div_by(it.r0 + r, a.by_g), h = (it.r0 + r) - t * a.G;
-    const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
-    float *dst = (it.part < 0 ? a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD
-                              : a.part_o + pr * HD) + CW * CD * part;
     const float f = it.part < 0 ? 1.f / l[n] : 1.f;
 #pragma unroll
-    for (int c = 0; c < CW; ++c)
+    for (int c = 0; c < CW; ++c) {
 #pragma unroll
       for (int e = 0; e < 4 * VD; e += 4) {  // dims VD (4 g + e / VD) + e % VD of the chunk
         f4 x;
 #pragma unroll
         for (int u = 0; u < 4; ++u) x[u] = o[n][c * VD + (e + u) % VD][(e + u) / VD] * f;
-        *reinterpret_cast<f4 *>(dst + c * CD + 4 * VD * g + e) = x;
+        *reinterpret_cast<f4 *>(own + (ln & 15) * LD + 4 * VD * (ln >> 4) + e) = x;
       }
-    if (it.part >= 0 && g == 0 && part == 0) {
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int j = 0; j < 16 * C4 / 64; ++j) {
+        const int i = 64 * j + ln, r = r_wave + 16 * n + i / C4, d = CD * (CW * part + c) + i % C4 * 4;
+        const f4 x = *reinterpret_cast<const f4 *>(own + i / C4 * LD + i % C4 * 4);
+        if (r >= nrows) continue;
+        const int t = (int)div_by(it.r0 + r, a.by_g), h = (it.r0 + r) - t * a.G;
+        float *dst = it.part < 0 ? a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD
+                                 : a.part_o + (((size_t)it.part * a.n_kv + kvh) * a.part_rows + r) * HD;
+        *reinterpret_cast<f4 *>(dst + d) = x;
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    const int r = r_wave + 16 * n + ln;
+    if (it.part >= 0 && ln < 16 && part == 0 && r < nrows) {
+      const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
       a.part_ml[pr * 2] = m[n];
       a.part_ml[pr * 2 + 1] = l[n];
     }
