@@ -129,8 +129,9 @@ __device__ inline void store_kv(void *pool, size_t at, V x) {
 }
 
 // A thread takes N values and the N that turn with them (or 2 N side by side that do not turn) of
-// one head of a row: q heads, k heads, v heads.  Bound by memory: 3001 rows of 40 + 8 + 8
-// heads of 128 dims into bf16 pools, 161 MB.
+// one head of a row: q heads, k heads, v heads.  Bound by memory: 3001 rows of 40 + 8 + 8 heads
+// of 128 dims into bf16 pools, 161 MB, in 30 us (with one pair a thread 43 us); a step of single
+// tokens by its launch (2.2 to 2.6 us).
 template <int DT, int N>
 __global__ void k_paged_append(AppendArgs a) {
   typedef float V __attribute__((ext_vector_type(N)));

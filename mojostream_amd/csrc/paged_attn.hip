@@ -1,4 +1,19 @@
 // Attention of a ragged batch's new rows over a paged KV cache.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = e^(scale q.k_j - m),  max(0, pos - window + 1) <= j <= pos,
+//
+// one pass over the keys with a running maximum m and sum, cut into spans of keys whose
+// results are merged.
+//
+//  k_paged_tile   up to 32 (row, head) pairs of a kv head: single tokens, or a few
+//                 (item_by_tile).  Bound by memory: 48 tokens over up to 4096 keys, 14B class, bf16,
+//                 458 MB in 92 to 97 us; 32 tokens over up to 4096 keys in fp32, 8 kv heads of 128
+//                 dims, 5.1 TB/s, 2 of 512 dims, 5.6 TB/s (a large copy: 4.6 TB/s).
+//  k_paged_block  longer chunks, and single tokens beside them (item_by_block, item_by_tile).
+//                 Bound by the matrix cores: 4096 rows over 16384 keys, 14B class, bf16 (three
+//                 products a multiplication): 2.7 to 2.9 ms, 1.3 PFLOP/s of bf16 products, MFMA
+//                 busy 56% of the time at 2.1 GHz (a large bf16 matrix product: 1.2 PFLOP/s).
+//  k_paged_merge  the spans' results.
 #include <algorithm>
 #include <cmath>
 #include <exception>
@@ -611,19 +626,20 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
 // the sums then stays in its registers (two waves a SIMD).
 template <int HD, int DT>
 struct Shape {
-  // (two query tiles a wave where the registers hold them: a fragment then serves six products)
+  // two query tiles a wave where the registers hold them: a fragment then serves six products
   static constexpr int NQ = HD == 64 || (HD == 128 && DT != MS_KV_F32) ? 2 : 1;
-  static constexpr int W = NQ == 2 ? 4 : 8, SP = HD == 512 ? 2 : 1;
+  // the fragments of K and V take turns in one buffer where LDS has no room for both (fp32, 512 dims:
+  // 96 KB each; 1024 rows over 4096 keys, 8 heads: 0.57 ms, by item_by_tile 0.70 ms, with two waves a
+  // group, whose registers spill, 1.0 ms)
+  static constexpr bool ONE = HD == 512 && DT == MS_KV_F32;
+  static constexpr int W = NQ == 2 ? 4 : 8, SP = ONE ? 4 : HD == 512 ? 2 : 1;
   static constexpr int PAIRS = 16 * NQ * W / SP;
-  static constexpr int FRAG = kTile * HD * 2 * Form<DT>::KP;  // bytes of K's or V's fragments
-  static constexpr int XS = SP > 1 ? W * NQ * 2 * 64 * 16 : 0;
   static constexpr int VD = HD / (16 * W) < 2 ? 2 : HD / (16 * W);  // dims of a value row a lane loads
-  static constexpr int USED = 2 * FRAG + XS + 2 * kTile * 4, OUT = W * 16 * (16 * VD + 4) * 4;
+  static constexpr int FRAG = kTile * HD * 2 * Form<DT>::KP;        // bytes of K's or V's fragments
+  static constexpr int XS_AT = FRAG * (ONE ? 1 : 2), XS = SP > 1 ? W * NQ * 2 * 64 * 16 : 0;
+  static constexpr int ROWS_AT = XS_AT + XS, USED = ROWS_AT + 2 * kTile * 4;
+  static constexpr int OUT = W * 16 * (16 * VD + 4) * 4;
   static constexpr int LDS = USED > OUT ? USED : OUT;
-  // (fragments of fp32 pools of 512 dims take more LDS than there is; in turns in one buffer the
-  // waves ran out of registers: 1.0 to 1.2 ms where item_by_tile takes 0.61 ms, 1024 rows over 4096
-  // keys, 8 heads)
-  static constexpr bool FITS = LDS <= 160 * 1024;
 };
 
 // The attention of one item of a longer chunk.  The waves go over the item's 32-key tiles
@@ -652,9 +668,9 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   const int grp = wave / SP, part = wave % SP;
   const int nrows = min(B::PAIRS, it.n_new * a.G - it.r0), base = it.len - it.n_new;
   u4 *kf = reinterpret_cast<u4 *>(lds);                        // [half][ks][part][64], slots turned by (ks, g)
-  u4 *vf = kf + B::FRAG / 16;                                  // [c][t][part][64]
-  f4 *xs = reinterpret_cast<f4 *>(lds + 2 * B::FRAG);           // [wave][nq][half][64]
-  uint32_t *rows = reinterpret_cast<uint32_t *>(lds + B::LDS - 2 * kTile * 4);  // [2][32]
+  u4 *vf = B::ONE ? kf : kf + B::FRAG / 16;                    // [c][t][part][64]
+  f4 *xs = reinterpret_cast<f4 *>(lds + B::XS_AT);             // [wave][nq][half][64]
+  uint32_t *rows = reinterpret_cast<uint32_t *>(lds + B::ROWS_AT);  // [2][32]
 
   float sc[NQ], down[NQ], m[NQ], l[NQ];
   const int t_first = (int)div_by(it.r0, a.by_g), r_wave = 16 * NQ * grp;
@@ -742,6 +758,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   f4 o[NQ][CW * VD] = {};
   for (int tile = 0; tile < n_tiles; ++tile) {
     const int kb = it.k0 + tile * kTile;
+    if (B::ONE && tile) __syncthreads();
 #pragma unroll
     for (int u = 0; u < UK; ++u) {
       const int key = (tid + 64 * W * u) / D8, d8 = tid % D8;
@@ -801,6 +818,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
       }
       if constexpr (SP == 1) probabilities<DT, NQ>(s, kb, edge, sc, span, m, l, o, pf);
     }
+    if (B::ONE) __syncthreads();
     if (tid < kTile) rows[((tile + 1) & 1) * kTile + tid] = next;
     if (v_busy) {
 #pragma unroll
@@ -947,7 +965,8 @@ __global__ __launch_bounds__(NT, 2) void k_paged_block(PagedAttnArgs a) {
 
 // The parts of one result, weighted by e^(their maximum - the largest).  A block takes RPB rows,
 // its NT threads being HD / 4 columns of RPB rows by GRP groups of parts: many rows of a few parts
-// (chunks) or one row of many (a single token over a long context).
+// (chunks) or one row of many (a single token over a long context).  Bound by the launch and a chain of
+// three loads: 3.5 to 4.2 us for a few parts, 5.9 us for 256 of a row, 9.2 us for 46 MB of them.
 template <int HD, int NT>
 __global__ __launch_bounds__(NT) void k_paged_merge(PagedAttnArgs a, const PagedMerge *merge, int rpb) {
   constexpr int COLS = HD / 4, ALL = NT / COLS;
@@ -1028,7 +1047,7 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
       const int t0 = r0 / p->G, t1 = std::min((r0 + p->rows - 1) / p->G, b->n_new[s] - 1);
       const int lo = p->window ? std::max(0, base + t0 - p->window + 1) : 0;
       const int k0 = lo / kTile * kTile, k1 = base + t1 + 1, n = (k1 - k0 + kTile - 1) / kTile;
-      spans.push_back({s, r0, k0, k1, n, p->rows > 32 && pairs - r0 > 16 ? 4 : p->tile_cost});
+      spans.push_back({s, r0, k0, k1, n, p->block && pairs - r0 > 16 ? 4 : p->tile_cost});
       work += (int64_t)n * spans.back().cost;
       longest = std::max(longest, n * spans.back().cost);
     }
@@ -1087,11 +1106,11 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
   return MS_OK;
 }
 
-int plan_for(ms_paged_batch *b, int G, int rows, int n_kv, int window, int blocks, int tile_cost,
-             PagedPlan **out) {
+int plan_for(ms_paged_batch *b, int G, int rows, bool block, int n_kv, int window, int blocks,
+             int tile_cost, PagedPlan **out) {
   PagedPlan *p = nullptr;
   for (PagedPlan *x : b->plans)
-    if (x->G == G && x->rows == rows && x->n_kv == n_kv && x->window == window && x->blocks == blocks &&
+    if (x->G == G && x->rows == rows && x->block == block && x->n_kv == n_kv && x->window == window && x->blocks == blocks &&
         x->tile_cost == tile_cost)
       p = x;
   if (!p) {
@@ -1106,6 +1125,7 @@ int plan_for(ms_paged_batch *b, int G, int rows, int n_kv, int window, int block
     p->valid = false;
     p->G = G;
     p->rows = rows;
+    p->block = block;
     p->blocks = blocks;
     p->tile_cost = tile_cost;
     p->n_kv = n_kv;
@@ -1123,11 +1143,12 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   // at larger ones, whose second item finds its keys in the caches (head dim 256: 44 us, 52 us with two
   // query tiles, 64 us by blocks).
   constexpr bool TWO = HD <= 128;
-  const int rows = most <= 16 ? 16 : most <= 32 ? (TWO ? 32 : 16) : B::FITS ? B::PAIRS : 16;
+  const bool block = most > 32;
+  const int rows = block ? B::PAIRS : most > 16 && TWO ? 32 : 16;
   PagedPlan *p = nullptr;
   // blocks that run at once; a step of single tokens takes a tile for every group of waves
-  const int w = rows > 32 ? B::W : 4, cost = std::max(1, 4 * tile_split<HD>() / w);
-  if (int rc = plan_for(b, a.G, rows, a.n_kv, a.window, 8 / w * ctx().n_cu, cost, &p)) return rc;
+  const int w = block ? B::W : 4, cost = std::max(1, 4 * tile_split<HD>() / w);
+  if (int rc = plan_for(b, a.G, rows, block, a.n_kv, a.window, 8 / w * ctx().n_cu, cost, &p)) return rc;
   a.part_rows = p->most;
   if (const size_t n = (size_t)p->n_parts * a.n_kv * a.part_rows) {
     void *buf = nullptr;
@@ -1137,13 +1158,13 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   }
   a.items = reinterpret_cast<const PagedItem *>(p->up.d);
   const dim3 grid(p->n_items * a.n_kv);
-  if (rows == 16)
+  if (block) {
+    hipLaunchKernelGGL((k_paged_block<HD, DT>), grid, dim3(64 * B::W), 0, st, a);
+  } else if (rows == 16) {
     hipLaunchKernelGGL((k_paged_tile<HD, DT, 1>), grid, dim3(256), 0, st, a);
-  else if (rows == 32) {
+  } else {
     if constexpr (TWO) hipLaunchKernelGGL((k_paged_tile<HD, DT, 2>), grid, dim3(256), 0, st, a);
   }
-  else if constexpr (B::FITS)
-    hipLaunchKernelGGL((k_paged_block<HD, DT>), grid, dim3(64 * B::W), 0, st, a);
   if (p->n_merge) {
     // about four parts a thread, more of them in a larger block
     const PagedMerge *merge = reinterpret_cast<const PagedMerge *>(p->up.d + p->merge_at);
