@@ -269,7 +269,8 @@ int ms_paged_batch_set(ms_paged_batch *b, int n_seqs, const int32_t *h_new,
 /* cos and sin [n_pos][rot_dim/2] of positions pos0.. for ms_paged_append.
  * wide = 0: the reference's fp32 angles (kernels.mojo:563-577), the values
  * ms_rope and the model use; wide = 1: angles pos * theta^(-2i/rot_dim) in 64
- * bits, rounded once: at position 100000 the fp32 angles are off by up to 0.05. */
+ * bits, rounded once: at position 100000 and theta 1e4 the fp32 angles are off by
+ * up to 0.006. */
 int ms_rope_table(float *d_cos, float *d_sin, int rot_dim, float theta, int pos0, int n_pos,
                   int wide);
 /* The rows' k (rotated) and v into their pages, and q (rotated) to d_q_out.  Row
@@ -289,7 +290,8 @@ int ms_paged_append(const ms_paged_layer *layer, const ms_paged_batch *b, const 
  * among them: append first), d_q and d_out rows as in ms_paged_append, which must
  * not overlap.  The row at position p attends to positions max(0, p - window +
  * 1) .. p.  Products take q, the probabilities and the pools' values with all
- * their bits, sums are fp32.  Slots outside the attended positions are never
+ * their bits (over fp16 pools 22 bits of q and of the probabilities), sums are
+ * fp32.  Slots outside the attended positions are never
  * used, whatever they hold; a value that is not finite reaches only the rows
  * that attend to it.  Rows behind the last sequence's are left as they were. */
 int ms_paged_attention(const ms_paged_layer *layer, ms_paged_batch *b, const float *d_q,

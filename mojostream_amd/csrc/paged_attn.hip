@@ -373,7 +373,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   const char *kb0 = static_cast<const char *>(a.k) + ((size_t)kvh * HD + HW * part + 8 * g) * ES;
   const char *vb0 = static_cast<const char *>(a.v) + ((size_t)kvh * HD + HW * part + VD * c16) * ES;
   // The next tile's keys are loaded once this one's are multiplied, its values once these are, where
-  // there are registers for it (not for fp32 pools and one query tile: 160 us with spills, 126 us with
+  // there are registers for it (not for fp32 pools and one query tile: 160 us with spills, 118 us with
   // both loaded as the tile begins; 32 tokens over 4096 keys, 8 kv heads of 128 dims).
   constexpr bool AHEAD = F16 ? NQ == 1 : ES == 2 || NQ == 2;
   u4 kr[2][KS][ES / 2], vr[8][NC];
