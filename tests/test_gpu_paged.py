@@ -233,6 +233,20 @@ def test_attention_sizes_of_q(gpu, dtype, new, hd):
             assert np.array_equal(got[r, h], v[best, h // 2].astype(np.float32))
 
 
+@pytest.mark.parametrize("new,hd", [(1, 128), (6, 128), (1, 512), (60, 64), (60, 512)])
+@pytest.mark.parametrize("dtype,tiny", [("f16", 2.0 ** -19), ("bf16", 2.0 ** -100), ("f32", 2.0 ** -90)])
+def test_attention_tiny_values(gpu, dtype, tiny, new, hd):
+    """Values far below 1 (fp16: below its smallest normal number) keep what their type holds."""
+    say(f"attention, tiny values: {dtype} {tiny} new={new} hd={hd}")
+    st = Setup(gpu, [(new, 100)], 4, 2, hd, dtype, 16, seed=21)
+    for n in "kv":
+        x = decode(st.pool[n], dtype) * tiny
+        st.pool[n] = encode(x.astype(np.float32), dtype)
+    st.upload()
+    st.layer.scale = st.scale = 1.0
+    st.check_attention(scale=0.1 / tiny)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("new,length,window", [(1, 400, 0), (40, 170, 0), (40, 170, 50), (3, 1200, 0)])
 def test_attention_not_finite(gpu, dtype, new, length, window):
@@ -260,6 +274,32 @@ def test_attention_not_finite(gpu, dtype, new, length, window):
         assert fine.any()
         assert np.all(np.abs(got[fine] - want[fine]) <= tol[fine]), kind
         st.pool = st2
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("new,hd", [(1, 128), (8, 64), (50, 128), (50, 512)])
+def test_attention_rows_not_finite(gpu, dtype, new, hd):
+    """A query that is not finite spoils its own row alone; a row all of whose keys score minus
+    infinity has no result (NaN, as the formula)."""
+    ms = gpu
+    say(f"attention, rows not finite: {dtype} new={new} hd={hd}")
+    st = Setup(ms, [(new, 90), (1, 40)], 4, 2, hd, dtype, 16, seed=23)
+    q = f32(st.rows, 4, hd, seed=24)
+    q[0, 1, 3], q[new // 2, 2, 7] = np.nan, np.inf
+    want, tol = st.attend(q.reshape(st.rows, -1))
+    got = st.run_attention(q.reshape(st.rows, -1))
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isnan(want).any()
+    fine = np.isfinite(want)
+    assert np.all(np.abs(got[fine] - want[fine]) <= tol[fine])
+    # every key of kv head 1
+    g = st.slots(0, 0, 90)
+    x = decode(st.pool["k"][g], dtype).astype(np.float32)
+    x[:, 1, 0] = -np.inf
+    st.pool["k"][g] = encode(x, dtype)
+    st.upload()
+    q = np.abs(f32(st.rows, 4, hd, seed=25)) + 0.1
+    got = st.run_attention(q.reshape(st.rows, -1)).reshape(st.rows, 4, hd)
+    assert np.isnan(got[:new, 2:]).all() and np.isfinite(got[:new, :2]).all() and np.isfinite(got[new]).all()
 
 
 def test_attention_freed_pages(gpu):
@@ -331,6 +371,9 @@ def test_far_pages(gpu):
     b.set([n], [n], pages)
     ms.paged_append(layer, b, dk, dv, kv * hd)
     st.batch, st.layer, old = b, layer, (st.batch, st.layer)
+    st.check_attention()
+    b.set([1], [n], pages)  # a single token takes another way
+    st.new, st.rows = [1], 1
     st.check_attention()
     out = np.empty((page, kv * hd), np.float32)
     ms.synchronize()
