@@ -54,7 +54,7 @@ struct PagedMerge {
 
 // A split of the batch's work, for layers of the same shape.
 struct PagedPlan {
-  int G = 0, rows = 0, n_kv = 0, window = 0, blocks = 0, tile_cost = 0;
+  int G = 0, rows = 0, n_kv = 0, window = 0, blocks = 0, tile_cost = 0, merge_cost = 0;
   bool block = false;  // items of more than 16 pairs go to item_by_block
   bool valid = false;
   int n_items = 0, n_merge = 0, n_parts = 0;

@@ -1053,7 +1053,8 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
     }
   }
   // The longest part a block gets, `per`: at least a step, and no more than kMaxParts of them; from an even share up, where its end is soonest: all blocks at once
-  // are done with the longest, more of them after about half of one more.
+  // are done with the longest, more of them after about half of one more; then the merge, if there is
+  // anything to merge.
   auto cuts_of = [](const Span &x, int per) { return (x.tiles * x.cost + per - 1) / per; };
   const int64_t fill = std::max((work * p->n_kv + blocks - 1) / blocks,
                                 ((int64_t)b->max_pos / kTile * 4 + kMaxParts) / kMaxParts);
@@ -1067,7 +1068,9 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
       top = std::max<int64_t>(top, (x.tiles + cuts - 1) / cuts * x.cost);
     }
     n *= p->n_kv;
-    const int64_t end = n <= blocks ? top : std::max(top, work * p->n_kv / blocks) + top / 2;
+    const bool cut = n > (int64_t)spans.size() * p->n_kv;
+    const int64_t end = (n <= blocks ? top : std::max(top, work * p->n_kv / blocks) + top / 2) +
+                        (cut ? p->merge_cost : 0);
     if (end < best) {
       best = end;
       per = (int)c;
@@ -1107,11 +1110,11 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
 }
 
 int plan_for(ms_paged_batch *b, int G, int rows, bool block, int n_kv, int window, int blocks,
-             int tile_cost, PagedPlan **out) {
+             int tile_cost, int merge_cost, PagedPlan **out) {
   PagedPlan *p = nullptr;
   for (PagedPlan *x : b->plans)
     if (x->G == G && x->rows == rows && x->block == block && x->n_kv == n_kv && x->window == window && x->blocks == blocks &&
-        x->tile_cost == tile_cost)
+        x->tile_cost == tile_cost && x->merge_cost == merge_cost)
       p = x;
   if (!p) {
     // (a model has a few shapes of layers; more than that reuse the oldest place)
@@ -1128,6 +1131,7 @@ int plan_for(ms_paged_batch *b, int G, int rows, bool block, int n_kv, int windo
     p->block = block;
     p->blocks = blocks;
     p->tile_cost = tile_cost;
+    p->merge_cost = merge_cost;
     p->n_kv = n_kv;
     p->window = window;
   }
@@ -1148,7 +1152,11 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   PagedPlan *p = nullptr;
   // blocks that run at once; a step of single tokens takes a tile for every group of waves
   const int w = block ? B::W : 4, cost = std::max(1, 4 * tile_split<HD>() / w);
-  if (int rc = plan_for(b, a.G, rows, block, a.n_kv, a.window, 8 / w * ctx().n_cu, cost, &p)) return rc;
+  // A merge's launch takes 3.4 us; a step of a single token (4 in the plan's measure) 0.7 us at head dim 64,
+  // 1.15 at 128 and 1.4 to 1.6 at 256 and 512 over 16-bit pools, 1.7 to 5 us over fp32 ones: one token over 250
+  // keys of 64 dims (bf16) 5.4 us in one block a head, 9.0 us cut and merged; over 1500 keys 12.4 and 9.1 us.
+  const int merge = block ? 8 : DT == MS_KV_F32 ? 4 : HD == 64 ? 20 : HD == 128 ? 12 : 8;
+  if (int rc = plan_for(b, a.G, rows, block, a.n_kv, a.window, 8 / w * ctx().n_cu, cost, merge, &p)) return rc;
   a.part_rows = p->most;
   if (const size_t n = (size_t)p->n_parts * a.n_kv * a.part_rows) {
     void *buf = nullptr;
