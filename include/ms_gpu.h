@@ -270,7 +270,7 @@ int ms_paged_batch_set(ms_paged_batch *b, int n_seqs, const int32_t *h_new,
  * wide = 0: the reference's fp32 angles (kernels.mojo:563-577), the values
  * ms_rope and the model use; wide = 1: angles pos * theta^(-2i/rot_dim) in 64
  * bits, rounded once: at position 100000 and theta 1e4 the fp32 angles are off by
- * up to 0.006. */
+ * up to 0.006.  At most 2^31 entries a table. */
 int ms_rope_table(float *d_cos, float *d_sin, int rot_dim, float theta, int pos0, int n_pos,
                   int wide);
 /* The rows' k (rotated) and v into their pages, and q (rotated) to d_q_out.  Row

@@ -304,12 +304,13 @@ extern "C" int ms_rope_table(float *d_cos, float *d_sin, int rot_dim, float thet
   MS_CHECK_ARG(rot_dim >= 2 && rot_dim % 2 == 0 && theta > 0.f && theta < INFINITY && pos0 >= 0 &&
                    n_pos >= 0 && (int64_t)pos0 + n_pos < ((int64_t)1 << 31),
                "rope_table: bad arguments");
+  // (a launch has fewer than 2^32 threads)
+  MS_CHECK_ARG((int64_t)n_pos * (rot_dim / 2) <= ((int64_t)1 << 31), "rope_table: table too large");
   if (int rc = require_init()) return rc;
   if (!n_pos) return MS_OK;
   OnDevice on;
   const long total = (long)n_pos * (rot_dim / 2);
   if (wide) {
-    MS_CHECK_ARG(total <= ((long)1 << 38), "rope_table: table too large");
     hipLaunchKernelGGL(k_rope_table, dim3(cdiv(total, kBlock)), dim3(kBlock), 0, ctx().stream,
                        d_cos, d_sin, rot_dim / 2, -2.0 * std::log((double)theta) / rot_dim, pos0,
                        total);

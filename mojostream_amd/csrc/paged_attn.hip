@@ -1052,9 +1052,9 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
       longest = std::max(longest, n * spans.back().cost);
     }
   }
-  // The longest part a block gets, `per`: at least a step, and no more than kMaxParts of them; from an even share up, where its end is soonest: all blocks at once
-  // are done with the longest, more of them after about half of one more; then the merge, if there is
-  // anything to merge.
+  // The longest part a block gets, `per`: at least a step, and no more than kMaxParts of them; from an
+  // even share up, where its end is soonest: all blocks at once are done with the longest, more of
+  // them after about half of one more; then the merge, if there is anything to merge.
   auto cuts_of = [](const Span &x, int per) { return (x.tiles * x.cost + per - 1) / per; };
   const int64_t fill = std::max((work * p->n_kv + blocks - 1) / blocks,
                                 ((int64_t)b->max_pos / kTile * 4 + kMaxParts) / kMaxParts);
@@ -1165,6 +1165,9 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
     a.part_ml = a.part_o + n * HD;
   }
   a.items = reinterpret_cast<const PagedItem *>(p->up.d);
+  // (a launch has fewer than 2^32 threads)
+  MS_CHECK_ARG((int64_t)p->n_items * a.n_kv * 64 * w < ((int64_t)1 << 32),
+               "paged_attention: too many rows for one call");
   const dim3 grid(p->n_items * a.n_kv);
   if (block) {
     hipLaunchKernelGGL((k_paged_block<HD, DT>), grid, dim3(64 * B::W), 0, st, a);
@@ -1202,8 +1205,12 @@ using namespace ms;
 extern "C" int ms_paged_attention(const ms_paged_layer *L, ms_paged_batch *b, const float *d_q,
                                   size_t q_stride, float *d_out, size_t out_stride) {
   MS_CHECK_ARG(L, "paged_attention: null layer or batch");
-  MS_CHECK_ARG(std::fabs(L->scale) < INFINITY, "paged_attention: the scale is not a finite number");
+  // (log2(e) times it, what the kernels take, is finite too)
+  MS_CHECK_ARG(std::fabs(L->scale * 1.4426950408889634) <= 0x1.fffffep+127,
+               "paged_attention: the scale is not finite or too large");
   if (int rc = paged_check("paged_attention", L, b)) return rc;
+  MS_CHECK_ARG((int64_t)b->rows * L->n_heads < ((int64_t)1 << 30),
+               "paged_attention: too many rows for one call");
   const int q_dim = L->n_heads * L->head_dim, hd = L->head_dim, G = L->n_heads / L->n_kv_heads;
   int most = 0;
   for (int s = 0; s < b->n_seqs; ++s) {
@@ -1213,8 +1220,6 @@ extern "C" int ms_paged_attention(const ms_paged_layer *L, ms_paged_batch *b, co
                                        " attends to a position whose page is -1");
     most = std::max(most, b->n_new[s] * G);
   }
-  MS_CHECK_ARG((int64_t)b->rows * L->n_heads < ((int64_t)1 << 30),
-               "paged_attention: too many rows for one call");
   if (b->rows == 0) return require_init();
   MS_CHECK_ARG(d_q && d_out && aligned16(d_q) && aligned16(d_out) && q_stride % 4 == 0 &&
                    out_stride % 4 == 0 && q_stride >= (size_t)q_dim &&

@@ -125,6 +125,19 @@ def test_rope_table(args, wide):
     assert ms.lib().ms_rope_table(*args, wide) == INVALID
 
 
+@pytest.mark.parametrize("wide", [0, 1])
+def test_rope_table_size(wide):
+    assert ms.lib().ms_rope_table(64, 64, 64, 1e4, 0, 2 ** 26 + 1, wide) == INVALID
+    assert "too large" in err()
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38])
+def test_scale_past_fp32_in_log2(batch, scale):
+    layer = ms.PagedLayer(**{**GOOD, "scale": scale})
+    assert ms.lib().ms_paged_attention(C.byref(layer), batch.h, 64, 512, 64, 512) == INVALID
+    assert "scale" in err()
+
+
 def _logits(row=None, n=1, vocab=100, x=4096, ldx=100, y=8192, ldy=100, hist=64, nh=10, ids=64, vals=64, nb=5,
             masks=64, nm=2):
     rows = (ms.LogitsRow * max(n, 1))(*[row or ms.LogitsRow()] * max(n, 1))
