@@ -289,9 +289,9 @@ int ms_paged_append(const ms_paged_layer *layer, const ms_paged_batch *b, const 
 /* Causal GQA attention of the batch's rows over the pages (the rows' own keys
  * among them: append first), d_q and d_out rows as in ms_paged_append, which must
  * not overlap.  The row at position p attends to positions max(0, p - window +
- * 1) .. p.  Products take q, the probabilities and the pools' values with all
- * their bits (over fp16 pools 22 bits of q and of the probabilities), sums are
- * fp32.  Slots outside the attended positions are never
+ * 1) .. p.  Products take q times the scale (rounded once to fp32), the
+ * probabilities and the pools' values with all their bits (over fp16 pools 22
+ * bits of q and of the probabilities), sums are fp32.  Slots outside the attended positions are never
  * used, whatever they hold; a value that is not finite reaches only the rows
  * that attend to it.  Rows behind the last sequence's are left as they were. */
 int ms_paged_attention(const ms_paged_layer *layer, ms_paged_batch *b, const float *d_q,

@@ -37,7 +37,8 @@ struct PagedAttnArgs {
   const PagedItem *items;
   int n_kv, G, window, page_size, page_rows;
   FastDiv by_page, by_g;  // n / page_size, n / G
-  float scale;            // of the scores, log2(e) in it
+  // The scores' scale, log2(e) in it, is q_scale (0.5 to 1 in size) times s_scale (a power of two).
+  float q_scale, s_scale;
   float *part_o, *part_ml;  // [part][kv head][part_rows][head dim], [part][kv head][part_rows][2]
   int part_rows;          // (row, head) pairs of the longest item
 };
@@ -155,7 +156,8 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
         const size_t row = (size_t)a.pages[(size_t)it.seq * a.stride + pg] * a.page_rows +
                            (key - pg * a.page_size);
         const size_t at = (row * a.n_kv + kvh) * HD;
-        for (int d = 0; d < HD; ++d) s += q[d] * a.scale * load_kv<DT>(a.k, at + d);
+        for (int d = 0; d < HD; ++d) s += q[d] * a.q_scale * load_kv<DT>(a.k, at + d);
+        s *= a.s_scale;
       }
       float mx = on ? s : -INFINITY;
       for (int off = 1; off < 64; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
@@ -211,7 +213,10 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
 // A tile's probabilities as the operand of the second product, from its scores: t = s sc - m,
 // m the running maximum, in log2; p = 2^t.  `edge`: some row does not attend to some key.
 // m serves all of a query's keys and may lag behind by kLag, so that a tile needs neither a
-// cross-lane maximum nor a rescaling of the sums, unless a score exceeds it.
+// cross-lane maximum nor a rescaling of the sums, unless a score exceeds it.  sc is a power of two, so
+// that s sc is exact: t of the key that m was raised to is 0 whatever the scores' size.  (With a rounded
+// product in m and not in t it was off by up to half of m's last place: from 2^29 on rows came out
+// as 0 or NaN.)
 // span(n, &low, &high): the keys that the lane's query of query tile n attends to.
 template <int DT, int NQ, int ND, class Span>
 __device__ __forceinline__ void probabilities(const f4 (&s)[2][NQ], int kb, bool edge,
@@ -279,11 +284,12 @@ __device__ inline void lift_of(float big, float *up, float *down) {
   *down = __uint_as_float((uint32_t)(127 - e) << 23);
 }
 
-// KS 32-dim steps of a query's dims from qp on (that lane's eight of each) in parts, as the first
-// product's operand; 0 where the query is not real.  What their product has to be multiplied by: *down.
+// KS 32-dim steps of a query's dims from qp on (that lane's eight of each), times `scale` (0.5 to 1 in
+// size; one rounding), in parts, as the first product's operand; 0 where the query is not real.  What
+// their product has to be multiplied by, a power of two: *down.
 template <int DT, int KS>
-__device__ __forceinline__ void load_q(const float *qp, bool real, u4 (&q)[KS][Form<DT>::QP],
-                                       float *down) {
+__device__ __forceinline__ void load_q(const float *qp, bool real, float scale,
+                                       u4 (&q)[KS][Form<DT>::QP], float *down) {
   constexpr bool F16 = Form<DT>::F16;
   constexpr int QP = Form<DT>::QP;
   f4 x[KS][2];
@@ -303,6 +309,7 @@ __device__ __forceinline__ void load_q(const float *qp, bool real, u4 (&q)[KS][F
       for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[ks][j >> 2][j & 3]));
     lift_of(max_groups(big), &up, down);
   }
+  up *= scale;
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     uint32_t p[QP][4];
@@ -424,8 +431,8 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
     const bool real = r < nrows;
     const int t = real ? (int)div_by(it.r0 + r, a.by_g) : t_first, h = real ? it.r0 + r - t * a.G : 0;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
-    load_q<DT, KS>(qp + HW * part, real, q[n], &down[n]);
-    sc[n] = SP == 1 ? a.scale * down[n] : a.scale;
+    load_q<DT, KS>(qp + HW * part, real, a.q_scale, q[n], &down[n]);
+    sc[n] = SP == 1 ? a.s_scale * down[n] : a.s_scale;
   }
 
   f4 o[NQ][NC * VD] = {};
@@ -752,8 +759,8 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     m[n] = kLow;
     l[n] = 0.f;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
-    load_q<DT, KW>(qp + 32 * KW * part, real, q[n], &down[n]);
-    sc[n] = SP == 1 ? a.scale * down[n] : a.scale;
+    load_q<DT, KW>(qp + 32 * KW * part, real, a.q_scale, q[n], &down[n]);
+    sc[n] = SP == 1 ? a.s_scale * down[n] : a.s_scale;
   }
   f4 o[NQ][CW * VD] = {};
   for (int tile = 0; tile < n_tiles; ++tile) {
@@ -1247,7 +1254,11 @@ extern "C" int ms_paged_attention(const ms_paged_layer *L, ms_paged_batch *b, co
   a.page_rows = page_rows(L, b);
   a.by_page = fast_div(b->page_size);
   a.by_g = fast_div(G);
-  a.scale = (float)((L->scale == 0.f ? 1.0 / std::sqrt((double)hd) : L->scale) * 1.4426950408889634);
+  int e = 0;
+  const double scale = (L->scale == 0.f ? 1.0 / std::sqrt((double)hd) : L->scale) * 1.4426950408889634;
+  const double part = std::frexp(scale, &e);  // (e <= 128; 2^127 is the largest power that fp32 holds)
+  a.q_scale = (float)(e > 127 ? 2 * part : part);
+  a.s_scale = (float)std::ldexp(1.0, e > 127 ? e - 1 : e);
   try {
     switch (hd) {
       case 64: return launch_type<64>(a, b, L->dtype, most, st);

@@ -302,6 +302,59 @@ def test_attention_rows_not_finite(gpu, dtype, new, hd):
     assert np.isnan(got[:new, 2:]).all() and np.isfinite(got[:new, :2]).all() and np.isfinite(got[new]).all()
 
 
+def one_key_takes_all(st, q):
+    """Rows and heads whose best key takes all, and those keys' values, in 64 bits.  A score may be off
+    by (hd + 8) 2^-24 of the sum of its products' magnitudes; a key that is behind by twice
+    that and 150 has a weight below fp32's smallest number (e^-150 < 2^-149 2^-67)."""
+    G = st.heads // st.kv
+    want, sure = np.zeros((st.rows, st.heads, st.hd), np.float32), np.zeros((st.rows, st.heads), bool)
+    q, sc = q.reshape(st.rows, st.heads, st.hd).astype(np.float64), st.scale or 1 / np.sqrt(st.hd)
+    for r, (s, p) in enumerate(st.row_of()):
+        k, v = (decode(st.pool[n][st.slots(s, 0, p + 1)], st.dtype) for n in "kv")
+        for h in range(st.heads):
+            x = k[:, h // G] @ q[r, h] * sc
+            off = (st.hd + 8) * 2.0 ** -24 * (np.abs(k[:, h // G]) @ np.abs(q[r, h])).max() * abs(sc)
+            best = np.argmax(x)
+            want[r, h] = v[best, h // G]
+            sure[r, h] = len(x) == 1 or x[best] - np.delete(x, best).max() > 2 * off + 150
+    return want, sure
+
+
+@pytest.mark.parametrize("size", [3e8, 1e9, 1e10, 1e30])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("seqs,hd", [([(1, 20)] * 150, 128), ([(1, 9)] * 60, 64), ([(1, 30)] * 60, 256),
+                                     ([(1, 30)] * 60, 512), ([(1, 3000)] * 3, 128), ([(40, 40), (1, 20)], 128),
+                                     ([(40, 60), (1, 20)], 512)])
+def test_attention_large_scores(gpu, seqs, hd, dtype, size):
+    """Finite scores of any size: where one key is far above the others the result is its value,
+    also for a row that has an item to itself (1 pair a kv head)."""
+    say(f"attention, large scores: {len(seqs)} x {seqs[0]} hd={hd} {dtype} q x {size}")
+    st = Setup(gpu, seqs, 2, 2, hd, dtype, 32, seed=31)
+    q = f32(st.rows, 2 * hd, seed=32) * np.float32(size)
+    want, sure = one_key_takes_all(st, q)
+    assert sure.mean() > 0.9
+    got = st.run_attention(q).reshape(want.shape)
+    assert np.array_equal(got[sure], want[sure])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new,hd", [(2, 128), (50, 64)])
+def test_attention_large_scale_beside_nan(gpu, dtype, new, hd):
+    """A row beside one whose key is NaN, with a scale whose product with q alone
+    passes fp32 (1e30 * 1e10), while the scores do not."""
+    say(f"attention, large scale beside NaN: {dtype} new={new} hd={hd}")
+    st = Setup(gpu, [(new, 90)], 2, 2, hd, dtype, 16, seed=33, scale=1e30)
+    st.pool["k"] = encode((decode(st.pool["k"], dtype) * 1e-20).astype(np.float32), dtype)
+    g = st.slots(0, 89, 90)
+    st.pool["k"][g] = encode(np.full((1, 2, hd), np.nan, np.float32), dtype)
+    st.upload()
+    q = f32(new, 2 * hd, seed=34) * np.float32(1e10)
+    got = st.run_attention(q).reshape(new, 2, hd)
+    st.new, st.len, st.rows = [new - 1], [89], new - 1
+    want, sure = one_key_takes_all(st, q[:-1])
+    assert sure.mean() > 0.9 and np.isnan(got[-1]).all()
+    assert np.array_equal(got[:-1][sure], want[sure])
+
 def test_attention_freed_pages(gpu):
     """Pages behind a window may be given back: -1 in the table; full attention is refused."""
     ms = gpu
