@@ -1046,7 +1046,7 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
   };
   std::vector<Span> spans;
   int64_t work = 0;
-  int most = 0, longest = 0;
+  int most = 0, longest = 0, most_tiles = 0;
   for (int s = 0; s < b->n_seqs; ++s) {
     const int pairs = b->n_new[s] * p->G, base = b->len[s] - b->n_new[s];
     most = std::max(most, std::min(pairs, p->rows));
@@ -1057,14 +1057,16 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
       spans.push_back({s, r0, k0, k1, n, p->block && pairs - r0 > 16 ? 4 : p->tile_cost});
       work += (int64_t)n * spans.back().cost;
       longest = std::max(longest, n * spans.back().cost);
+      most_tiles = std::max(most_tiles, n);
     }
   }
   // The longest part a block gets, `per`: at least a step, and no more than kMaxParts of them; from an
   // even share up, where its end is soonest: all blocks at once are done with the longest, more of
   // them after about half of one more; then the merge, if there is anything to merge.
   auto cuts_of = [](const Span &x, int per) { return (x.tiles * x.cost + per - 1) / per; };
+  // (by the tiles that the longest span has: a sliding window's are the same at every position)
   const int64_t fill = std::max((work * p->n_kv + blocks - 1) / blocks,
-                                ((int64_t)b->max_pos / kTile * 4 + kMaxParts) / kMaxParts);
+                                ((int64_t)most_tiles * 4 + kMaxParts) / kMaxParts);
   int per = (int)((fill + 3) / 4 * 4);
   int64_t best = INT64_MAX;
   for (int64_t c = per;; c += std::max<int64_t>(4, c / 8 / 4 * 4)) {

@@ -355,6 +355,24 @@ def test_attention_large_scale_beside_nan(gpu, dtype, new, hd):
     assert sure.mean() > 0.9 and np.isnan(got[-1]).all()
     assert np.array_equal(got[:-1][sure], want[sure])
 
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_window_far_along(gpu, dtype):
+    """A sliding window's work is that of its keys: a token at position 599 and one at 128599,
+    with the same keys in the window, are computed alike, to the bit."""
+    ms = gpu
+    say(f"attention: a window far along, {dtype}")
+    near = Setup(ms, [(1, 600)], 8, 2, 256, dtype, 16, window=512, seed=35)
+    q, want = near.check_attention()
+    ahead = 128000  # whole pages and whole tiles of keys
+    pages = np.full((1, (ahead + 600 + 15) // 16), -1, np.int32)
+    pages[0, ahead // 16:] = near.pages[0]
+    pages[0, :(ahead + 599 - 511) // 16] = -1
+    near.batch = ms.PagedBatch(16, near.n_pages, 1, 1, pages.shape[1])
+    near.batch.set([1], [ahead + 600], pages)
+    assert np.array_equal(near.run_attention(q), want)
+
+
 def test_attention_freed_pages(gpu):
     """Pages behind a window may be given back: -1 in the table; full attention is refused."""
     ms = gpu
