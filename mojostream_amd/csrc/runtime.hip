@@ -14,6 +14,8 @@ static Ctx g_ctx;
 void set_error(const std::string &msg) { g_err = msg; }
 int fail(int code, const std::string &msg) {
   g_err = msg;
+  // The caller has the code: the runtime's own copy would be taken for the next launch's error.
+  if (code == MS_E_HIP || code == MS_E_NOMEM) (void)hipGetLastError();
   return code;
 }
 Ctx &ctx() { return g_ctx; }

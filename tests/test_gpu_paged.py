@@ -474,3 +474,21 @@ def test_refusals_with_a_batch(gpu):
                    dict(o=p + 4096 + 1024), dict(o=p + 4096, os=260), dict(o=p), dict(v=far, o=far)):
         a = {**good, **change}
         assert ap(L, h, a["k"], a["v"], a["kvs"], a["q"], a["qs"], a["o"], a["os"], a["c"], a["s"], a["n"]) == -1, change
+
+
+def test_call_after_a_failed_allocation(gpu):
+    """An allocation that fails leaves no error behind for the calls that follow it."""
+    ms = gpu
+    say("paged: calls after a failed allocation")
+    st = Setup(ms, [(3, 20)], 4, 2, 64, "f32", 16, seed=36)
+    q = f32(3, 4 * 64, seed=37)
+    d = ms.DeviceBuffer.from_array(q)
+    for _ in range(2):
+        with pytest.raises(ms.MSError, match="memory"):
+            ms.DeviceBuffer(1 << 50)
+        ms.paged_append(st.layer, st.batch, d, d, 128)
+        with pytest.raises(ms.MSError, match="memory"):
+            ms.DeviceBuffer(1 << 50)
+        st.run_attention(q)
+    c, s = ms.rope_table(64, 1e4, 3, wide=True)
+    ms.synchronize()
