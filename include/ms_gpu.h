@@ -319,7 +319,8 @@ typedef struct {
  * (vocab + 31) / 32 words, id i in bit i % 32 of word i / 32.  Ids outside
  * [0, vocab) are passed over.  A mask that allows nothing leaves a row of
  * -infinity.  h_rows is read before the call returns.  n_history, n_bias and n_masks
- * are the sizes of the device arrays; a row that reaches past them is refused. */
+ * are the sizes of the device arrays; a row that reaches past them is refused, and one of
+ * 2^30 or more history ids or biases. */
 int ms_logits_process(const float *d_logits, size_t in_stride, float *d_out, size_t out_stride,
                       int rows, int vocab, const ms_logits_row *h_rows,
                       const int32_t *d_history, size_t n_history, const int32_t *d_bias_ids,

@@ -212,7 +212,7 @@ extern "C" int ms_logits_process(const float *d_logits, size_t in_stride, float 
     MS_CHECK_ARG(h < (1 << 30) && w.history >= 0 && (uint64_t)w.history <= n_history &&
                      (uint64_t)h <= n_history - (uint64_t)w.history && (h == 0 || d_history),
                  at("the history reaches past d_history"));
-    MS_CHECK_ARG(w.bias >= 0 && (uint64_t)w.bias <= n_bias &&
+    MS_CHECK_ARG(w.n_bias < (1 << 30) && w.bias >= 0 && (uint64_t)w.bias <= n_bias &&
                      (uint64_t)w.n_bias <= n_bias - (uint64_t)w.bias &&
                      (w.n_bias == 0 || (d_bias_ids && d_bias)),
                  at("the biases reach past d_bias"));

@@ -159,6 +159,15 @@ def test_logits_rows(row, say):
     assert "row 0" in err() and say in err(), err()
 
 
+@pytest.mark.parametrize("row,say", [(dict(n_bias=2 ** 30), "biases"), (dict(n_bias=2 ** 31 - 1), "biases"),
+                                     (dict(n_prompt=2 ** 30), "history"),
+                                     (dict(n_prompt=2 ** 30 - 1, n_generated=1), "history")])
+def test_logits_counts(row, say):
+    """Counts that the kernel's 32-bit indexes do not hold, over arrays that would be large enough."""
+    assert _logits(ms.LogitsRow(**row), hist=64, nh=2 ** 33, nb=2 ** 33) == INVALID
+    assert "row 0" in err() and say in err(), err()
+
+
 def test_logits_arguments():
     assert _logits(n=-1) == INVALID
     assert _logits(vocab=0) == INVALID
