@@ -1065,8 +1065,9 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
   // them after about half of one more; then the merge, if there is anything to merge.
   auto cuts_of = [](const Span &x, int per) { return (x.tiles * x.cost + per - 1) / per; };
   // (by the tiles that the longest span has: a sliding window's are the same at every position)
-  const int64_t fill = std::max((work * p->n_kv + blocks - 1) / blocks,
-                                ((int64_t)most_tiles * 4 + kMaxParts) / kMaxParts);
+  // (an even share of more than the longest span: nothing is cut; unbounded it passes 32 bits)
+  const int64_t fill = std::min<int64_t>(longest, std::max((work * p->n_kv + blocks - 1) / blocks,
+                                                           ((int64_t)most_tiles * 4 + kMaxParts) / kMaxParts));
   int per = (int)((fill + 3) / 4 * 4);
   int64_t best = INT64_MAX;
   for (int64_t c = per;; c += std::max<int64_t>(4, c / 8 / 4 * 4)) {

@@ -492,3 +492,21 @@ def test_call_after_a_failed_allocation(gpu):
         st.run_attention(q)
     c, s = ms.rope_table(64, 1e4, 3, wide=True)
     ms.synchronize()
+
+
+def test_plan_of_the_longest_batch(gpu):
+    """A batch whose even share of work passes 32 bits is planned, and refused for its number of
+    blocks before anything is launched (the pools' and rows' addresses are not memory)."""
+    ms = gpu
+    say("paged: a plan past 32 bits")
+    rows, page, n_pages = (1 << 20) - 1, 1 << 20, 1 << 10
+    batch = ms.PagedBatch(page, n_pages, 1, rows, n_pages)
+    batch.set([rows], [page * n_pages], np.arange(n_pages)[None])
+
+    class At:
+        def __init__(self, ptr):
+            self.ptr = ptr
+
+    layer = ms.PagedLayer(n_heads=1024, n_kv_heads=1024, head_dim=512, dtype=1, k=4096, v=8192)
+    with pytest.raises(ms.MSError, match="too many rows for one call"):
+        ms.paged_attention(layer, batch, At(4096), 1024 * 512, At(1 << 43), 1024 * 512)
