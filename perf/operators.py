@@ -6,7 +6,9 @@
     logits   penalties for tokens that occurred, biases, and grammar masks on the logits
 
 Where `own` is false, run() computes them in plain torch operations in 32 bits; where it
-is true, through ms_paged_append, ms_paged_attention and ms_logits_process.
+is true, through ms_paged_append, ms_paged_attention and ms_logits_process: these calls are
+asynchronous on the library's own stream, so results are read, and inputs changed, behind
+mojostream_amd.synchronize() or a device-wide wait.
 """
 import ctypes
 import math
@@ -279,6 +281,7 @@ def _logits_plain(st):
 def _handles(st):
     import mojostream_amd as ms
     ms.init(0)
+    torch.cuda.synchronize()  # the library's stream does not wait for torch's, which fills the inputs
     c = st["case"]
     st["ms"] = ms
     if c["kind"] == "logits":
