@@ -1067,7 +1067,7 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
   // (by the tiles that the longest span has: a sliding window's are the same at every position)
   // (an even share of more than the longest span: nothing is cut; unbounded it passes 32 bits)
   const int64_t fill = std::min<int64_t>(longest, std::max((work * p->n_kv + blocks - 1) / blocks,
-                                                           ((int64_t)most_tiles * 4 + kMaxParts) / kMaxParts));
+                                                           ((int64_t)most_tiles * 4 + kMaxParts - 1) / kMaxParts));
   int per = (int)((fill + 3) / 4 * 4);
   int64_t best = INT64_MAX;
   for (int64_t c = per;; c += std::max<int64_t>(4, c / 8 / 4 * 4)) {
