@@ -309,14 +309,15 @@ __device__ __forceinline__ void load_q(const float *qp, bool real, float scale,
       for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[ks][j >> 2][j & 3]));
     lift_of(max_groups(big), &up, down);
   }
-  up *= scale;
+  // (a factor of 0 in place of a choice for each value: an item beside a row whose q is not finite may
+  // then be done again key by key)
+  up = real ? up * scale : 0.f;
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     uint32_t p[QP][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      split2<F16, QP>(real ? x[ks][j >> 1][2 * (j & 1)] * up : 0.f,
-                      real ? x[ks][j >> 1][2 * (j & 1) + 1] * up : 0.f, &p[0][j], 4);
+      split2<F16, QP>(x[ks][j >> 1][2 * (j & 1)] * up, x[ks][j >> 1][2 * (j & 1) + 1] * up, &p[0][j], 4);
 #pragma unroll
     for (int i = 0; i < QP; ++i) q[ks][i] = u4{p[i][0], p[i][1], p[i][2], p[i][3]};
   }
