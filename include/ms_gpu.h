@@ -291,7 +291,9 @@ int ms_paged_append(const ms_paged_layer *layer, const ms_paged_batch *b, const 
  * not overlap.  The row at position p attends to positions max(0, p - window +
  * 1) .. p.  Products take q times the scale (rounded once to fp32), the
  * probabilities and the pools' values with all their bits (over fp16 pools 22
- * bits of q and of the probabilities), sums are fp32.  Slots outside the attended positions are never
+ * bits of q and of the probabilities, of these nothing below 2^-32 of a row's
+ * largest).  Sums are fp32 and divided at the end: n positions of values past 2^128 / n
+ * may overflow.  Slots outside the attended positions are never
  * used, whatever they hold; a value that is not finite reaches only the rows
  * that attend to it.  Rows behind the last sequence's are left as they were. */
 int ms_paged_attention(const ms_paged_layer *layer, ms_paged_batch *b, const float *d_q,

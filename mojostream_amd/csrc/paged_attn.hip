@@ -11,8 +11,9 @@
 //                 dims, 5.1 TB/s, 2 of 512 dims, 5.6 TB/s (a large copy: 4.6 TB/s).
 //  k_paged_block  longer chunks, and single tokens beside them (item_by_block, item_by_tile).
 //                 Bound by the matrix cores: 4096 rows over 16384 keys, 14B class, bf16 (three
-//                 products a multiplication): 2.7 to 2.9 ms, 1.3 PFLOP/s of bf16 products, MFMA
-//                 busy 56% of the time at 2.1 GHz (a large bf16 matrix product: 1.2 PFLOP/s).
+//                 products a multiplication): 2.7 to 2.9 ms among other calls (2.9 to 3.1 in ten
+//                 passes under the profiler), 1.3 PFLOP/s of bf16 products, MFMA busy 56% of the time
+//                 at 2.1 GHz (a large bf16 matrix product: 1.2 PFLOP/s).
 //  k_paged_merge  the spans' results.
 #include <algorithm>
 #include <cmath>
@@ -323,8 +324,8 @@ __device__ __forceinline__ void load_q(const float *qp, bool real, float scale,
   }
 }
 
-// Waves that share a tile in item_by_tile: 128 dims each at most, so that a wave's whole tile is
-// in flight at once.
+// Waves that share a tile in item_by_tile: 128 dims each at most, so that a wave's registers hold its
+// whole tile.
 template <int HD>
 constexpr int tile_split() {
   return HD <= 128 ? 1 : HD / 128;
@@ -382,7 +383,9 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   const char *vb0 = static_cast<const char *>(a.v) + ((size_t)kvh * HD + HW * part + VD * c16) * ES;
   // The next tile's keys are loaded once this one's are multiplied, its values once these are, where
   // there are registers for it (not for fp32 pools and one query tile: 160 us with spills, 118 us with
-  // both loaded as the tile begins; 32 tokens over 4096 keys, 8 kv heads of 128 dims).
+  // the tile's own loads in it; 32 tokens over 4096 keys, 8 kv heads of 128 dims).  Of those the compiler
+  // issues four of a tile's keys at a time, between the products, and most of the values behind them:
+  // where a block has one tile that chain is most of its time.
   constexpr bool AHEAD = F16 ? NQ == 1 : ES == 2 || NQ == 2;
   u4 kr[2][KS][ES / 2], vr[8][NC];
   auto load_k = [&](int row) {
@@ -656,7 +659,8 @@ struct Shape {
 // registers; the waves read both without bank conflicts.  (item_by_tile's loads of K take 16
 // bytes of 16 rows a quarter wave, sixteen cache accesses where a row's take one or two; with
 // many queries these accesses bound it.)  The next tile's rows are loaded beside the second
-// product of this one and wait in registers.  Where a group has several waves each computes the scores over
+// product of this one and wait in registers; where its pages lie the first wave finds before its own
+// first product, a load that it waits for.  Where a group has several waves each computes the scores over
 // its dims, and all take the sum, in the same order.
 template <int HD, int DT>
 __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const PagedItem &it, int kvh,
