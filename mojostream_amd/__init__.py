@@ -353,6 +353,21 @@ def _ptr(b):
     return b.ptr if b is not None else None
 
 
+def _int32(x, what: str):
+    """x as an int32 array of the same numbers."""
+    a = np.asarray(x)
+    if a.dtype == np.int32:
+        return a
+    try:
+        with np.errstate(invalid="ignore"):
+            b = a.astype(np.int32)
+    except (OverflowError, TypeError, ValueError):
+        b = None
+    if b is None or not np.array_equal(a, b):
+        raise MSError(f"{what}: a number is not a 32-bit integer")
+    return b
+
+
 class PagedBatch:
     """Owner of an ms_paged_batch handle: a step's sequences and their page tables, for
     every layer's paged_append and paged_attention."""
@@ -369,9 +384,8 @@ class PagedBatch:
     def set(self, new: Sequence[int], length: Sequence[int], pages) -> None:
         """new[s] new rows of length[s] positions in all; pages [n_seqs][at most max_pages]
         (-1: no page)."""
-        n = np.ascontiguousarray(new, dtype=np.int32)
-        l = np.ascontiguousarray(length, dtype=np.int32)
-        p = np.asarray(pages, dtype=np.int32)
+        n, l = (np.ascontiguousarray(_int32(x, "PagedBatch.set")) for x in (new, length))
+        p = _int32(pages, "PagedBatch.set")
         if n.ndim != 1 or l.shape != n.shape or p.ndim != 2 or p.shape[0] != n.size or \
                 p.shape[1] > self.max_pages:
             raise MSError("PagedBatch.set: shapes do not fit")

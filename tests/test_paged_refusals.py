@@ -83,6 +83,15 @@ def test_batch_null(batch):
         batch.set([1], [1, 2], np.zeros((1, 5), np.int32))
 
 
+@pytest.mark.parametrize("new,length,pages", [
+    ([1], [1], [[2 ** 32 + 3]]), ([2 ** 32 + 1], [2 ** 32 + 1], [[3]]), ([1], [2 ** 32 + 1], [[3]]),
+    ([1], [1], [[1.5]]), ([0.5], [1], [[3]]), ([1], [float("nan")], [[3]]), ([1], [2 ** 70], [[3]])])
+def test_set_takes_int32_values(batch, new, length, pages):
+    """Numbers that 32 bits do not hold are refused, not wrapped to others."""
+    with pytest.raises(ms.MSError, match="32-bit"):
+        batch.set(np.array(new), np.array(length), np.array(pages))
+
+
 GOOD = dict(n_heads=8, n_kv_heads=2, head_dim=64, rot_dim=64, window=0, dtype=0, page_rows=0, scale=0.0,
             k=4096, v=8192)
 
