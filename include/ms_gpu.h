@@ -299,6 +299,48 @@ int ms_paged_append(const ms_paged_layer *layer, const ms_paged_batch *b, const 
 int ms_paged_attention(const ms_paged_layer *layer, ms_paged_batch *b, const float *d_q,
                        size_t q_stride, float *d_out, size_t out_stride);
 
+/* ---- paged KV cache: 8-bit pools, normed heads, capped scores --------------- */
+/* No reference counterpart.  What ms_paged_layer has no place for, for the calls
+ * named _ext below, which otherwise are ms_paged_append and ms_paged_attention. */
+#define MS_KV_E4M3 4 /* base.dtype: 8-bit floats of 4 exponent and 3 mantissa bits, to 448, no infinities */
+#define MS_KV_I8 5   /* 8-bit integers, -127 to 127 */
+#define MS_NORM_Q 1
+#define MS_NORM_K 2
+#define MS_NORM_V 4
+#define MS_ROPE_HALVES 0 /* dims i and i + rot_dim/2 turn together */
+#define MS_ROPE_PAIRS 1  /* dims 2i and 2i + 1 do */
+typedef struct {
+  ms_paged_layer base;
+  /* 8-bit pools: a head's values at a position are its codes times one fp32 scale, that of page p,
+   * kv head h and slot s at k_scale[(p * n_kv_heads + h) * page_rows + s] (page_rows 0: page_size);
+   * unused otherwise. */
+  float *k_scale, *v_scale;
+  float score_cap;  /* attention: a score s becomes score_cap * tanh(s / score_cap); 0: none; else 2^-60 to 2^60 */
+  int norm;         /* append: MS_NORM_*, whose heads are normed before they are rotated; 0: none */
+  float norm_eps;   /* x / sqrt(mean of a head's x^2 + norm_eps) * gamma */
+  const float *q_gamma, *k_gamma; /* device, [head_dim]; NULL: 1 (v has none) */
+  int rope;         /* append: MS_ROPE_* */
+} ms_paged_layer_ext;
+/* ms_paged_append with norms, either rotation and 8-bit pools.  An 8-bit head's scale is its largest
+ * magnitude by 448 (MS_KV_I8: by 127), rounded to fp32, at least 2^-126 (and so that the largest code times it is finite), and its codes are the nearest to value / scale,
+ * even where two are as near.  A head that holds a value that is not finite gets NaN as its scale, so that
+ * every value of it is NaN.  The squares are summed in 64 bits. */
+int ms_paged_append_ext(const ms_paged_layer_ext *layer, const ms_paged_batch *b, const float *d_k,
+                        const float *d_v, size_t kv_stride, const float *d_q, size_t q_stride,
+                        float *d_q_out, size_t q_out_stride, const float *d_cos,
+                        const float *d_sin, int n_pos);
+/* ms_paged_attention over any of the pools, with capped scores or not.  Over 8-bit pools the products take
+ * the codes with all their bits, 22 bits of q times the scale of the scores (of these nothing below 2^-32 of a row's largest),
+ * and the probabilities times the values' scales with all theirs.  A cap holds for infinite scores too. */
+int ms_paged_attention_ext(const ms_paged_layer_ext *layer, ms_paged_batch *b, const float *d_q,
+                           size_t q_stride, float *d_out, size_t out_stride);
+/* Positions pos0 .. pos0 + n - 1 of sequence seq out of the pages (any pool), in fp32: position
+ * pos0 + r's n_kv_heads * head_dim values at d_k + r * stride and d_v + r * stride (in floats, a
+ * multiple of 4; pointers 16-byte aligned; either may be NULL; the two must not overlap).  Only
+ * positions of the sequence whose page was not freed. */
+int ms_paged_read(const ms_paged_layer_ext *layer, const ms_paged_batch *b, int seq, int pos0, int n,
+                  float *d_k, float *d_v, size_t stride);
+
 /* ---- logits: penalties, biases, grammar masks ------------------------------- */
 /* One row of ms_logits_process. */
 typedef struct {
@@ -327,6 +369,30 @@ int ms_logits_process(const float *d_logits, size_t in_stride, float *d_out, siz
                       int rows, int vocab, const ms_logits_row *h_rows,
                       const int32_t *d_history, size_t n_history, const int32_t *d_bias_ids,
                       const float *d_bias, size_t n_bias, const uint32_t *d_masks, int n_masks);
+/* One row of ms_sample_rows. */
+typedef struct {
+  float temperature; /* 0: the best id */
+  int32_t top_k;     /* 0: all */
+  float top_p;       /* 0 to 1; 1: all */
+  float min_p;       /* 0 to 1; 0: all */
+} ms_sample_row;
+/* A token id for each row of logits, beside ms_sample (the reference's: one row, temperature alone,
+ * an id that comes back to the host).  Id i weighs w_i = e^((x_i - max) / temperature).  In order of falling
+ * logits, the lower id first among equals,
+ *   top_k   leaves the first top_k ids,
+ *   top_p   the fewest of these, from the first, that weigh at least top_p of them,
+ *   min_p   those of w_i >= min_p;
+ * the first id always stays.  The draw is the first id, in order of ids, at which the running weight of
+ * what is left passes d_u[row] times the whole (d_u: 0 <= u < 1; anything below counts as 0, NaN too, anything
+ * above leaves the last id).  Weights are 64-bit, rounded to whole multiples of 2^-63 times the vocabulary
+ * (rounded up to a power of two) before they are added: sums are exact and the same whatever their order.  An id
+ * of logit -infinity or NaN is never drawn; a row without any other has id -1, probability 0, none kept.
+ * d_logits rows of in_stride floats are only read; d_ids [rows]; d_prob (may be NULL): the id's weight by that of
+ * what is left; d_kept (may be NULL): how many ids were left.  h_rows is read before the call returns.
+ * Asynchronous on the library's stream. */
+int ms_sample_rows(const float *d_logits, size_t in_stride, int rows, int vocab,
+                   const ms_sample_row *h_rows, const float *d_u, int32_t *d_ids, float *d_prob,
+                   int32_t *d_kept);
 
 /* ---- tokenizers (host only, no device use) ----------------------------------
  * Strings are byte strings: the reference builds its text from chr(byte), so

@@ -24,6 +24,11 @@ MS_CACHE_CIRCULAR = 1
 MS_KV_F32 = 0
 MS_KV_BF16 = 1
 MS_KV_F16 = 2
+MS_KV_E4M3 = 4
+MS_KV_I8 = 5
+MS_NORM_Q, MS_NORM_K, MS_NORM_V = 1, 2, 4
+MS_ROPE_HALVES = 0
+MS_ROPE_PAIRS = 1
 MAT_NAMES = ("Q", "K", "V", "O", "Gate", "Up", "Down")
 
 
@@ -109,6 +114,22 @@ class LogitsRow(C.Structure):
                          n_bias, mask)
 
 
+class PagedLayerExt(C.Structure):
+    """ms_paged_layer_ext: a layer with 8-bit pools, normed heads or capped scores."""
+    _fields_ = [("base", PagedLayer), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("score_cap", C.c_float), ("norm", C.c_int), ("norm_eps", C.c_float),
+                ("q_gamma", C.c_void_p), ("k_gamma", C.c_void_p), ("rope", C.c_int)]
+
+
+class SampleRow(C.Structure):
+    """ms_sample_row: one row's temperature, top-k, top-p and min-p."""
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float),
+                ("min_p", C.c_float)]
+
+    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        super().__init__(temperature, top_k, top_p, min_p)
+
+
 _P = C.c_void_p
 _I = C.c_int
 _SZ = C.c_size_t
@@ -145,6 +166,10 @@ _SIGS = {
     "ms_paged_attention": [C.POINTER(PagedLayer), _P, _P, _SZ, _P, _SZ],
     "ms_logits_process": [_P, _SZ, _P, _SZ, _I, _I, C.POINTER(LogitsRow), _P, _SZ, _P, _P, _SZ,
                           _P, _I],
+    "ms_paged_append_ext": [C.POINTER(PagedLayerExt), _P, _P, _P, _SZ, _P, _SZ, _P, _SZ, _P, _P, _I],
+    "ms_paged_attention_ext": [C.POINTER(PagedLayerExt), _P, _P, _SZ, _P, _SZ],
+    "ms_paged_read": [C.POINTER(PagedLayerExt), _P, _I, _I, _I, _P, _P, _SZ],
+    "ms_sample_rows": [_P, _SZ, _I, _I, C.POINTER(SampleRow), _P, _P, _P, _P],
     "ms_model_create": [C.POINTER(ModelDesc), C.POINTER(LayerDesc), C.POINTER(C.c_void_p)],
     "ms_model_destroy": [_P],
     "ms_model_set_matrix": [_P, _I, _I, _P, _I, _F],
@@ -415,20 +440,29 @@ def rope_table(rot_dim: int, theta: float, n_pos: int, pos0: int = 0, wide: bool
     return c, s
 
 
-def paged_append(layer: PagedLayer, batch: PagedBatch, k, v, kv_stride: int, q=None,
+def paged_append(layer, batch: PagedBatch, k, v, kv_stride: int, q=None,
                  q_stride: int = 0, q_out=None, q_out_stride: int = 0, cos=None, sin=None,
                  n_pos: int = 0) -> None:
     """The batch's new k (rotated) and v rows into their pages, q rotated to q_out
-    (ms_paged_append; buffers are objects with a device address `ptr`)."""
-    check(_lib.ms_paged_append(C.byref(layer), batch.h, _ptr(k), _ptr(v), kv_stride, _ptr(q),
-                               q_stride, _ptr(q_out), q_out_stride, _ptr(cos), _ptr(sin), n_pos))
+    (ms_paged_append; of a PagedLayerExt ms_paged_append_ext, which norms heads and writes
+    8-bit pools too; buffers are objects with a device address `ptr`)."""
+    f = _lib.ms_paged_append_ext if isinstance(layer, PagedLayerExt) else _lib.ms_paged_append
+    check(f(C.byref(layer), batch.h, _ptr(k), _ptr(v), kv_stride, _ptr(q), q_stride, _ptr(q_out),
+            q_out_stride, _ptr(cos), _ptr(sin), n_pos))
 
 
-def paged_attention(layer: PagedLayer, batch: PagedBatch, q, q_stride: int, out,
-                    out_stride: int) -> None:
-    """Causal attention of the batch's rows over the pages (ms_paged_attention)."""
-    check(_lib.ms_paged_attention(C.byref(layer), batch.h, _ptr(q), q_stride, _ptr(out),
-                                  out_stride))
+def paged_attention(layer, batch: PagedBatch, q, q_stride: int, out, out_stride: int) -> None:
+    """Causal attention of the batch's rows over the pages (ms_paged_attention; of a
+    PagedLayerExt ms_paged_attention_ext: 8-bit pools, capped scores)."""
+    f = _lib.ms_paged_attention_ext if isinstance(layer, PagedLayerExt) else _lib.ms_paged_attention
+    check(f(C.byref(layer), batch.h, _ptr(q), q_stride, _ptr(out), out_stride))
+
+
+def paged_read(layer: PagedLayerExt, batch: PagedBatch, seq: int, pos0: int, n: int, k, v,
+               stride: int) -> None:
+    """n positions of a sequence's keys and values out of the pages, in fp32 (ms_paged_read; k
+    or v None: not read)."""
+    check(_lib.ms_paged_read(C.byref(layer), batch.h, seq, pos0, n, _ptr(k), _ptr(v), stride))
 
 
 def logits_process(logits, in_stride: int, out, out_stride: int, vocab: int,
@@ -439,6 +473,15 @@ def logits_process(logits, in_stride: int, out, out_stride: int, vocab: int,
     check(_lib.ms_logits_process(_ptr(logits), in_stride, _ptr(out), out_stride, len(rows), vocab,
                                  arr, _ptr(history), n_history, _ptr(bias_ids), _ptr(bias),
                                  n_bias, _ptr(masks), n_masks))
+
+
+def sample_rows(logits, in_stride: int, vocab: int, rows: Sequence[SampleRow], u, ids, prob=None,
+                kept=None) -> None:
+    """A token id for each logits row by temperature, top-k, top-p and min-p from the random
+    numbers u, on the device (ms_sample_rows)."""
+    arr = (SampleRow * max(len(rows), 1))(*rows)
+    check(_lib.ms_sample_rows(_ptr(logits), in_stride, len(rows), vocab, arr, _ptr(u), _ptr(ids),
+                              _ptr(prob), _ptr(kept)))
 
 
 # ---- architecture presets -------------------------------------------------------

@@ -97,8 +97,35 @@ __device__ inline uint32_t div_by(uint32_t n, FastDiv f) {
   return (uint32_t)(((uint64_t)n * f.mul) >> 31 >> f.shift);
 }
 
+typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+
+// One or four values of a pool, rounded to nearest even.
+template <int DT, class V>
+__device__ inline void store_kv(void *pool, size_t at, V x) {
+  constexpr bool ONE = sizeof(V) == 4;
+  if constexpr (DT == MS_KV_F32)
+    *reinterpret_cast<V *>(static_cast<float *>(pool) + at) = x;
+  else if constexpr (DT == MS_KV_BF16 && ONE)
+    static_cast<__bf16 *>(pool)[at] = (__bf16)x;
+  else if constexpr (DT == MS_KV_BF16)
+    *reinterpret_cast<bf4 *>(static_cast<__bf16 *>(pool) + at) = __builtin_convertvector(x, bf4);
+  else if constexpr (ONE)
+    static_cast<_Float16 *>(pool)[at] = (_Float16)x;
+  else
+    *reinterpret_cast<half4_t *>(static_cast<_Float16 *>(pool) + at) = __builtin_convertvector(x, half4_t);
+}
+
 // The layer's shape and pools, and that they fit the batch.
 int paged_check(const char *what, const ms_paged_layer *L, const ms_paged_batch *b);
+// The same of a layer that may have 8-bit pools.
+int paged_check_ext(const char *what, const ms_paged_layer_ext *L, const ms_paged_batch *b);
+// The arguments of ms_paged_append, or with X those that ms_paged_append_ext has too.
+int append_check(const char *what, const ms_paged_layer *L, const ms_paged_layer_ext *X,
+                 const ms_paged_batch *b, const float *d_k, const float *d_v, size_t kv_stride,
+                 const float *d_q, size_t q_stride, const float *d_q_out, size_t q_out_stride,
+                 const float *d_cos, const float *d_sin, int n_pos);
+inline bool is_8bit(int dtype) { return dtype == MS_KV_E4M3 || dtype == MS_KV_I8; }
 inline int page_rows(const ms_paged_layer *L, const ms_paged_batch *b) {
   return L->page_rows ? L->page_rows : b->page_size;
 }

@@ -46,7 +46,9 @@ void Upload::release() {
   cap = 0;
 }
 
-int paged_check(const char *what, const ms_paged_layer *L, const ms_paged_batch *b) {
+namespace {
+
+int check(const char *what, const ms_paged_layer *L, const ms_paged_batch *b, bool eight) {
   auto w = [what](const char *msg) { return std::string(what) + msg; };
   MS_CHECK_ARG(L && b, w(": null layer or batch"));
   MS_CHECK_ARG(L->n_kv_heads >= 1 && L->n_heads >= 1 && L->n_heads % L->n_kv_heads == 0,
@@ -55,7 +57,8 @@ int paged_check(const char *what, const ms_paged_layer *L, const ms_paged_batch 
   MS_CHECK_ARG(L->head_dim == 64 || L->head_dim == 128 || L->head_dim == 256 ||
                    L->head_dim == 512,
                w(": head_dim must be 64, 128, 256 or 512"));
-  MS_CHECK_ARG(L->dtype == MS_KV_F32 || L->dtype == MS_KV_BF16 || L->dtype == MS_KV_F16,
+  MS_CHECK_ARG(L->dtype == MS_KV_F32 || L->dtype == MS_KV_BF16 || L->dtype == MS_KV_F16 ||
+                   (eight && is_8bit(L->dtype)),
                w(": unknown pool type"));
   MS_CHECK_ARG(L->window >= 0, w(": negative window"));
   MS_CHECK_ARG(L->page_rows == 0 || L->page_rows >= b->page_size,
@@ -67,6 +70,22 @@ int paged_check(const char *what, const ms_paged_layer *L, const ms_paged_batch 
                w(": the pools must be 16-byte aligned"));
   MS_CHECK_ARG(b->set, w(": the batch was not set"));
   return MS_OK;
+}
+
+}  // namespace
+
+int paged_check(const char *what, const ms_paged_layer *L, const ms_paged_batch *b) {
+  return check(what, L, b, false);
+}
+
+int paged_check_ext(const char *what, const ms_paged_layer_ext *L, const ms_paged_batch *b) {
+  MS_CHECK_ARG(L && b, std::string(what) + ": null layer or batch");
+  if (is_8bit(L->base.dtype)) {
+    MS_CHECK_ARG(L->k_scale && L->v_scale, std::string(what) + ": an 8-bit pool has scales");
+    MS_CHECK_ARG(((reinterpret_cast<uintptr_t>(L->k_scale) | reinterpret_cast<uintptr_t>(L->v_scale)) & 3) == 0,
+                 std::string(what) + ": the scales must be 4-byte aligned");
+  }
+  return check(what, &L->base, b, true);
 }
 
 bool rows_overlap(const void *a, size_t stride_a, int na, const void *b, size_t stride_b, int nb,
@@ -108,25 +127,6 @@ struct AppendArgs {
   long total;
   FastDiv by_row;  // total < 2^31
 };
-
-typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
-typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
-
-// One or four values of a pool, rounded to nearest even.
-template <int DT, class V>
-__device__ inline void store_kv(void *pool, size_t at, V x) {
-  constexpr bool ONE = sizeof(V) == 4;
-  if constexpr (DT == MS_KV_F32)
-    *reinterpret_cast<V *>(static_cast<float *>(pool) + at) = x;
-  else if constexpr (DT == MS_KV_BF16 && ONE)
-    static_cast<__bf16 *>(pool)[at] = (__bf16)x;
-  else if constexpr (DT == MS_KV_BF16)
-    *reinterpret_cast<bf4 *>(static_cast<__bf16 *>(pool) + at) = __builtin_convertvector(x, bf4);
-  else if constexpr (ONE)
-    static_cast<_Float16 *>(pool)[at] = (_Float16)x;
-  else
-    *reinterpret_cast<half4_t *>(static_cast<_Float16 *>(pool) + at) = __builtin_convertvector(x, half4_t);
-}
 
 // A thread takes N values and the N that turn with them (or 2 N side by side that do not turn) of
 // one head of a row: q heads, k heads, v heads.  Bound by memory: 3001 rows of 40 + 8 + 8 heads
@@ -329,35 +329,50 @@ extern "C" int ms_rope_table(float *d_cos, float *d_sin, int rot_dim, float thet
   return MS_OK;
 }
 
-extern "C" int ms_paged_append(const ms_paged_layer *L, const ms_paged_batch *b, const float *d_k,
-                               const float *d_v, size_t kv_stride, const float *d_q,
-                               size_t q_stride, float *d_q_out, size_t q_out_stride,
-                               const float *d_cos, const float *d_sin, int n_pos) {
-  MS_CHECK_ARG(L, "paged_append: null layer or batch");
+namespace ms {
+
+int append_check(const char *what, const ms_paged_layer *L, const ms_paged_layer_ext *X,
+                 const ms_paged_batch *b, const float *d_k, const float *d_v, size_t kv_stride,
+                 const float *d_q, size_t q_stride, const float *d_q_out, size_t q_out_stride,
+                 const float *d_cos, const float *d_sin, int n_pos) {
+  auto w = [what](const char *msg) { return std::string(what) + msg; };
+  MS_CHECK_ARG(L, w(": null layer or batch"));
   MS_CHECK_ARG(L->rot_dim >= 0 && L->rot_dim % 2 == 0 && L->rot_dim <= L->head_dim,
-               "paged_append: rot_dim must be even and at most head_dim");
-  MS_CHECK_ARG(L->rot_dim == 0 || (d_cos && d_sin), "paged_append: rotary tables missing");
-  if (int rc = paged_check("paged_append", L, b)) return rc;
+               w(": rot_dim must be even and at most head_dim"));
+  MS_CHECK_ARG(L->rot_dim == 0 || (d_cos && d_sin), w(": rotary tables missing"));
+  if (int rc = X ? paged_check_ext(what, X, b) : paged_check(what, L, b)) return rc;
   const int kv_dim = L->n_kv_heads * L->head_dim, q_dim = L->n_heads * L->head_dim;
-  MS_CHECK_ARG(L->rot_dim == 0 || b->max_pos <= n_pos,
-               "paged_append: a position past the rotary tables");
-  if (b->rows == 0) return require_init();
+  MS_CHECK_ARG(L->rot_dim == 0 || b->max_pos <= n_pos, w(": a position past the rotary tables"));
+  if (b->rows == 0) return MS_OK;
   MS_CHECK_ARG(d_k && d_v && aligned16(d_k) && aligned16(d_v) && kv_stride % 4 == 0 &&
                    kv_stride >= (size_t)kv_dim && kv_stride < ((size_t)1 << 31),
-               "paged_append: bad k or v rows");
+               w(": bad k or v rows"));
   if (d_q) {
     MS_CHECK_ARG(d_q_out && aligned16(d_q) && aligned16(d_q_out) && q_stride % 4 == 0 &&
                      q_out_stride % 4 == 0 && q_stride >= (size_t)q_dim &&
                      q_out_stride >= (size_t)q_dim && q_stride < ((size_t)1 << 31) &&
                      q_out_stride < ((size_t)1 << 31),
-                 "paged_append: bad q rows");
+                 w(": bad q rows"));
     MS_CHECK_ARG((d_q_out == d_q && q_out_stride == q_stride) ||
                      !rows_overlap(d_q, q_stride, q_dim, d_q_out, q_out_stride, q_dim, b->rows),
-                 "paged_append: d_q and d_q_out overlap");
+                 w(": d_q and d_q_out overlap"));
     MS_CHECK_ARG(!rows_overlap(d_k, kv_stride, kv_dim, d_q_out, q_out_stride, q_dim, b->rows) &&
                      !rows_overlap(d_v, kv_stride, kv_dim, d_q_out, q_out_stride, q_dim, b->rows),
-                 "paged_append: d_q_out overlaps the k or v rows");
+                 w(": d_q_out overlaps the k or v rows"));
   }
+  return MS_OK;
+}
+
+}  // namespace ms
+
+extern "C" int ms_paged_append(const ms_paged_layer *L, const ms_paged_batch *b, const float *d_k,
+                               const float *d_v, size_t kv_stride, const float *d_q,
+                               size_t q_stride, float *d_q_out, size_t q_out_stride,
+                               const float *d_cos, const float *d_sin, int n_pos) {
+  if (int rc = append_check("paged_append", L, nullptr, b, d_k, d_v, kv_stride, d_q, q_stride, d_q_out,
+                            q_out_stride, d_cos, d_sin, n_pos))
+    return rc;
+  if (b->rows == 0) return require_init();
   AppendArgs a{};
   a.rows = b->d_rows();
   a.q = d_q;
