@@ -14,7 +14,7 @@ def say(msg):
 
 def weights(x, temperature, n):
     """Whole weights of logits x (64 bits, the largest first)."""
-    s = 63 - (n - 1).bit_length()
+    s = min(49, 63 - (n - 1).bit_length())
     with np.errstate(invalid="ignore", over="ignore"):
         w = np.where(x == x[0], 1.0, np.exp((x - x[0]) / np.float64(np.float32(temperature))))
     return w, [int(v) for v in np.rint(np.ldexp(w, s))]
@@ -70,7 +70,7 @@ def draw(ms, x, rows, u, pad=0, prob=True, kept=True):
 
 def check(ms, x, settings, u, pad=0):
     """All rows; ids and counts are those of the definition, probabilities to fp32's rounding and what the weights'
-    (2^-45 of the largest, at 2^18 ids) and exp's own leave."""
+    (2^-44 of the largest, at 2^18 ids) and exp's own leave."""
     rows = [ms.SampleRow(**s) for s in settings]
     ids, kept, prob = draw(ms, x, rows, u, pad)
     far = 0
