@@ -21,13 +21,13 @@
 namespace ms {
 namespace {
 
-constexpr int kRows = 128;      // rows of a launch: their settings are kernel arguments
+constexpr int kRows = 64;       // rows of a launch: their settings are kernel arguments
 constexpr int kNT = 1024;
-constexpr int kBins = 2048;     // buckets of a slice's histogram; the last takes what lies below
+constexpr int kBins = 2048;     // buckets of a slice's histogram, in 64 groups of 32
 constexpr int kList = 8192;     // candidates of a row
 constexpr int kMostK = 2048;    // the largest top-k by the list
-constexpr int kPer = 16;        // logits of a thread; a wave's 1024 are a chunk
 constexpr int kMostSlices = 64;
+constexpr int kWave = 256;      // candidates that one wave goes through alone
 constexpr int kSliceBits = 49;  // S of a slice of up to 2^14 logits; S of a row is at most that
 
 struct RowInfo {
@@ -35,6 +35,14 @@ struct RowInfo {
   int ref;                   // weights are 2^(x log2(e) / T - ref)
   float top;                 // the largest logit
   unsigned long long want;   // top-p: weight still to be reached within the bucket
+};
+// A row's settings.
+struct RowSet {
+  double c;         // log2(e) / T; T = 0: 0
+  double log_min;   // log2(min_p)
+  float grain;      // buckets by weight: 32 of an octave
+  float temperature, top_p, min_p;
+  int k;            // ids that top-k leaves; 0: all
 };
 enum { kNone, kBest, kSum, kSlow };  // nothing to draw; by the list; by sums (and the list); digit by digit
 
@@ -48,15 +56,15 @@ struct SampleRowsArgs {
   float *prob;
   // workspace
   unsigned long long *hist;  // [row][slice][kBins], top-k: uint32
-  unsigned long long *sum;   // [row][slice]: its whole weight
+  unsigned long long *coarse;  // [row][slice][64]: of each group of buckets
   float *top;                // [row][slice]
   uint32_t *real;            // [row][slice]: logits that can be drawn
   RowInfo *info;
   uint32_t *n_list;          // [row]
   unsigned long long *list;  // [row][kList]
-  unsigned long long *chunk; // [row][slices * slice / 1024]
+  unsigned long long *chunk; // [row][slices * 16]: of a wave's part of a slice
   uint32_t *chunk_n;
-  ms_sample_row rows[kRows];
+  RowSet rows[kRows];
 };
 
 // Logits as unsigned numbers of the same order; -infinity and NaN, which are never drawn, as 0.
@@ -65,6 +73,25 @@ __device__ inline uint32_t key_of(float x) {
   return !(x > -INFINITY) ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ inline float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+
+// 2^(j/64)
+__device__ const double kExp2[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
 // 2^t as a whole number of 2^-bits, bits <= 51: 2^(j/64) from a table, a polynomial of degree 5 over a 64th of an octave
 // (its remainder is below 2^-54).
@@ -87,20 +114,10 @@ struct Exp2 {
 __device__ inline unsigned long long weight_of(const Exp2 &exp2, float x, double c, int ref, int bits) {
   return exp2(__builtin_fma((double)x, c, (double)-ref), bits);
 }
-// log2 of the least share, T and the largest logit in it, that min_p leaves
-__device__ inline double least_of(float top, double c, float min_p) {
-  return min_p > 0.f ? __builtin_fma((double)top, c, log2((double)min_p)) : -INFINITY;
-}
 __device__ inline void exp2_table(double *t) {
-  if (threadIdx.x < 64) t[threadIdx.x] = exp2(threadIdx.x / 64.0);
+  if (threadIdx.x < 64) t[threadIdx.x] = kExp2[threadIdx.x];
 }
 
-// How a row is done.
-__device__ inline int best_of(const ms_sample_row &s, int n) {  // ids that top-k leaves; 0: all
-  return s.temperature == 0.f ? 1 : s.top_k > 0 && s.top_k < n ? s.top_k : 0;
-}
-__device__ inline bool by_sums(const ms_sample_row &s, int n) { return best_of(s, n) == 0; }
-__device__ inline float grain(const ms_sample_row &s) { return 32.f * 1.44269504f / s.temperature; }
 constexpr float kMostGrain = 0x1p60f;
 // A logit's bucket, in the order of logits.  Top-k: the exponent and eight bits of the mantissa, whatever
 // the logits' size; sums: 1/32 of an octave of the weights.
@@ -108,11 +125,11 @@ __device__ inline int bucket_of(float x, bool sums, float grain) {
   return sums ? (int)fminf(fmaxf(floorf(x * grain), -0x1p29f), 0x1p29f) : (int)(key_of(x) >> 15);
 }
 
-template <bool VEC>
-__device__ inline void load_chunk(const float *x, int n, int at, float (&v)[kPer]) {
+template <int PER, bool VEC>
+__device__ inline void load_chunk(const float *x, int n, int at, float (&v)[PER]) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int j = 0; j < kPer / 4; ++j) {
+  for (int j = 0; j < PER / 4; ++j) {
     const int i = at + 256 * j + 4 * lane;
     if (VEC && i + 3 < n) {
       const float4 y = ldg<float4>(x + i);
@@ -126,31 +143,34 @@ __device__ inline void load_chunk(const float *x, int n, int at, float (&v)[kPer
     }
   }
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) v[j] = v[j] > -INFINITY ? v[j] : -INFINITY;  // (NaN too)
+  for (int j = 0; j < PER; ++j) v[j] = v[j] > -INFINITY ? v[j] : -INFINITY;  // (NaN too)
 }
 
-template <int NT, bool VEC>
-__global__ __launch_bounds__(NT) void k_rows_scan(SampleRowsArgs a) {
+// A slice's buckets are counted from the top of its largest logit's group down: those of two slices
+// lie whole groups apart.
+__device__ inline int top_of(int bucket) { return bucket | 31; }
+
+// A thread has PER logits, a wave a chunk of 64 PER.
+template <int PER, bool VEC>
+__global__ __launch_bounds__(kNT) void k_rows_scan(SampleRowsArgs a) {
   __shared__ __align__(16) unsigned long long hist[kBins];
   __shared__ double table[64];
-  __shared__ float tops[NT / 64];
-  __shared__ uint32_t reals[NT / 64];
-  __shared__ unsigned long long sums[NT / 64];
+  __shared__ float tops[kNT / 64];
+  __shared__ uint32_t reals[kNT / 64];
   uint32_t *count = reinterpret_cast<uint32_t *>(hist);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y;
-  const ms_sample_row &set = a.rows[row];
-  const int k = best_of(set, a.n);
-  const bool sums_of = k == 0, bins = sums_of ? set.top_p < 1.f && grain(set) < kMostGrain : k <= kMostK;
-  float v[kPer];
-  load_chunk<VEC>(a.x + row * a.ld, a.n, blockIdx.x * a.slice + wave * 1024, v);
+  const RowSet &set = a.rows[row];
+  const bool sums = set.k == 0, bins = sums ? set.top_p < 1.f && set.grain < kMostGrain : set.k <= kMostK;
+  float v[PER];
+  load_chunk<PER, VEC>(a.x + row * a.ld, a.n, blockIdx.x * a.slice + wave * 64 * PER, v);
   if (bins) {
-    for (int i = tid; i < (sums_of ? kBins : kBins / 2); i += NT) hist[i] = 0;
+    for (int i = tid; i < (sums ? kBins : kBins / 2); i += kNT) hist[i] = 0;
     exp2_table(table);
   }
   float top = -INFINITY;
   uint32_t real = 0;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     top = fmaxf(top, v[j]);
     real += v[j] > -INFINITY;
   }
@@ -163,181 +183,242 @@ __global__ __launch_bounds__(NT) void k_rows_scan(SampleRowsArgs a) {
     reals[wave] = real;
   }
   __syncthreads();
-  real = 0;
+  top = tops[0];
 #pragma unroll
-  for (int w = 0; w < NT / 64; ++w) {
-    top = fmaxf(top, tops[w]);
-    real += reals[w];
-  }
+  for (int w = 1; w < kNT / 64; ++w) top = fmaxf(top, tops[w]);
   const size_t at = (size_t)row * a.slices + blockIdx.x;
   if (tid == 0) {
+    real = 0;
+    for (int w = 0; w < kNT / 64; ++w) real += reals[w];
     a.top[at] = top;
     a.real[at] = real;
     if (blockIdx.x == 0) a.n_list[row] = 0;
   }
-  if (!bins || real == 0 || top == INFINITY) return;
-  const float gr = grain(set);
-  const int g_top = bucket_of(top, sums_of, gr);
-  if (sums_of) {
+  if (!bins || !(top > -INFINITY && top < INFINITY)) return;
+  const int base = top_of(bucket_of(top, sums, set.grain));
+  if (sums) {
     const Exp2 exp2{table};
-    const double c = 1.4426950408889634 / (double)set.temperature;
-    const int ref = (g_top >> 5) + 1;
-    unsigned long long sum = 0;
+    const int ref = (base >> 5) + 1;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const unsigned long long w = weight_of(exp2, v[j], c, ref, kSliceBits);
-      if (w) atomicAdd(&hist[min(max(g_top - bucket_of(v[j], true, gr), 0), kBins - 1)], w);
-      sum += w;
+    for (int j = 0; j < PER; ++j) {
+      const unsigned long long w = weight_of(exp2, v[j], set.c, ref, kSliceBits);
+      if (w) atomicAdd(&hist[min(max(base - bucket_of(v[j], true, set.grain), 0), kBins - 1)], w);
     }
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) sums[wave] = sum;
   } else {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int d = g_top - bucket_of(v[j], false, gr);
-      if (d < kBins - 1) atomicAdd(&count[d], 1u);
+    for (int j = 0; j < PER; ++j) {
+      const int d = base - bucket_of(v[j], false, 0.f);
+      if (d < kBins) atomicAdd(&count[d], 1u);
     }
   }
   __syncthreads();
-  if (sums_of) {
-    for (int i = tid; i < kBins; i += NT) a.hist[at * kBins + i] = hist[i];
-    if (tid == 0) {
-      unsigned long long sum = 0;
-      for (int w = 0; w < NT / 64; ++w) sum += sums[w];
-      a.sum[at] = sum;
-    }
+  // two buckets a thread, a group 16 threads
+  unsigned long long two;
+  if (sums) {
+    const unsigned long long h0 = hist[2 * tid], h1 = hist[2 * tid + 1];
+    a.hist[at * kBins + 2 * tid] = h0;
+    a.hist[at * kBins + 2 * tid + 1] = h1;
+    two = h0 + h1;
   } else {
-    for (int i = tid; i < kBins / 2; i += NT) a.hist[at * kBins + i] = hist[i];
+    const unsigned long long h = hist[tid];
+    a.hist[at * kBins + tid] = h;
+    two = (h & 0xFFFFFFFFu) + (h >> 32);
   }
+  for (int o = 1; o < 16; o <<= 1) two += __shfl_xor(two, o, 64);
+  if ((tid & 15) == 0) a.coarse[at * 64 + tid / 16] = two;
 }
 
-template <int NT, bool VEC>
-__global__ __launch_bounds__(NT) void k_rows_pick(SampleRowsArgs a) {
-  constexpr int GR = NT / 256;
-  __shared__ double table[64];
-  __shared__ int g_of[kMostSlices];
-  __shared__ unsigned long long part[GR][256];
-  __shared__ unsigned long long wsum[4], found_before;
-  __shared__ int found;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y;
-  const ms_sample_row &set = a.rows[row];
-  const int k = best_of(set, a.n);
-  const bool sums = k == 0, cut = sums && set.top_p < 1.f;
-  const int id0 = blockIdx.x * a.slice + wave * 1024;
-  float v[kPer];
-  load_chunk<VEC>(a.x + row * a.ld, a.n, id0, v);
+__device__ inline unsigned long long scan_wave(unsigned long long v) {
+  const int lane = threadIdx.x & 63;
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned long long y = __shfl_up(v, o, 64);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
 
-  // ---- the row's maximum
-  const size_t at = (size_t)row * a.slices;
-  const float gr = grain(set);
-  float top = lane < a.slices ? ldg<float>(a.top + at + lane) : -INFINITY;
-  const float mine = top;
+__device__ inline unsigned long long share_of(float p, unsigned long long total) {
+  const unsigned long long t = (unsigned long long)ceil((double)p * (double)total);
+  return t ? t : 1;
+}
+
+struct CutLds {
+  unsigned long long part[kNT / 64][64];
+  unsigned long long goal, before;
+  int group;
+  RowInfo info;
+};
+
+// What a row's slices say: the state, and the bucket in which the cut lies.  Each wave adds up the buckets of its
+// share of the slices, the first wave looks for the cut in the sum: among the groups, then in the one it lies in.  (By
+// the first wave alone 11 us for 64 slices.)
+template <bool SUMS>
+__device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size_t at, CutLds &lds) {
+  constexpr int W = kNT / 64, Q = kMostSlices / W;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float mine = lane < a.slices ? ldg<float>(a.top + at + lane) : -INFINITY;
   uint32_t real = lane < a.slices ? ldg<uint32_t>(a.real + at + lane) : 0;
+  float top = mine;
   for (int o = 1; o < 64; o <<= 1) {
     top = fmaxf(top, __shfl_xor(top, o, 64));
     real += (uint32_t)__shfl_xor((int)real, o, 64);
   }
-  exp2_table(table);
-  // (a weight's bucket is a whole number that fp32 holds to a quarter)
-  int state = real == 0 ? kNone : top == INFINITY || k > kMostK ? kSlow : !sums ? kBest : kSum;
-  if (state == kSum && !(fabsf(top) * gr < 0x1p22f && gr < kMostGrain)) state = kSlow;
-  int bucket = INT_MIN, ref = 0;
-  unsigned long long want = 0;
-  const int g_top = state == kBest || state == kSum ? bucket_of(top, sums, gr) : 0;
-  if (state == kSum) ref = (g_top >> 5) + 1;
-  const double c = set.temperature == 0.f ? 0.0 : 1.4426950408889634 / (double)set.temperature;
-
-  // ---- the bucket of the cut
-  if (state == kBest || (state == kSum && cut)) {
-    if (wave == 0) g_of[lane] = mine > -INFINITY ? bucket_of(mine, sums, gr) : INT_MIN;
-    if (tid == 0) found = -1;
+  RowInfo in{real == 0 ? kNone : top == INFINITY || set.k > kMostK ? kSlow : SUMS ? kSum : kBest, INT_MIN, 0, top, 0};
+  // (a bucket by weight is a whole number that fp32 holds to a quarter)
+  if (in.state == kSum && !(fabsf(top) * set.grain < 0x1p22f && set.grain < kMostGrain)) in.state = kSlow;
+  const bool done = in.state == kNone || in.state == kSlow || (SUMS && set.top_p >= 1.f);
+  const int base = done && in.state != kSum ? 0 : top_of(bucket_of(top, SUMS, set.grain));
+  if (in.state == kSum) in.ref = (base >> 5) + 1;
+  if (done) {
+    if (threadIdx.x == 0) lds.info = in;
     __syncthreads();
-    // a slice's weights in the row's unit, rounded
-    auto in_unit = [&](unsigned long long w, int g) {
-      const int sh = kSliceBits - a.bits + ref - ((g >> 5) + 1);
-      return sh == 0 ? w : sh > 63 ? 0ull : ((w >> (sh - 1)) + 1) >> 1;
-    };
-    unsigned long long goal = (unsigned long long)k;
-    if (sums) {
-      unsigned long long all = 0;
-      if (lane < a.slices && g_of[lane] != INT_MIN) all = in_unit(ldg<unsigned long long>(a.sum + at + lane), g_of[lane]);
-      for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o, 64);
-      goal = (unsigned long long)ceil((double)set.top_p * (double)all);
-      if (goal == 0) goal = 1;
-    }
-    unsigned long long before = 0;
-    for (int b0 = 0; b0 < kBins - 1; b0 += 256) {
-      const int j = b0 + (tid & 255);
-      unsigned long long s = 0;
-      if (j < kBins - 1)
-        for (int q = tid >> 8; q < a.slices; q += GR) {
-          const int g = g_of[q], i = j - (g_top - g);
-          if (g == INT_MIN || i < 0) continue;
-          const unsigned long long *h = a.hist + (at + q) * kBins;
-          s += sums ? in_unit(ldg<unsigned long long>(h + i), g) : ldg<uint32_t>(reinterpret_cast<const uint32_t *>(h) + i);
-        }
-      if (GR > 1) {
-        part[tid >> 8][tid & 255] = s;
-        __syncthreads();
-        if (tid < 256) {
-          s = 0;
-#pragma unroll
-          for (int q = 0; q < GR; ++q) s += part[q][tid];
-        }
-      }
-      unsigned long long upto = s;
-      for (int o = 1; o < 64; o <<= 1) {
-        const unsigned long long y = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += y;
-      }
-      if (wave < 4 && lane == 63) wsum[wave] = upto;
-      __syncthreads();
-      if (tid < 256) {
-        upto += before;
-        for (int w = 0; w < wave; ++w) upto += wsum[w];
-        if (upto >= goal && upto - s < goal) {
-          found = j;
-          found_before = upto - s;
-        }
-      }
-      before += wsum[0] + wsum[1] + wsum[2] + wsum[3];
-      __syncthreads();
-      if (found >= 0) break;
-    }
-    if (found >= 0) {
-      bucket = g_top - found;
-      want = goal - found_before;
-    } else if (sums || real > kList) {
-      state = kSlow;
-    }  // (else all that can be drawn is in the list)
+    return;
   }
-  if (blockIdx.x == 0 && tid == 0) a.info[row] = RowInfo{state, bucket, ref, top, want};
+  // groups that a slice's buckets begin below the row's
+  const int down = mine > -INFINITY ? (base - top_of(bucket_of(mine, SUMS, set.grain))) >> 5 : kBins;
+  // a slice's weights in the row's unit, rounded
+  auto in_unit = [&](unsigned long long w, int down) {
+    if constexpr (!SUMS) return w;
+    const int sh = min(kSliceBits - a.bits + down, 63);  // (2^63 at most: that and more leave 0 or 1)
+    return (w >> sh) + (sh ? w >> (sh - 1) & 1 : 0);
+  };
+  unsigned long long h[Q], s = 0;
+  int d[Q];
+#pragma unroll
+  for (int e = 0; e < Q; ++e) {
+    const int q = min(wave + W * e, a.slices - 1);
+    d[e] = __builtin_amdgcn_readlane(down, q);
+    h[e] = ldg<unsigned long long>(a.coarse + (at + q) * 64 + max(lane - d[e], 0));
+  }
+#pragma unroll
+  for (int e = 0; e < Q; ++e) s += wave + W * e < a.slices && lane >= d[e] ? in_unit(h[e], d[e]) : 0;
+  lds.part[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0) {
+    s = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += lds.part[w][lane];
+    const unsigned long long upto = scan_wave(s);
+    unsigned long long goal = (unsigned long long)set.k;
+    if (SUMS) goal = share_of(set.top_p, __shfl(upto, 63, 64));
+    const unsigned long long hit = __ballot(upto >= goal);
+    const int group = hit ? __ffsll(hit) - 1 : -1;
+    const unsigned long long before = __shfl(upto - s, max(group, 0), 64);
+    if (lane == 0) {
+      // (top-k: all that can be drawn is in the list, if it holds that)
+      if (group < 0 && (SUMS || real > kList)) in.state = kSlow;
+      lds.info = in;
+      lds.group = group;
+      lds.goal = goal;
+      lds.before = before;
+    }
+  }
+  __syncthreads();
+  const int group = lds.group;
+  if (group < 0) return;
+  // ---- the group's 32 buckets: two slices at a time
+  s = 0;
+#pragma unroll
+  for (int e = 0; e < Q / 2; ++e) {
+    const int q = min(2 * (wave + W * e) + (lane >> 5), a.slices - 1);
+    d[e] = __shfl(down, q, 64);
+    const size_t i = 32 * max(group - d[e], 0) + (lane & 31);
+    const unsigned long long *from = a.hist + (at + q) * kBins;
+    if constexpr (SUMS)
+      h[e] = ldg<unsigned long long>(from + i);
+    else
+      h[e] = ldg<uint32_t>(reinterpret_cast<const uint32_t *>(from) + i);
+  }
+#pragma unroll
+  for (int e = 0; e < Q / 2; ++e)
+    s += 2 * (wave + W * e) + (lane >> 5) < a.slices && group >= d[e] ? in_unit(h[e], d[e]) : 0;
+  lds.part[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0) {
+    s = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += lds.part[w][lane & 31] + lds.part[w][32 + (lane & 31)];
+    if (lane >= 32) s = 0;
+    const unsigned long long goal = lds.goal, upto = lds.before + scan_wave(s), hit = __ballot(upto >= goal && lane < 32);
+    // (buckets are rounded one by one: the group's last, should they stay below the goal)
+    const int bin = hit ? __ffsll(hit) - 1 : 31;
+    const unsigned long long under = __shfl(upto - s, bin, 64);
+    if (lane == 0) {
+      lds.info.bucket = base - 32 * group - bin;
+      lds.info.want = goal > under ? goal - under : 1;
+    }
+  }
+  __syncthreads();
+}
+
+template <int PER, bool VEC>
+__global__ __launch_bounds__(kNT) void k_rows_pick(SampleRowsArgs a) {
+  __shared__ double table[64];
+  __shared__ CutLds lds;
+  __shared__ uint32_t places[kNT / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y;
+  const RowSet &set = a.rows[row];
+  const bool sums = set.k == 0, cut = sums && set.top_p < 1.f;
+  const size_t at = (size_t)row * a.slices;
+  const int id0 = blockIdx.x * a.slice + wave * 64 * PER;
+  float v[PER];
+  load_chunk<PER, VEC>(a.x + row * a.ld, a.n, id0, v);
+  exp2_table(table);
+  if (sums)
+    find_cut<true>(a, set, at, lds);
+  else
+    find_cut<false>(a, set, at, lds);
+  if (blockIdx.x == 0 && tid == 0) a.info[row] = lds.info;
+  const int state = lds.info.state, bucket = lds.info.bucket, ref = lds.info.ref;
+  const float top = lds.info.top;
   if (state == kNone || state == kSlow) return;
-  __syncthreads();  // (the table)
 
   // ---- the slice once more
   const Exp2 exp2{table};
-  const double least = least_of(top, c, set.min_p);
+  const double least = __builtin_fma((double)top, set.c, set.log_min);
   unsigned long long sum = 0;
-  uint32_t num = 0;
+  uint32_t num = 0, listed = 0;  // bit j: logit j goes to the list
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int g = bucket_of(v[j], sums, gr);
-    const bool on = v[j] > -INFINITY && g >= bucket && (!sums || v[j] == top || (double)v[j] * c >= least);
-    const bool listed = on && (!sums || (cut && g == bucket));
-    const unsigned long long m = __ballot(listed);
-    if (m) {
-      uint32_t base = 0;
-      if (lane == 0) base = atomicAdd(a.n_list + row, (uint32_t)__popcll(m));
-      base = (uint32_t)__shfl((int)base, 0, 64) + __popcll(m & ((1ull << lane) - 1));
-      if (listed && base < kList)
-        a.list[(size_t)row * kList + base] = (unsigned long long)key_of(v[j]) << 32 |
-                                             (0xFFFFFFFFu - (uint32_t)(id0 + 256 * (j / 4) + 4 * lane + j % 4));
-    }
-    if (sums && on && !listed) {
-      sum += weight_of(exp2, v[j], c, ref, a.bits);
+  for (int j = 0; j < PER; ++j) {
+    const int g = bucket_of(v[j], sums, set.grain);
+    if (!(v[j] > -INFINITY && g >= bucket && (!sums || v[j] == top || (double)v[j] * set.c >= least))) continue;
+    if (!sums || (cut && g == bucket)) {
+      listed |= 1u << j;
+    } else {
+      sum += weight_of(exp2, v[j], set.c, ref, a.bits);
       ++num;
     }
+  }
+  // the block's candidates: one place in the list for all (a round trip for each would be most of the time)
+  if (!sums || cut) {
+    uint32_t mine = __popc(listed), upto = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t y = (uint32_t)__shfl_up((int)upto, o, 64);
+      if (lane >= o) upto += y;
+    }
+    if (lane == 63) places[wave] = upto;
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t p = lane < kNT / 64 ? places[lane] : 0, q = p;
+      for (int o = 1; o < kNT / 64; o <<= 1) {
+        const uint32_t y = (uint32_t)__shfl_up((int)q, o, 64);
+        if (lane >= o) q += y;
+      }
+      uint32_t base = 0;
+      if (lane == kNT / 64 - 1 && q) base = atomicAdd(a.n_list + row, q);
+      base = (uint32_t)__shfl((int)base, kNT / 64 - 1, 64);
+      if (lane < kNT / 64) places[lane] = base + q - p;
+    }
+    __syncthreads();
+    uint32_t at_list = places[wave] + upto - mine;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (listed >> j & 1) {
+        if (at_list < kList)
+          a.list[(size_t)row * kList + at_list] = (unsigned long long)key_of(v[j]) << 32 |
+                                                  (0xFFFFFFFFu - (uint32_t)(id0 + 256 * (j / 4) + 4 * lane + j % 4));
+        ++at_list;
+      }
   }
   if (sums) {
     for (int o = 1; o < 64; o <<= 1) {
@@ -345,7 +426,7 @@ __global__ __launch_bounds__(NT) void k_rows_pick(SampleRowsArgs a) {
       num += (uint32_t)__shfl_xor((int)num, o, 64);
     }
     if (lane == 0) {
-      const size_t ch = (size_t)row * a.slices * (a.slice / 1024) + id0 / 1024;
+      const size_t ch = (at + blockIdx.x) * (kNT / 64) + wave;
       a.chunk[ch] = sum;
       a.chunk_n[ch] = num;
     }
@@ -374,7 +455,7 @@ __device__ void row_by_digits(const SampleRowsArgs &a, DigitLds &lds) {
   unsigned long long *wt = lds.wt, *part = lds.part, &s_above = lds.s_above;
   int &s_id = lds.s_id;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n;
-  const ms_sample_row set = a.rows[blockIdx.x];
+  const RowSet &set = a.rows[blockIdx.x];
   const float *x = a.x + blockIdx.x * a.ld;
 
   // ---- maximum, and how many can be drawn
@@ -459,7 +540,7 @@ __device__ void row_by_digits(const SampleRowsArgs &a, DigitLds &lds) {
 
   uint32_t key = 1;  // (below every number's)
   uint32_t eq = 0, eq_all = 0;  // of the logits equal to the cut, the first eq are left
-  const unsigned long long all_k = set.temperature == 0.f ? 1 : set.top_k > 0 ? set.top_k : real;
+  const unsigned long long all_k = set.k > 0 ? set.k : real;
   if (all_k < real) {
     find(false, all_k, 1, 0);
     key = cut_key;
@@ -573,12 +654,43 @@ __device__ void row_by_digits(const SampleRowsArgs &a, DigitLds &lds) {
   }
 }
 
-// Falling order of n numbers, n a power of two.
+// Falling order of n numbers, n a power of two from 64 on.  A wave does the steps within 128 numbers of its own
+// without waiting for the others.
 __device__ inline void sort_falling(unsigned long long *x, int n) {
+  const int lane = threadIdx.x & 63;
+  auto swap = [&](int t, int size, int step) {
+    const int i = 2 * t - (t & (step - 1)), j = i + step;
+    const unsigned long long p = x[i], q = x[j];
+    if ((p < q) == ((i & size) == 0)) {
+      x[i] = q;
+      x[j] = p;
+    }
+  };
+  auto near = [&](int size, int step) {  // steps of up to 64: pairs t of a wave lie among its 128 numbers
+    for (int t = threadIdx.x; t - lane < n / 2; t += kNT)
+      for (int s = step; s > 0; s >>= 1) {
+        if (t < n / 2) swap(t, size, s);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (no instruction: LDS accesses stay in their order)
+      }
+  };
+  __syncthreads();
+  for (int size = 2; size <= 128 && size <= n; size <<= 1) near(size, size / 2);
+  for (int size = 256; size <= n; size <<= 1) {
+    for (int step = size / 2; step > 64; step >>= 1) {
+      __syncthreads();
+      for (int t = threadIdx.x; t < n / 2; t += kNT) swap(t, size, step);
+    }
+    __syncthreads();
+    near(size, 64);
+  }
+  __syncthreads();
+}
+// The same by one wave.
+__device__ inline void sort_by_wave(unsigned long long *x, int n) {
+  const int lane = threadIdx.x & 63;
   for (int size = 2; size <= n; size <<= 1)
     for (int step = size / 2; step > 0; step >>= 1) {
-      __syncthreads();
-      for (int t = threadIdx.x; t < n / 2; t += kNT) {
+      for (int t = lane; t < n / 2; t += 64) {
         const int i = 2 * t - (t & (step - 1)), j = i + step;
         const unsigned long long p = x[i], q = x[j];
         if ((p < q) == ((i & size) == 0)) {
@@ -586,8 +698,8 @@ __device__ inline void sort_falling(unsigned long long *x, int n) {
           x[j] = p;
         }
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-  __syncthreads();
 }
 __device__ inline int power_of_two(int n) {
   int p = 64;
@@ -598,10 +710,7 @@ __device__ inline int power_of_two(int n) {
 // Running sum over the block's threads, this one's value among it; *all: the whole.
 __device__ inline unsigned long long run_sum(unsigned long long v, unsigned long long *part, unsigned long long *all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long y = __shfl_up(v, o, 64);
-    if (lane >= o) v += y;
-  }
+  v = scan_wave(v);
   __syncthreads();
   if (lane == 63) part[wave] = v;
   __syncthreads();
@@ -619,26 +728,101 @@ __device__ inline unsigned long long target_of(float u, unsigned long long total
   const unsigned long long t = !(u > 0.f) ? 0 : u >= 1.f ? total - 1 : (unsigned long long)((double)u * (double)total);
   return t < total ? t : total - 1;
 }
+__device__ inline uint32_t id_of(unsigned long long entry) { return 0xFFFFFFFFu - (uint32_t)entry; }
+__device__ inline float logit_of(unsigned long long entry) { return of_key((uint32_t)(entry >> 32)); }
+__device__ inline void write_row(const SampleRowsArgs &a, int row, int id, float prob, uint32_t kept) {
+  a.ids[row] = id;
+  if (a.prob) a.prob[row] = prob;
+  if (a.kept) a.kept[row] = (int)kept;
+}
+
+// The draw of a row whose best ids are the sorted list's first, nk of them, E of these a lane (a thread).  BLOCK: by
+// all threads, else by one wave.
+template <bool BLOCK, int E>
+__device__ inline void draw_best(const SampleRowsArgs &a, const RowSet &set, int row, float top, int nk, float u,
+                                 const Exp2 &exp2, unsigned long long *list, unsigned long long *by_place,
+                                 unsigned long long *part, uint32_t *counts) {
+  const int at = (BLOCK ? threadIdx.x : threadIdx.x & 63) * E;
+  auto run = [&](unsigned long long v, unsigned long long *all) {
+    if constexpr (BLOCK) return run_sum(v, part, all);
+    v = scan_wave(v);
+    *all = __shfl(v, 63, 64);
+    return v;
+  };
+  unsigned long long w[E], sum = 0, total;
+  uint32_t id[E], over = 0, under = 0;  // how many min_p leaves, and top-p
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool in = at + e < nk;
+    const unsigned long long x = in ? list[at + e] : 0;
+    const float v = logit_of(x);
+    id[e] = id_of(x);
+    const double t = v == top ? 0.0 : ((double)v - (double)top) * set.c;
+    w[e] = in ? exp2(t, a.bits) : 0;
+    over += in && (v == top || t >= set.log_min);
+    sum += w[e];
+  }
+  unsigned long long upto = run(sum, &total) - sum;
+  const unsigned long long goal = set.temperature != 0.f && set.top_p < 1.f ? share_of(set.top_p, total) : ~0ull;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    under += at + e < nk && upto < goal;
+    upto += w[e];
+  }
+  for (int o = 1; o < 64; o <<= 1) {
+    over += (uint32_t)__shfl_xor((int)over, o, 64);
+    under += (uint32_t)__shfl_xor((int)under, o, 64);
+  }
+  if constexpr (BLOCK) {
+    if ((threadIdx.x & 63) == 0) {
+      atomicAdd(counts, over);
+      atomicAdd(counts + 1, under);
+    }
+    __syncthreads();
+    over = counts[0];
+    under = counts[1];
+  }
+  const int n = (int)min(over, under), size = power_of_two(n);
+  // ---- in the order of ids: (id, place) sorted, the weights by their places
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (at + e < size) list[at + e] = at + e < n ? (unsigned long long)(0xFFFFFFFFu - id[e]) << 32 | (uint32_t)(at + e) : 0;
+    if (at + e < n) by_place[at + e] = w[e];
+  }
+  if constexpr (BLOCK)
+    sort_falling(list, size);
+  else
+    sort_by_wave(list, size);
+  sum = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const unsigned long long x = at + e < n ? list[at + e] : 0;
+    id[e] = 0xFFFFFFFFu - (uint32_t)(x >> 32);
+    w[e] = at + e < n ? by_place[(uint32_t)x] : 0;
+    sum += w[e];
+  }
+  upto = run(sum, &total) - sum;
+  const unsigned long long target = target_of(u, total);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (upto <= target && upto + w[e] > target) write_row(a, row, (int)id[e], (float)((double)w[e] / (double)total), n);
+    upto += w[e];
+  }
+}
 
 __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   __shared__ __align__(16) unsigned long long list[kList];
-  __shared__ unsigned long long chunk[kMostSlices * 16];
+  __shared__ __align__(16) unsigned long long chunk[kMostSlices * 16];
   __shared__ double table[64];
   __shared__ unsigned long long part[16];
   __shared__ DigitLds digits;
-  __shared__ int hit;
-  __shared__ unsigned long long hit_before;
-  const int tid = threadIdx.x, row = blockIdx.x;
-  const ms_sample_row &set = a.rows[row];
+  __shared__ uint32_t counts[2];
+  const int tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
+  const RowSet &set = a.rows[row];
   const RowInfo in = a.info[row];
   const uint32_t n_list = a.n_list[row];
-  auto write = [&](int id, float prob, uint32_t kept) {
-    a.ids[row] = id;
-    if (a.prob) a.prob[row] = prob;
-    if (a.kept) a.kept[row] = (int)kept;
-  };
   if (in.state == kNone) {
-    if (tid == 0) write(-1, 0.f, 0);
+    if (tid == 0) write_row(a, row, -1, 0.f, 0);
     return;
   }
   if (in.state == kSlow || n_list > kList) {
@@ -647,131 +831,100 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   }
   exp2_table(table);
   const Exp2 exp2{table};
-  const float *x = a.x + row * a.ld;
-  const double c = set.temperature == 0.f ? 0.0 : 1.4426950408889634 / (double)set.temperature;
+  const float u = ldg<float>(a.u + row);
+  const int n_chunks = a.slices * (kNT / 64), chunk_len = a.slice / (kNT / 64);
+  uint32_t kept = 0;
+  if (in.state == kSum && tid < n_chunks) {
+    chunk[tid] = a.chunk[(size_t)row * n_chunks + tid];
+    kept = a.chunk_n[(size_t)row * n_chunks + tid];
+  }
   const int size = n_list ? power_of_two((int)n_list) : 0;
   for (int i = tid; i < size; i += kNT) list[i] = i < (int)n_list ? a.list[(size_t)row * kList + i] : 0;
-  sort_falling(list, size);
-  const float u = ldg<float>(a.u + row);
-  auto id_of = [](unsigned long long e) { return 0xFFFFFFFFu - (uint32_t)e; };
-  auto logit_of = [](unsigned long long e) { return of_key((uint32_t)(e >> 32)); };
-
+  if (tid < 2) counts[tid] = 0;
+  __syncthreads();
   if (in.state == kBest) {
-    // ---- everything that may be left is in the list: two of its first kMostK a thread
-    const int best = best_of(set, a.n), nk = min(best, (int)n_list);
-    unsigned long long w[2] = {};
-    const double least = set.min_p > 0.f ? log2((double)set.min_p) : -INFINITY;
-    uint32_t over = 0;  // of the two, how many min_p leaves
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * tid + e;
-      if (i >= nk) continue;
-      const float v = logit_of(list[i]);
-      const double t = v == in.top ? 0.0 : ((double)v - (double)in.top) * c;
-      w[e] = exp2(t, a.bits);
-      over += v == in.top || t >= least;
-    }
-    unsigned long long total, left, most;
-    unsigned long long upto = run_sum(w[0] + w[1], part, &total);
-    unsigned long long goal = ~0ull;
-    if (set.temperature != 0.f && set.top_p < 1.f) {
-      goal = (unsigned long long)ceil((double)set.top_p * (double)total);
-      if (goal == 0) goal = 1;
-    }
-    const uint32_t under = (2 * tid < nk && upto - w[0] - w[1] < goal) + (2 * tid + 1 < nk && upto - w[1] < goal);
-    run_sum(under, part, &left);
-    run_sum(over, part, &most);
-    const int n = (int)(left < most ? left : most);
-    // in order of ids: (id, place) sorted, the weights by their places
-    __syncthreads();
-    unsigned long long *by_place = list + 4096;
-    uint32_t id[2] = {};
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (2 * tid + e < n) id[e] = id_of(list[2 * tid + e]);
-    __syncthreads();
-    const int size2 = power_of_two(n);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * tid + e;
-      if (i < size2) list[i] = i < n ? (unsigned long long)(0xFFFFFFFFu - id[e]) << 32 | (uint32_t)i : 0;
-      if (i < n) by_place[i] = w[e];
-    }
-    sort_falling(list, size2);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) w[e] = 2 * tid + e < n ? by_place[(uint32_t)list[2 * tid + e]] : 0;
-    upto = run_sum(w[0] + w[1], part, &total);
-    const unsigned long long target = target_of(u, total);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const unsigned long long to = e ? upto : upto - w[1];
-      if (to > target && to - w[e] <= target)
-        write((int)(0xFFFFFFFFu - (uint32_t)(list[2 * tid + e] >> 32)), (float)((double)w[e] / (double)total), n);
+    const int nk = min(set.k, (int)n_list);
+    if (n_list <= kWave) {
+      if (tid >= 64) return;
+      sort_by_wave(list, size);
+      draw_best<false, kWave / 64>(a, set, row, in.top, nk, u, exp2, list, list + 4096, part, counts);
+    } else {
+      sort_falling(list, size);
+      draw_best<true, kMostK / kNT>(a, set, row, in.top, nk, u, exp2, list, list + 4096, part, counts);
     }
     return;
   }
 
-  // ---- sums of the chunks; of the candidates as many as it takes
-  const int n_chunks = a.slices * (a.slice / 1024);
-  unsigned long long kept = 0, total;
-  if (tid < n_chunks) {
-    chunk[tid] = a.chunk[(size_t)row * n_chunks + tid];
-    kept = a.chunk_n[(size_t)row * n_chunks + tid];
+  // ---- the weights of the chunks, and of the candidates as many as it takes
+  for (int o = 1; o < 64; o <<= 1) kept += (uint32_t)__shfl_xor((int)kept, o, 64);
+  if (lane == 0 && kept) atomicAdd(counts, kept);
+  if (n_list > kWave)
+    sort_falling(list, size);
+  else
+    __syncthreads();
+  if (tid >= 64) return;
+  if (n_list <= kWave) sort_by_wave(list, size);
+  unsigned long long before = 0, cut = ~0ull;
+  uint32_t taken = 0;
+  for (int i0 = 0; i0 < (int)n_list && before < in.want; i0 += 64) {
+    const int i = i0 + lane;
+    const unsigned long long x = i < (int)n_list ? list[i] : 0;
+    const unsigned long long w = i < (int)n_list ? weight_of(exp2, logit_of(x), set.c, in.ref, a.bits) : 0;
+    const unsigned long long upto = before + scan_wave(w);
+    const bool take = i < (int)n_list && upto - w < in.want;
+    if (take) atomicAdd(&chunk[id_of(x) / chunk_len], w);
+    const unsigned long long m = __ballot(take);
+    if (m) cut = __shfl(x, 63 - __clzll(m), 64);
+    taken += __popcll(m);
+    before = __shfl(upto, 63, 64);
   }
-  __syncthreads();
-  unsigned long long before = 0;
-  int taken = 0;
-  for (int i0 = 0; i0 < (int)n_list; i0 += kNT) {
-    const int i = i0 + tid;
-    unsigned long long w = 0, all;
-    if (i < (int)n_list) w = weight_of(exp2, logit_of(list[i]), c, in.ref, a.bits);
-    const unsigned long long upto = run_sum(w, part, &all);
-    const bool take = i < (int)n_list && before + upto - w < in.want;
-    if (take) atomicAdd(&chunk[id_of(list[i]) >> 10], w);
-    unsigned long long num;
-    run_sum(take, part, &num);
-    taken += (int)num;
-    before += all;
-    if (before >= in.want) break;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  // ---- the chunk, then the id, at which the running weight passes the target
+  const int per = (n_chunks + 63) / 64;
+  unsigned long long sum = 0;
+  for (int i = 0; i < per; ++i) sum += per * lane + i < n_chunks ? chunk[per * lane + i] : 0;
+  unsigned long long upto = scan_wave(sum);
+  const unsigned long long total = __shfl(upto, 63, 64), target = target_of(u, total);
+  const int l = __ffsll((unsigned long long)__ballot(upto > target)) - 1;
+  before = __shfl(upto - sum, l, 64);
+  int hit = per * l;
+  while (before + chunk[hit] <= target) before += chunk[hit++];
+  const double least = __builtin_fma((double)in.top, set.c, set.log_min);
+  const float *x = a.x + row * a.ld;
+  float v[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int id = hit * chunk_len + 64 * e + lane;
+    v[e] = 64 * e < chunk_len && id < a.n ? ldg<float>(x + id) : -INFINITY;
   }
-  const unsigned long long cut = taken ? list[taken - 1] : ~0ull;
-  __syncthreads();
-  {
-    unsigned long long num;
-    run_sum(kept, part, &num);
-    kept = num + taken;
-  }
-  const unsigned long long w = tid < n_chunks ? chunk[tid] : 0, upto = run_sum(w, part, &total);
-  const unsigned long long target = target_of(u, total);
-  if (upto > target && upto - w <= target) {
-    hit = tid;
-    hit_before = upto - w;
-  }
-  __syncthreads();
-  {
-    const int id = hit * 1024 + tid;
-    const float v = id < a.n ? ldg<float>(x + id) : -INFINITY;
-    unsigned long long w = 0, all;
-    if (v > -INFINITY) {
-      const int g = bucket_of(v, true, grain(set));
-      const bool in_cut = g > in.bucket || ((unsigned long long)key_of(v) << 32 | (0xFFFFFFFFu - (uint32_t)id)) >= cut;
-      if ((in.bucket == INT_MIN || in_cut) && (v == in.top || (double)v * c >= least_of(in.top, c, set.min_p)))
-        w = weight_of(exp2, v, c, in.ref, a.bits);
+  for (int e = 0; 64 * e < chunk_len; ++e) {
+    const int id = hit * chunk_len + 64 * e + lane;
+    float y = v[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) y = i == e ? v[i] : y;
+    unsigned long long w = 0;
+    if (y > -INFINITY) {
+      const bool in_cut = bucket_of(y, true, set.grain) > in.bucket ||
+                          ((unsigned long long)key_of(y) << 32 | (0xFFFFFFFFu - (uint32_t)id)) >= cut;
+      if ((in.bucket == INT_MIN || in_cut) && (y == in.top || (double)y * set.c >= least))
+        w = weight_of(exp2, y, set.c, in.ref, a.bits);
     }
-    const unsigned long long upto = hit_before + run_sum(w, part, &all);
-    if (upto > target && upto - w <= target) write(id, (float)((double)w / (double)total), (uint32_t)kept);
+    const unsigned long long upto = before + scan_wave(w);
+    if (upto > target && upto - w <= target) write_row(a, row, id, (float)((double)w / (double)total), counts[0] + taken);
+    before = __shfl(upto, 63, 64);
+    if (before > target) break;
   }
 }
 
-template <int NT>
+template <int PER>
 void launch_slices(const SampleRowsArgs &a, int rows, bool vec, hipStream_t st) {
-  const dim3 grid(a.slices, rows), blk(NT);
+  const dim3 grid(a.slices, rows), blk(kNT);
   if (vec) {
-    hipLaunchKernelGGL((k_rows_scan<NT, true>), grid, blk, 0, st, a);
-    hipLaunchKernelGGL((k_rows_pick<NT, true>), grid, blk, 0, st, a);
+    hipLaunchKernelGGL((k_rows_scan<PER, true>), grid, blk, 0, st, a);
+    hipLaunchKernelGGL((k_rows_pick<PER, true>), grid, blk, 0, st, a);
   } else {
-    hipLaunchKernelGGL((k_rows_scan<NT, false>), grid, blk, 0, st, a);
-    hipLaunchKernelGGL((k_rows_pick<NT, false>), grid, blk, 0, st, a);
+    hipLaunchKernelGGL((k_rows_scan<PER, false>), grid, blk, 0, st, a);
+    hipLaunchKernelGGL((k_rows_pick<PER, false>), grid, blk, 0, st, a);
   }
 }
 
@@ -818,12 +971,12 @@ extern "C" int ms_sample_rows(const float *d_logits, size_t in_stride, int rows,
   a.slices = cdiv(vocab, a.slice);
   const bool sliced = a.slices <= kMostSlices, vec = aligned16(d_logits) && in_stride % 4 == 0;
   if (sliced) {
-    const size_t cells = (size_t)m0 * a.slices, chunks = cells * (a.slice / 1024);
+    const size_t cells = (size_t)m0 * a.slices, chunks = cells * (kNT / 64);
     void *buf = nullptr;
-    if (int rc = scratch(cells * (kBins * 8 + 16) + chunks * 12 + m0 * (kList * 8 + sizeof(RowInfo) + 4) + 64, &buf)) return rc;
+    if (int rc = scratch(cells * (kBins * 8 + 64 * 8 + 8) + chunks * 12 + m0 * (kList * 8 + sizeof(RowInfo) + 4) + 64, &buf)) return rc;
     a.hist = static_cast<unsigned long long *>(buf);
-    a.sum = a.hist + cells * kBins;
-    a.list = a.sum + cells;
+    a.coarse = a.hist + cells * kBins;
+    a.list = a.coarse + cells * 64;
     a.chunk = a.list + (size_t)m0 * kList;
     a.info = reinterpret_cast<RowInfo *>(a.chunk + chunks);
     a.top = reinterpret_cast<float *>(a.info + m0);
@@ -838,14 +991,24 @@ extern "C" int ms_sample_rows(const float *d_logits, size_t in_stride, int rows,
     a.ids = d_ids + r0;
     a.prob = d_prob ? d_prob + r0 : nullptr;
     a.kept = d_kept ? d_kept + r0 : nullptr;
-    for (int r = 0; r < kRows; ++r) a.rows[r] = h_rows[r0 + (r < m ? r : 0)];
+    for (int r = 0; r < kRows; ++r) {
+      const ms_sample_row &w = h_rows[r0 + (r < m ? r : 0)];
+      const bool best = w.temperature == 0.f;
+      a.rows[r].c = best ? 0.0 : 1.4426950408889634 / (double)w.temperature;
+      a.rows[r].log_min = w.min_p > 0.f ? std::log2((double)w.min_p) : -INFINITY;
+      a.rows[r].grain = best ? 0.f : (float)(32 * 1.4426950408889634 / (double)w.temperature);
+      a.rows[r].temperature = w.temperature;
+      a.rows[r].top_p = w.top_p;
+      a.rows[r].min_p = w.min_p;
+      a.rows[r].k = best ? 1 : w.top_k > 0 && w.top_k < vocab ? w.top_k : 0;
+    }
     if (!sliced) {
       hipLaunchKernelGGL(k_rows_digits, dim3(m), dim3(kNT), 0, st, a);
     } else {
       if (large)
-        launch_slices<1024>(a, m, vec, st);
+        launch_slices<16>(a, m, vec, st);
       else
-        launch_slices<256>(a, m, vec, st);
+        launch_slices<4>(a, m, vec, st);
       hipLaunchKernelGGL(k_rows_draw, dim3(m), dim3(kNT), 0, st, a);
     }
     MS_HIP_TRY(hipGetLastError());
