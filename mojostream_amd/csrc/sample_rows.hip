@@ -72,7 +72,48 @@ __device__ inline uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);  // (-0 and 0 are equal)
   return !(x > -INFINITY) ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ inline float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+// (0: -infinity)
+__device__ inline float of_key(uint32_t k) {
+  return k == 0 ? -INFINITY : __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+// One step across a wave's lanes: the value of a lane below (row_shr 1, 2, 4, 8 within 16 lanes; the last
+// lane of a row of 16 to the next row, of the first half to the second), `old` where there is none.
+template <int CTRL, int ROWS>
+__device__ inline uint32_t from_below(uint32_t old, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 15, false);
+}
+template <int CTRL, int ROWS>
+__device__ inline unsigned long long from_below(unsigned long long old, unsigned long long v) {
+  return (unsigned long long)from_below<CTRL, ROWS>((uint32_t)(old >> 32), (uint32_t)(v >> 32)) << 32 |
+         from_below<CTRL, ROWS>((uint32_t)old, (uint32_t)v);
+}
+// Running sum over a wave's lanes, a lane's own value in it.
+template <class T>
+__device__ inline T scan_wave(T v) {
+  v += from_below<0x111, 15>((T)0, v);
+  v += from_below<0x112, 15>((T)0, v);
+  v += from_below<0x114, 15>((T)0, v);
+  v += from_below<0x118, 15>((T)0, v);
+  v += from_below<0x142, 10>((T)0, v);
+  return v + from_below<0x143, 12>((T)0, v);
+}
+__device__ inline uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+__device__ inline unsigned long long last_lane(unsigned long long v) {
+  return (unsigned long long)last_lane((uint32_t)(v >> 32)) << 32 | last_lane((uint32_t)v);
+}
+template <class T>
+__device__ inline T sum_wave(T v) {
+  return last_lane(scan_wave(v));
+}
+__device__ inline uint32_t max_wave(uint32_t v) {
+  v = max(v, from_below<0x111, 15>(v, v));
+  v = max(v, from_below<0x112, 15>(v, v));
+  v = max(v, from_below<0x114, 15>(v, v));
+  v = max(v, from_below<0x118, 15>(v, v));
+  v = max(v, from_below<0x142, 10>(v, v));
+  return last_lane(max(v, from_below<0x143, 12>(v, v)));
+}
 
 // 2^(j/64)
 __device__ const double kExp2[64] = {
@@ -174,10 +215,8 @@ __global__ __launch_bounds__(kNT) void k_rows_scan(SampleRowsArgs a) {
     top = fmaxf(top, v[j]);
     real += v[j] > -INFINITY;
   }
-  for (int o = 1; o < 64; o <<= 1) {
-    top = fmaxf(top, __shfl_xor(top, o, 64));
-    real += (uint32_t)__shfl_xor((int)real, o, 64);
-  }
+  top = of_key(max_wave(key_of(top)));
+  real = sum_wave(real);
   if (lane == 0) {
     tops[wave] = top;
     reals[wave] = real;
@@ -228,15 +267,6 @@ __global__ __launch_bounds__(kNT) void k_rows_scan(SampleRowsArgs a) {
   if ((tid & 15) == 0) a.coarse[at * 64 + tid / 16] = two;
 }
 
-__device__ inline unsigned long long scan_wave(unsigned long long v) {
-  const int lane = threadIdx.x & 63;
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long y = __shfl_up(v, o, 64);
-    if (lane >= o) v += y;
-  }
-  return v;
-}
-
 __device__ inline unsigned long long share_of(float p, unsigned long long total) {
   const unsigned long long t = (unsigned long long)ceil((double)p * (double)total);
   return t ? t : 1;
@@ -258,11 +288,8 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float mine = lane < a.slices ? ldg<float>(a.top + at + lane) : -INFINITY;
   uint32_t real = lane < a.slices ? ldg<uint32_t>(a.real + at + lane) : 0;
-  float top = mine;
-  for (int o = 1; o < 64; o <<= 1) {
-    top = fmaxf(top, __shfl_xor(top, o, 64));
-    real += (uint32_t)__shfl_xor((int)real, o, 64);
-  }
+  const float top = of_key(max_wave(key_of(mine)));
+  real = sum_wave(real);
   RowInfo in{real == 0 ? kNone : top == INFINITY || set.k > kMostK ? kSlow : SUMS ? kSum : kBest, INT_MIN, 0, top, 0};
   // (a bucket by weight is a whole number that fp32 holds to a quarter)
   if (in.state == kSum && !(fabsf(top) * set.grain < 0x1p22f && set.grain < kMostGrain)) in.state = kSlow;
@@ -300,7 +327,7 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
     for (int w = 0; w < W; ++w) s += lds.part[w][lane];
     const unsigned long long upto = scan_wave(s);
     unsigned long long goal = (unsigned long long)set.k;
-    if (SUMS) goal = share_of(set.top_p, __shfl(upto, 63, 64));
+    if (SUMS) goal = share_of(set.top_p, last_lane(upto));
     const unsigned long long hit = __ballot(upto >= goal);
     const int group = hit ? __ffsll(hit) - 1 : -1;
     const unsigned long long before = __shfl(upto - s, max(group, 0), 64);
@@ -391,22 +418,14 @@ __global__ __launch_bounds__(kNT) void k_rows_pick(SampleRowsArgs a) {
   }
   // the block's candidates: one place in the list for all (a round trip for each would be most of the time)
   if (!sums || cut) {
-    uint32_t mine = __popc(listed), upto = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t y = (uint32_t)__shfl_up((int)upto, o, 64);
-      if (lane >= o) upto += y;
-    }
+    const uint32_t mine = __popc(listed), upto = scan_wave(mine);
     if (lane == 63) places[wave] = upto;
     __syncthreads();
     if (wave == 0) {
-      uint32_t p = lane < kNT / 64 ? places[lane] : 0, q = p;
-      for (int o = 1; o < kNT / 64; o <<= 1) {
-        const uint32_t y = (uint32_t)__shfl_up((int)q, o, 64);
-        if (lane >= o) q += y;
-      }
+      const uint32_t p = lane < kNT / 64 ? places[lane] : 0, q = scan_wave(p);
       uint32_t base = 0;
-      if (lane == kNT / 64 - 1 && q) base = atomicAdd(a.n_list + row, q);
-      base = (uint32_t)__shfl((int)base, kNT / 64 - 1, 64);
+      if (lane == 63 && q) base = atomicAdd(a.n_list + row, q);
+      base = last_lane(base);
       if (lane < kNT / 64) places[lane] = base + q - p;
     }
     __syncthreads();
@@ -421,21 +440,14 @@ __global__ __launch_bounds__(kNT) void k_rows_pick(SampleRowsArgs a) {
       }
   }
   if (sums) {
-    for (int o = 1; o < 64; o <<= 1) {
-      sum += __shfl_xor(sum, o, 64);
-      num += (uint32_t)__shfl_xor((int)num, o, 64);
-    }
+    sum = sum_wave(sum);
+    num = sum_wave(num);
     if (lane == 0) {
       const size_t ch = (at + blockIdx.x) * (kNT / 64) + wave;
       a.chunk[ch] = sum;
       a.chunk_n[ch] = num;
     }
   }
-}
-
-__device__ inline uint64_t add_over_wave(uint64_t v) {
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor((unsigned long long)v, o, 64);
-  return v;
 }
 
 struct DigitLds {
@@ -465,10 +477,8 @@ __device__ void row_by_digits(const SampleRowsArgs &a, DigitLds &lds) {
     top = max(top, k);
     real += k != 0;
   }
-  for (int o = 1; o < 64; o <<= 1) {
-    top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-    real += __shfl_xor((int)real, o, 64);
-  }
+  top = max_wave(top);
+  real = sum_wave(real);
   if (lane == 0) {
     red[wave] = top;
     cnt[wave] = real;
@@ -549,7 +559,7 @@ __device__ void row_by_digits(const SampleRowsArgs &a, DigitLds &lds) {
   }
   uint32_t last_eq = 0xFFFFFFFFu;  // the last id of those equal to the cut
   auto block_sum = [&](unsigned long long v) {
-    v = add_over_wave(v);
+    v = sum_wave(v);
     __syncthreads();
     if (lane == 0) part[wave] = v;
     __syncthreads();
@@ -615,7 +625,7 @@ __device__ void row_by_digits(const SampleRowsArgs &a, DigitLds &lds) {
         ++num;
       }
     }
-    sum = add_over_wave(sum);
+    sum = sum_wave(sum);
     if (first) num = block_sum(num);
     __syncthreads();
     if (lane == 0) part[wave] = sum;
@@ -639,11 +649,7 @@ __device__ void row_by_digits(const SampleRowsArgs &a, DigitLds &lds) {
       const float v = ldg<float>(x + i);
       if (left(v, i)) w = weight(v);
     }
-    unsigned long long upto = w;
-    for (int o = 1; o < 64; o <<= 1) {
-      const unsigned long long y = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += y;
-    }
+    const unsigned long long upto = scan_wave(w);
     const unsigned long long hit = __ballot(before + upto > target);
     const int l = __ffsll((unsigned long long)hit) - 1;
     if (lane == l) {
@@ -685,21 +691,35 @@ __device__ inline void sort_falling(unsigned long long *x, int n) {
   }
   __syncthreads();
 }
-// The same by one wave.
-__device__ inline void sort_by_wave(unsigned long long *x, int n) {
+// The same by one wave, of n <= 64 E numbers that differ: each goes to the place that says how many are larger.
+// (64 numbers 0.6 us; sorted as above 3.6 us, a chain of 21 LDS round trips)
+template <int E>
+__device__ inline void rank_by_wave(unsigned long long *x, int n) {
   const int lane = threadIdx.x & 63;
-  for (int size = 2; size <= n; size <<= 1)
-    for (int step = size / 2; step > 0; step >>= 1) {
-      for (int t = lane; t < n / 2; t += 64) {
-        const int i = 2 * t - (t & (step - 1)), j = i + step;
-        const unsigned long long p = x[i], q = x[j];
-        if ((p < q) == ((i & size) == 0)) {
-          x[i] = q;
-          x[j] = p;
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  unsigned long long v[E];
+  int place[E] = {};
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = 64 * e + lane < n ? x[64 * e + lane] : 0;
+#pragma unroll
+  for (int f = 0; f < E; ++f)
+    for (int l = 0; l < min(64, n - 64 * f); ++l) {
+      const unsigned long long y = (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v[f] >> 32), l) << 32 |
+                                   (uint32_t)__builtin_amdgcn_readlane((int)v[f], l);
+#pragma unroll
+      for (int e = 0; e < E; ++e) place[e] += y > v[e];
     }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (64 * e + lane < n) x[place[e]] = v[e];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+__device__ inline void sort_by_wave(unsigned long long *x, int n) {
+  if (n <= 64)
+    rank_by_wave<1>(x, n);
+  else if (n <= 128)
+    rank_by_wave<2>(x, n);
+  else
+    rank_by_wave<kWave / 64>(x, n);
 }
 __device__ inline int power_of_two(int n) {
   int p = 64;
@@ -746,7 +766,7 @@ __device__ inline void draw_best(const SampleRowsArgs &a, const RowSet &set, int
   auto run = [&](unsigned long long v, unsigned long long *all) {
     if constexpr (BLOCK) return run_sum(v, part, all);
     v = scan_wave(v);
-    *all = __shfl(v, 63, 64);
+    *all = last_lane(v);
     return v;
   };
   unsigned long long w[E], sum = 0, total;
@@ -759,19 +779,15 @@ __device__ inline void draw_best(const SampleRowsArgs &a, const RowSet &set, int
     id[e] = id_of(x);
     const double t = v == top ? 0.0 : ((double)v - (double)top) * set.c;
     w[e] = in ? exp2(t, a.bits) : 0;
-    over += in && (v == top || t >= set.log_min);
+    over += __popcll(__ballot(in && (v == top || t >= set.log_min)));
     sum += w[e];
   }
   unsigned long long upto = run(sum, &total) - sum;
   const unsigned long long goal = set.temperature != 0.f && set.top_p < 1.f ? share_of(set.top_p, total) : ~0ull;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    under += at + e < nk && upto < goal;
+    under += __popcll(__ballot(at + e < nk && upto < goal));
     upto += w[e];
-  }
-  for (int o = 1; o < 64; o <<= 1) {
-    over += (uint32_t)__shfl_xor((int)over, o, 64);
-    under += (uint32_t)__shfl_xor((int)under, o, 64);
   }
   if constexpr (BLOCK) {
     if ((threadIdx.x & 63) == 0) {
@@ -792,7 +808,7 @@ __device__ inline void draw_best(const SampleRowsArgs &a, const RowSet &set, int
   if constexpr (BLOCK)
     sort_falling(list, size);
   else
-    sort_by_wave(list, size);
+    sort_by_wave(list, n);
   sum = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -846,8 +862,11 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
     const int nk = min(set.k, (int)n_list);
     if (n_list <= kWave) {
       if (tid >= 64) return;
-      sort_by_wave(list, size);
-      draw_best<false, kWave / 64>(a, set, row, in.top, nk, u, exp2, list, list + 4096, part, counts);
+      sort_by_wave(list, (int)n_list);
+      if (nk <= 64)
+        draw_best<false, 1>(a, set, row, in.top, nk, u, exp2, list, list + 4096, part, counts);
+      else
+        draw_best<false, kWave / 64>(a, set, row, in.top, nk, u, exp2, list, list + 4096, part, counts);
     } else {
       sort_falling(list, size);
       draw_best<true, kMostK / kNT>(a, set, row, in.top, nk, u, exp2, list, list + 4096, part, counts);
@@ -856,14 +875,14 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   }
 
   // ---- the weights of the chunks, and of the candidates as many as it takes
-  for (int o = 1; o < 64; o <<= 1) kept += (uint32_t)__shfl_xor((int)kept, o, 64);
+  kept = sum_wave(kept);
   if (lane == 0 && kept) atomicAdd(counts, kept);
   if (n_list > kWave)
     sort_falling(list, size);
   else
     __syncthreads();
   if (tid >= 64) return;
-  if (n_list <= kWave) sort_by_wave(list, size);
+  if (n_list <= kWave) sort_by_wave(list, (int)n_list);
   unsigned long long before = 0, cut = ~0ull;
   uint32_t taken = 0;
   for (int i0 = 0; i0 < (int)n_list && before < in.want; i0 += 64) {
@@ -876,7 +895,7 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
     const unsigned long long m = __ballot(take);
     if (m) cut = __shfl(x, 63 - __clzll(m), 64);
     taken += __popcll(m);
-    before = __shfl(upto, 63, 64);
+    before = last_lane(upto);
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   // ---- the chunk, then the id, at which the running weight passes the target
@@ -884,7 +903,7 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   unsigned long long sum = 0;
   for (int i = 0; i < per; ++i) sum += per * lane + i < n_chunks ? chunk[per * lane + i] : 0;
   unsigned long long upto = scan_wave(sum);
-  const unsigned long long total = __shfl(upto, 63, 64), target = target_of(u, total);
+  const unsigned long long total = last_lane(upto), target = target_of(u, total);
   const int l = __ffsll((unsigned long long)__ballot(upto > target)) - 1;
   before = __shfl(upto - sum, l, 64);
   int hit = per * l;
@@ -911,7 +930,7 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
     }
     const unsigned long long upto = before + scan_wave(w);
     if (upto > target && upto - w <= target) write_row(a, row, id, (float)((double)w / (double)total), counts[0] + taken);
-    before = __shfl(upto, 63, 64);
+    before = last_lane(upto);
     if (before > target) break;
   }
 }
