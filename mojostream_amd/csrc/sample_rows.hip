@@ -21,26 +21,28 @@
 namespace ms {
 namespace {
 
+constexpr float MAX32 = 0x1.fffffep+127f;
 constexpr int kRows = 64;       // rows of a launch: their settings are kernel arguments
 constexpr int kNT = 1024;
 constexpr int kBins = 2048;     // buckets of a slice's histogram, in 64 groups of 32
 constexpr int kList = 8192;     // candidates of a row
+constexpr int kSliceList = 2048;  // of one of its slices
 constexpr int kMostK = 2048;    // the largest top-k by the list
 constexpr int kMostSlices = 64;
 constexpr int kWave = 256;      // candidates that one wave goes through alone
 constexpr int kSliceBits = 49;  // S of a slice of up to 2^14 logits; S of a row is at most that
 
 struct RowInfo {
-  int state, bucket;         // kNone ..; the cut's bucket
-  int ref;                   // weights are 2^(x log2(e) / T - ref)
-  float top;                 // the largest logit
-  unsigned long long want;   // top-p: weight still to be reached within the bucket
+  int state;                // kNone ..
+  int ref;                  // weights are 2^(x log2(e) / T - ref)
+  float top;                // the largest logit
+  float lo, hi;             // the cut lies among the logits lo <= x < hi (the candidates); what lies above stays
+  unsigned long long want;  // top-p: weight still to be reached by the candidates
 };
 // A row's settings.
 struct RowSet {
-  double c;         // log2(e) / T; T = 0: 0
-  double log_min;   // log2(min_p)
-  float grain;      // buckets by weight: 32 of an octave
+  double c64, by;   // 64 log2(e) / T (T = 0: 0), and its inverse
+  double min64;     // 64 log2(min_p)
   float temperature, top_p, min_p;
   int k;            // ids that top-k leaves; 0: all
 };
@@ -58,10 +60,11 @@ struct SampleRowsArgs {
   unsigned long long *hist;  // [row][slice][kBins], top-k: uint32
   unsigned long long *coarse;  // [row][slice][64]: of each group of buckets
   float *top;                // [row][slice]
+  float *chunk_top;          // [row][slices * 16]
   uint32_t *real;            // [row][slice]: logits that can be drawn
   RowInfo *info;
-  uint32_t *n_list;          // [row]
-  unsigned long long *list;  // [row][kList]
+  uint32_t *n_list;          // [row][slice]
+  unsigned long long *list;  // [row][slice][kSliceList]
   unsigned long long *chunk; // [row][slices * 16]: of a wave's part of a slice
   uint32_t *chunk_n;
   RowSet rows[kRows];
@@ -134,36 +137,45 @@ __device__ const double kExp2[64] = {
     0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
-// 2^t as a whole number of 2^-bits, bits <= 51: 2^(j/64) from a table, a polynomial of degree 5 over a 64th of an octave
-// (its remainder is below 2^-54).
+// 2^(z/64) as a whole number of 2^-bits, bits <= 49: 2^(j/64) from a table, a polynomial of degree 4 over a 64th of an
+// octave (off by 4e-14 of it at most); the sums with large constants round to whole numbers.  *n: z rounded.  (With rint,
+// ldexp and conversions in place of the constants the 12.6 million weights of 48 rows took 20 us more.)
 struct Exp2 {
   const double *table;  // LDS, [64]
-  __device__ unsigned long long operator()(double t, int bits) const {
-    if (!(t > -60.0)) return 0;
-    const double n = rint(t * 64.0), r = __builtin_fma(t, 64.0, -n) * 0.010830424696249145;
-    double p = __builtin_fma(r, 1.0 / 120, 1.0 / 24);
-    p = __builtin_fma(r, p, 1.0 / 6);
-    p = __builtin_fma(r, p, 0.5);
+  __device__ unsigned long long operator()(double z, int bits, int *n) const {
+    constexpr double L = 0.010830424696249145;  // ln(2) / 64
+    z = __builtin_fmax(z, -3840.0);             // (2^-60: none)
+    const double m = z + 0x1.8p52, r = z - (m - 0x1.8p52);
+    const int k = (int)__double_as_longlong(m);
+    double p = __builtin_fma(r, L * L * L * L / 24, L * L * L / 6);
+    p = __builtin_fma(r, p, L * L / 2);
+    p = __builtin_fma(r, p, L);
     p = __builtin_fma(r, p, 1.0);
-    p = __builtin_fma(r, p, 1.0);
-    const int e = (int)n;
-    const double v = ldexp(p * table[e & 63], (e >> 6) + bits) + 0x1p52;
-    return (unsigned long long)__double_as_longlong(v) & 0xFFFFFFFFFFFFFull;
+    const long long t = __double_as_longlong(table[k & 63]) + ((long long)((k >> 6) + bits) << 52);
+    *n = k;
+    return (unsigned long long)__double_as_longlong(__builtin_fma(p, __longlong_as_double(t), 0x1p52)) & 0xFFFFFFFFFFFFFull;
   }
 };
-// A logit's weight by sums: the same instructions in every kernel, which count on the same number.
-__device__ inline unsigned long long weight_of(const Exp2 &exp2, float x, double c, int ref, int bits) {
-  return exp2(__builtin_fma((double)x, c, (double)-ref), bits);
-}
 __device__ inline void exp2_table(double *t) {
   if (threadIdx.x < 64) t[threadIdx.x] = kExp2[threadIdx.x];
 }
-
-constexpr float kMostGrain = 0x1p60f;
-// A logit's bucket, in the order of logits.  Top-k: the exponent and eight bits of the mantissa, whatever
-// the logits' size; sums: 1/32 of an octave of the weights.
-__device__ inline int bucket_of(float x, bool sums, float grain) {
-  return sums ? (int)fminf(fmaxf(floorf(x * grain), -0x1p29f), 0x1p29f) : (int)(key_of(x) >> 15);
+// A logit's weight by sums: the same instructions in every kernel, which count on the same number.  *n: 64ths of an
+// octave below the reference.
+__device__ inline unsigned long long weight_of(const Exp2 &exp2, float x, double c64, int ref, int bits, int *n) {
+  return exp2(__builtin_fma((double)x, c64, -64.0 * ref), bits, n);
+}
+// The reference of a largest logit: a whole octave that rounds above it.  Logits by sums have buckets of 1/32 of an octave,
+// 32 ref - 1 - b for bucket b from the reference down; 2^17 octaves are the most.
+__device__ inline bool in_range(float top, double c64) { return fabs((double)top * c64) < 0x1p23; }
+__device__ inline int ref_of(float top, double c64) { return ((int)rint((double)top * c64) >> 6) + 1; }
+// By counts: a bucket is the exponent and eight bits of the mantissa, whatever the logits' size.
+__device__ inline int bucket_of(float x) { return (int)(key_of(x) >> 15); }
+// The least number whose product with c64 is at least z.  (by: 1 / c64, by which the first guess is off by one place at most)
+__device__ inline float least_float(double z, double c64, double by) {
+  const float x = fmaxf((float)(z * by), -MAX32);
+  auto ok = [&](float y) { return (double)y * c64 >= z; };
+  const float below = of_key(key_of(x) - 1);
+  return !ok(x) ? of_key(key_of(x) + 1) : ok(below) ? below : x;
 }
 
 template <int PER, bool VEC>
@@ -187,84 +199,12 @@ __device__ inline void load_chunk(const float *x, int n, int at, float (&v)[PER]
   for (int j = 0; j < PER; ++j) v[j] = v[j] > -INFINITY ? v[j] : -INFINITY;  // (NaN too)
 }
 
-// A slice's buckets are counted from the top of its largest logit's group down: those of two slices
-// lie whole groups apart.
-__device__ inline int top_of(int bucket) { return bucket | 31; }
-
-// A thread has PER logits, a wave a chunk of 64 PER.
-template <int PER, bool VEC>
-__global__ __launch_bounds__(kNT) void k_rows_scan(SampleRowsArgs a) {
-  __shared__ __align__(16) unsigned long long hist[kBins];
-  __shared__ double table[64];
-  __shared__ float tops[kNT / 64];
-  __shared__ uint32_t reals[kNT / 64];
-  uint32_t *count = reinterpret_cast<uint32_t *>(hist);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y;
-  const RowSet &set = a.rows[row];
-  const bool sums = set.k == 0, bins = sums ? set.top_p < 1.f && set.grain < kMostGrain : set.k <= kMostK;
-  float v[PER];
-  load_chunk<PER, VEC>(a.x + row * a.ld, a.n, blockIdx.x * a.slice + wave * 64 * PER, v);
-  if (bins) {
-    for (int i = tid; i < (sums ? kBins : kBins / 2); i += kNT) hist[i] = 0;
-    exp2_table(table);
-  }
-  float top = -INFINITY;
-  uint32_t real = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    top = fmaxf(top, v[j]);
-    real += v[j] > -INFINITY;
-  }
-  top = of_key(max_wave(key_of(top)));
-  real = sum_wave(real);
-  if (lane == 0) {
-    tops[wave] = top;
-    reals[wave] = real;
-  }
-  __syncthreads();
-  top = tops[0];
-#pragma unroll
-  for (int w = 1; w < kNT / 64; ++w) top = fmaxf(top, tops[w]);
-  const size_t at = (size_t)row * a.slices + blockIdx.x;
-  if (tid == 0) {
-    real = 0;
-    for (int w = 0; w < kNT / 64; ++w) real += reals[w];
-    a.top[at] = top;
-    a.real[at] = real;
-    if (blockIdx.x == 0) a.n_list[row] = 0;
-  }
-  if (!bins || !(top > -INFINITY && top < INFINITY)) return;
-  const int base = top_of(bucket_of(top, sums, set.grain));
-  if (sums) {
-    const Exp2 exp2{table};
-    const int ref = (base >> 5) + 1;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const unsigned long long w = weight_of(exp2, v[j], set.c, ref, kSliceBits);
-      if (w) atomicAdd(&hist[min(max(base - bucket_of(v[j], true, set.grain), 0), kBins - 1)], w);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int d = base - bucket_of(v[j], false, 0.f);
-      if (d < kBins) atomicAdd(&count[d], 1u);
-    }
-  }
-  __syncthreads();
-  // two buckets a thread, a group 16 threads
-  unsigned long long two;
-  if (sums) {
-    const unsigned long long h0 = hist[2 * tid], h1 = hist[2 * tid + 1];
-    a.hist[at * kBins + 2 * tid] = h0;
-    a.hist[at * kBins + 2 * tid + 1] = h1;
-    two = h0 + h1;
-  } else {
-    const unsigned long long h = hist[tid];
-    a.hist[at * kBins + tid] = h;
-    two = (h & 0xFFFFFFFFu) + (h >> 32);
-  }
-  for (int o = 1; o < 16; o <<= 1) two += __shfl_xor(two, o, 64);
-  if ((tid & 15) == 0) a.coarse[at * 64 + tid / 16] = two;
+// A slice's buckets are counted from the top of its largest logit's group of 32 down: those of two slices
+// lie whole groups apart.  That group's number:
+template <bool SUMS>
+__device__ inline int group_of(float top, double c64) {
+  if constexpr (SUMS) return ref_of(top, c64);
+  return (bucket_of(top) >> 5) + 1;
 }
 
 __device__ inline unsigned long long share_of(float p, unsigned long long total) {
@@ -290,19 +230,31 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
   uint32_t real = lane < a.slices ? ldg<uint32_t>(a.real + at + lane) : 0;
   const float top = of_key(max_wave(key_of(mine)));
   real = sum_wave(real);
-  RowInfo in{real == 0 ? kNone : top == INFINITY || set.k > kMostK ? kSlow : SUMS ? kSum : kBest, INT_MIN, 0, top, 0};
-  // (a bucket by weight is a whole number that fp32 holds to a quarter)
-  if (in.state == kSum && !(fabsf(top) * set.grain < 0x1p22f && set.grain < kMostGrain)) in.state = kSlow;
-  const bool done = in.state == kNone || in.state == kSlow || (SUMS && set.top_p >= 1.f);
-  const int base = done && in.state != kSum ? 0 : top_of(bucket_of(top, SUMS, set.grain));
-  if (in.state == kSum) in.ref = (base >> 5) + 1;
-  if (done) {
-    if (threadIdx.x == 0) lds.info = in;
+  RowInfo in{real == 0 ? kNone : top == INFINITY || set.k > kMostK ? kSlow : SUMS ? kSum : kBest, 0, top, -MAX32, -MAX32, 0};
+  if (in.state == kSum && !in_range(top, set.c64)) in.state = kSlow;
+  const bool all = SUMS && set.top_p >= 1.f;
+  const int group0 = in.state == kSum || in.state == kBest ? group_of<SUMS>(top, set.c64) : 0;
+  if (in.state == kSum) in.ref = group0;
+  // the bounds that start z64 = lo and hi, and min_p's (the largest logit stays), each by a lane
+  auto bounds = [&](double lo, double hi) {
+    const bool least = set.min_p > 0.f;
+    const double z = lane == 0 ? lo : lane == 1 ? hi : __builtin_fma((double)top, set.c64, set.min64);
+    const float x = least_float(z, set.c64, set.by);
+    const float m = least ? fminf(top, __shfl(x, 2, 64)) : -MAX32;
+    in.lo = fmaxf(__shfl(x, 0, 64), m);
+    in.hi = fmaxf(__shfl(x, 1, 64), m);
+  };
+  if (in.state == kNone || in.state == kSlow || all) {
+    if (wave == 0) {
+      if (SUMS && in.state == kSum && set.min_p > 0.f) bounds(-INFINITY, -INFINITY);
+      if (lane == 0) lds.info = in;
+    }
     __syncthreads();
     return;
   }
   // groups that a slice's buckets begin below the row's
-  const int down = mine > -INFINITY ? (base - top_of(bucket_of(mine, SUMS, set.grain))) >> 5 : kBins;
+  const bool has = mine > -INFINITY && (!SUMS || in_range(mine, set.c64));
+  const int down = has ? group0 - group_of<SUMS>(mine, set.c64) : kBins;
   // a slice's weights in the row's unit, rounded
   auto in_unit = [&](unsigned long long w, int down) {
     if constexpr (!SUMS) return w;
@@ -313,12 +265,16 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
   int d[Q];
 #pragma unroll
   for (int e = 0; e < Q; ++e) {
+    if (W * e >= a.slices) break;
     const int q = min(wave + W * e, a.slices - 1);
     d[e] = __builtin_amdgcn_readlane(down, q);
     h[e] = ldg<unsigned long long>(a.coarse + (at + q) * 64 + max(lane - d[e], 0));
   }
 #pragma unroll
-  for (int e = 0; e < Q; ++e) s += wave + W * e < a.slices && lane >= d[e] ? in_unit(h[e], d[e]) : 0;
+  for (int e = 0; e < Q; ++e) {
+    if (W * e >= a.slices) break;
+    s += wave + W * e < a.slices && lane >= d[e] ? in_unit(h[e], d[e]) : 0;
+  }
   lds.part[wave][lane] = s;
   __syncthreads();
   if (wave == 0) {
@@ -334,6 +290,7 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
     if (lane == 0) {
       // (top-k: all that can be drawn is in the list, if it holds that)
       if (group < 0 && (SUMS || real > kList)) in.state = kSlow;
+      if (!SUMS) in.hi = INFINITY;
       lds.info = in;
       lds.group = group;
       lds.goal = goal;
@@ -347,6 +304,7 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
   s = 0;
 #pragma unroll
   for (int e = 0; e < Q / 2; ++e) {
+    if (2 * W * e >= a.slices) break;
     const int q = min(2 * (wave + W * e) + (lane >> 5), a.slices - 1);
     d[e] = __shfl(down, q, 64);
     const size_t i = 32 * max(group - d[e], 0) + (lane & 31);
@@ -357,8 +315,10 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
       h[e] = ldg<uint32_t>(reinterpret_cast<const uint32_t *>(from) + i);
   }
 #pragma unroll
-  for (int e = 0; e < Q / 2; ++e)
+  for (int e = 0; e < Q / 2; ++e) {
+    if (2 * W * e >= a.slices) break;
     s += 2 * (wave + W * e) + (lane >> 5) < a.slices && group >= d[e] ? in_unit(h[e], d[e]) : 0;
+  }
   lds.part[wave][lane] = s;
   __syncthreads();
   if (wave == 0) {
@@ -370,83 +330,167 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
     // (buckets are rounded one by one: the group's last, should they stay below the goal)
     const int bin = hit ? __ffsll(hit) - 1 : 31;
     const unsigned long long under = __shfl(upto - s, bin, 64);
-    if (lane == 0) {
-      lds.info.bucket = base - 32 * group - bin;
-      lds.info.want = goal > under ? goal - under : 1;
+    const int bucket = 32 * (group0 - group) - 1 - bin;
+    if constexpr (SUMS) {
+      bounds(2.0 * bucket - 0.5, 2.0 * bucket + 1.5);
+    } else {
+      in.lo = of_key((uint32_t)bucket << 15);
+      in.hi = INFINITY;
     }
+    in.want = goal > under ? goal - under : 1;
+    if (lane == 0) lds.info = in;
   }
   __syncthreads();
 }
 
+// A thread has PER logits, a wave a chunk of 64 PER.
+template <int PER, bool VEC>
+__global__ __launch_bounds__(kNT) void k_rows_scan(SampleRowsArgs a) {
+  __shared__ __align__(16) unsigned long long hist[kBins];
+  __shared__ double table[64];
+  __shared__ uint32_t tops[kNT / 64], reals[kNT / 64];
+  uint32_t *count = reinterpret_cast<uint32_t *>(hist);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y;
+  const RowSet &set = a.rows[row];
+  const bool sums = set.k == 0, bins = sums ? set.top_p < 1.f : set.k <= kMostK;
+  float v[PER];
+  load_chunk<PER, VEC>(a.x + row * a.ld, a.n, blockIdx.x * a.slice + wave * 64 * PER, v);
+  if (bins) {
+    for (int i = tid; i < (sums ? kBins : kBins / 2); i += kNT) hist[i] = 0;
+    exp2_table(table);
+  }
+  float most = -INFINITY;
+  uint32_t real = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    most = fmaxf(most, v[j]);
+    real += v[j] > -INFINITY;
+  }
+  uint32_t key = max_wave(key_of(most));
+  real = sum_wave(real);
+  const size_t at = (size_t)row * a.slices + blockIdx.x;
+  if (lane == 0) {
+    tops[wave] = key;
+    reals[wave] = real;
+    a.chunk_top[at * (kNT / 64) + wave] = of_key(key);
+  }
+  __syncthreads();
+  key = 0;
+#pragma unroll
+  for (int w = 0; w < kNT / 64; ++w) key = max(key, tops[w]);
+  const float top = of_key(key);
+  if (tid == 0) {
+    real = 0;
+    for (int w = 0; w < kNT / 64; ++w) real += reals[w];
+    a.top[at] = top;
+    a.real[at] = real;
+  }
+  if (bins && top > -INFINITY && top < INFINITY && (!sums || in_range(top, set.c64))) {
+    if (sums) {
+      const Exp2 exp2{table};
+      const int ref = ref_of(top, set.c64);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        int n;
+        const unsigned long long w = weight_of(exp2, v[j], set.c64, ref, kSliceBits, &n);
+        // (n is below 0, and above -64 50 where there is any weight)
+        if (w) atomicAdd(&hist[max(-1 - (n >> 1), 0) & (kBins - 1)], w);
+      }
+    } else {
+      const int base = bucket_of(top) | 31;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int d = base - bucket_of(v[j]);
+        if (d < kBins) atomicAdd(&count[d], 1u);
+      }
+    }
+    __syncthreads();
+    // two buckets a thread, a group 16 threads
+    unsigned long long two;
+    if (sums) {
+      const unsigned long long h0 = hist[2 * tid], h1 = hist[2 * tid + 1];
+      a.hist[at * kBins + 2 * tid] = h0;
+      a.hist[at * kBins + 2 * tid + 1] = h1;
+      two = h0 + h1;
+    } else {
+      const unsigned long long h = hist[tid];
+      a.hist[at * kBins + tid] = h;
+      two = (h & 0xFFFFFFFFu) + (h >> 32);
+    }
+    for (int o = 1; o < 16; o <<= 1) two += __shfl_xor(two, o, 64);
+    if ((tid & 15) == 0) a.coarse[at * 64 + tid / 16] = two;
+  }
+}
+
+// Each block looks for the cut (in a kernel of its own, a block a row: 5 us and a launch, 2 to 4 us here); then a wave goes
+// over its chunk once more, but for one whose largest logit lies below the cut.
 template <int PER, bool VEC>
 __global__ __launch_bounds__(kNT) void k_rows_pick(SampleRowsArgs a) {
   __shared__ double table[64];
-  __shared__ CutLds lds;
   __shared__ uint32_t places[kNT / 64];
+  __shared__ CutLds lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y;
   const RowSet &set = a.rows[row];
   const bool sums = set.k == 0, cut = sums && set.top_p < 1.f;
-  const size_t at = (size_t)row * a.slices;
+  const size_t slice = (size_t)row * a.slices + blockIdx.x, ch = slice * (kNT / 64) + wave;
   const int id0 = blockIdx.x * a.slice + wave * 64 * PER;
-  float v[PER];
-  load_chunk<PER, VEC>(a.x + row * a.ld, a.n, id0, v);
+  const float chunk_top = ldg<float>(a.chunk_top + ch);
   exp2_table(table);
   if (sums)
-    find_cut<true>(a, set, at, lds);
+    find_cut<true>(a, set, (size_t)row * a.slices, lds);
   else
-    find_cut<false>(a, set, at, lds);
-  if (blockIdx.x == 0 && tid == 0) a.info[row] = lds.info;
-  const int state = lds.info.state, bucket = lds.info.bucket, ref = lds.info.ref;
-  const float top = lds.info.top;
-  if (state == kNone || state == kSlow) return;
-
-  // ---- the slice once more
+    find_cut<false>(a, set, (size_t)row * a.slices, lds);
+  const RowInfo in = lds.info;
+  if (blockIdx.x == 0 && tid == 0) a.info[row] = in;
+  if (in.state == kNone || in.state == kSlow) return;
   const Exp2 exp2{table};
-  const double least = __builtin_fma((double)top, set.c, set.log_min);
   unsigned long long sum = 0;
   uint32_t num = 0, listed = 0;  // bit j: logit j goes to the list
+  float v[PER];
+  if (chunk_top >= in.lo) {
+    load_chunk<PER, VEC>(a.x + row * a.ld, a.n, id0, v);
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int g = bucket_of(v[j], sums, set.grain);
-    if (!(v[j] > -INFINITY && g >= bucket && (!sums || v[j] == top || (double)v[j] * set.c >= least))) continue;
-    if (!sums || (cut && g == bucket)) {
-      listed |= 1u << j;
-    } else {
-      sum += weight_of(exp2, v[j], set.c, ref, a.bits);
-      ++num;
+    for (int j = 0; j < PER; ++j) {
+      listed |= (uint32_t)(v[j] >= in.lo && v[j] < in.hi) << j;
+      int n;
+      if (v[j] >= in.hi) {
+        sum += weight_of(exp2, v[j], set.c64, in.ref, a.bits, &n);
+        ++num;
+      }
+    }
+    if (sums) {
+      sum = sum_wave(sum);
+      num = sum_wave(num);
     }
   }
-  // the block's candidates: one place in the list for all (a round trip for each would be most of the time)
+  if (sums && lane == 0) {
+    a.chunk[ch] = sum;
+    a.chunk_n[ch] = num;
+  }
+  // the slice's candidates, in a place of their own (a list for the row, whose end blocks ask for by an atomic: 4 us, one
+  // block after the other)
   if (!sums || cut) {
     const uint32_t mine = __popc(listed), upto = scan_wave(mine);
     if (lane == 63) places[wave] = upto;
     __syncthreads();
-    if (wave == 0) {
-      const uint32_t p = lane < kNT / 64 ? places[lane] : 0, q = scan_wave(p);
-      uint32_t base = 0;
-      if (lane == 63 && q) base = atomicAdd(a.n_list + row, q);
-      base = last_lane(base);
-      if (lane < kNT / 64) places[lane] = base + q - p;
+    uint32_t at = upto - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < kNT / 64; ++w) {
+      const uint32_t p = places[w];
+      at += w < wave ? p : 0;
+      all += p;
     }
-    __syncthreads();
-    uint32_t at_list = places[wave] + upto - mine;
+    if (tid == 0) a.n_list[slice] = all;
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (listed >> j & 1) {
-        if (at_list < kList)
-          a.list[(size_t)row * kList + at_list] = (unsigned long long)key_of(v[j]) << 32 |
-                                                  (0xFFFFFFFFu - (uint32_t)(id0 + 256 * (j / 4) + 4 * lane + j % 4));
-        ++at_list;
+        if (at < kSliceList)
+          a.list[slice * kSliceList + at] = (unsigned long long)key_of(v[j]) << 32 |
+                                            (0xFFFFFFFFu - (uint32_t)(id0 + 256 * (j / 4) + 4 * lane + j % 4));
+        ++at;
       }
-  }
-  if (sums) {
-    sum = sum_wave(sum);
-    num = sum_wave(num);
-    if (lane == 0) {
-      const size_t ch = (at + blockIdx.x) * (kNT / 64) + wave;
-      a.chunk[ch] = sum;
-      a.chunk_n[ch] = num;
-    }
+  } else if (tid == 0) {
+    a.n_list[slice] = 0;
   }
 }
 
@@ -756,20 +800,12 @@ __device__ inline void write_row(const SampleRowsArgs &a, int row, int id, float
   if (a.kept) a.kept[row] = (int)kept;
 }
 
-// The draw of a row whose best ids are the sorted list's first, nk of them, E of these a lane (a thread).  BLOCK: by
-// all threads, else by one wave.
-template <bool BLOCK, int E>
-__device__ inline void draw_best(const SampleRowsArgs &a, const RowSet &set, int row, float top, int nk, float u,
-                                 const Exp2 &exp2, unsigned long long *list, unsigned long long *by_place,
-                                 unsigned long long *part, uint32_t *counts) {
-  const int at = (BLOCK ? threadIdx.x : threadIdx.x & 63) * E;
-  auto run = [&](unsigned long long v, unsigned long long *all) {
-    if constexpr (BLOCK) return run_sum(v, part, all);
-    v = scan_wave(v);
-    *all = last_lane(v);
-    return v;
-  };
-  unsigned long long w[E], sum = 0, total;
+// The draw of a row whose best ids are the sorted list's first, nk of them, E of these a lane, by one wave.
+template <int E>
+__device__ inline void draw_few(const SampleRowsArgs &a, const RowSet &set, int row, float top, int nk, float u,
+                                const Exp2 &exp2, unsigned long long *list, unsigned long long *by_place) {
+  const int at = (threadIdx.x & 63) * E;
+  unsigned long long w[E], sum = 0;
   uint32_t id[E], over = 0, under = 0;  // how many min_p leaves, and top-p
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -777,38 +813,29 @@ __device__ inline void draw_best(const SampleRowsArgs &a, const RowSet &set, int
     const unsigned long long x = in ? list[at + e] : 0;
     const float v = logit_of(x);
     id[e] = id_of(x);
-    const double t = v == top ? 0.0 : ((double)v - (double)top) * set.c;
-    w[e] = in ? exp2(t, a.bits) : 0;
-    over += __popcll(__ballot(in && (v == top || t >= set.log_min)));
+    const double z = v == top ? 0.0 : ((double)v - (double)top) * set.c64;
+    int n;
+    w[e] = in ? exp2(z, a.bits, &n) : 0;
+    over += __popcll(__ballot(in && (v == top || z >= set.min64)));
     sum += w[e];
   }
-  unsigned long long upto = run(sum, &total) - sum;
+  unsigned long long upto = scan_wave(sum), total = last_lane(upto);
+  upto -= sum;
   const unsigned long long goal = set.temperature != 0.f && set.top_p < 1.f ? share_of(set.top_p, total) : ~0ull;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     under += __popcll(__ballot(at + e < nk && upto < goal));
     upto += w[e];
   }
-  if constexpr (BLOCK) {
-    if ((threadIdx.x & 63) == 0) {
-      atomicAdd(counts, over);
-      atomicAdd(counts + 1, under);
-    }
-    __syncthreads();
-    over = counts[0];
-    under = counts[1];
-  }
-  const int n = (int)min(over, under), size = power_of_two(n);
+  const int n = (int)min(over, under);
   // ---- in the order of ids: (id, place) sorted, the weights by their places
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (at + e < size) list[at + e] = at + e < n ? (unsigned long long)(0xFFFFFFFFu - id[e]) << 32 | (uint32_t)(at + e) : 0;
-    if (at + e < n) by_place[at + e] = w[e];
-  }
-  if constexpr (BLOCK)
-    sort_falling(list, size);
-  else
-    sort_by_wave(list, n);
+  for (int e = 0; e < E; ++e)
+    if (at + e < n) {
+      list[at + e] = (unsigned long long)(0xFFFFFFFFu - id[e]) << 32 | (uint32_t)(at + e);
+      by_place[at + e] = w[e];
+    }
+  sort_by_wave(list, n);
   sum = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -817,7 +844,9 @@ __device__ inline void draw_best(const SampleRowsArgs &a, const RowSet &set, int
     w[e] = at + e < n ? by_place[(uint32_t)x] : 0;
     sum += w[e];
   }
-  upto = run(sum, &total) - sum;
+  upto = scan_wave(sum);
+  total = last_lane(upto);
+  upto -= sum;
   const unsigned long long target = target_of(u, total);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -826,69 +855,236 @@ __device__ inline void draw_best(const SampleRowsArgs &a, const RowSet &set, int
   }
 }
 
+// The chunk in which the running weight passes the target, by one wave: *before, what the chunks before it weigh.
+__device__ inline int find_chunk(const unsigned long long *chunk, int n_chunks, float u, unsigned long long *total,
+                                 unsigned long long *target, unsigned long long *before) {
+  const int lane = threadIdx.x & 63, per = (n_chunks + 63) / 64;
+  unsigned long long sum = 0;
+  for (int i = 0; i < per; ++i) sum += per * lane + i < n_chunks ? chunk[per * lane + i] : 0;
+  const unsigned long long upto = scan_wave(sum);
+  *total = last_lane(upto);
+  *target = target_of(u, *total);
+  const int l = __ffsll((unsigned long long)__ballot(upto > *target)) - 1;
+  unsigned long long b = __shfl(upto - sum, l, 64);
+  int hit = per * l;
+  while (b + chunk[hit] <= *target) b += chunk[hit++];
+  *before = b;
+  return hit;
+}
+
+struct ManyLds {
+  unsigned long long bin[kBins];
+  unsigned long long part[kNT / 64];
+  unsigned long long before, cut;
+  int found;
+  uint32_t num, kept;
+};
+
+// The same of a longer list, by all threads.  Nothing is sorted but what lies in the bucket of a cut (top-k's, then
+// top-p's) and in the chunk of ids in which the draw falls.  (Sorted as a whole, 1000 ids of 48 rows: 20 us.)
+__device__ inline void draw_many(const SampleRowsArgs &a, const RowSet &set, int row, const RowInfo &in, int n_list,
+                                 float u, const Exp2 &exp2, unsigned long long *list, unsigned long long *chunk,
+                                 int n_chunks, int chunk_len, ManyLds &lds) {
+  constexpr int E = kList / kNT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  unsigned long long x[E], w[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = kNT * e + tid < n_list ? list[kNT * e + tid] : 0;
+  // those that `which` says, into the list from its start, the largest first
+  auto gather = [&](const auto &which) {
+    __syncthreads();
+    if (tid == 0) lds.num = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (kNT * e >= n_list) break;
+      const bool is = x[e] && which(x[e]);
+      const unsigned long long m = __ballot(is);
+      uint32_t at = 0;
+      if (m) {
+        if (lane == 0) at = atomicAdd(&lds.num, (uint32_t)__popcll(m));
+        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + __popcll(m & ((1ull << lane) - 1));
+      }
+      if (is) list[at] = x[e];
+    }
+    __syncthreads();
+    const int num = (int)lds.num;
+    if (num <= kWave) {
+      if (wave == 0) sort_by_wave(list, num);
+      __syncthreads();
+    } else {
+      const int size = power_of_two(num);
+      for (int i = num + tid; i < size; i += kNT) list[i] = 0;
+      sort_falling(list, size);
+    }
+    return num;
+  };
+
+  // ---- top-k: of the last bucket's, as many as it takes
+  if (n_list > set.k) {
+    const uint32_t last = key_of(in.lo) >> 15;
+    gather([&](unsigned long long y) { return (uint32_t)(y >> 47) == last; });
+    const unsigned long long cut = list[in.want - 1];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (x[e] < cut) x[e] = 0;
+  }
+  // ---- weights, min_p, and for top-p their histogram
+  const uint32_t base = key_of(in.top) >> 15;
+  const bool cut_p = set.top_p < 1.f;
+  for (int i = tid; i < kBins; i += kNT) lds.bin[i] = 0;
+  for (int i = tid; i < n_chunks; i += kNT) chunk[i] = 0;
+  if (tid == 0) lds.kept = 0;
+  __syncthreads();
+  auto bin_of = [&](unsigned long long y) { return min((int)(base - (uint32_t)(y >> 47)), kBins - 1); };
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (kNT * e >= n_list) break;
+    const double z = logit_of(x[e]) == in.top ? 0.0 : ((double)logit_of(x[e]) - (double)in.top) * set.c64;
+    int n;
+    w[e] = x[e] ? exp2(z, a.bits, &n) : 0;
+    if (cut_p && w[e]) atomicAdd(&lds.bin[bin_of(x[e])], w[e]);
+  }
+  if (cut_p) {
+    __syncthreads();
+    const unsigned long long h0 = lds.bin[2 * tid], h1 = lds.bin[2 * tid + 1];
+    unsigned long long total;
+    const unsigned long long upto = run_sum(h0 + h1, lds.part, &total), goal = share_of(set.top_p, total);
+    if (upto >= goal && upto - h0 - h1 < goal) {
+      const bool second = upto - h1 < goal;
+      lds.found = 2 * tid + second;
+      lds.before = second ? upto - h1 : upto - h0 - h1;
+    }
+    __syncthreads();
+    const int found = lds.found;
+    const int num = gather([&](unsigned long long y) { return bin_of(y) == found; });
+    if (wave == 0) {
+      unsigned long long before = lds.before, cut = 0;
+      for (int i0 = 0; i0 < num && before < goal; i0 += 64) {
+        const unsigned long long y = i0 + lane < num ? list[i0 + lane] : 0;
+        const double z = logit_of(y) == in.top ? 0.0 : ((double)logit_of(y) - (double)in.top) * set.c64;
+        int n;
+        const unsigned long long v = y ? exp2(z, a.bits, &n) : 0, upto = before + scan_wave(v);
+        const unsigned long long m = __ballot(y && upto - v < goal);
+        if (m) cut = __shfl(y, 63 - __clzll(m), 64);
+        before = last_lane(upto);
+      }
+      if (lane == 0) lds.cut = cut;
+    }
+    __syncthreads();
+    const unsigned long long cut = lds.cut;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (x[e] < cut) x[e] = 0;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (kNT * e >= n_list) break;
+    const float v = logit_of(x[e]);
+    if (x[e] && !(v == in.top || ((double)v - (double)in.top) * set.c64 >= set.min64)) x[e] = 0;
+    const unsigned long long m = __ballot(x[e] != 0);
+    if (lane == 0 && m) atomicAdd(&lds.kept, (uint32_t)__popcll(m));
+    if (x[e]) atomicAdd(&chunk[id_of(x[e]) / chunk_len], w[e]);
+  }
+  __syncthreads();
+  unsigned long long total, target, before;
+  int hit = 0;
+  if (wave == 0) {
+    hit = find_chunk(chunk, n_chunks, u, &total, &target, &before);
+    if (lane == 0) lds.found = hit;
+  }
+  __syncthreads();
+  hit = lds.found;
+  // (turned to the order of ids: the lowest id first is the largest number)
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = x[e] ? x[e] << 32 | x[e] >> 32 : 0;
+  const int num = gather([&](unsigned long long y) { return (int)((0xFFFFFFFFu - (uint32_t)(y >> 32)) / chunk_len) == hit; });
+  if (wave != 0) return;
+  for (int i0 = 0; i0 < num; i0 += 64) {
+    const unsigned long long y = i0 + lane < num ? list[i0 + lane] : 0;
+    const float v = of_key((uint32_t)y);
+    const double z = v == in.top ? 0.0 : ((double)v - (double)in.top) * set.c64;
+    int n;
+    const unsigned long long w = y ? exp2(z, a.bits, &n) : 0, upto = before + scan_wave(w);
+    if (upto > target && upto - w <= target)
+      write_row(a, row, (int)(0xFFFFFFFFu - (uint32_t)(y >> 32)), (float)((double)w / (double)total), lds.kept);
+    before = last_lane(upto);
+  }
+}
+
+template <int PER>
 __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   __shared__ __align__(16) unsigned long long list[kList];
   __shared__ __align__(16) unsigned long long chunk[kMostSlices * 16];
   __shared__ double table[64];
-  __shared__ unsigned long long part[16];
-  __shared__ DigitLds digits;
-  __shared__ uint32_t counts[2];
+  __shared__ union { DigitLds digits; ManyLds many; } lds;
+  __shared__ uint32_t counted;
+  constexpr int chunk_len = 64 * PER;
   const int tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
   const RowSet &set = a.rows[row];
   const RowInfo in = a.info[row];
-  const uint32_t n_list = a.n_list[row];
+  // the slices' candidates, one after the other; what a wave copies: every 16th slice's
+  const size_t at = (size_t)row * a.slices;
+  const int wave = tid >> 6;
+  const uint32_t mine = in.state != kNone && in.state != kSlow && lane < a.slices ? ldg<uint32_t>(a.n_list + at + lane) : 0;
+  const bool fits = !__any(mine > kSliceList);
+  const uint32_t listed = scan_wave(mine), n_list = last_lane(listed);
   if (in.state == kNone) {
     if (tid == 0) write_row(a, row, -1, 0.f, 0);
     return;
   }
-  if (in.state == kSlow || n_list > kList) {
-    row_by_digits(a, digits);
+  if (in.state == kSlow || !fits || n_list > kList) {
+    row_by_digits(a, lds.digits);
     return;
   }
   exp2_table(table);
   const Exp2 exp2{table};
   const float u = ldg<float>(a.u + row);
-  const int n_chunks = a.slices * (kNT / 64), chunk_len = a.slice / (kNT / 64);
+  const int n_chunks = a.slices * (kNT / 64);
   uint32_t kept = 0;
   if (in.state == kSum && tid < n_chunks) {
-    chunk[tid] = a.chunk[(size_t)row * n_chunks + tid];
-    kept = a.chunk_n[(size_t)row * n_chunks + tid];
+    chunk[tid] = a.chunk[at * (kNT / 64) + tid];
+    kept = a.chunk_n[at * (kNT / 64) + tid];
   }
-  const int size = n_list ? power_of_two((int)n_list) : 0;
-  for (int i = tid; i < size; i += kNT) list[i] = i < (int)n_list ? a.list[(size_t)row * kList + i] : 0;
-  if (tid < 2) counts[tid] = 0;
+  for (int q = wave; q < a.slices; q += kNT / 64) {
+    const int num = __builtin_amdgcn_readlane((int)mine, q), from = __builtin_amdgcn_readlane((int)(listed - mine), q);
+    for (int i = lane; i < num; i += 64) list[from + i] = ldg<unsigned long long>(a.list + (at + q) * kSliceList + i);
+  }
+  if (tid == 0) counted = 0;
   __syncthreads();
   if (in.state == kBest) {
-    const int nk = min(set.k, (int)n_list);
-    if (n_list <= kWave) {
-      if (tid >= 64) return;
+    if (n_list > kWave) {
+      draw_many(a, set, row, in, (int)n_list, u, exp2, list, chunk, n_chunks, chunk_len, lds.many);
+    } else if (wave == 0) {
+      const int nk = min(set.k, (int)n_list);
       sort_by_wave(list, (int)n_list);
       if (nk <= 64)
-        draw_best<false, 1>(a, set, row, in.top, nk, u, exp2, list, list + 4096, part, counts);
+        draw_few<1>(a, set, row, in.top, nk, u, exp2, list, list + kWave);
       else
-        draw_best<false, kWave / 64>(a, set, row, in.top, nk, u, exp2, list, list + 4096, part, counts);
-    } else {
-      sort_falling(list, size);
-      draw_best<true, kMostK / kNT>(a, set, row, in.top, nk, u, exp2, list, list + 4096, part, counts);
+        draw_few<kWave / 64>(a, set, row, in.top, nk, u, exp2, list, list + kWave);
     }
     return;
   }
 
   // ---- the weights of the chunks, and of the candidates as many as it takes
   kept = sum_wave(kept);
-  if (lane == 0 && kept) atomicAdd(counts, kept);
-  if (n_list > kWave)
+  if (lane == 0 && kept) atomicAdd(&counted, kept);
+  if (n_list > kWave) {
+    const int size = power_of_two((int)n_list);
+    for (int i = (int)n_list + tid; i < size; i += kNT) list[i] = 0;
     sort_falling(list, size);
-  else
+  } else {
     __syncthreads();
-  if (tid >= 64) return;
+  }
+  if (wave != 0) return;
   if (n_list <= kWave) sort_by_wave(list, (int)n_list);
   unsigned long long before = 0, cut = ~0ull;
   uint32_t taken = 0;
   for (int i0 = 0; i0 < (int)n_list && before < in.want; i0 += 64) {
     const int i = i0 + lane;
     const unsigned long long x = i < (int)n_list ? list[i] : 0;
-    const unsigned long long w = i < (int)n_list ? weight_of(exp2, logit_of(x), set.c, in.ref, a.bits) : 0;
+    int n;
+    const unsigned long long w = i < (int)n_list ? weight_of(exp2, logit_of(x), set.c64, in.ref, a.bits, &n) : 0;
     const unsigned long long upto = before + scan_wave(w);
     const bool take = i < (int)n_list && upto - w < in.want;
     if (take) atomicAdd(&chunk[id_of(x) / chunk_len], w);
@@ -899,39 +1095,29 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   // ---- the chunk, then the id, at which the running weight passes the target
-  const int per = (n_chunks + 63) / 64;
-  unsigned long long sum = 0;
-  for (int i = 0; i < per; ++i) sum += per * lane + i < n_chunks ? chunk[per * lane + i] : 0;
-  unsigned long long upto = scan_wave(sum);
-  const unsigned long long total = last_lane(upto), target = target_of(u, total);
-  const int l = __ffsll((unsigned long long)__ballot(upto > target)) - 1;
-  before = __shfl(upto - sum, l, 64);
-  int hit = per * l;
-  while (before + chunk[hit] <= target) before += chunk[hit++];
-  const double least = __builtin_fma((double)in.top, set.c, set.log_min);
+  unsigned long long total, target;
+  const int hit = find_chunk(chunk, n_chunks, u, &total, &target, &before);
   const float *x = a.x + row * a.ld;
-  float v[16];
+  const int id0 = hit * chunk_len + PER * lane;
+  float v[PER];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int id = hit * chunk_len + 64 * e + lane;
-    v[e] = 64 * e < chunk_len && id < a.n ? ldg<float>(x + id) : -INFINITY;
+  for (int e = 0; e < PER; ++e) v[e] = id0 + e < a.n ? ldg<float>(x + id0 + e) : -INFINITY;
+  unsigned long long w[PER], sum = 0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    int n;
+    w[e] = 0;
+    if (v[e] >= in.hi ||
+        (v[e] >= in.lo && ((unsigned long long)key_of(v[e]) << 32 | (0xFFFFFFFFu - (uint32_t)(id0 + e))) >= cut))
+      w[e] = weight_of(exp2, v[e], set.c64, in.ref, a.bits, &n);
+    sum += w[e];
   }
-  for (int e = 0; 64 * e < chunk_len; ++e) {
-    const int id = hit * chunk_len + 64 * e + lane;
-    float y = v[0];
+  unsigned long long upto = before + scan_wave(sum) - sum;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) y = i == e ? v[i] : y;
-    unsigned long long w = 0;
-    if (y > -INFINITY) {
-      const bool in_cut = bucket_of(y, true, set.grain) > in.bucket ||
-                          ((unsigned long long)key_of(y) << 32 | (0xFFFFFFFFu - (uint32_t)id)) >= cut;
-      if ((in.bucket == INT_MIN || in_cut) && (y == in.top || (double)y * set.c >= least))
-        w = weight_of(exp2, y, set.c, in.ref, a.bits);
-    }
-    const unsigned long long upto = before + scan_wave(w);
-    if (upto > target && upto - w <= target) write_row(a, row, id, (float)((double)w / (double)total), counts[0] + taken);
-    before = last_lane(upto);
-    if (before > target) break;
+  for (int e = 0; e < PER; ++e) {
+    if (upto <= target && upto + w[e] > target)
+      write_row(a, row, id0 + e, (float)((double)w[e] / (double)total), counted + taken);
+    upto += w[e];
   }
 }
 
@@ -945,6 +1131,7 @@ void launch_slices(const SampleRowsArgs &a, int rows, bool vec, hipStream_t st) 
     hipLaunchKernelGGL((k_rows_scan<PER, false>), grid, blk, 0, st, a);
     hipLaunchKernelGGL((k_rows_pick<PER, false>), grid, blk, 0, st, a);
   }
+  hipLaunchKernelGGL(k_rows_draw<PER>, dim3(rows), blk, 0, st, a);
 }
 
 // Rows of more ids than the slices hold.
@@ -992,16 +1179,17 @@ extern "C" int ms_sample_rows(const float *d_logits, size_t in_stride, int rows,
   if (sliced) {
     const size_t cells = (size_t)m0 * a.slices, chunks = cells * (kNT / 64);
     void *buf = nullptr;
-    if (int rc = scratch(cells * (kBins * 8 + 64 * 8 + 8) + chunks * 12 + m0 * (kList * 8 + sizeof(RowInfo) + 4) + 64, &buf)) return rc;
+    if (int rc = scratch(cells * ((kBins + 64 + kSliceList) * 8 + 12) + chunks * 16 + m0 * sizeof(RowInfo) + 64, &buf)) return rc;
     a.hist = static_cast<unsigned long long *>(buf);
     a.coarse = a.hist + cells * kBins;
     a.list = a.coarse + cells * 64;
-    a.chunk = a.list + (size_t)m0 * kList;
+    a.chunk = a.list + cells * kSliceList;
     a.info = reinterpret_cast<RowInfo *>(a.chunk + chunks);
     a.top = reinterpret_cast<float *>(a.info + m0);
     a.real = reinterpret_cast<uint32_t *>(a.top + cells);
     a.n_list = a.real + cells;
-    a.chunk_n = a.n_list + m0;
+    a.chunk_n = a.n_list + cells;
+    a.chunk_top = reinterpret_cast<float *>(a.chunk_n + chunks);
   }
   for (int r0 = 0; r0 < rows; r0 += kRows) {
     const int m = rows - r0 < kRows ? rows - r0 : kRows;
@@ -1013,9 +1201,9 @@ extern "C" int ms_sample_rows(const float *d_logits, size_t in_stride, int rows,
     for (int r = 0; r < kRows; ++r) {
       const ms_sample_row &w = h_rows[r0 + (r < m ? r : 0)];
       const bool best = w.temperature == 0.f;
-      a.rows[r].c = best ? 0.0 : 1.4426950408889634 / (double)w.temperature;
-      a.rows[r].log_min = w.min_p > 0.f ? std::log2((double)w.min_p) : -INFINITY;
-      a.rows[r].grain = best ? 0.f : (float)(32 * 1.4426950408889634 / (double)w.temperature);
+      a.rows[r].c64 = best ? 0.0 : 64 * 1.4426950408889634 / (double)w.temperature;
+      a.rows[r].by = best ? 0.0 : 1.0 / a.rows[r].c64;
+      a.rows[r].min64 = w.min_p > 0.f ? 64 * std::log2((double)w.min_p) : -INFINITY;
       a.rows[r].temperature = w.temperature;
       a.rows[r].top_p = w.top_p;
       a.rows[r].min_p = w.min_p;
@@ -1028,7 +1216,6 @@ extern "C" int ms_sample_rows(const float *d_logits, size_t in_stride, int rows,
         launch_slices<16>(a, m, vec, st);
       else
         launch_slices<4>(a, m, vec, st);
-      hipLaunchKernelGGL(k_rows_draw, dim3(m), dim3(kNT), 0, st, a);
     }
     MS_HIP_TRY(hipGetLastError());
   }
