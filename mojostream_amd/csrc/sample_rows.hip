@@ -11,7 +11,7 @@
 //               candidates (top-k: all down to the cut's bucket; top-p: those in it) into a list, the weights
 //               of what lies above it added up by chunks of 1024 ids
 //  k_rows_draw  a block a row: sorts the candidates, finds the cut and draws.  Rows that this does not
-//               fit (more candidates than the list holds, a large top-k, infinite logits) it goes over digit by digit.
+//               fit (more candidates than the list holds, a large top-k, infinite logits) it goes over as a whole.
 #include <climits>
 #include <cmath>
 
@@ -46,7 +46,7 @@ struct RowSet {
   float temperature, top_p, min_p;
   int k;            // ids that top-k leaves; 0: all
 };
-enum { kNone, kBest, kSum, kSlow };  // nothing to draw; by the list; by sums (and the list); digit by digit
+enum { kNone, kBest, kSum, kSlow };  // nothing to draw; by the list; by sums (and the list); as a whole
 
 struct SampleRowsArgs {
   const float *x;
@@ -494,216 +494,6 @@ __global__ __launch_bounds__(kNT) void k_rows_pick(SampleRowsArgs a) {
   }
 }
 
-struct DigitLds {
-  uint32_t cnt[256];
-  unsigned long long wt[256];
-  unsigned long long part[16];
-  uint32_t red[16];
-  uint32_t s_key, s_count;
-  unsigned long long s_above;
-  int s_id;
-};
-
-// The whole of a row, by one block.  The cut is found digit by digit of the logits' keys: a histogram
-// of the counts (top-k) or weights (top-p) of the logits that agree with the digits found so far.
-__device__ void row_by_digits(const SampleRowsArgs &a, DigitLds &lds) {
-  uint32_t *cnt = lds.cnt, *red = lds.red, &s_key = lds.s_key, &s_count = lds.s_count;
-  unsigned long long *wt = lds.wt, *part = lds.part, &s_above = lds.s_above;
-  int &s_id = lds.s_id;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n;
-  const RowSet &set = a.rows[blockIdx.x];
-  const float *x = a.x + blockIdx.x * a.ld;
-
-  // ---- maximum, and how many can be drawn
-  uint32_t top = 0, real = 0;
-  for (int i = tid; i < n; i += kNT) {
-    const uint32_t k = key_of(ldg<float>(x + i));
-    top = max(top, k);
-    real += k != 0;
-  }
-  top = max_wave(top);
-  real = sum_wave(real);
-  if (lane == 0) {
-    red[wave] = top;
-    cnt[wave] = real;
-  }
-  __syncthreads();
-  real = 0;
-  for (int w = 0; w < kNT / 64; ++w) {
-    top = max(top, red[w]);
-    real += cnt[w];
-  }
-  if (real == 0) {
-    if (tid == 0) {
-      a.ids[blockIdx.x] = -1;
-      if (a.prob) a.prob[blockIdx.x] = 0.f;
-      if (a.kept) a.kept[blockIdx.x] = 0;
-    }
-    return;
-  }
-  const double vmax = of_key(top), temp = set.temperature;
-  auto share = [&](float v) { return v == (float)vmax ? 1.0 : exp(((double)v - vmax) / temp); };
-  auto weight = [&](float v) { return (unsigned long long)rint(ldexp(share(v), a.bits)); };
-
-  // The cut where the count (or weight) from the top reaches `want`, of what lies at or above `floor` (of
-  // those equal to it, floor_count): key, how many of the logits equal to it, what lies above it.
-  uint32_t cut_key, cut_count;
-  unsigned long long above;
-  auto find = [&](bool by_weight, unsigned long long want, uint32_t floor, uint32_t floor_count) {
-    uint32_t prefix = 0;
-    above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (tid < 256) {
-        cnt[tid] = 0;
-        wt[tid] = 0;
-      }
-      __syncthreads();
-      for (int i = tid; i < n; i += kNT) {
-        const float v = ldg<float>(x + i);
-        const uint32_t k = key_of(v);
-        if (k < floor || k == 0 || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
-        atomicAdd(&cnt[k >> shift & 255], 1u);
-        if (by_weight && k > floor) atomicAdd(&wt[k >> shift & 255], weight(v));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        unsigned long long sum = above;
-        const unsigned long long at_floor = by_weight ? floor_count * weight(of_key(floor)) : 0;
-        int d = 255;
-        for (; d > 0; --d) {
-          unsigned long long w = cnt[d];
-          if (by_weight) {
-            w = wt[d];
-            if ((prefix << 8 | d) == floor >> shift) w += at_floor;
-          }
-          if (sum + w >= want) break;
-          sum += w;
-        }
-        s_key = prefix << 8 | d;
-        s_above = sum;
-        s_count = cnt[d];
-      }
-      __syncthreads();
-      prefix = s_key;
-      above = s_above;
-    }
-    cut_key = prefix;
-    cut_count = s_count;
-  };
-
-  uint32_t key = 1;  // (below every number's)
-  uint32_t eq = 0, eq_all = 0;  // of the logits equal to the cut, the first eq are left
-  const unsigned long long all_k = set.k > 0 ? set.k : real;
-  if (all_k < real) {
-    find(false, all_k, 1, 0);
-    key = cut_key;
-    eq = (uint32_t)(all_k - above);
-    eq_all = cut_count;
-  }
-  uint32_t last_eq = 0xFFFFFFFFu;  // the last id of those equal to the cut
-  auto block_sum = [&](unsigned long long v) {
-    v = sum_wave(v);
-    __syncthreads();
-    if (lane == 0) part[wave] = v;
-    __syncthreads();
-    v = 0;
-    for (int w = 0; w < kNT / 64; ++w) v += part[w];
-    return v;
-  };
-  if (set.temperature != 0.f && set.top_p < 1.f) {
-    unsigned long long sum = 0;
-    for (int i = tid; i < n; i += kNT) {
-      const float v = ldg<float>(x + i);
-      if (key_of(v) > key) sum += weight(v);
-    }
-    sum = block_sum(sum);
-    const unsigned long long w_eq = key > 1 ? weight(of_key(key)) : 0;
-    sum += eq * w_eq;
-    unsigned long long want = (unsigned long long)ceil((double)set.top_p * (double)sum);
-    if (want == 0) want = 1;
-    find(true, want, key, key > 1 ? eq : 0);
-    const uint32_t have = cut_key == key && key > 1 ? eq : cut_count;
-    const unsigned long long w = weight(of_key(cut_key));
-    const unsigned long long take = w ? (want - above + w - 1) / w : 1;
-    key = cut_key;
-    eq = (uint32_t)(take < have ? take : have);
-    eq_all = cut_count;
-  }
-  if (eq < eq_all) {
-    // ---- the eq-th id that is equal to the cut
-    uint32_t seen = 0;
-    for (int i0 = 0; i0 < n; i0 += kNT) {
-      const int i = i0 + tid;
-      const bool is = i < n && key_of(ldg<float>(x + i)) == key;
-      const unsigned long long m = __ballot(is);
-      __syncthreads();
-      if (lane == 0) red[wave] = __popcll(m);
-      __syncthreads();
-      uint32_t before = seen;
-      for (int w = 0; w < kNT / 64; ++w) {
-        if (w < wave) before += red[w];
-        seen += red[w];
-      }
-      if (is && before + __popcll(m & ((1ull << lane) - 1)) == eq - 1) s_id = i;
-      if (seen >= eq) break;
-    }
-    __syncthreads();
-    last_eq = (uint32_t)s_id;
-  }
-  auto left = [&](float v, int i) {
-    const uint32_t k = key_of(v);
-    if (k < key || k == 0 || (k == key && (uint32_t)i > last_eq)) return false;
-    return k == top || share(v) >= (double)set.min_p;
-  };
-  // ---- the draw: the wave, then the sixteenth of its part, and so on, in which the running weight passes the target
-  unsigned long long total = 0, target = 0, before = 0, count = 0;
-  int lo = 0, len = n;
-  for (bool first = true; len > 64 || first; first = false) {
-    const int per = ((len + 15) / 16 + 63) / 64 * 64, b0 = lo + min(len, wave * per), b1 = lo + min(len, wave * per + per);
-    unsigned long long sum = 0, num = 0;
-    for (int i = b0 + lane; i < b1; i += 64) {
-      const float v = ldg<float>(x + i);
-      if (left(v, i)) {
-        sum += weight(v);
-        ++num;
-      }
-    }
-    sum = sum_wave(sum);
-    if (first) num = block_sum(num);
-    __syncthreads();
-    if (lane == 0) part[wave] = sum;
-    __syncthreads();
-    if (first) {
-      count = num;
-      for (int w = 0; w < 16; ++w) total += part[w];
-      const float u = ldg<float>(a.u + blockIdx.x);
-      target = !(u > 0.f) ? 0 : u >= 1.f ? total - 1 : (unsigned long long)((double)u * (double)total);
-      if (target >= total) target = total - 1;
-    }
-    int w = 0;
-    while (w < 15 && before + part[w] <= target) before += part[w++];
-    lo += min(len, w * per);
-    len = min(len - min(len, w * per), per);
-  }
-  if (wave == 0) {
-    const int i = lo + lane;
-    unsigned long long w = 0;
-    if (lane < len) {
-      const float v = ldg<float>(x + i);
-      if (left(v, i)) w = weight(v);
-    }
-    const unsigned long long upto = scan_wave(w);
-    const unsigned long long hit = __ballot(before + upto > target);
-    const int l = __ffsll((unsigned long long)hit) - 1;
-    if (lane == l) {
-      a.ids[blockIdx.x] = i;
-      if (a.prob) a.prob[blockIdx.x] = (float)((double)w / (double)total);
-      if (a.kept) a.kept[blockIdx.x] = (int)count;
-    }
-  }
-}
-
 // Falling order of n numbers, n a power of two from 64 on.  A wave does the steps within 128 numbers of its own
 // without waiting for the others.
 __device__ inline void sort_falling(unsigned long long *x, int n) {
@@ -800,6 +590,188 @@ __device__ inline void write_row(const SampleRowsArgs &a, int row, int id, float
   if (a.kept) a.kept[row] = (int)kept;
 }
 
+struct RowLds {
+  unsigned long long bin[kBins];
+  unsigned long long part[kNT / 64];
+  unsigned long long before, cut;
+  int found;
+  uint32_t num, kept;
+};
+
+// The bin (of two of each thread's) at which the running sum reaches goal: to lds.found, what lies before it to lds.before.
+__device__ inline void find_bin(RowLds &lds, unsigned long long before, unsigned long long goal) {
+  const unsigned long long h0 = lds.bin[2 * threadIdx.x], h1 = lds.bin[2 * threadIdx.x + 1];
+  unsigned long long total;
+  const unsigned long long upto = before + run_sum(h0 + h1, lds.part, &total);
+  if (upto >= goal && upto - h0 - h1 < goal) {
+    const bool second = upto - h1 < goal;
+    lds.found = 2 * threadIdx.x + second;
+    lds.before = second ? upto - h1 : upto - h0 - h1;
+  }
+  __syncthreads();
+}
+
+// The whole of a row, by one block.  The cut's logit is found by histograms over the keys of a range,
+// by counts (top-k) or weights (top-p), the range then being the bin that the cut lies in.  (One row of 262144
+// logits that are all alike, about ten times over the row: 0.5 ms.)
+__device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, RowLds &lds) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n, row = blockIdx.x;
+  const RowSet &set = a.rows[row];
+  const float *x = a.x + row * a.ld;
+  auto each = [&](int from, int to, int step, const auto &f) {  // eight loads in flight
+    for (int i0 = from; i0 < to; i0 += 8 * step) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = ldg<float>(x + min(i0 + e * step, to - 1));
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i0 + e * step < to) f(v[e], i0 + e * step);
+    }
+  };
+  auto over_block = [&](unsigned long long v) {
+    unsigned long long all;
+    run_sum(v, lds.part, &all);
+    __syncthreads();
+    return all;
+  };
+
+  // ---- largest and least logit, and how many can be drawn
+  uint32_t top = 0, least = 0xFFFFFFFFu, mine = 0;
+  each(tid, n, kNT, [&](float v, int) {
+    const uint32_t k = key_of(v);
+    top = max(top, k);
+    least = min(least, k ? k : 0xFFFFFFFFu);
+    mine += k != 0;
+  });
+  const uint32_t real = (uint32_t)over_block(mine);
+  if (real == 0) {
+    if (tid == 0) write_row(a, row, -1, 0.f, 0);
+    return;
+  }
+  if (tid == 0) lds.before = lds.cut = 0;
+  __syncthreads();
+  top = max_wave(top);
+  least = ~max_wave(~least);
+  if (lane == 0) {
+    atomicMax(&lds.before, (unsigned long long)top);
+    atomicMax(&lds.cut, (unsigned long long)~least);
+  }
+  __syncthreads();
+  top = (uint32_t)lds.before;
+  least = ~(uint32_t)lds.cut;
+  const double vmax = of_key(top);
+  auto place = [&](float v) { return v == (float)vmax ? 0.0 : ((double)v - vmax) * set.c64; };
+  auto weight = [&](float v) {
+    int k;
+    return exp2(place(v), a.bits, &k);
+  };
+
+  // Where the count (or weight) from the top reaches `want`, of what lies at or above `floor` (of those equal
+  // to it, floor_n): the key; what lies above it.
+  unsigned long long above;
+  auto find = [&](bool by_weight, unsigned long long want, uint32_t floor, uint32_t floor_n) {
+    uint32_t hi = top, lo = floor;
+    above = 0;
+    for (;;) {
+      const int shift = hi - lo < kBins ? 0 : 21 - __clz(hi - lo);
+      __syncthreads();
+      for (int i = tid; i < kBins; i += kNT) lds.bin[i] = 0;
+      __syncthreads();
+      each(tid, n, kNT, [&](float v, int) {
+        const uint32_t k = key_of(v);
+        if (k >= lo && k <= hi && (!by_weight || k > floor)) atomicAdd(&lds.bin[(hi - k) >> shift], by_weight ? weight(v) : 1ull);
+      });
+      if (by_weight && tid == 0 && lo == floor) atomicAdd(&lds.bin[(hi - floor) >> shift], floor_n * weight(of_key(floor)));
+      __syncthreads();
+      find_bin(lds, above, want);
+      above = lds.before;
+      hi -= (uint32_t)lds.found << shift;
+      if (shift == 0) return hi;
+      lo = max(lo, hi - ((1u << shift) - 1));
+    }
+  };
+  auto equal_to = [&](uint32_t key) {
+    uint32_t num = 0;
+    each(tid, n, kNT, [&](float v, int) { num += key_of(v) == key; });
+    return (uint32_t)over_block(num);
+  };
+
+  uint32_t key = least, eq = 0xFFFFFFFFu;  // of the logits equal to the cut, the first eq are left
+  if (set.k > 0 && (uint32_t)set.k < real) {
+    key = find(false, set.k, least, 0);
+    eq = (uint32_t)(set.k - above);
+  }
+  if (set.temperature != 0.f && set.top_p < 1.f) {
+    unsigned long long sum = 0;
+    each(tid, n, kNT, [&](float v, int) {
+      if (key_of(v) > key) sum += weight(v);
+    });
+    const uint32_t floor_n = min(eq, equal_to(key));
+    sum = over_block(sum) + floor_n * weight(of_key(key));
+    const unsigned long long want = share_of(set.top_p, sum);
+    const uint32_t floor = key;
+    key = find(true, want, floor, floor_n);
+    const unsigned long long w = weight(of_key(key)), take = (want - above + w - 1) / w;
+    eq = (uint32_t)min(take, (unsigned long long)(key == floor ? floor_n : 0xFFFFFFFFu));
+  }
+  uint32_t last_eq = 0xFFFFFFFFu;  // the last id of those equal to the cut that is left
+  if (eq < equal_to(key)) {
+    uint32_t seen = 0;
+    for (int i0 = 0; i0 < n; i0 += kNT) {
+      const int i = i0 + tid;
+      const bool is = i < n && key_of(ldg<float>(x + i)) == key;
+      unsigned long long all;
+      const uint32_t upto = seen + (uint32_t)run_sum(is, lds.part, &all);
+      if (is && upto == eq) lds.found = i;
+      seen += (uint32_t)all;
+      if (seen >= eq) break;
+    }
+    __syncthreads();
+    last_eq = (uint32_t)lds.found;
+  }
+  auto left = [&](float v, int i) {
+    const uint32_t k = key_of(v);
+    return k > key || (k == key && (uint32_t)i <= last_eq) ? k == top || place(v) >= set.min64 : false;
+  };
+  // ---- the draw: the wave, then the sixteenth of its part, and so on, in which the running weight passes the target
+  unsigned long long total = 0, target = 0, before = 0;
+  uint32_t count = 0;
+  int lo = 0, len = n;
+  for (bool first = true; len > 64 || first; first = false) {
+    const int per = ((len + 15) / 16 + 63) / 64 * 64, b0 = lo + min(len, wave * per), b1 = lo + min(len, wave * per + per);
+    unsigned long long sum = 0;
+    uint32_t num = 0;
+    each(b0 + lane, b1, 64, [&](float v, int i) {
+      if (left(v, i)) {
+        sum += weight(v);
+        ++num;
+      }
+    });
+    if (first) count = (uint32_t)over_block(num);
+    sum = sum_wave(sum);
+    __syncthreads();
+    if (lane == 0) lds.part[wave] = sum;
+    __syncthreads();
+    if (first) {
+      for (int w = 0; w < 16; ++w) total += lds.part[w];
+      target = target_of(ldg<float>(a.u + row), total);
+    }
+    int w = 0;
+    while (w < 15 && before + lds.part[w] <= target) before += lds.part[w++];
+    lo += min(len, w * per);
+    len = min(len - min(len, w * per), per);
+  }
+  if (wave != 0) return;
+  const int i = lo + lane;
+  unsigned long long w = 0;
+  if (lane < len) {
+    const float v = ldg<float>(x + i);
+    if (left(v, i)) w = weight(v);
+  }
+  const unsigned long long upto = before + scan_wave(w);
+  if (upto > target && upto - w <= target) write_row(a, row, i, (float)((double)w / (double)total), count);
+}
+
 // The draw of a row whose best ids are the sorted list's first, nk of them, E of these a lane, by one wave.
 template <int E>
 __device__ inline void draw_few(const SampleRowsArgs &a, const RowSet &set, int row, float top, int nk, float u,
@@ -872,19 +844,11 @@ __device__ inline int find_chunk(const unsigned long long *chunk, int n_chunks, 
   return hit;
 }
 
-struct ManyLds {
-  unsigned long long bin[kBins];
-  unsigned long long part[kNT / 64];
-  unsigned long long before, cut;
-  int found;
-  uint32_t num, kept;
-};
-
 // The same of a longer list, by all threads.  Nothing is sorted but what lies in the bucket of a cut (top-k's, then
 // top-p's) and in the chunk of ids in which the draw falls.  (Sorted as a whole, 1000 ids of 48 rows: 20 us.)
 __device__ inline void draw_many(const SampleRowsArgs &a, const RowSet &set, int row, const RowInfo &in, int n_list,
                                  float u, const Exp2 &exp2, unsigned long long *list, unsigned long long *chunk,
-                                 int n_chunks, int chunk_len, ManyLds &lds) {
+                                 int n_chunks, int chunk_len, RowLds &lds) {
   constexpr int E = kList / kNT;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   unsigned long long x[E], w[E];
@@ -947,15 +911,13 @@ __device__ inline void draw_many(const SampleRowsArgs &a, const RowSet &set, int
   }
   if (cut_p) {
     __syncthreads();
-    const unsigned long long h0 = lds.bin[2 * tid], h1 = lds.bin[2 * tid + 1];
-    unsigned long long total;
-    const unsigned long long upto = run_sum(h0 + h1, lds.part, &total), goal = share_of(set.top_p, total);
-    if (upto >= goal && upto - h0 - h1 < goal) {
-      const bool second = upto - h1 < goal;
-      lds.found = 2 * tid + second;
-      lds.before = second ? upto - h1 : upto - h0 - h1;
-    }
-    __syncthreads();
+    unsigned long long sum = 0, total;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (kNT * e < n_list) sum += w[e];
+    run_sum(sum, lds.part, &total);
+    const unsigned long long goal = share_of(set.top_p, total);
+    find_bin(lds, 0, goal);
     const int found = lds.found;
     const int num = gather([&](unsigned long long y) { return bin_of(y) == found; });
     if (wave == 0) {
@@ -1017,12 +979,14 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   __shared__ __align__(16) unsigned long long list[kList];
   __shared__ __align__(16) unsigned long long chunk[kMostSlices * 16];
   __shared__ double table[64];
-  __shared__ union { DigitLds digits; ManyLds many; } lds;
+  __shared__ RowLds lds;
   __shared__ uint32_t counted;
   constexpr int chunk_len = 64 * PER;
   const int tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
   const RowSet &set = a.rows[row];
   const RowInfo in = a.info[row];
+  exp2_table(table);
+  const Exp2 exp2{table};
   // the slices' candidates, one after the other; what a wave copies: every 16th slice's
   const size_t at = (size_t)row * a.slices;
   const int wave = tid >> 6;
@@ -1034,11 +998,10 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
     return;
   }
   if (in.state == kSlow || !fits || n_list > kList) {
-    row_by_digits(a, lds.digits);
+    __syncthreads();  // (the table)
+    row_by_ranges(a, exp2, lds);
     return;
   }
-  exp2_table(table);
-  const Exp2 exp2{table};
   const float u = ldg<float>(a.u + row);
   const int n_chunks = a.slices * (kNT / 64);
   uint32_t kept = 0;
@@ -1054,7 +1017,7 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   __syncthreads();
   if (in.state == kBest) {
     if (n_list > kWave) {
-      draw_many(a, set, row, in, (int)n_list, u, exp2, list, chunk, n_chunks, chunk_len, lds.many);
+      draw_many(a, set, row, in, (int)n_list, u, exp2, list, chunk, n_chunks, chunk_len, lds);
     } else if (wave == 0) {
       const int nk = min(set.k, (int)n_list);
       sort_by_wave(list, (int)n_list);
@@ -1135,9 +1098,12 @@ void launch_slices(const SampleRowsArgs &a, int rows, bool vec, hipStream_t st) 
 }
 
 // Rows of more ids than the slices hold.
-__global__ __launch_bounds__(kNT) void k_rows_digits(SampleRowsArgs a) {
-  __shared__ DigitLds digits;
-  row_by_digits(a, digits);
+__global__ __launch_bounds__(kNT) void k_rows_whole(SampleRowsArgs a) {
+  __shared__ double table[64];
+  __shared__ RowLds lds;
+  exp2_table(table);
+  __syncthreads();
+  row_by_ranges(a, Exp2{table}, lds);
 }
 
 }  // namespace
@@ -1210,7 +1176,7 @@ extern "C" int ms_sample_rows(const float *d_logits, size_t in_stride, int rows,
       a.rows[r].k = best ? 1 : w.top_k > 0 && w.top_k < vocab ? w.top_k : 0;
     }
     if (!sliced) {
-      hipLaunchKernelGGL(k_rows_digits, dim3(m), dim3(kNT), 0, st, a);
+      hipLaunchKernelGGL(k_rows_whole, dim3(m), dim3(kNT), 0, st, a);
     } else {
       if (large)
         launch_slices<16>(a, m, vec, st);
