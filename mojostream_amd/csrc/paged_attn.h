@@ -40,6 +40,7 @@ struct PagedAttnArgs {
   float *part_o, *part_ml;  // [part][kv head][part_rows][head dim], [part][kv head][part_rows][2]
   int part_rows;          // (row, head) pairs of the longest item
   const float *k_scale, *v_scale;  // 8-bit pools: [page][kv head][slot]
+  int hp_log;             // 8-bit pools, item_by_tile: log2 of the kv heads of a block
   float cap, inv_cap;     // capped scores: log2(e) times the cap, and its inverse
 };
 
@@ -440,17 +441,19 @@ __host__ __device__ constexpr int v_dims() {
 // zeros of masked keys too; where the end finds such a sum the item is done again key by
 // key.
 template <int HD, int DT, int NQ, int W, bool CAP>
-__device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const PagedItem &it, int kvh,
-                                             char *lds) {
+__device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const PagedItem &it, int kvh0,
+                                             int hp_log, char *lds) {
   using F = Form<DT>;
   constexpr bool F16 = F::F16;
-  constexpr int SP = tile_split<HD>(), NG = W / SP, HW = HD / SP;
+  constexpr int SP = tile_split<HD>(), HW = HD / SP;
   constexpr bool E8 = F::E8;
   constexpr int QP = F::QP, PP = F::PP, KP = F::KP, KS = HW / 32, ES = F::ES;
   constexpr int KL = E8 ? KS / 2 : KS, KB = E8 ? 64 : 32 * ES;  // loads of 16 or 32 bytes of a key, bytes between them
   constexpr int VD = v_dims<HD, DT>(), CD = 16 * VD, NC = HW / CD;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
-  const int grp = wave / SP, part = wave % SP;
+  // kv head, group of the waves of its head, part of the head's dims
+  const int hp = E8 && SP == 1 ? hp_log : 0, NG = W / SP >> hp;
+  const int kvh = kvh0 + (wave & ((1 << hp) - 1)), grp = wave / SP >> hp, part = wave % SP;
   const int nrows = min(16 * NQ, it.n_new * a.G - it.r0), base = it.len - it.n_new;
   const int t_first = (int)div_by(it.r0, a.by_g), t_last = (int)div_by(it.r0 + nrows - 1, a.by_g);
   const int low_key = a.window ? max(it.k0, base + t_first - a.window + 1) : it.k0;
@@ -682,17 +685,20 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   }
   // (also: every wave is done with xs)
   if (__syncthreads_or(bad)) {
-    item_by_key<HD, DT, 64 * W, CAP>(a, it, kvh, 16 * NQ, reinterpret_cast<float *>(lds));
+    for (int h = 0; h < 1 << hp; ++h)
+      item_by_key<HD, DT, 64 * W, CAP>(a, it, kvh0 + h, 16 * NQ, reinterpret_cast<float *>(lds));
     return;
   }
-  float *ml = reinterpret_cast<float *>(lds);  // [2][group][16 NQ]
+  float *ml = reinterpret_cast<float *>(lds);  // [2][group][head][16 NQ]
+  constexpr int NS = W / SP;                   // groups by heads
+  const int sub = wave & ((1 << hp) - 1);
   constexpr int LD = CD + 4, ROWS = 16 * NQ;
-  float *os = ml + 2 * NG * ROWS;              // [wave][16][LD]
+  float *os = ml + 2 * NS * ROWS;              // [wave][16][LD]
   if (g == 0 && part == 0)
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      ml[grp * ROWS + 16 * n + c16] = m[n];
-      ml[(NG + grp) * ROWS + 16 * n + c16] = l[n];
+      ml[((grp << hp) + sub) * ROWS + 16 * n + c16] = m[n];
+      ml[(NS + (grp << hp) + sub) * ROWS + 16 * n + c16] = l[n];
     }
   __syncthreads();
 #pragma unroll
@@ -700,7 +706,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
     if (16 * n >= nrows) break;
     float top = kLow;
 #pragma unroll
-    for (int w = 0; w < NG; ++w) top = fmaxf(top, ml[w * ROWS + 16 * n + c16]);
+    for (int w = 0; w < NG; ++w) top = fmaxf(top, ml[((w << hp) + sub) * ROWS + 16 * n + c16]);
     const float f = __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -715,25 +721,27 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
           *reinterpret_cast<f4 *>(os + (wave * 16 + c16) * LD + VD * (4 * g + e) + t) = x;
         }
       __syncthreads();
-      for (int i = tid; i < 16 * SP * (CD / 4); i += 64 * W) {
+      for (int i0 = tid; i0 < 16 * SP * (CD / 4) << hp; i0 += 64 * W) {
+        const int h_of = i0 & ((1 << hp) - 1), i = i0 >> hp;
         const int d = i % (CD / 4) * 4, pt = i / (CD / 4) % SP, r16 = i / (CD / 4 * SP), r = 16 * n + r16;
         if (r >= nrows) break;
         float mt = kLow, ls = 0.f;
 #pragma unroll
-        for (int w = 0; w < NG; ++w) mt = fmaxf(mt, ml[w * ROWS + r]);
+        for (int w = 0; w < NG; ++w) mt = fmaxf(mt, ml[((w << hp) + h_of) * ROWS + r]);
         f4 x = {};
 #pragma unroll
         for (int w = 0; w < NG; ++w) {
-          ls += ml[(NG + w) * ROWS + r] * __builtin_amdgcn_exp2f(ml[w * ROWS + r] - mt);
-          x += *reinterpret_cast<const f4 *>(os + ((w * SP + pt) * 16 + r16) * LD + d);
+          const int at = (w << hp) + h_of;
+          ls += ml[(NS + at) * ROWS + r] * __builtin_amdgcn_exp2f(ml[at * ROWS + r] - mt);
+          x += *reinterpret_cast<const f4 *>(os + ((at * SP + pt) * 16 + r16) * LD + d);
         }
         const int dim = pt * HW + c * CD + d;
         if (it.part < 0) {
           const int t = (int)div_by(it.r0 + r, a.by_g), h = it.r0 + r - t * a.G;
-          *reinterpret_cast<f4 *>(a.out + (size_t)(it.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD + dim) =
+          *reinterpret_cast<f4 *>(a.out + (size_t)(it.row + t) * a.out_ld + (size_t)((kvh0 + h_of) * a.G + h) * HD + dim) =
               x / ls;
         } else {
-          const size_t pr = ((size_t)it.part * a.n_kv + kvh) * a.part_rows + r;
+          const size_t pr = ((size_t)it.part * a.n_kv + kvh0 + h_of) * a.part_rows + r;
           *reinterpret_cast<f4 *>(a.part_o + pr * HD + dim) = x;
           if (dim == 0) {
             a.part_ml[pr * 2] = mt;
@@ -1130,12 +1138,29 @@ constexpr int tile_lds() {
   return x > e ? x : e;
 }
 
+// Blocks go to the eight dies in turn: those of an item's heads to one die, whose cache then finds the rows of a page
+// whole (8 heads of 64 dims in 8 bits, 48 tokens: 83 us where a die has one head of all items, 50 us; the items of the last
+// groups of eight that are not whole as they come).
+struct BlockOf {
+  int item, head;
+};
+__device__ inline BlockOf block_of(int block, int n_blocks, int heads) {
+  const int per = 8 * heads;
+  if (block >= n_blocks / per * per) return {block / heads, block % heads};
+  return {block / per * 8 + block % 8, block % per / 8};
+}
+
 // Items of at most 16 NQ pairs: single tokens, or a few of them.  (Two query tiles of three parts do
 // not fit the registers of two waves a SIMD: with spills 110 us where one wave takes 72 us.)
 template <int HD, int DT, int NQ, bool CAP>
 __global__ __launch_bounds__(256, NQ == 2 && DT != MS_KV_F16 ? 1 : 2) void k_paged_tile(PagedAttnArgs a) {
   __shared__ __align__(16) char lds[tile_lds<HD, DT, NQ, 4>()];
-  item_by_tile<HD, DT, NQ, 4, CAP>(a, a.items[blockIdx.x / a.n_kv], blockIdx.x % a.n_kv, lds);
+  if constexpr (Form<DT>::E8) {
+    const BlockOf b = block_of(blockIdx.x, gridDim.x, a.n_kv >> a.hp_log);
+    item_by_tile<HD, DT, NQ, 4, CAP>(a, a.items[b.item], b.head << a.hp_log, a.hp_log, lds);
+  } else {
+    item_by_tile<HD, DT, NQ, 4, CAP>(a, a.items[blockIdx.x / a.n_kv], blockIdx.x % a.n_kv, 0, lds);
+  }
 }
 
 // Items of longer chunks, and single tokens beside them.
@@ -1145,7 +1170,7 @@ __global__ __launch_bounds__(NT, 2) void k_paged_block(PagedAttnArgs a) {
   __shared__ __align__(16) char lds[A > B ? A : B];
   const PagedItem it = a.items[blockIdx.x / a.n_kv];
   if (it.n_new * a.G - it.r0 <= 16)
-    item_by_tile<HD, DT, 1, Shape<HD, DT>::W, CAP>(a, it, blockIdx.x % a.n_kv, lds);
+    item_by_tile<HD, DT, 1, Shape<HD, DT>::W, CAP>(a, it, blockIdx.x % a.n_kv, 0, lds);
   else
     item_by_block<HD, DT, CAP>(a, it, blockIdx.x % a.n_kv, lds);
 }
@@ -1230,12 +1255,18 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   const int rows = block ? B::PAIRS : most > 16 && TWO ? 32 : 16;
   PagedPlan *p = nullptr;
   // blocks that run at once; a step of single tokens takes a tile for every group of waves
-  const int w = block ? B::W : 4, cost = std::max(1, 4 * tile_split<HD>() / w);
+  const int w = block ? B::W : 4;
+  // 8-bit pools: a block's waves share two heads of 128 dims, four of 64, so that 256 bytes of a row are read about
+  // at once
+  if constexpr (Form<DT>::E8)
+    if (!block)
+      while (HD << a.hp_log < 256 && a.n_kv % (2 << a.hp_log) == 0) ++a.hp_log;
+  const int cost = std::max(1, (4 << a.hp_log) * tile_split<HD>() / w);
   // A merge's launch takes 3.4 us; a step of a single token (4 in the plan's measure) 0.7 us at head dim 64,
   // 1.15 at 128 and 1.4 to 1.6 at 256 and 512 over 16-bit pools, 1.7 to 5 us over fp32 ones: one token over 250
   // keys of 64 dims (bf16) 5.4 us in one block a head, 9.0 us cut and merged; over 1500 keys 12.4 and 9.1 us.
   const int merge = block ? 8 : DT == MS_KV_F32 ? 4 : HD == 64 ? 20 : HD == 128 ? 12 : 8;
-  if (int rc = plan_for(b, a.G, rows, block, a.n_kv, a.window, 8 / w * ctx().n_cu, cost, merge, &p)) return rc;
+  if (int rc = plan_for(b, a.G, rows, block, a.n_kv >> a.hp_log, a.window, 8 / w * ctx().n_cu, cost, merge, &p)) return rc;
   a.part_rows = p->most;
   if (const size_t n = (size_t)p->n_parts * a.n_kv * a.part_rows) {
     void *buf = nullptr;
@@ -1247,7 +1278,7 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   // (a launch has fewer than 2^32 threads)
   MS_CHECK_ARG((int64_t)p->n_items * a.n_kv * 64 * w < ((int64_t)1 << 32),
                "paged_attention: too many rows for one call");
-  const dim3 grid(p->n_items * a.n_kv);
+  const dim3 grid(p->n_items * (a.n_kv >> a.hp_log));
   if (block) {
     hipLaunchKernelGGL((k_paged_block<HD, DT, CAP>), grid, dim3(64 * B::W), 0, st, a);
   } else if (rows == 16) {
