@@ -330,8 +330,8 @@ int ms_paged_append_ext(const ms_paged_layer_ext *layer, const ms_paged_batch *b
                         float *d_q_out, size_t q_out_stride, const float *d_cos,
                         const float *d_sin, int n_pos);
 /* ms_paged_attention over any of the pools, with capped scores or not.  Over 8-bit pools the products take
- * the codes with all their bits, 22 bits of q times the scale of the scores (of these nothing below 2^-32 of a row's largest),
- * and the probabilities times the values' scales with all theirs.  A cap holds for infinite scores too. */
+ * the codes with all their bits, and 22 bits of q times the scores' scale (of these nothing below 2^-32 of a row's largest) and
+ * of the probabilities times the values' scales (nothing below 2^-32 of the largest scale that the row attends to).  A cap holds for infinite scores too. */
 int ms_paged_attention_ext(const ms_paged_layer_ext *layer, ms_paged_batch *b, const float *d_q,
                            size_t q_stride, float *d_out, size_t out_stride);
 /* Positions pos0 .. pos0 + n - 1 of sequence seq out of the pages (any pool), in fp32: position

@@ -88,15 +88,18 @@ constexpr float kLag = 8.0f;
 //   fp32  three bf16 parts each, six products (what is dropped is below 2^-25)
 //   fp16  q and p in two fp16 parts (22 bits): q scaled by a power of two to below 2^15, p by
 //         2^kLift, so that what falls below fp16's smallest step is below 2^-32 of the largest
-//   8-bit the codes, which fp16 and bf16 hold exactly.  The keys' with q in two fp16 parts, their
-//         scales multiply the scores; the values' scales multiply the probabilities, which then may have any
-//         size: three bf16 parts
+//   8-bit the codes, which fp16 holds exactly, and two fp16 parts of q and of p times the values'
+//         scales, in units of the smallest power of two above the scales that the row has attended to
+//         (a scale's head has a code of full size, so that what is lost is below 2^-32 of that too).  The keys' scales
+//         multiply the scores.  With three bf16 parts of p times the scales as they are the chunk of 4096 rows over 16384
+//         keys took 2.6 ms
 template <int DT>
 struct Form {
   static constexpr bool E8 = DT == MS_KV_E4M3 || DT == MS_KV_I8;
   static constexpr int ES = DT == MS_KV_F32 ? 4 : E8 ? 1 : 2;  // bytes of a pool's value
-  static constexpr bool F16 = DT == MS_KV_F16 || E8, P16 = DT == MS_KV_F16;  // fp16 parts of q, of p
-  static constexpr int QP = F16 ? 2 : 3, PP = P16 ? 2 : 3, KP = DT == MS_KV_F32 ? 3 : 1;
+  static constexpr bool F16 = DT == MS_KV_F16 || E8;           // fp16 parts
+  static constexpr bool LIFT = DT == MS_KV_F16;                // the sum of p too is lifted
+  static constexpr int QP = F16 ? 2 : 3, KP = DT == MS_KV_F32 ? 3 : 1;
 };
 constexpr float kLift = 7.0f;
 
@@ -127,28 +130,18 @@ __device__ inline void split2(float a, float b, uint32_t *p, int step) {
     }
   }
 }
-// Four 8-bit codes as fp16, or as bf16: those of bytes 0 and 1 to lo, 2 and 3 to hi.
-template <int DT, bool F16>
+// Four 8-bit codes as fp16: those of bytes 0 and 1 to lo, 2 and 3 to hi.
+template <int DT>
 __device__ inline void codes4(uint32_t w, uint32_t *lo, uint32_t *hi) {
-  if constexpr (DT == MS_KV_E4M3 && F16) {
+  if constexpr (DT == MS_KV_E4M3) {
     *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
     *hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true));
-  } else if constexpr (DT == MS_KV_E4M3) {
-    *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
-    *hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true));
-  } else if constexpr (F16) {
+  } else {
     // 1024 + (c + 128) has c + 128 in fp16's low bits
     constexpr half2_t off = {(_Float16)1152.f, (_Float16)1152.f};
     w ^= 0x80808080u;
     *lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - off);
     *hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - off);
-  } else {
-    // (a code has at most eight bits: the low half of its fp32 form is 0)
-    uint32_t f[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = __float_as_uint((float)(int8_t)(w >> (8 * i)));
-    *lo = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);
-    *hi = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
   }
 }
 template <bool F16>
@@ -234,7 +227,7 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
       for (int w = 1; w < NW; ++w) mx = fmaxf(mx, red[w]);
       const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;
       // (lifted like the tiles' probabilities: parts of both kinds are merged)
-      const float p = on ? __builtin_amdgcn_exp2f(Form<DT>::P16 ? s - base + kLift : s - base) : 0.f;
+      const float p = on ? __builtin_amdgcn_exp2f(Form<DT>::LIFT ? s - base + kLift : s - base) : 0.f;
       p_of[tid] = on ? p : -1.f;
       float sum = p;
       for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
@@ -287,13 +280,14 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
 // product in m and not in t it was off by up to half of m's last place: from 2^29 on rows came out
 // as 0 or NaN.)
 // span(n, &low, &high): the keys that the lane's query of query tile n attends to.
-// ks, vs: an 8-bit pool's scales of keys 4 g .. 4 g + 3 of both half tiles.  CAP: the scores are capped.
+// ks, vs: an 8-bit pool's scales of keys 4 g .. 4 g + 3 of both half tiles; vtop: the power of two that the values' scales
+// are taken in, above all that the query has attended to.  CAP: the scores are capped.
 template <int DT, bool CAP, int NQ, int ND, class Span>
 __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2][NQ], int kb, bool edge,
                                               const float (&scale)[NQ], const f4 (&ks)[2], const f4 (&vs)[2],
-                                              const Span &span, float (&m)[NQ], float (&l)[NQ], f4 (&o)[NQ][ND],
-                                              uint32_t (&pf)[NQ][Form<DT>::PP][4]) {
-  constexpr bool F16 = Form<DT>::P16, E8 = Form<DT>::E8;
+                                              const Span &span, float (&vtop)[NQ], float (&m)[NQ], float (&l)[NQ],
+                                              f4 (&o)[NQ][ND], uint32_t (&pf)[NQ][Form<DT>::QP][4]) {
+  constexpr bool F16 = Form<DT>::F16, E8 = Form<DT>::E8;
   float sc[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -346,18 +340,41 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
         if (t[n][j] != -INFINITY) t[n][j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], -mn);
     }
   }
+  if constexpr (E8) {
+    float big[NQ];
+    bool more = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      big[n] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        big[n] = fmaxf(big[n], edge && t[n][j] == -INFINITY ? 0.f : vs[j >> 2][j & 3]);
+      more |= big[n] > vtop[n];
+    }
+    if (__any(more))
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const uint32_t up = (__float_as_uint(max_groups(big[n])) + 0x7FFFFFu) & 0x7F800000u;
+        const float to = fmaxf(vtop[n], __uint_as_float(up)), f = vtop[n] / to;
+        vtop[n] = to;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[n][d] *= f;
+      }
+  }
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     float *p = t[n];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(F16 ? p[j] + kLift : p[j]);
+    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(Form<DT>::LIFT ? p[j] + kLift : p[j]);
     l[n] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-    if constexpr (E8)
+    if constexpr (E8) {
+      const float by = __uint_as_float(((254u + (int)kLift) << 23) - __float_as_uint(vtop[n]));  // 2^kLift / vtop
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] *= vs[j >> 2][j & 3];
+      for (int j = 0; j < 8; ++j) p[j] *= vs[j >> 2][j & 3] * by;
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      split2<F16, Form<DT>::PP>(p[2 * j], p[2 * j + 1], &pf[n][0][j], 4);
+      split2<F16, Form<DT>::QP>(p[2 * j], p[2 * j + 1], &pf[n][0][j], 4);
   }
 }
 
@@ -447,7 +464,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   constexpr bool F16 = F::F16;
   constexpr int SP = tile_split<HD>(), HW = HD / SP;
   constexpr bool E8 = F::E8;
-  constexpr int QP = F::QP, PP = F::PP, KP = F::KP, KS = HW / 32, ES = F::ES;
+  constexpr int QP = F::QP, KP = F::KP, KS = HW / 32, ES = F::ES;
   constexpr int KL = E8 ? KS / 2 : KS, KB = E8 ? 64 : 32 * ES;  // loads of 16 or 32 bytes of a key, bytes between them
   constexpr int VD = v_dims<HD, DT>(), CD = 16 * VD, NC = HW / CD;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
@@ -539,11 +556,12 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   }
 
   f4 o[NQ][NC * VD] = {};
-  float m[NQ], l[NQ];
+  float m[NQ], l[NQ], vtop[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     m[n] = kLow;
     l[n] = 0.f;
+    vtop[n] = 0x1p-119f;
   }
   auto span = [&](int n, int *low, int *high) {
     const int pos = base + (int)div_by(it.r0 + min(16 * n + c16, nrows - 1), a.by_g);
@@ -580,8 +598,8 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
         for (int i = 0; i < 2; ++i) {
           uint32_t kf[KP][4];
           if constexpr (E8) {
-            codes4<DT, true>(kr[i][ks / 2][0][2 * (ks & 1)], &kf[0][0], &kf[0][1]);
-            codes4<DT, true>(kr[i][ks / 2][0][2 * (ks & 1) + 1], &kf[0][2], &kf[0][3]);
+            codes4<DT>(kr[i][ks / 2][0][2 * (ks & 1)], &kf[0][0], &kf[0][1]);
+            codes4<DT>(kr[i][ks / 2][0][2 * (ks & 1) + 1], &kf[0][2], &kf[0][3]);
           } else if constexpr (ES == 2) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) kf[0][j] = kr[i][ks][0][j];
@@ -629,8 +647,8 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
         }
     }
     if (!work) continue;
-    uint32_t pf[NQ][PP][4];
-    probabilities<DT, CAP, NQ>(a, s, kb, kb < all_lo || kb + kTile - 1 > all_hi, sc, ks8, vs8, span, m, l, o, pf);
+    uint32_t pf[NQ][QP][4];
+    probabilities<DT, CAP, NQ>(a, s, kb, kb < all_lo || kb + kTile - 1 > all_hi, sc, ks8, vs8, span, vtop, m, l, o, pf);
 
     // ---- values
 #pragma unroll
@@ -641,7 +659,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
         for (int t = 0; t < VD; t += 2)
 #pragma unroll
           for (int d = 0; d < 4; ++d)  // dims t and t + 1 of both keys, then each dim's pair
-            codes4<DT, false>(__builtin_amdgcn_perm(vr[2 * d + 1][c][t / 4], vr[2 * d][c][t / 4],
+            codes4<DT>(__builtin_amdgcn_perm(vr[2 * d + 1][c][t / 4], vr[2 * d][c][t / 4],
                                                     t & 2 ? 0x07030602u : 0x05010400u),
                               &vf[t][0][d], &vf[t + 1][0][d]);
 #pragma unroll
@@ -656,15 +674,15 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
                               &vf[t][0][d], 4);
         }
 #pragma unroll
-      for (int pa = PP - 1; pa >= 0; --pa)
+      for (int pa = QP - 1; pa >= 0; --pa)
 #pragma unroll
         for (int pb = KP - 1; pb >= 0; --pb) {
-          if (pa + pb >= PP) continue;
+          if (pa + pb >= QP) continue;
 #pragma unroll
           for (int t = 0; t < VD; ++t)
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
-              o[n][c * VD + t] = mfma<F::P16>(u4{vf[t][pb][0], vf[t][pb][1], vf[t][pb][2], vf[t][pb][3]},
+              o[n][c * VD + t] = mfma<F16>(u4{vf[t][pb][0], vf[t][pb][1], vf[t][pb][2], vf[t][pb][3]},
                                            u4{pf[n][pa][0], pf[n][pa][1], pf[n][pa][2], pf[n][pa][3]},
                                            o[n][c * VD + t]);
         }
@@ -678,6 +696,9 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   for (int n = 0; n < NQ; ++n) {
     l[n] = sum_groups(l[n]);
     bad |= !(fabsf(l[n]) < INFINITY);
+    if constexpr (E8)
+#pragma unroll
+      for (int d = 0; d < NC * VD; ++d) o[n][d] *= vtop[n] * 0x1p-7f;
 #pragma unroll
     for (int d = 0; d < NC * VD; ++d)
 #pragma unroll
@@ -795,7 +816,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   constexpr bool F16 = F::F16;
   constexpr int NQ = B::NQ, W = B::W, SP = B::SP;
   constexpr bool E8 = F::E8;
-  constexpr int QP = F::QP, PP = F::PP, KP = F::KP, KS = HD / 32, ES = F::ES;
+  constexpr int QP = F::QP, KP = F::KP, KS = HD / 32, ES = F::ES;
   constexpr int VD = B::VD, CD = 16 * VD, NC = HD / CD;
   constexpr int KW = KS / SP, CW = NC / SP;  // a wave's 32-dim steps and chunks of CD dims
   constexpr int D8 = HD / 8, UK = kTile * D8 / (64 * W);  // K units of 8 dims a thread
@@ -811,7 +832,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   uint32_t *rows = reinterpret_cast<uint32_t *>(lds + B::ROWS_AT);  // [2][32]
   float *scl = reinterpret_cast<float *>(lds + B::SCL_AT);     // [2][keys', values'][32]
 
-  float sc[NQ], down[NQ], m[NQ], l[NQ];
+  float sc[NQ], down[NQ], m[NQ], l[NQ], vtop[NQ];
   const int t_first = (int)div_by(it.r0, a.by_g), r_wave = 16 * NQ * grp;
   const int low_key = a.window ? max(it.k0, base + t_first - a.window + 1) : it.k0;
   const bool busy = r_wave < nrows;
@@ -905,6 +926,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     const int t = real ? (int)div_by(it.r0 + r, a.by_g) : t_first, h = real ? (it.r0 + r) - t * a.G : 0;
     m[n] = kLow;
     l[n] = 0.f;
+    vtop[n] = 0x1p-119f;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
     load_q<DT, KW>(qp + 32 * KW * part, real, a.q_scale, q[n], &down[n]);
     sc[n] = SP == 1 ? a.s_scale * down[n] : a.s_scale;
@@ -920,10 +942,10 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
       if constexpr (E8) {
         u4 x;
         uint32_t lo, hi;
-        codes4<DT, true>(kr[u][0], &lo, &hi);
+        codes4<DT>(kr[u][0], &lo, &hi);
         x[0] = lo;
         x[1] = hi;
-        codes4<DT, true>(kr[u][1], &lo, &hi);
+        codes4<DT>(kr[u][1], &lo, &hi);
         x[2] = lo;
         x[3] = hi;
         dst[0] = x;
@@ -947,7 +969,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     __syncthreads();
     int next = 0;
     if (tid < kTile) next = find(min(tile + 1, n_tiles - 1));
-    uint32_t pf[NQ][PP][4];
+    uint32_t pf[NQ][QP][4];
     f4 ks8[2] = {}, vs8[2] = {};
     if constexpr (E8)
 #pragma unroll
@@ -992,7 +1014,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
         }
         if constexpr (STRICT) __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (SP == 1) probabilities<DT, CAP, NQ>(a, s, kb, edge, sc, ks8, vs8, span, m, l, o, pf);
+      if constexpr (SP == 1) probabilities<DT, CAP, NQ>(a, s, kb, edge, sc, ks8, vs8, span, vtop, m, l, o, pf);
     }
     if (B::ONE) __syncthreads();
     if (tid < kTile) rows[((tile + 1) & 1) * kTile + tid] = next;
@@ -1002,7 +1024,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
         uint32_t p[2][4 / B::VH];
 #pragma unroll
         for (int d = 0; d < 4 / B::VH; ++d)
-          codes4<DT, false>(__builtin_amdgcn_perm(vr[2 * d + 1][t / 4], vr[2 * d][t / 4],
+          codes4<DT>(__builtin_amdgcn_perm(vr[2 * d + 1][t / 4], vr[2 * d][t / 4],
                                                   t & 2 ? 0x07030602u : 0x05010400u), &p[0][d], &p[1][d]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -1051,7 +1073,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
             }
           __builtin_amdgcn_sched_barrier(0);
         }
-        probabilities<DT, CAP, NQ>(a, s, kb, edge, sc, ks8, vs8, span, m, l, o, pf);
+        probabilities<DT, CAP, NQ>(a, s, kb, edge, sc, ks8, vs8, span, vtop, m, l, o, pf);
       }
       u4 x[RING];
       auto read = [&](int f) {
@@ -1064,11 +1086,11 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
         const int d = f / KP, pb = KP - 1 - f % KP;
         if (f + RING - 1 < CW * VD * KP) read(f + RING - 1);
 #pragma unroll
-        for (int pa = PP - 1; pa >= 0; --pa) {
-          if (pa + pb >= PP) continue;
+        for (int pa = QP - 1; pa >= 0; --pa) {
+          if (pa + pb >= QP) continue;
 #pragma unroll
           for (int n = 0; n < NQ; ++n)
-            o[n][d] = mfma<F::P16>(x[f % RING], u4{pf[n][pa][0], pf[n][pa][1], pf[n][pa][2], pf[n][pa][3]}, o[n][d]);
+            o[n][d] = mfma<F16>(x[f % RING], u4{pf[n][pa][0], pf[n][pa][1], pf[n][pa][2], pf[n][pa][3]}, o[n][d]);
         }
         if constexpr (STRICT) __builtin_amdgcn_sched_barrier(0);
       }
@@ -1081,6 +1103,9 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   for (int n = 0; n < NQ; ++n) {
     l[n] = sum_groups(l[n]);
     bad |= !(fabsf(l[n]) < INFINITY);
+    if constexpr (E8)
+#pragma unroll
+      for (int d = 0; d < CW * VD; ++d) o[n][d] *= vtop[n] * 0x1p-7f;
 #pragma unroll
     for (int d = 0; d < CW * VD; ++d)
 #pragma unroll

@@ -114,7 +114,11 @@ class SetupExt(Setup):
         Setup.attend derives (an 8-bit key's scale is one more rounding of its score, q's 22 bits four: its eight spare
         ones), and with a cap what tanh adds.  tanh never grows an error; its own: below 0.6 2^-23 of it; above, from
         t = e^-2|z| <= 0.3 with an argument off by 2^-23, so (1 - t) / (1 + t) by at most 2^-21 of it; z itself is off by 2^-22 of it, which
-        moves tanh by less than 2^-22 of it: 2^-20 of the capped score in all."""
+        moves tanh by less than 2^-22 of it: 2^-20 of the capped score in all.
+        An 8-bit value's probability times its scale is taken in two fp16 parts: off by 2^-22 of itself (eight spare
+        ones hold that) or, where that is less, by half of fp16's smallest step, 2^-25, in units of 2^-7 of a power of two that
+        is at most twice the largest scale the row attends to, the best key having a probability of 1 at least: 2^-31 of that
+        scale for each key, times its code."""
         G = self.heads // self.kv
         out, tol = (np.zeros((self.rows, self.heads, self.hd)) for _ in range(2))
         q = q.reshape(self.rows, self.heads, self.hd).astype(np.float64)
@@ -124,8 +128,10 @@ class SetupExt(Setup):
             if s not in cache:
                 g = self.slots(s, 0, self.len[s])
                 cache = {s: [decode(self.pool[n][g], self.dtype) for n in "kv"]}
+                if self.eight:
+                    cache[s] += [np.abs(VALUE[self.kind][self.raw["v"][g]]), self.scales["v"].transpose(0, 2, 1)[g]]
             lo = max(0, p - self.window + 1) if self.window else 0
-            k, v = (x[lo:p + 1] for x in cache[s])
+            k, v = (x[lo:p + 1] for x in cache[s][:2])
             for h in range(self.heads):
                 kk, vv = k[:, h // G], v[:, h // G]
                 with np.errstate(invalid="ignore", over="ignore"):
@@ -138,6 +144,9 @@ class SetupExt(Setup):
                     w = e / e.sum()
                     out[r, h] = w @ vv
                     tol[r, h] = 2 * (d + (p - lo + 9) * 2.0 ** -24) * (w @ np.abs(vv)) + 1e-30
+                    if self.eight:
+                        code, scale = (x[lo:p + 1, h // G] for x in cache[s][2:])
+                        tol[r, h] += 2.0 ** -31 * np.float64(scale.max()) * code.sum(0)
         return out.reshape(self.rows, -1), tol.reshape(self.rows, -1)
 
     def check(self, seed=1, pad=0, scale=1.5):
