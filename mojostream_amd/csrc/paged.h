@@ -56,6 +56,7 @@ struct PagedMerge {
 struct PagedPlan {
   int G = 0, rows = 0, n_kv = 0, window = 0, blocks = 0, tile_cost = 0, merge_cost = 0;
   bool block = false;  // items of more than 16 pairs go to item_by_block
+  bool tail = false;   // a last turn of whole spans that does not fill the blocks is cut
   bool valid = false;
   int n_items = 0, n_merge = 0, n_parts = 0;
   int most = 0, most_parts = 0;  // (row, head) pairs of the longest item; parts of one result

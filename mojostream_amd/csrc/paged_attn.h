@@ -16,6 +16,7 @@
 //                 at 2.1 GHz (a large bf16 matrix product: 1.2 PFLOP/s).
 //  k_paged_merge  the spans' results.
 #pragma once
+#include <cmath>
 #include <type_traits>
 
 #include "devutil.h"
@@ -41,12 +42,15 @@ struct PagedAttnArgs {
   int part_rows;          // (row, head) pairs of the longest item
   const float *k_scale, *v_scale;  // 8-bit pools: [page][kv head][slot]
   int hp_log;             // 8-bit pools, item_by_tile: log2 of the kv heads of a block
-  float cap, inv_cap;     // capped scores: log2(e) times the cap, and its inverse
+  // Capped scores: log2(e) times the cap is cap_p[0] (0.5 to 1) times cap_to (a power of two); inv_cap its
+  // inverse (0: not capped); cap_p[1..5] the coefficients of tanh's near form, times cap_p[0] (cap_args).
+  float cap_to, inv_cap, cap_p[6];
 };
 
-// The split of the batch's work for a shape of layers (made anew after each set).
+// The split of the batch's work for a shape of layers (made anew after each set).  tail: a last turn of whole spans that
+// does not fill the blocks is cut.
 int plan_for(ms_paged_batch *b, int G, int rows, bool block, int n_kv, int window, int blocks,
-             int tile_cost, int merge_cost, PagedPlan **out);
+             int tile_cost, int merge_cost, bool tail, PagedPlan **out);
 
 // The launches of pools of 8 bits (dtype MS_KV_E4M3, MS_KV_I8; scores capped or not) and of the other pools
 // with capped scores: each in a source of its own.
@@ -171,17 +175,29 @@ __device__ inline float sum_groups(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// tanh.  To 0.6 z + z^3 P(z^2), P a polynomial fitted here by least squares, reweighted until its
-// largest relative error (3e-9) is least: scores far below the cap keep all their bits; past it from e^(-2 |z|).
-__device__ inline float tanh_of(float z) {
-  const float z2 = z * z, t = __builtin_amdgcn_exp2f(-2.f * 1.44269504f * fabsf(z));
-  float p = -0.00589513639f;
-  p = __builtin_fmaf(p, z2, 0.0207959525f);
-  p = __builtin_fmaf(p, z2, -0.0537838228f);
-  p = __builtin_fmaf(p, z2, 0.133319244f);
-  p = __builtin_fmaf(p, z2, -0.333332986f);
-  const float far = (1.f - t) * __builtin_amdgcn_rcpf(1.f + t);
-  return fabsf(z) < 0.6f ? __builtin_fmaf(z * z2, p, z) : copysignf(far, z);
+// Capped scores: c tanh(z), c = cap_p[0].  To |z| = 0.6, z2 < kNear, c z (1 + z^2 P(z^2)), P a polynomial fitted here
+// by least squares, reweighted until its largest relative error (3e-9) is least: scores far below the cap keep
+// all their bits; past it from e^(-2 |z|).
+constexpr float kNear = 0.36f;
+inline void cap_args(PagedAttnArgs *a, float cap) {
+  constexpr double p[6] = {1, -0.333332986, 0.133319244, -0.0537838228, 0.0207959525, -0.00589513639};
+  int e = 0;
+  const double c = cap * 1.4426950408889634, part = std::frexp(c, &e);
+  a->cap_to = (float)std::ldexp(1.0, e);
+  a->inv_cap = (float)(1.0 / c);
+  for (int i = 0; i < 6; ++i) a->cap_p[i] = (float)(part * p[i]);
+}
+__device__ inline float cap_near(const PagedAttnArgs &a, float z) {
+  const float z2 = z * z;
+  float p = a.cap_p[5];
+#pragma unroll
+  for (int i = 4; i >= 0; --i) p = __builtin_fmaf(p, z2, a.cap_p[i]);
+  return z * p;
+}
+__device__ inline float cap_any(const PagedAttnArgs &a, float z) {
+  const float t = __builtin_amdgcn_exp2f(-2.f * 1.44269504f * fabsf(z));
+  const float far = a.cap_p[0] * ((1.f - t) * __builtin_amdgcn_rcpf(1.f + t));
+  return z * z < kNear ? cap_near(a, z) : copysignf(far, z);
 }
 
 // Of an 8-bit pool's scales: where that of a page's slot is.
@@ -217,7 +233,7 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
         if constexpr (Form<DT>::E8)
           s *= ldg<float>(a.k_scale + scale_at(a, a.pages[(size_t)it.seq * a.stride + pg], key - pg * a.page_size, kvh));
         s *= a.s_scale;
-        if constexpr (CAP) s = a.cap * tanh_of(s * a.inv_cap);
+        if constexpr (CAP) s = a.cap_to * cap_any(a, s * a.inv_cap);
       }
       float mx = on ? s : -INFINITY;
       for (int off = 1; off < 64; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
@@ -288,16 +304,33 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
                                               const Span &span, float (&vtop)[NQ], float (&m)[NQ], float (&l)[NQ],
                                               f4 (&o)[NQ][ND], uint32_t (&pf)[NQ][Form<DT>::QP][4]) {
   constexpr bool F16 = Form<DT>::F16, E8 = Form<DT>::E8;
-  float sc[NQ];
+  float sc[NQ], z2 = 0.f;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    sc[n] = CAP ? 1.f : scale[n];
+    sc[n] = CAP ? a.cap_to : scale[n];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if constexpr (E8) s[i][n] *= ks[i];
-      if constexpr (CAP)
+      if constexpr (CAP) {
+        s[i][n] *= scale[n] * a.inv_cap;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][n][e] = a.cap * tanh_of(s[i][n][e] * scale[n] * a.inv_cap);
+        for (int e = 0; e < 4; ++e) z2 = fmaxf(z2, s[i][n][e] * s[i][n][e]);
+      }
+    }
+  }
+  // (both forms for each score of every tile: 4096 rows over 16384 keys, i8, 3.5 ms; the near one alone where a
+  // tile's scores allow it: @@ ms; uncapped 2.6 ms)
+  if constexpr (CAP) {
+    if (__any(z2 >= kNear)) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j >> 2][n][j & 3] = cap_any(a, s[j >> 2][n][j & 3]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j >> 2][n][j & 3] = cap_near(a, s[j >> 2][n][j & 3]);
     }
   }
   const int g = (threadIdx.x & 63) >> 4;
@@ -1291,7 +1324,10 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   // 1.15 at 128 and 1.4 to 1.6 at 256 and 512 over 16-bit pools, 1.7 to 5 us over fp32 ones: one token over 250
   // keys of 64 dims (bf16) 5.4 us in one block a head, 9.0 us cut and merged; over 1500 keys 12.4 and 9.1 us.
   const int merge = block ? 8 : DT == MS_KV_F32 ? 4 : HD == 64 ? 20 : HD == 128 ? 12 : 8;
-  if (int rc = plan_for(b, a.G, rows, block, a.n_kv >> a.hp_log, a.window, 8 / w * ctx().n_cu, cost, merge, &p)) return rc;
+  // (pools and scores that the plain calls take keep their split, and so their results to the last bit)
+  const bool tail = block && (Form<DT>::E8 || CAP);
+  if (int rc = plan_for(b, a.G, rows, block, a.n_kv >> a.hp_log, a.window, 8 / w * ctx().n_cu, cost, merge, tail, &p))
+    return rc;
   a.part_rows = p->most;
   if (const size_t n = (size_t)p->n_parts * a.n_kv * a.part_rows) {
     void *buf = nullptr;
