@@ -855,6 +855,10 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   constexpr int D8 = HD / 8, UK = kTile * D8 / (64 * W);  // K units of 8 dims a thread
   constexpr bool STRICT = KW * KP >= 8;
   constexpr int RING = 3;
+  // 8-bit keys, few registers, are loaded from the time on that the last tile's are in LDS, so that the first
+  // product and the softmax too lie before their use; their rows are then found two tiles ahead.
+  // (4096 rows over 16384 keys, 14B class, e4m3: 2.48 -> 2.44 ms; 16-bit keys of 256 dims: no gain)
+  constexpr bool EARLY = E8;
   static_assert(CW >= 1 && UK >= 1 && 64 * W / D8 * UK == kTile, "shape");
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
   const int grp = wave / SP, part = wave % SP;
@@ -886,8 +890,8 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   const int v_chunk = wave / B::VH, v_half = wave % B::VH;
   const char *vb0 = static_cast<const char *>(a.v) + ((size_t)kvh * HD + v_chunk * CD + VD * c16) * ES;
   // Pool row of a tile's key `tid`, never one outside the attended keys; two tiles' rows in LDS.
-  // Those of the next are written between the two barriers of a tile, in place of the last's,
-  // whose readers are past the first of them.
+  // Those of the next (EARLY: of the one behind it, in place of this one's) are written between the two barriers of a
+  // tile, in place of the last's, whose readers are past the first of them.
   float k_scl = 0.f, v_scl = 0.f;  // of the next tile's key `tid`
   size_t scl_from = 0;
   auto find = [&](int tile) {
@@ -944,11 +948,14 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     }
   };
   const bool v_busy = v_chunk < NC;
-  if (tid < kTile) rows[tid] = find(0);
+  if (tid < kTile) {
+    rows[tid] = find(0);
+    if constexpr (E8) load_scales();
+    if constexpr (EARLY) rows[kTile + tid] = find(min(1, n_tiles - 1));
+  }
   __syncthreads();
   load_k(0);
   if (v_busy) load_v(0);
-  if (E8 && tid < kTile) load_scales();
 
   // ---- q, beside the first tile's loads
   u4 q[NQ][KW][QP];
@@ -1001,7 +1008,11 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     }
     __syncthreads();
     int next = 0;
-    if (tid < kTile) next = find(min(tile + 1, n_tiles - 1));
+    if (tid < kTile) {
+      if constexpr (EARLY) load_scales();
+      next = find(min(tile + (EARLY ? 2 : 1), n_tiles - 1));
+    }
+    if (EARLY && tile + 1 < n_tiles) load_k(tile + 1);
     uint32_t pf[NQ][QP][4];
     f4 ks8[2] = {}, vs8[2] = {};
     if constexpr (E8)
@@ -1050,7 +1061,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
       if constexpr (SP == 1) probabilities<DT, CAP, NQ>(a, s, kb, edge, sc, ks8, vs8, span, vtop, m, l, o, pf);
     }
     if (B::ONE) __syncthreads();
-    if (tid < kTile) rows[((tile + 1) & 1) * kTile + tid] = next;
+    if (tid < kTile) rows[((tile + (EARLY ? 0 : 1)) & 1) * kTile + tid] = next;
     if (E8 && v_busy) {
 #pragma unroll
       for (int t = 0; t < VD; t += 2) {
@@ -1089,9 +1100,8 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     }
     __syncthreads();
     if (tile + 1 < n_tiles) {
-      load_k(tile + 1);
+      if constexpr (!EARLY) load_k(tile + 1);
       if (v_busy) load_v(tile + 1);
-      if (E8 && tid < kTile) load_scales();
     }
     if (work) {
       if constexpr (SP > 1) {
@@ -1301,6 +1311,60 @@ __global__ __launch_bounds__(NT) void k_paged_merge(PagedAttnArgs a, const Paged
       o / l;
 }
 
+// The same where a row has many parts: a block takes 32 dims of one row, its threads being 8 columns by 128
+// groups of parts.  A block per row (k_paged_merge) reads all of the row's parts through one CU: 512 parts of 8 rows
+// of 128 dims, 2 MB, 8.4 us; by four blocks each 5.5 us.
+template <int HD>
+__global__ __launch_bounds__(1024) void k_paged_merge_cols(PagedAttnArgs a, const PagedMerge *merge) {
+  constexpr int W = 16, GRP = 128, AHEAD = 4;
+  __shared__ f4 os[W][8];
+  __shared__ f2 ls[W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kvh = blockIdx.x % a.n_kv;
+  const int col = 8 * blockIdx.z + (tid & 7), r = blockIdx.y;
+  const PagedMerge g = merge[blockIdx.x / a.n_kv];
+  if (r >= g.n_new * a.G - g.r0 || r >= a.part_rows) return;
+  const size_t step = (size_t)a.n_kv * a.part_rows;
+  const size_t pr = ((size_t)g.part * a.n_kv + kvh) * a.part_rows + r;
+  float m = kLow, l = 0.f;
+  f4 o = {};
+  // (weights are of what both have: a part that is not there has kLow, and 0 of everything)
+  auto join = [&](float m2, float l2, f4 o2) {
+    const float mn = fmaxf(m, m2), f = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(m2 - mn);
+    m = mn;
+    l = l * f + l2 * w;
+    o = o * f + o2 * w;
+  };
+  const float *po = a.part_o + pr * HD + 4 * col;
+  for (int p0 = tid / 8; p0 < g.n; p0 += AHEAD * GRP) {
+    f2 ml[AHEAD];
+    f4 x[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int p = min(p0 + i * GRP, g.n - 1);
+      ml[i] = ldg<f2>(a.part_ml + (pr + p * step) * 2);
+      x[i] = ldg<f4>(po + p * step * HD);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (p0 + i * GRP < g.n) join(ml[i].x, ml[i].y, x[i]);
+  }
+#pragma unroll
+  for (int off = 8; off < 64; off <<= 1) {
+    f4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = __shfl_xor(o[e], off, 64);
+    join(__shfl_xor(m, off, 64), __shfl_xor(l, off, 64), y);
+  }
+  if (lane < 8) os[wave][lane] = o;
+  if (lane == 0) ls[wave] = f2{m, l};
+  __syncthreads();
+  if (tid >= 8) return;
+#pragma unroll
+  for (int w = 1; w < W; ++w) join(ls[w].x, ls[w].y, os[w][tid]);
+  const int t = (int)div_by(g.r0 + r, a.by_g), h = g.r0 + r - t * a.G;
+  *reinterpret_cast<f4 *>(a.out + (size_t)(g.row + t) * a.out_ld + (size_t)(kvh * a.G + h) * HD + 4 * col) = o / l;
+}
+
 template <int HD, int DT, bool CAP>
 int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   using B = Shape<HD, DT>;
@@ -1353,10 +1417,13 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
     int rpb = 1024 / HD;
     while (rpb > 1 && 1024 / HD / rpb * 4 < p->most_parts) rpb /= 2;
     const dim3 mg(p->n_merge * a.n_kv, cdiv(p->most, rpb));
-    if (1024 / HD * 4 < p->most_parts)
-      hipLaunchKernelGGL((k_paged_merge<HD, 1024>), mg, dim3(1024), 0, st, a, merge, rpb);
-    else
+    // (the plain calls keep their order of sums, and so their results to the last bit)
+    if (1024 / HD * 4 >= p->most_parts)
       hipLaunchKernelGGL((k_paged_merge<HD, 256>), mg, dim3(256), 0, st, a, merge, rpb);
+    else if (Form<DT>::E8 || CAP)
+      hipLaunchKernelGGL(k_paged_merge_cols<HD>, dim3(p->n_merge * a.n_kv, p->most, HD / 32), dim3(1024), 0, st, a, merge);
+    else
+      hipLaunchKernelGGL((k_paged_merge<HD, 1024>), mg, dim3(1024), 0, st, a, merge, rpb);
   }
   MS_HIP_TRY(hipGetLastError());
   return MS_OK;
