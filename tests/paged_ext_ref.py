@@ -109,7 +109,7 @@ class SetupExt(Setup):
         return ({n: d.download(np.uint8, self.raw[n].shape) for n, d in (("k", self.dk), ("v", self.dv))},
                 {n: d.download(np.float32, self.scales[n].shape) for n, d in (("k", self.dks), ("v", self.dvs))})
 
-    def attend(self, q):
+    def attend(self, q, only=None):
         """The rows' attention in 64 bits, capped, and per value how far an fp32 result may be off: what
         Setup.attend derives (an 8-bit key's scale is one more rounding of its score, q's 22 bits four: its eight spare
         ones), and with a cap what tanh adds.  tanh never grows an error; its own: below 0.6 2^-23 of it; above, from
@@ -118,13 +118,16 @@ class SetupExt(Setup):
         An 8-bit value's probability times its scale is taken in two fp16 parts: off by 2^-22 of itself (eight spare
         ones hold that) or, where that is less, by half of fp16's smallest step, 2^-25, in units of 2^-7 of a power of two that
         is at most twice the largest scale the row attends to, the best key having a probability of 1 at least: 2^-31 of that
-        scale for each key, times its code."""
+        scale for each key, times its code.
+        only: of these rows."""
         G = self.heads // self.kv
         out, tol = (np.zeros((self.rows, self.heads, self.hd)) for _ in range(2))
         q = q.reshape(self.rows, self.heads, self.hd).astype(np.float64)
         sc = self.scale or 1 / np.sqrt(self.hd)
         cache = {}
         for r, (s, p) in enumerate(self.row_of()):
+            if only is not None and r not in only:
+                continue
             if s not in cache:
                 g = self.slots(s, 0, self.len[s])
                 cache = {s: [decode(self.pool[n][g], self.dtype) for n in "kv"]}
@@ -149,11 +152,12 @@ class SetupExt(Setup):
                         tol[r, h] += 2.0 ** -31 * np.float64(scale.max()) * code.sum(0)
         return out.reshape(self.rows, -1), tol.reshape(self.rows, -1)
 
-    def check(self, seed=1, pad=0, scale=1.5):
+    def check(self, seed=1, pad=0, scale=1.5, only=None):
         q = (np.random.default_rng(seed).standard_normal((self.rows, self.heads * self.hd)) * scale).astype(np.float32)
-        want, tol = self.attend(q)
+        want, tol = self.attend(q, only)
         got = self.run_attention(q, pad)
-        bad = ~(np.abs(got - want) <= tol)
+        at = slice(None) if only is None else list(only)
+        bad = ~(np.abs(got - want)[at] <= tol[at])
         assert not bad.any(), (np.argwhere(bad)[:4], np.abs(got - want).max(), bad.sum())
         return q, got
 

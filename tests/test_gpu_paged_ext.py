@@ -277,6 +277,25 @@ def test_attention_capped(gpu, case):
     st.check(pad=4 * (case % 3), scale=3.0)
 
 
+@pytest.mark.parametrize("dtype,hd,kv,G,rows,cap", [
+    ("e4m3", 512, 32, 2, 320, 0.0), ("i8", 128, 64, 1, 1280, 20.0), ("bf16", 512, 32, 2, 290, 20.0), ("e4m3", 64, 64, 2, 641, 5.0)])
+def test_attention_last_turn(gpu, dtype, hd, kv, G, rows, cap):
+    """Chunks whose blocks are all busy more than once, the last time few of them: some rows' keys are cut, others not."""
+    say(f"attention, a short last turn: {dtype} hd={hd} {rows} rows")
+    st = SetupExt(gpu, [(rows, rows + 1200)], kv * G, kv, hd, dtype, 64, cap=cap, seed=21)
+    st.check(only=(0, 1, 17, 31, 63, 64, 100, 127, 128, rows // 2, rows - 33, rows - 1))
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "i8", "f32", "bf16", "f16"])
+@pytest.mark.parametrize("seqs,heads,kv,hd", [([(1, 40000), (1, 3)], 3, 1, 64), ([(2, 12000)], 6, 2, 128), ([(1, 9000)], 16, 1, 256),
+                                              ([(3, 5000), (1, 1)], 4, 1, 512)])
+def test_attention_many_parts(gpu, seqs, heads, kv, hd, dtype):
+    """Few rows over many keys, whose parts are merged by several blocks."""
+    say(f"attention, many parts: {dtype} {seqs} hd={hd}")
+    st = SetupExt(gpu, seqs, heads, kv, hd, dtype, 32, cap=25.0, seed=22)
+    st.check()
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256, 512])
 @pytest.mark.parametrize("dtype", ["e4m3", "i8", "f32", "bf16", "f16"])
 @pytest.mark.parametrize("new", [1, 3, 40])

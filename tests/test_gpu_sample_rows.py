@@ -48,7 +48,8 @@ def pick(row, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, u=0.5):
     j = int(np.searchsorted(upto, target, side="right"))
     if 0 < u < 1:
         close |= bool(min(abs(float(upto[j]) - u * float(total)), abs(float(upto[max(j - 1, 0)]) - u * float(total))) < 2e-14 * float(total))
-    return int(left[j]), n, at[left[j]] / total, close
+    # (weights of 1 are whole numbers without any rounding: every border is exact)
+    return int(left[j]), n, at[left[j]] / total, close and not np.all(w == 1)
 
 
 def draw(ms, x, rows, u, pad=0, prob=True, kept=True):
@@ -105,6 +106,26 @@ def test_settings(gpu, vocab, pad):
     say(f"sample_rows: {vocab} ids, every setting")
     R = len(SETTINGS)
     check(gpu, logits(R, vocab, vocab), SETTINGS, np.random.default_rng(vocab + 1).random(R).astype(np.float32), pad)
+
+
+@pytest.mark.parametrize("vocab,pad", [(262144, 4), (262145, 0), (300001, 2), (1 << 20, 0), ((1 << 20) + 1, 3)])
+def test_large_vocabularies(gpu, vocab, pad):
+    """Few rows of many ids: small and large slices, rows gone over as a whole, rows at any alignment."""
+    say(f"sample_rows: few rows of {vocab} ids")
+    settings = [SETTINGS[i] for i in (0, 1, 3, 6, 16)]
+    x = logits(len(settings), vocab, vocab)
+    x[2, : vocab // 2] = -np.inf  # (slices without any id)
+    check(gpu, x, settings, np.random.default_rng(vocab).random(len(settings)).astype(np.float32), pad)
+
+
+def test_flat_large_slices(gpu):
+    """More candidates in a slice than it may list."""
+    say("sample_rows: flat rows of 300000 ids")
+    settings = [dict(), dict(top_p=0.3), dict(top_k=3000), dict(top_k=40, top_p=0.5), dict(temperature=0.0)]
+    rng = np.random.default_rng(31)
+    x = (1e-6 * rng.integers(0, 3, (len(settings), 300000))).astype(np.float32)
+    x[3] = 0.0
+    check(gpu, x, settings, rng.random(len(settings)).astype(np.float32))
 
 
 @pytest.mark.parametrize("std", [0.0, 1e-3, 0.5, 30.0, 1e4])
