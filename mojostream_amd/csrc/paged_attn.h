@@ -43,8 +43,9 @@ struct PagedAttnArgs {
   const float *k_scale, *v_scale;  // 8-bit pools: [page][kv head][slot]
   int hp_log;             // 8-bit pools, item_by_tile: log2 of the kv heads of a block
   // Capped scores: log2(e) times the cap is cap_p[0] (0.5 to 1) times cap_to (a power of two); inv_cap its
-  // inverse (0: not capped); cap_p[1..5] the coefficients of tanh's near form, times cap_p[0] (cap_args).
-  float cap_to, inv_cap, cap_p[6];
+  // inverse (0: not capped); cap_p[1..5] the coefficients of tanh's near form, times cap_p[0]; cap_2 is
+  // 2 cap_p[0] in log2, inv_2 its inverse (cap_args).
+  float cap_to, inv_cap, cap_p[6], cap_2, inv_2;
 };
 
 // The split of the batch's work for a shape of layers (made anew after each set).  tail: a last turn of whole spans that
@@ -177,7 +178,8 @@ __device__ inline float sum_groups(float v) {
 
 // Capped scores: c tanh(z), c = cap_p[0].  To |z| = 0.6, z2 < kNear, c z (1 + z^2 P(z^2)), P a polynomial fitted here
 // by least squares, reweighted until its largest relative error (3e-9) is least: scores far below the cap keep
-// all their bits; past it from e^(-2 |z|).
+// all their bits.  Past it c - 2 c t / (1 + t), t = e^(-2 z); scores near the cap are told apart by the second term: as
+// 32-bit numbers of the cap's size (50: 72 in log2) each would be off by up to 4e-6.
 constexpr float kNear = 0.36f;
 inline void cap_args(PagedAttnArgs *a, float cap) {
   constexpr double p[6] = {1, -0.333332986, 0.133319244, -0.0537838228, 0.0207959525, -0.00589513639};
@@ -186,18 +188,22 @@ inline void cap_args(PagedAttnArgs *a, float cap) {
   a->cap_to = (float)std::ldexp(1.0, e);
   a->inv_cap = (float)(1.0 / c);
   for (int i = 0; i < 6; ++i) a->cap_p[i] = (float)(part * p[i]);
+  a->cap_2 = (float)std::log2(2 * part);
+  a->inv_2 = (float)(0.5 / part);
 }
-__device__ inline float cap_near(const PagedAttnArgs &a, float z) {
+// Both less h.
+__device__ inline float cap_near(const PagedAttnArgs &a, float z, float h) {
   const float z2 = z * z;
   float p = a.cap_p[5];
 #pragma unroll
-  for (int i = 4; i >= 0; --i) p = __builtin_fmaf(p, z2, a.cap_p[i]);
-  return z * p;
+  for (int i = 4; i > 0; --i) p = __builtin_fmaf(p, z2, a.cap_p[i]);
+  return __builtin_fmaf(z * z2, p, __builtin_fmaf(z, a.cap_p[0], -h));
 }
-__device__ inline float cap_any(const PagedAttnArgs &a, float z) {
-  const float t = __builtin_amdgcn_exp2f(-2.f * 1.44269504f * fabsf(z));
-  const float far = a.cap_p[0] * ((1.f - t) * __builtin_amdgcn_rcpf(1.f + t));
-  return z * z < kNear ? cap_near(a, z) : copysignf(far, z);
+__device__ inline float cap_any(const PagedAttnArgs &a, float z, float h) {
+  // (2 c t; 2^100: the second term is 2 c)
+  const float t = __builtin_amdgcn_exp2f(fminf(__builtin_fmaf(z, -2.f * 1.44269504f, a.cap_2), 100.f));
+  const float far = __builtin_fmaf(-t, __builtin_amdgcn_rcpf(__builtin_fmaf(t, a.inv_2, 1.f)), a.cap_p[0] - h);
+  return z * z >= kNear ? far : cap_near(a, z, h);
 }
 
 // Of an 8-bit pool's scales: where that of a page's slot is.
@@ -233,7 +239,7 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
         if constexpr (Form<DT>::E8)
           s *= ldg<float>(a.k_scale + scale_at(a, a.pages[(size_t)it.seq * a.stride + pg], key - pg * a.page_size, kvh));
         s *= a.s_scale;
-        if constexpr (CAP) s = a.cap_to * cap_any(a, s * a.inv_cap);
+        if constexpr (CAP) s = a.cap_to * cap_any(a, s * a.inv_cap, 0.f);
       }
       float mx = on ? s : -INFINITY;
       for (int off = 1; off < 64; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
@@ -318,19 +324,29 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
       }
     }
   }
-  // (both forms for each score of every tile: 4096 rows over 16384 keys, i8, 3.5 ms; the near one alone where a
-  // tile's scores allow it: @@ ms; uncapped 2.6 ms)
+  // A lane that has a score of query n past kNear takes all eight in their distance to the cap, `from`: cap - m is exact
+  // where m is near it, and t then has an error of its own size.  (The lane's smaller scores are off by up to 2^-25 of the
+  // cap, what those at half of it are in any case; the smaller the less they weigh beside the one past it.)
+  float from[NQ] = {};
+  // (both forms for each score of every tile: 4096 rows over 16384 keys, 14B class, i8, 3.5 ms; the near one alone
+  // where a tile's scores allow it, 3.2 ms; uncapped 2.5 ms)
   if constexpr (CAP) {
     if (__any(z2 >= kNear)) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+      for (int n = 0; n < NQ; ++n) {
+        float most = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j >> 2][n][j & 3] = cap_any(a, s[j >> 2][n][j & 3]);
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, s[j >> 2][n][j & 3]);
+        const float h = most * most >= kNear ? a.cap_p[0] : 0.f;
+        from[n] = h * a.cap_to;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j >> 2][n][j & 3] = cap_any(a, s[j >> 2][n][j & 3], h);
+      }
     } else {
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j >> 2][n][j & 3] = cap_near(a, s[j >> 2][n][j & 3]);
+        for (int j = 0; j < 8; ++j) s[j >> 2][n][j & 3] = cap_near(a, s[j >> 2][n][j & 3], 0.f);
     }
   }
   const int g = (threadIdx.x & 63) >> 4;
@@ -338,7 +354,7 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
 #pragma unroll
   for (int n = 0; n < NQ; ++n)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[n][j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], -m[n]);
+    for (int j = 0; j < 8; ++j) t[n][j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], CAP ? from[n] - m[n] : -m[n]);
   if (edge) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -362,7 +378,9 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        mx = fmaxf(mx, t[n][j] == -INFINITY ? -INFINITY : s[j >> 2][n][j & 3] * sc[n]);
+        mx = fmaxf(mx, t[n][j] == -INFINITY ? -INFINITY
+                       : CAP                ? __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], from[n])
+                                            : s[j >> 2][n][j & 3] * sc[n]);
       const float mn = fmaxf(m[n], max_groups(mx)), al = __builtin_amdgcn_exp2f(m[n] - mn);
       m[n] = mn;
       l[n] *= al;
@@ -370,7 +388,7 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
       for (int d = 0; d < ND; ++d) o[n][d] *= al;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (t[n][j] != -INFINITY) t[n][j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], -mn);
+        if (t[n][j] != -INFINITY) t[n][j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], CAP ? from[n] - mn : -mn);
     }
   }
   if constexpr (E8) {
