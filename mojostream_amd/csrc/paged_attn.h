@@ -8,13 +8,15 @@
 //  k_paged_tile   up to 32 (row, head) pairs of a kv head: single tokens, or a few
 //                 (item_by_tile).  Bound by memory: 48 tokens over up to 4096 keys, 14B class, bf16,
 //                 458 MB in 92 to 97 us; 32 tokens over up to 4096 keys in fp32, 8 kv heads of 128
-//                 dims, 5.1 TB/s, 2 of 512 dims, 5.6 TB/s (a large copy: 4.6 TB/s).
+//                 dims, 5.1 TB/s, 2 of 512 dims, 5.6 TB/s (a large copy: 4.6 TB/s).  8-bit pools: the 48 tokens'
+//                 237 MB in 47 to 51 us (4.6 to 5.0 TB/s); one token over 131065 keys, 2 kv heads of 128 dims, capped, 69 MB in 19 us.
 //  k_paged_block  longer chunks, and single tokens beside them (item_by_block, item_by_tile).
 //                 Bound by the matrix cores: 4096 rows over 16384 keys, 14B class, bf16 (three
 //                 products a multiplication): 2.7 to 2.9 ms among other calls (2.9 to 3.1 in ten
 //                 passes under the profiler), 1.3 PFLOP/s of bf16 products, MFMA busy 56% of the time
-//                 at 2.1 GHz (a large bf16 matrix product: 1.2 PFLOP/s).
-//  k_paged_merge  the spans' results.
+//                 at 2.1 GHz (a large bf16 matrix product: 1.2 PFLOP/s).  8-bit pools (two products): 2.39 to 2.48 ms,
+//                 with a cap 3.2 to 3.4 ms; capped over bf16 3.0 to 3.15 ms.
+//  k_paged_merge  the spans' results (k_paged_merge_cols: of many spans a row, over 8-bit pools or capped).
 #pragma once
 #include <cmath>
 #include <type_traits>
@@ -96,8 +98,8 @@ constexpr float kLag = 8.0f;
 //   8-bit the codes, which fp16 holds exactly, and two fp16 parts of q and of p times the values'
 //         scales, in units of the smallest power of two above the scales that the row has attended to
 //         (a scale's head has a code of full size, so that what is lost is below 2^-32 of that too).  The keys' scales
-//         multiply the scores.  With three bf16 parts of p times the scales as they are the chunk of 4096 rows over 16384
-//         keys took 2.6 ms
+//         multiply the scores.  (Three bf16 parts of p times the scales as they are: the chunk of 4096 rows over 16384
+//         keys 2.60 ms, so 2.53, before its last spans were cut and its keys loaded earlier)
 template <int DT>
 struct Form {
   static constexpr bool E8 = DT == MS_KV_E4M3 || DT == MS_KV_I8;
@@ -1436,12 +1438,14 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
     while (rpb > 1 && 1024 / HD / rpb * 4 < p->most_parts) rpb /= 2;
     const dim3 mg(p->n_merge * a.n_kv, cdiv(p->most, rpb));
     // (the plain calls keep their order of sums, and so their results to the last bit)
-    if (1024 / HD * 4 >= p->most_parts)
+    constexpr bool COLS = Form<DT>::E8 || CAP;
+    if (1024 / HD * 4 >= p->most_parts) {
       hipLaunchKernelGGL((k_paged_merge<HD, 256>), mg, dim3(256), 0, st, a, merge, rpb);
-    else if (Form<DT>::E8 || CAP)
+    } else if constexpr (COLS) {
       hipLaunchKernelGGL(k_paged_merge_cols<HD>, dim3(p->n_merge * a.n_kv, p->most, HD / 32), dim3(1024), 0, st, a, merge);
-    else
+    } else {
       hipLaunchKernelGGL((k_paged_merge<HD, 1024>), mg, dim3(1024), 0, st, a, merge, rpb);
+    }
   }
   MS_HIP_TRY(hipGetLastError());
   return MS_OK;

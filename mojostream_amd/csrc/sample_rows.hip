@@ -9,9 +9,13 @@
 //               (top-p) over buckets of its logits
 //  k_rows_pick  finds, from the slices' histograms, the bucket in which the cut lies; the slice once more: the
 //               candidates (top-k: all down to the cut's bucket; top-p: those in it) into a list, the weights
-//               of what lies above it added up by chunks of 1024 ids
+//               of what lies above it added up by chunks of a wave's 256 or 1024 ids
 //  k_rows_draw  a block a row: sorts the candidates, finds the cut and draws.  Rows that this does not
 //               fit (more candidates than the list holds, a large top-k, infinite logits) it goes over as a whole.
+//
+// Three launches, each with a chain of loads behind the last one's results: 4.8 + 7.2 + 6.6 us for a row of 262144 ids; 48 such
+// rows, 50 MB, 17 + 17 + 12 us (the first without its weights and sums 17 as well; in slices of 28672 ids, whose
+// blocks are all there at once, 20 + 16 + 14).
 #include <climits>
 #include <cmath>
 
