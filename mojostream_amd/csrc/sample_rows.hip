@@ -41,7 +41,7 @@ struct RowInfo {
   int ref;                  // weights are 2^(x log2(e) / T - ref)
   float top;                // the largest logit
   float lo, hi;             // the cut lies among the logits lo <= x < hi (the candidates); what lies above stays
-  unsigned long long want;  // top-p: weight still to be reached by the candidates
+  unsigned long long want;  // top-p: weight still to be reached by the candidates; top-k: ids of the cut's bucket
 };
 // A row's settings.
 struct RowSet {
@@ -292,7 +292,8 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
     const int group = hit ? __ffsll(hit) - 1 : -1;
     const unsigned long long before = __shfl(upto - s, max(group, 0), 64);
     if (lane == 0) {
-      // (top-k: all that can be drawn is in the list, if it holds that)
+      // (top-k, whose buckets end eight octaves below the largest logit: all that can be drawn is in the list, if it holds
+      // that, and nothing is `want`ed of a bucket)
       if (group < 0 && (SUMS || real > kList)) in.state = kSlow;
       if (!SUMS) in.hi = INFINITY;
       lds.info = in;
@@ -888,11 +889,12 @@ __device__ inline void draw_many(const SampleRowsArgs &a, const RowSet &set, int
     return num;
   };
 
-  // ---- top-k: of the last bucket's, as many as it takes
+  // ---- top-k: of the last bucket's, as many as it takes; of all, where the buckets end above the cut
   if (n_list > set.k) {
     const uint32_t last = key_of(in.lo) >> 15;
-    gather([&](unsigned long long y) { return (uint32_t)(y >> 47) == last; });
-    const unsigned long long cut = list[in.want - 1];
+    const bool beyond = in.want == 0;
+    gather([&](unsigned long long y) { return beyond || (uint32_t)(y >> 47) == last; });
+    const unsigned long long cut = list[(beyond ? (unsigned long long)set.k : in.want) - 1];
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (x[e] < cut) x[e] = 0;

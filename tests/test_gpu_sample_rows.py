@@ -118,6 +118,23 @@ def test_large_vocabularies(gpu, vocab, pad):
     check(gpu, x, settings, np.random.default_rng(vocab).random(len(settings)).astype(np.float32), pad)
 
 
+@pytest.mark.parametrize("vocab,shift", [(1250, 0.0), (1700, 0.0), (2300, 0.0), (6000, -1.0), (3000, -30.0), (9000, 0.0), (100003, 0.0)])
+def test_top_k_across_zero(gpu, vocab, shift):
+    """Cuts far below the largest logit in size, at zero and beyond, by top-k alone and with the others; few ids that can be drawn."""
+    say(f"sample_rows: top-k down to logits about zero, {vocab} ids")
+    settings = [dict(top_k=k, temperature=t, top_p=p, min_p=m)
+                for k in (300, 1000, 1800, 2048) for t, p, m in ((1.5, 0.6, 0.0), (1.0, 1.0, 0.0), (30.0, 0.97, 0.0), (5.0, 1.0, 0.01))]
+    rng = np.random.default_rng(vocab)
+    x = logits(len(settings), vocab, vocab + 1) + np.float32(shift)
+    if shift:
+        x[:, 17] = -1e-3  # (the largest logit is the smallest in size)
+        x = np.minimum(x, np.float32(-1e-3))
+    x[::3][rng.random(x[::3].shape) < 0.3] = -np.inf
+    if vocab > 50000:
+        x[rng.random(x.shape) < 0.97] = -np.inf
+    check(gpu, x, settings, rng.random(len(settings)).astype(np.float32))
+
+
 def test_flat_large_slices(gpu):
     """More candidates in a slice than it may list."""
     say("sample_rows: flat rows of 300000 ids")
