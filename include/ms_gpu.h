@@ -315,7 +315,8 @@ typedef struct {
    * kv head h and slot s at k_scale[(p * n_kv_heads + h) * page_rows + s] (page_rows 0: page_size);
    * unused otherwise. */
   float *k_scale, *v_scale;
-  float score_cap;  /* attention: a score s becomes score_cap * tanh(s / score_cap); 0: none; else 2^-60 to 2^60 */
+  float score_cap;  /* attention: a score s becomes score_cap * tanh(s / score_cap); 0: none; else 2^-60 to 2^60
+                        (scale / score_cap: 2^-126 to 2^127 in size) */
   int norm;         /* append: MS_NORM_*, whose heads are normed before they are rotated; 0: none */
   float norm_eps;   /* x / sqrt(mean of a head's x^2 + norm_eps) * gamma */
   const float *q_gamma, *k_gamma; /* device, [head_dim]; NULL: 1 (v has none) */

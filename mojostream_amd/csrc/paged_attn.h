@@ -38,16 +38,17 @@ struct PagedAttnArgs {
   const PagedItem *items;
   int n_kv, G, window, page_size, page_rows;
   FastDiv by_page, by_g;  // n / page_size, n / G
-  // The scores' scale, log2(e) in it, is q_scale (0.5 to 1 in size) times s_scale (a power of two).
+  // The scores' scale, log2(e) in it (capped scores: over the cap), is q_scale (0.5 to 1 in size) times s_scale (a power
+  // of two).
   float q_scale, s_scale;
   float *part_o, *part_ml;  // [part][kv head][part_rows][head dim], [part][kv head][part_rows][2]
   int part_rows;          // (row, head) pairs of the longest item
   const float *k_scale, *v_scale;  // 8-bit pools: [page][kv head][slot]
   int hp_log;             // 8-bit pools, item_by_tile: log2 of the kv heads of a block
-  // Capped scores: log2(e) times the cap is cap_p[0] (0.5 to 1) times cap_to (a power of two); inv_cap its
-  // inverse (0: not capped); cap_p[1..5] the coefficients of tanh's near form, times cap_p[0]; cap_2 is
+  // Capped scores: log2(e) times the cap is cap_p[0] (0.5 to 1) times cap_to (a power of two; 0: not
+  // capped); cap_p[1..5] the coefficients of tanh's near form, times cap_p[0]; cap_2 is
   // 2 cap_p[0] in log2, inv_2 its inverse (cap_args).
-  float cap_to, inv_cap, cap_p[6], cap_2, inv_2;
+  float cap_to, cap_p[6], cap_2, inv_2;
 };
 
 // The split of the batch's work for a shape of layers (made anew after each set).  tail: a last turn of whole spans that
@@ -188,7 +189,6 @@ inline void cap_args(PagedAttnArgs *a, float cap) {
   int e = 0;
   const double c = cap * 1.4426950408889634, part = std::frexp(c, &e);
   a->cap_to = (float)std::ldexp(1.0, e);
-  a->inv_cap = (float)(1.0 / c);
   for (int i = 0; i < 6; ++i) a->cap_p[i] = (float)(part * p[i]);
   a->cap_2 = (float)std::log2(2 * part);
   a->inv_2 = (float)(0.5 / part);
@@ -241,7 +241,7 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
         if constexpr (Form<DT>::E8)
           s *= ldg<float>(a.k_scale + scale_at(a, a.pages[(size_t)it.seq * a.stride + pg], key - pg * a.page_size, kvh));
         s *= a.s_scale;
-        if constexpr (CAP) s = a.cap_to * cap_any(a, s * a.inv_cap, 0.f);
+        if constexpr (CAP) s = a.cap_to * cap_any(a, s, 0.f);
       }
       float mx = on ? s : -INFINITY;
       for (int off = 1; off < 64; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
@@ -320,7 +320,7 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
     for (int i = 0; i < 2; ++i) {
       if constexpr (E8) s[i][n] *= ks[i];
       if constexpr (CAP) {
-        s[i][n] *= scale[n] * a.inv_cap;
+        s[i][n] *= scale[n];
 #pragma unroll
         for (int e = 0; e < 4; ++e) z2 = fmaxf(z2, s[i][n][e] * s[i][n][e]);
       }
@@ -437,6 +437,13 @@ __device__ inline void lift_of(float big, float *up, float *down) {
   e = max(-126, min(126, e));
   *up = __uint_as_float((uint32_t)(127 + e) << 23);
   *down = __uint_as_float((uint32_t)(127 - e) << 23);
+}
+
+// What a query's products are multiplied by.  (Capped: finite, so that a score of 0 stays 0 however far q is from the cap.)
+template <bool CAP>
+__device__ inline float score_scale(const PagedAttnArgs &a, float down) {
+  const float s = a.s_scale * down;
+  return CAP ? fminf(s, 0x1p127f) : s;
 }
 
 // KS 32-dim steps of a query's dims from qp on (that lane's eight of each; WIDE: its sixteen of two), times `scale` (0.5 to 1 in
@@ -605,7 +612,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
     const int t = real ? (int)div_by(it.r0 + r, a.by_g) : t_first, h = real ? it.r0 + r - t * a.G : 0;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + LD8 * g;
     load_q<DT, KS, E8>(qp + HW * part, real, a.q_scale, q[n], &down[n]);
-    sc[n] = SP == 1 ? a.s_scale * down[n] : a.s_scale;
+    sc[n] = SP == 1 ? score_scale<CAP>(a, down[n]) : a.s_scale;
   }
 
   f4 o[NQ][NC * VD] = {};
@@ -989,7 +996,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     vtop[n] = 0x1p-119f;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
     load_q<DT, KW>(qp + 32 * KW * part, real, a.q_scale, q[n], &down[n]);
-    sc[n] = SP == 1 ? a.s_scale * down[n] : a.s_scale;
+    sc[n] = SP == 1 ? score_scale<CAP>(a, down[n]) : a.s_scale;
   }
   f4 o[NQ][CW * VD] = {};
   for (int tile = 0; tile < n_tiles; ++tile) {

@@ -154,9 +154,11 @@ int attend(const char *what, const ms_paged_layer *L, const ms_paged_layer_ext *
   // (log2(e) times it, what the kernels take, is finite too)
   MS_CHECK_ARG(std::fabs(L->scale * 1.4426950408889634) <= 0x1.fffffep+127,
                w("the scale is not finite or too large"));
-  if (int rc = X ? paged_check_ext(what, X, b) : paged_check(what, L, b)) return rc;
   const float cap = X ? X->score_cap : 0.f;
   MS_CHECK_ARG(cap == 0.f || (cap >= 0x1p-60f && cap <= 0x1p60f), w("score_cap must be 0 or 2^-60 to 2^60"));
+  const double ratio = cap == 0.f || L->scale == 0.f ? 1.0 : std::fabs(L->scale / (double)cap);
+  MS_CHECK_ARG(ratio >= 0x1p-126 && ratio <= 0x1.fffffep+127, w("the scale over score_cap must be 2^-126 to 2^127 in size"));
+  if (int rc = X ? paged_check_ext(what, X, b) : paged_check(what, L, b)) return rc;
   MS_CHECK_ARG((int64_t)b->rows * L->n_heads < ((int64_t)1 << 30), w("too many rows for one call"));
   const int q_dim = L->n_heads * L->head_dim, hd = L->head_dim, G = L->n_heads / L->n_kv_heads;
   int most = 0;
@@ -195,7 +197,8 @@ int attend(const char *what, const ms_paged_layer *L, const ms_paged_layer_ext *
   a.by_page = fast_div(b->page_size);
   a.by_g = fast_div(G);
   int e = 0;
-  const double scale = (L->scale == 0.f ? 1.0 / std::sqrt((double)hd) : L->scale) * 1.4426950408889634;
+  const double by = L->scale == 0.f ? 1.0 / std::sqrt((double)hd) : L->scale;
+  const double scale = cap == 0.f ? by * 1.4426950408889634 : by / cap;
   const double part = std::frexp(scale, &e);  // (e <= 128; 2^127 is the largest power that fp32 holds)
   a.q_scale = (float)(e > 127 ? 2 * part : part);
   a.s_scale = (float)std::ldexp(1.0, e > 127 ? e - 1 : e);

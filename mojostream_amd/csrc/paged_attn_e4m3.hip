@@ -4,8 +4,8 @@
 namespace ms {
 
 int launch_attn_e4m3(PagedAttnArgs &a, ms_paged_batch *b, int hd, int most, hipStream_t st) {
-  return a.inv_cap != 0.f ? launch_dims<MS_KV_E4M3, true>(a, b, hd, most, st)
-                      : launch_dims<MS_KV_E4M3, false>(a, b, hd, most, st);
+  return a.cap_to != 0.f ? launch_dims<MS_KV_E4M3, true>(a, b, hd, most, st)
+                        : launch_dims<MS_KV_E4M3, false>(a, b, hd, most, st);
 }
 
 }  // namespace ms

@@ -290,10 +290,7 @@ extern "C" int ms_paged_append_ext(const ms_paged_layer_ext *X, const ms_paged_b
                                    size_t q_out_stride, const float *d_cos, const float *d_sin,
                                    int n_pos) {
   const char *what = "paged_append_ext";
-  if (int rc = append_check(what, X ? &X->base : nullptr, X, b, d_k, d_v, kv_stride, d_q, q_stride,
-                            d_q_out, q_out_stride, d_cos, d_sin, n_pos))
-    return rc;
-  const ms_paged_layer *L = &X->base;
+  MS_CHECK_ARG(X, "paged_append_ext: null layer or batch");
   MS_CHECK_ARG(X->norm >= 0 && X->norm <= (MS_NORM_Q | MS_NORM_K | MS_NORM_V),
                "paged_append_ext: unknown norm");
   MS_CHECK_ARG(!X->norm || (X->norm_eps >= 0.f && X->norm_eps < INFINITY),
@@ -301,6 +298,10 @@ extern "C" int ms_paged_append_ext(const ms_paged_layer_ext *X, const ms_paged_b
   MS_CHECK_ARG(X->rope == MS_ROPE_HALVES || X->rope == MS_ROPE_PAIRS, "paged_append_ext: unknown rotation");
   MS_CHECK_ARG(((reinterpret_cast<uintptr_t>(X->q_gamma) | reinterpret_cast<uintptr_t>(X->k_gamma)) & 3) == 0,
                "paged_append_ext: the gammas must be 4-byte aligned");
+  if (int rc = append_check(what, &X->base, X, b, d_k, d_v, kv_stride, d_q, q_stride,
+                            d_q_out, q_out_stride, d_cos, d_sin, n_pos))
+    return rc;
+  const ms_paged_layer *L = &X->base;
   if (b->rows == 0) return require_init();
   if (!X->norm && !is_8bit(L->dtype) && (X->rope == MS_ROPE_HALVES || L->rot_dim == 0))
     return ms_paged_append(L, b, d_k, d_v, kv_stride, d_q, q_stride, d_q_out, q_out_stride, d_cos,

@@ -277,6 +277,28 @@ def test_attention_capped(gpu, case):
     st.check(pad=4 * (case % 3), scale=3.0)
 
 
+@pytest.mark.parametrize("dtype", ["e4m3", "i8", "bf16", "f16"])
+@pytest.mark.parametrize("new,hd", [(1, 64), (3, 128), (40, 128), (30, 512)])
+def test_attention_cap_far_from_scores(gpu, new, hd, dtype):
+    """Scores far past any cap, or far below it, among scores of 0."""
+    say(f"attention, cap and scores far apart: {dtype} new={new} hd={hd}")
+    st = SetupExt(gpu, [(new, 150)], 4, 2, hd, dtype, 16, cap=1.0, seed=24)
+    g = [i[::2] for i in st.slots(0, 0, 150)]
+    (st.raw if st.eight else st.pool)["k"][tuple(g)] = 0
+    st.upload()
+    for cap in (2.0 ** -60, 1.0, 2.0 ** 60):
+        st.cap = st.layer.score_cap = cap
+        for scale in (2.0 ** 90, 2.0 ** -90):
+            q, got = st.check(scale=scale)
+            assert np.all(np.isfinite(got))
+            if scale < 1 or cap < 1:  # (scores of 0 to fp32: the values' mean; tanh of +-infinity times the least cap, too)
+                v = decode(st.pool["v"][st.slots(0, 0, 150)], dtype)
+                want = (np.cumsum(v, 0) / np.arange(1, 151)[:, None, None])[150 - new:]
+                want = np.repeat(want, 2, 1).reshape(new, -1)
+                # (a probability off by 2^-22, 160 rounded sums, the division)
+                assert np.all(np.abs(got - want) <= 2 * (2.0 ** -22 + 160 * 2.0 ** -24) * np.abs(v).max())
+
+
 @pytest.mark.parametrize("dtype,hd,kv,G,rows,cap", [
     ("e4m3", 512, 32, 2, 320, 0.0), ("i8", 128, 64, 1, 1280, 20.0), ("bf16", 512, 32, 2, 290, 20.0), ("e4m3", 64, 64, 2, 641, 5.0)])
 def test_attention_last_turn(gpu, dtype, hd, kv, G, rows, cap):

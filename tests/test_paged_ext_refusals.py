@@ -57,6 +57,25 @@ def test_layers(batch, change, say):
         assert say in err(), err()
 
 
+@pytest.mark.parametrize("cap,scale,ok", [
+    (float("nan"), 0.0, False), (float("inf"), 0.0, False), (-1.0, 0.0, False), (2.0 ** -61, 0.0, False), (2.0 ** 61, 0.0, False),
+    (2.0 ** -60, 2.0 ** 70, False), (2.0 ** 60, 2.0 ** -70, False), (30.0, float("nan"), False), (30.0, float("inf"), False),
+    (2.0 ** -60, 2.0 ** 60, True), (2.0 ** 60, -(2.0 ** -60), True), (0.0, 2.0 ** -100, True)])
+def test_caps(batch, cap, scale, ok):
+    assert attend(layer(score_cap=cap, scale=scale), batch) == INVALID
+    assert ("was not set" in err()) == ok and (ok or "scale" in err() or "score_cap" in err()), err()
+
+
+@pytest.mark.parametrize("change,say", [
+    (dict(norm=8), "unknown norm"), (dict(norm=-1), "unknown norm"), (dict(norm=1, norm_eps=-1e-9), "norm_eps"),
+    (dict(norm=2, norm_eps=float("nan")), "norm_eps"), (dict(norm=4, norm_eps=float("inf")), "norm_eps"),
+    (dict(rope=2), "unknown rotation"), (dict(rope=-1), "unknown rotation"), (dict(q_gamma=4098), "gammas"),
+    (dict(k_gamma=4099), "gammas"), (dict(norm=7, norm_eps=0.0, rope=1, q_gamma=4100, k_gamma=4100), "was not set")])
+def test_norms_and_rotations(batch, change, say):
+    assert append(layer(**change), batch) == INVALID
+    assert say in err(), err()
+
+
 def test_null(batch):
     L = layer()
     for call in (attend, append, read):
