@@ -324,7 +324,7 @@ typedef struct {
 } ms_paged_layer_ext;
 /* ms_paged_append with norms, either rotation and 8-bit pools.  An 8-bit head's scale is its largest
  * magnitude by 448 (MS_KV_I8: by 127), rounded to fp32, at least 2^-126 (and so that the largest code times it is finite), and its codes are the nearest to value / scale,
- * even where two are as near.  A head that holds a value that is not finite gets NaN as its scale, so that
+ * even where two are as near.  A head that holds a value that fp32 does not hold as a finite one gets NaN as its scale, so that
  * every value of it is NaN.  The squares are summed in 64 bits. */
 int ms_paged_append_ext(const ms_paged_layer_ext *layer, const ms_paged_batch *b, const float *d_k,
                         const float *d_v, size_t kv_stride, const float *d_q, size_t q_stride,
@@ -332,7 +332,9 @@ int ms_paged_append_ext(const ms_paged_layer_ext *layer, const ms_paged_batch *b
                         const float *d_sin, int n_pos);
 /* ms_paged_attention over any of the pools, with capped scores or not.  Over 8-bit pools the products take
  * the codes with all their bits, and 22 bits of q times the scores' scale (of these nothing below 2^-32 of a row's largest) and
- * of the probabilities times the values' scales (nothing below 2^-32 of the largest scale that the row attends to).  A cap holds for infinite scores too. */
+ * of the probabilities times the values' scales (nothing below 2^-32 of the largest scale that the row attends to).  A cap holds for infinite scores too.
+ * A row's q is brought to about 2^15 by a power of two before it meets the keys: 8-bit keys past 2^100 in size may
+ * overflow. */
 int ms_paged_attention_ext(const ms_paged_layer_ext *layer, ms_paged_batch *b, const float *d_q,
                            size_t q_stride, float *d_out, size_t out_stride);
 /* Positions pos0 .. pos0 + n - 1 of sequence seq out of the pages (any pool), in fp32: position

@@ -111,18 +111,13 @@ __global__ __launch_bounds__(kBlock) void k_append_ext(AppendExtArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < 2 * N; ++j) y[u][j] = (T)v[u][j];
-      if (normed) {
+      for (int j = 0; j < 2 * N; ++j) y[u][j] = normed ? (T)((double)v[u][j] * inv) : (T)v[u][j];
+      if (normed && gamma) {
         float g[2 * N];
-        if (gamma) {
-          get(gamma + d0[u], g);
-          get(gamma + d1[u], g + N);
-        }
+        get(gamma + d0[u], g);
+        get(gamma + d1[u], g + N);
 #pragma unroll
-        for (int j = 0; j < 2 * N; ++j) {
-          y[u][j] *= (T)inv;
-          if (gamma) y[u][j] *= (T)g[j];
-        }
+        for (int j = 0; j < 2 * N; ++j) y[u][j] *= (T)g[j];
       }
       if (turn[u]) {
         const size_t t = (size_t)w.pos * half + (u * LANES + lane) * N;
@@ -150,8 +145,8 @@ __global__ __launch_bounds__(kBlock) void k_append_ext(AppendExtArgs a) {
           const double m = fabs(y[u][j]);
           big = m > big ? m : m <= big ? big : (double)INFINITY;  // (NaN counts as infinite)
         }
-      float scale = fmaxf((float)(max_over(big, LANES) / TOP), 0x1p-126f);
-      scale = scale < INFINITY ? fminf(scale, MOST) : NAN;
+      big = max_over(big, LANES);  // (a value past fp32's range is infinite: rotations and gammas may lead there)
+      const float scale = big <= 0x1.fffffep+127 ? fminf(fmaxf((float)(big / TOP), 0x1p-126f), MOST) : NAN;
       uint8_t *pool = static_cast<uint8_t *>(what == 1 ? a.kp : a.vp) +
                       (((size_t)w.page * a.page_rows + w.slot) * a.n_kv + h) * HD;
       if (lane == 0)

@@ -43,6 +43,7 @@ def scale_of(x, dtype):
     """The scale of rows x [..][hd] (64 bits)."""
     with np.errstate(over="ignore", invalid="ignore"):
         s = np.maximum((np.abs(x).max(-1) / TOP[dtype]).astype(np.float32), np.float32(2.0 ** -126))
+        s = np.where(np.abs(x).max(-1) > MAX32, np.float32(np.nan), s)
         over = np.isfinite(s) & (s.astype(np.float64) * TOP[dtype] > MAX32)
         s = np.where(over, np.nextafter(s, np.float32(0)), s)
     return np.where(np.isfinite(s), s, np.float32(np.nan))

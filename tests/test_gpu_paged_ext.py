@@ -161,6 +161,60 @@ def test_append_special_values(gpu, dtype):
         assert np.all(np.abs(got[~bad] - x[~bad].astype(np.float64)) <= half * (1 + 1e-6))
 
 
+@pytest.mark.parametrize("dtype", ["e4m3", "i8"])
+@pytest.mark.parametrize("pairs", [False, True])
+def test_append_past_the_range(gpu, dtype, pairs):
+    """Rotations and gammas that lead past fp32's largest number, or to it."""
+    ms = gpu
+    say(f"append: past the range, {dtype} pairs={pairs}")
+    st = SetupExt(ms, [(4, 4)], 2, 2, 64, dtype, 4, rot=64, pairs=pairs)
+    x = f32(4, 2, 64, seed=3)
+    x[0] = MAX32                            # sqrt 2 of it
+    x[1] *= np.float32(0.7 * MAX32) / np.abs(x[1]).max()
+    x[2] = np.float32(0.72 * MAX32)
+    x[2, 0, ::2], x[2, 0, 1::2] = 0, 0      # (zeros beside a head that is past it)
+    x[3] = -np.float32(0.707 * MAX32)
+    cs = np.full((4, 32), np.float32(np.sqrt(0.5)))
+    d, c = ms.DeviceBuffer.from_array(x), ms.DeviceBuffer.from_array(cs)
+    ms.paged_append(st.layer, st.batch, d, d, 128, cos=c, sin=c, n_pos=4)
+    ms.synchronize()
+    codes, scales = st.download8()
+    (_, wk, wv), _ = append_in_64(st, np.zeros((4, 2, 64)), x, x, cs, cs)
+    seen = []
+    for n, w in (("k", wk), ("v", wv)):
+        for r, (sq, p) in enumerate(st.row_of()):
+            pg, sl = st.pages[sq, p // 4], p % 4
+            s, want = scales[n][pg, :, sl], scale_of(w[r], dtype)
+            assert np.array_equal(np.isnan(s), np.isnan(want)) and np.all(np.isnan(s) | (np.abs(s / want - 1) <= 2.0 ** -23))
+            c_, near = nearest(w[r] / np.where(np.isnan(s), 1e300, s.astype(np.float64))[:, None], dtype)
+            ok = (VALUE[dtype][codes[n][pg, sl]] == VALUE[dtype][c_]) | near | np.isnan(s)[:, None]
+            assert ok.all()
+            seen += np.isnan(s).tolist()
+    assert 0 < sum(seen) < len(seen)
+
+
+def test_append_tiny_norms(gpu):
+    """Heads of the smallest numbers under a norm without eps: their inverse is past fp32's range, the result is not."""
+    ms = gpu
+    say("append: norms of tiny heads")
+    for dtype in ("f32", "bf16", "e4m3"):
+        st = SetupExt(ms, [(3, 3)], 2, 2, 128, dtype, 4, norm=7, eps=0.0)
+        x = (f32(3, 2, 128, seed=4).astype(np.float64) * np.array([1e-40, 1e-30, 1e37])[:, None, None]).astype(np.float32)
+        d, o = ms.DeviceBuffer.from_array(x), ms.DeviceBuffer(3 * 256 * 4)
+        ms.paged_append(st.layer, st.batch, d, d, 256, d, 256, o, 256)
+        ms.synchronize()
+        (wq, wk, wv), (tq, _, _) = append_in_64(st, x, x, x, None, None)
+        assert np.all(np.abs(o.download(np.float32, x.shape) - wq) <= tq) and np.all(np.isfinite(wq))
+        got = st.download8() if st.eight else st.download()
+        for r, (sq, p) in enumerate(st.row_of()):
+            pg, sl = st.pages[sq, p // 4], p % 4
+            for n, w in (("k", wk), ("v", wv)):
+                g = VALUE[dtype][got[0][n][pg, sl]] * got[1][n][pg, :, sl, None].astype(np.float64) if st.eight else decode(got[n][pg, sl], dtype)
+                step = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "e4m3": 2.0 ** -4}[dtype]
+                least = np.abs(w[r]).max() / 448 * 2.0 ** -10 if st.eight else 0.0
+                assert np.all(np.abs(g - w[r]) <= (step + 4 * 2.0 ** -24) * np.abs(w[r]) + least * 1.001)
+
+
 def test_append_norm_sizes(gpu):
     """Norms of very small and very large rows, and of zeros: the squares neither vanish nor overflow."""
     ms = gpu
