@@ -305,11 +305,12 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
 // as 0 or NaN.)
 // span(n, &low, &high): the keys that the lane's query of query tile n attends to.
 // ks, vs: an 8-bit pool's scales of keys 4 g .. 4 g + 3 of both half tiles; vtop: the power of two that the values' scales
-// are taken in, above all that the query has attended to.  CAP: the scores are capped.
+// are taken in, above all that the query has attended to.  CAP: the scores are capped.  l_far: 8-bit pools, the
+// sums of the tiles but for the last sixteen (fold).
 template <int DT, bool CAP, int NQ, int ND, class Span>
 __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2][NQ], int kb, bool edge,
                                               const float (&scale)[NQ], const f4 (&ks)[2], const f4 (&vs)[2],
-                                              const Span &span, float (&vtop)[NQ], float (&m)[NQ], float (&l)[NQ],
+                                              const Span &span, float (&vtop)[NQ], float (&m)[NQ], float (&l)[NQ], float (&l_far)[NQ],
                                               f4 (&o)[NQ][ND], uint32_t (&pf)[NQ][Form<DT>::QP][4]) {
   constexpr bool F16 = Form<DT>::F16, E8 = Form<DT>::E8;
   float sc[NQ], z2 = 0.f;
@@ -386,6 +387,7 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
       const float mn = fmaxf(m[n], max_groups(mx)), al = __builtin_amdgcn_exp2f(m[n] - mn);
       m[n] = mn;
       l[n] *= al;
+      if constexpr (E8) l_far[n] *= al;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[n][d] *= al;
 #pragma unroll
@@ -428,6 +430,18 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       split2<F16, Form<DT>::QP>(p[2 * j], p[2 * j + 1], &pf[n][0][j], 4);
+  }
+}
+
+// Every sixteenth of a wave's tiles.  One key may weigh as much as all others: added one after the other to a sum of its
+// size the tiles lost up to half of its last place each (16,000 rows over 65,536 keys: 2.8e-6 of the result, so 0.7e-6).
+template <int DT, int NQ>
+__device__ __forceinline__ void fold(int nth, float (&l)[NQ], float (&l_far)[NQ]) {
+  if (!Form<DT>::E8 || (nth & 15) != 0) return;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    l_far[n] += l[n];
+    l[n] = 0.f;
   }
 }
 
@@ -616,11 +630,11 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   }
 
   f4 o[NQ][NC * VD] = {};
-  float m[NQ], l[NQ], vtop[NQ];
+  float m[NQ], l[NQ], l_far[NQ], vtop[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     m[n] = kLow;
-    l[n] = 0.f;
+    l[n] = l_far[n] = 0.f;
     vtop[n] = 0x1p-119f;
   }
   auto span = [&](int n, int *low, int *high) {
@@ -636,6 +650,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
     const int tile = step * NG + grp, kb = it.k0 + tile * kTile;
     const bool work = SP == 1 || tile < n_tiles, more = tile + NG < n_tiles;
     if (SP == 1 && tile >= n_tiles) break;
+    fold<DT, NQ>(step, l, l_far);
     f4 s[2][NQ] = {}, ks8[2] = {}, vs8[2] = {};
     if (work) {
       if (!AHEAD) {
@@ -708,7 +723,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
     }
     if (!work) continue;
     uint32_t pf[NQ][QP][4];
-    probabilities<DT, CAP, NQ>(a, s, kb, kb < all_lo || kb + kTile - 1 > all_hi, sc, ks8, vs8, span, vtop, m, l, o, pf);
+    probabilities<DT, CAP, NQ>(a, s, kb, kb < all_lo || kb + kTile - 1 > all_hi, sc, ks8, vs8, span, vtop, m, l, l_far, o, pf);
 
     // ---- values
 #pragma unroll
@@ -754,7 +769,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   int bad = 0;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    l[n] = sum_groups(l[n]);
+    l[n] = sum_groups(E8 ? l[n] + l_far[n] : l[n]);
     bad |= !(fabsf(l[n]) < INFINITY);
     if constexpr (E8)
 #pragma unroll
@@ -896,7 +911,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   uint32_t *rows = reinterpret_cast<uint32_t *>(lds + B::ROWS_AT);  // [2][32]
   float *scl = reinterpret_cast<float *>(lds + B::SCL_AT);     // [2][keys', values'][32]
 
-  float sc[NQ], down[NQ], m[NQ], l[NQ], vtop[NQ];
+  float sc[NQ], down[NQ], m[NQ], l[NQ], l_far[NQ], vtop[NQ];
   const int t_first = (int)div_by(it.r0, a.by_g), r_wave = 16 * NQ * grp;
   const int low_key = a.window ? max(it.k0, base + t_first - a.window + 1) : it.k0;
   const bool busy = r_wave < nrows;
@@ -992,7 +1007,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     const bool real = r < nrows;
     const int t = real ? (int)div_by(it.r0 + r, a.by_g) : t_first, h = real ? (it.r0 + r) - t * a.G : 0;
     m[n] = kLow;
-    l[n] = 0.f;
+    l[n] = l_far[n] = 0.f;
     vtop[n] = 0x1p-119f;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
     load_q<DT, KW>(qp + 32 * KW * part, real, a.q_scale, q[n], &down[n]);
@@ -1002,6 +1017,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   for (int tile = 0; tile < n_tiles; ++tile) {
     const int kb = it.k0 + tile * kTile;
     if (B::ONE && tile) __syncthreads();
+    fold<DT, NQ>(tile, l, l_far);
 #pragma unroll
     for (int u = 0; u < UK; ++u) {
       const int key = (tid + 64 * W * u) / D8, d8 = tid % D8;
@@ -1085,7 +1101,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
         }
         if constexpr (STRICT) __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (SP == 1) probabilities<DT, CAP, NQ>(a, s, kb, edge, sc, ks8, vs8, span, vtop, m, l, o, pf);
+      if constexpr (SP == 1) probabilities<DT, CAP, NQ>(a, s, kb, edge, sc, ks8, vs8, span, vtop, m, l, l_far, o, pf);
     }
     if (B::ONE) __syncthreads();
     if (tid < kTile) rows[((tile + (EARLY ? 0 : 1)) & 1) * kTile + tid] = next;
@@ -1143,7 +1159,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
             }
           __builtin_amdgcn_sched_barrier(0);
         }
-        probabilities<DT, CAP, NQ>(a, s, kb, edge, sc, ks8, vs8, span, vtop, m, l, o, pf);
+        probabilities<DT, CAP, NQ>(a, s, kb, edge, sc, ks8, vs8, span, vtop, m, l, l_far, o, pf);
       }
       u4 x[RING];
       auto read = [&](int f) {
@@ -1171,7 +1187,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   int bad = 0;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    l[n] = sum_groups(l[n]);
+    l[n] = sum_groups(E8 ? l[n] + l_far[n] : l[n]);
     bad |= !(fabsf(l[n]) < INFINITY);
     if constexpr (E8)
 #pragma unroll
