@@ -453,11 +453,20 @@ __device__ inline void lift_of(float big, float *up, float *down) {
   *down = __uint_as_float((uint32_t)(127 - e) << 23);
 }
 
-// What a query's products are multiplied by.  (Capped: finite, so that a score of 0 stays 0 however far q is from the cap.)
-template <bool CAP>
-__device__ inline float score_scale(const PagedAttnArgs &a, float down) {
-  const float s = a.s_scale * down;
-  return CAP ? fminf(s, 0x1p127f) : s;
+// What a query's products are multiplied by (waves that share its dims have them brought down already).  Capped: finite, so
+// that a score of 0 stays 0 however far q is from the cap; and a value of its own: the compiler else moves the
+// kernel's arguments about it to LDS (1890 rows of 256 dims, bf16: 41 to 52 us).
+template <int DT, bool CAP, int SP>
+__device__ inline float score_scale(float s_scale, float down) {
+  constexpr bool OWN = Form<DT>::F16 && SP == 1;  // a lane's query's
+  float s = OWN ? s_scale * down : s_scale;
+  if constexpr (CAP && OWN) {
+    s = fminf(s, 0x1p127f);
+    asm volatile("" : "+v"(s));
+  } else if constexpr (CAP) {
+    asm volatile("" : "+s"(s));
+  }
+  return s;
 }
 
 // KS 32-dim steps of a query's dims from qp on (that lane's eight of each; WIDE: its sixteen of two), times `scale` (0.5 to 1 in
@@ -626,7 +635,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
     const int t = real ? (int)div_by(it.r0 + r, a.by_g) : t_first, h = real ? it.r0 + r - t * a.G : 0;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + LD8 * g;
     load_q<DT, KS, E8>(qp + HW * part, real, a.q_scale, q[n], &down[n]);
-    sc[n] = SP == 1 ? score_scale<CAP>(a, down[n]) : a.s_scale;
+    sc[n] = score_scale<DT, CAP, SP>(a.s_scale, down[n]);
   }
 
   f4 o[NQ][NC * VD] = {};
@@ -1011,7 +1020,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
     vtop[n] = 0x1p-119f;
     const float *qp = a.q + (size_t)(it.row + t) * a.q_ld + (size_t)(kvh * a.G + h) * HD + 8 * g;
     load_q<DT, KW>(qp + 32 * KW * part, real, a.q_scale, q[n], &down[n]);
-    sc[n] = SP == 1 ? score_scale<CAP>(a, down[n]) : a.s_scale;
+    sc[n] = score_scale<DT, CAP, SP>(a.s_scale, down[n]);
   }
   f4 o[NQ][CW * VD] = {};
   for (int tile = 0; tile < n_tiles; ++tile) {
