@@ -282,6 +282,24 @@ def test_read(gpu, dtype, kv, hd, page, pr):
                 assert np.all(got == -777)
 
 
+@pytest.mark.parametrize("dtype", ["i8", "bf16"])
+def test_read_many(gpu, dtype):
+    """More rows than the caches hold, and half of them."""
+    ms = gpu
+    say(f"read of 138 MB, {dtype}")
+    kv, hd, n = 8, 512, 4200
+    st = SetupExt(ms, [(0, n)], kv, kv, hd, dtype, 128, seed=8, max_rows=1)
+    buf = {x: ms.DeviceBuffer.from_array(np.full((n + 1, kv * hd), -777, np.float32)) for x in "kv"}
+    for which in ("k", "kv"):
+        ms.paged_read(st.layer, st.batch, 0, 0, n, buf["k"], buf["v"] if "v" in which else None, kv * hd)
+        ms.synchronize()
+        for x in "kv":
+            got = buf[x].download(np.float32, (n + 1, kv * hd))
+            assert np.all(got[n:] == -777)
+            want = decode(st.pool[x][st.slots(0, 0, n)], st.dtype).reshape(n, -1).astype(np.float32)
+            assert np.array_equal(got[:n], want) if x in which else np.all(got == -777)
+
+
 # ---- attention -------------------------------------------------------------------------
 ATTENDS = [
     # seqs, heads, kv, hd, page, page_rows, window
