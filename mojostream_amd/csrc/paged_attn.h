@@ -540,7 +540,7 @@ __host__ __device__ constexpr int v_dims() {
 // A value that is not finite makes the sums it is multiplied into not finite, with the
 // zeros of masked keys too; where the end finds such a sum the item is done again key by
 // key.
-template <int HD, int DT, int NQ, int W, bool CAP>
+template <int HD, int DT, int NQ, int W, bool CAP, bool ONCE>
 __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const PagedItem &it, int kvh0,
                                              int hp_log, char *lds) {
   using F = Form<DT>;
@@ -591,6 +591,15 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
         for (int j = 0; j < (ES == 4 ? 2 : 1); ++j) kr[i][ks][j] = ldg<u4>(p + ks * KB + 16 * j);
     }
   };
+  // 8-bit values that no other item reads are not kept in the caches, where those that are still to come are looked
+  // for; 14B class, 48 tokens over up to 4096 and 16384 keys, e4m3, not in the caches before: 56 to 52 and 190 to 175 us (two
+  // heads of 256 dims that are: 28 to 30 us; the keys too: 56 and 185; rows of 64 bytes: 36 to 37).
+  auto get_v = [&](const char *p) {
+    if constexpr (ONCE)
+      return __builtin_nontemporal_load(reinterpret_cast<const u2 *>(p));
+    else
+      return ldg<u2>(p);
+  };
   auto load_v = [&](int row) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -598,7 +607,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         if constexpr (E8 && VD == 8) {
-          vr[j][c] = ldg<u2>(p + c * CD);
+          vr[j][c] = get_v(p + c * CD);
         } else if constexpr (E8) {
           vr[j][c] = u2{ldg<uint32_t>(p + c * CD), 0};
         } else if constexpr (VD * ES == 16) {
@@ -1272,14 +1281,14 @@ __device__ inline BlockOf block_of(int block, int n_blocks, int heads) {
 
 // Items of at most 16 NQ pairs: single tokens, or a few of them.  (Two query tiles of three parts do
 // not fit the registers of two waves a SIMD: with spills 110 us where one wave takes 72 us.)
-template <int HD, int DT, int NQ, bool CAP>
+template <int HD, int DT, int NQ, bool CAP, bool ONCE = Form<DT>::E8>
 __global__ __launch_bounds__(256, NQ == 2 && DT != MS_KV_F16 ? 1 : 2) void k_paged_tile(PagedAttnArgs a) {
   __shared__ __align__(16) char lds[tile_lds<HD, DT, NQ, 4>()];
   if constexpr (Form<DT>::E8) {
     const BlockOf b = block_of(blockIdx.x, gridDim.x, a.n_kv >> a.hp_log);
-    item_by_tile<HD, DT, NQ, 4, CAP>(a, a.items[b.item], b.head << a.hp_log, a.hp_log, lds);
+    item_by_tile<HD, DT, NQ, 4, CAP, ONCE>(a, a.items[b.item], b.head << a.hp_log, a.hp_log, lds);
   } else {
-    item_by_tile<HD, DT, NQ, 4, CAP>(a, a.items[blockIdx.x / a.n_kv], blockIdx.x % a.n_kv, 0, lds);
+    item_by_tile<HD, DT, NQ, 4, CAP, false>(a, a.items[blockIdx.x / a.n_kv], blockIdx.x % a.n_kv, 0, lds);
   }
 }
 
@@ -1290,7 +1299,7 @@ __global__ __launch_bounds__(NT, 2) void k_paged_block(PagedAttnArgs a) {
   __shared__ __align__(16) char lds[A > B ? A : B];
   const PagedItem it = a.items[blockIdx.x / a.n_kv];
   if (it.n_new * a.G - it.r0 <= 16)
-    item_by_tile<HD, DT, 1, Shape<HD, DT>::W, CAP>(a, it, blockIdx.x % a.n_kv, 0, lds);
+    item_by_tile<HD, DT, 1, Shape<HD, DT>::W, CAP, Form<DT>::E8>(a, it, blockIdx.x % a.n_kv, 0, lds);
   else
     item_by_block<HD, DT, CAP>(a, it, blockIdx.x % a.n_kv, lds);
 }
@@ -1458,6 +1467,8 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   const dim3 grid(p->n_items * (a.n_kv >> a.hp_log));
   if (block) {
     hipLaunchKernelGGL((k_paged_block<HD, DT, CAP>), grid, dim3(64 * B::W), 0, st, a);
+  } else if (Form<DT>::E8 && !TWO && most > 16) {  // (two items have the same keys)
+    if constexpr (!TWO) hipLaunchKernelGGL((k_paged_tile<HD, DT, 1, CAP, false>), grid, dim3(256), 0, st, a);
   } else if (rows == 16) {
     hipLaunchKernelGGL((k_paged_tile<HD, DT, 1, CAP>), grid, dim3(256), 0, st, a);
   } else {
