@@ -9,7 +9,7 @@
 //                 (item_by_tile).  Bound by memory: 48 tokens over up to 4096 keys, 14B class, bf16,
 //                 458 MB in 92 to 97 us; 32 tokens over up to 4096 keys in fp32, 8 kv heads of 128
 //                 dims, 5.1 TB/s, 2 of 512 dims, 5.6 TB/s (a large copy: 4.6 TB/s).  8-bit pools: the 48 tokens'
-//                 237 MB in 47 to 51 us (4.6 to 5.0 TB/s); one token over 131065 keys, 2 kv heads of 128 dims, capped, 69 MB in 19 us.
+//                 237 MB in 44 us (5.4 TB/s); one token over 131065 keys, 2 kv heads of 128 dims, capped, 69 MB in 20 us.
 //  k_paged_block  longer chunks, and single tokens beside them (item_by_block, item_by_tile).
 //                 Bound by the matrix cores: 4096 rows over 16384 keys, 14B class, bf16 (three
 //                 products a multiplication): 2.7 to 2.9 ms among other calls (2.9 to 3.1 in ten
@@ -1481,7 +1481,8 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
     while (rpb > 1 && 1024 / HD / rpb * 4 < p->most_parts) rpb /= 2;
     const dim3 mg(p->n_merge * a.n_kv, cdiv(p->most, rpb));
     // many parts of few rows: by several blocks a row where these are no more than compute units in all (48
-    // sequences, 14B class, one of 131072 keys and 47 of 3000, int8: 131 us, with every row's so 143).  (The plain calls keep their order of sums, and so their results to the last bit.)
+    // sequences, 14B class, one of 131072 keys and 47 of 3000, int8: 131 us, with every row's so 143).  (The plain calls
+    // keep their order of sums, and so their results to the last bit.)
     constexpr bool COLS = Form<DT>::E8 || CAP;
     if (1024 / HD * 4 >= p->most_parts) {
       hipLaunchKernelGGL((k_paged_merge<HD, 256>), mg, dim3(256), 0, st, a, merge, rpb);
