@@ -331,6 +331,7 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
   // where m is near it, and t then has an error of its own size.  (The lane's smaller scores are off by up to 2^-25 of the
   // cap, what those at half of it are in any case; the smaller the less they weigh beside the one past it.)
   float from[NQ] = {};
+  const int g = (threadIdx.x & 63) >> 4;
   // (both forms for each score of every tile: 4096 rows over 16384 keys, 14B class, i8, 3.5 ms; the near one alone
   // where a tile's scores allow it, 3.2 ms; uncapped 2.5 ms)
   if constexpr (CAP) {
@@ -338,8 +339,18 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         float most = 0.f;
+        if (edge) {  // (of keys that the query attends to)
+          int low, high;
+          span(n, &low, &high);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, s[j >> 2][n][j & 3]);
+          for (int j = 0; j < 8; ++j) {
+            const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
+            most = fmaxf(most, key > high || key < low ? 0.f : s[j >> 2][n][j & 3]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) most = fmaxf(most, s[j >> 2][n][j & 3]);
+        }
         const float h = most * most >= kNear ? a.cap_p[0] : 0.f;
         from[n] = h * a.cap_to;
 #pragma unroll
@@ -352,7 +363,6 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
         for (int j = 0; j < 8; ++j) s[j >> 2][n][j & 3] = cap_near(a, s[j >> 2][n][j & 3], 0.f);
     }
   }
-  const int g = (threadIdx.x & 63) >> 4;
   float t[NQ][8], top = -INFINITY;
 #pragma unroll
   for (int n = 0; n < NQ; ++n)

@@ -371,6 +371,36 @@ def test_attention_cap_far_from_scores(gpu, new, hd, dtype):
                 assert np.all(np.abs(got - want) <= 2 * (2.0 ** -22 + 160 * 2.0 ** -24) * np.abs(v).max())
 
 
+@pytest.mark.parametrize("dtype", ["e4m3", "i8", "f32", "bf16", "f16"])
+def test_attention_cap_of_later_keys(gpu, dtype):
+    """Rows of small scores keep their bits where keys behind them are past the cap."""
+    say(f"attention, later keys past the cap: {dtype}")
+    heads, n = 16, 40
+    st = SetupExt(gpu, [(n, n)], heads, 1, 64, dtype, 16, cap=50.0, seed=25)
+    g = st.slots(0, 0, n)
+    k, v = np.zeros((n, 1, 64)), np.zeros((n, 1, 64))
+    k[:, 0, 0] = 448.0
+    k[0, 0, 0], k[1, 0, 0] = 1.0, -1.0
+    v[:, 0, 0] = 1.0
+    v[1, 0, 0] = -1.0
+    for name, x in (("k", k), ("v", v)):
+        if st.eight:
+            y = st.pool[name].copy()
+            y[g] = x
+            st.fill(name, y)
+        else:
+            st.pool[name][g] = encode(x.astype(np.float32), dtype)
+    st.upload()
+    q = np.zeros((n, heads, 64), np.float32)
+    q[:, :, 0] = 1.7 + 0.137 * np.arange(heads)  # scores 0.2 to 0.5 in size, of later keys 95 to 210
+    got = st.run_attention(q.reshape(n, -1)).reshape(n, heads, 64)[1, :, 0]
+    s = q[1, :, 0].astype(np.float64) / 8
+    want = np.tanh(50 * np.tanh(s / 50))
+    # scores of half a unit in log2, four roundings; their distance to the maximum, one; two powers of 2^-22; the sums
+    # and the division, four: below 2^-24 (4 + 2 + 8 + 4)
+    assert np.all(np.abs(got - want) <= 18 * 2.0 ** -24), np.abs(got - want).max()
+
+
 @pytest.mark.parametrize("dtype,hd,kv,G,rows,cap", [
     ("e4m3", 512, 32, 2, 320, 0.0), ("i8", 128, 64, 1, 1280, 20.0), ("bf16", 512, 32, 2, 290, 20.0), ("e4m3", 64, 64, 2, 641, 5.0)])
 def test_attention_last_turn(gpu, dtype, hd, kv, G, rows, cap):
