@@ -388,8 +388,9 @@ typedef struct {
  * the first id always stays.  The draw is the first id, in order of ids, at which the running weight of
  * what is left passes d_u[row] times the whole (d_u: 0 <= u < 1; anything below counts as 0, NaN too, anything
  * above leaves the last id).  Weights are computed in 64 bits and added as whole multiples of a fixed part of the
- * largest, 2^-49 of it up to 2^14 ids, twice that for each doubling (2^-44 at most at 2^18): a draw does not
- * depend on any order, and an id of less weight is never drawn.  An id
+ * largest, 2^-48 of it or less up to 2^14 ids, twice that for each doubling (2^-44 at 2^18); where top_p cuts without
+ * top_k, as whole multiples of that part of themselves, to 2^-63 of the largest.  So a draw depends neither on any order nor
+ * on the rows beside it, equal ids weigh the same, and an id of less weight than that part is never drawn.  An id
  * of logit -infinity or NaN is never drawn; a row without any other has id -1, probability 0, none kept.
  * d_logits rows of in_stride floats are only read; d_ids [rows]; d_prob (may be NULL): the id's weight by that of
  * what is left; d_kept (may be NULL): how many ids were left.  h_rows is read before the call returns.

@@ -5,6 +5,11 @@
 // (the lower id first among equals), a first part of the row: all logits above a cut and the
 // first few that are equal to it.
 //
+// Where top-p cuts a whole row the same weights are whole numbers of 2^-S of their own octave: a slice's sums, which know
+// nothing of the rest of the row, then are exact too, an octave's sum over all slices fits 64 bits and the row's, of
+// 64 octaves, 128.  (As whole numbers of a slice's part, rounded to the row's, they were off by one or two: of two equal
+// logits top-p 0.5 left both.)
+//
 //  k_rows_scan  a block has a slice of a row: its maximum, and a histogram of counts (top-k) or weights
 //               (top-p) over buckets of its logits
 //  k_rows_pick  finds, from the slices' histograms, the bucket in which the cut lies; the slice once more: the
@@ -25,6 +30,8 @@
 namespace ms {
 namespace {
 
+typedef unsigned __int128 u128;
+
 constexpr float MAX32 = 0x1.fffffep+127f;
 constexpr int kRows = 64;       // rows of a launch: their settings are kernel arguments
 constexpr int kNT = 1024;
@@ -34,14 +41,14 @@ constexpr int kSliceList = 2048;  // of one of its slices
 constexpr int kMostK = 2048;    // the largest top-k by the list
 constexpr int kMostSlices = 64;
 constexpr int kWave = 256;      // candidates that one wave goes through alone
-constexpr int kSliceBits = 49;  // S of a slice of up to 2^14 logits; S of a row is at most that
+constexpr int kMostBits = 49;   // S of up to 2^14 logits
 
 struct RowInfo {
   int state;                // kNone ..
   int ref;                  // weights are 2^(x log2(e) / T - ref)
   float top;                // the largest logit
   float lo, hi;             // the cut lies among the logits lo <= x < hi (the candidates); what lies above stays
-  unsigned long long want;  // top-p: weight still to be reached by the candidates; top-k: ids of the cut's bucket
+  unsigned long long want;  // top-p: weight (of its octave) that the candidates have to reach; top-k: ids of the cut's bucket
 };
 // A row's settings.
 struct RowSet {
@@ -95,6 +102,11 @@ __device__ inline unsigned long long from_below(unsigned long long old, unsigned
   return (unsigned long long)from_below<CTRL, ROWS>((uint32_t)(old >> 32), (uint32_t)(v >> 32)) << 32 |
          from_below<CTRL, ROWS>((uint32_t)old, (uint32_t)v);
 }
+template <int CTRL, int ROWS>
+__device__ inline u128 from_below(u128 old, u128 v) {
+  return (u128)from_below<CTRL, ROWS>((unsigned long long)(old >> 64), (unsigned long long)(v >> 64)) << 64 |
+         from_below<CTRL, ROWS>((unsigned long long)old, (unsigned long long)v);
+}
 // Running sum over a wave's lanes, a lane's own value in it.
 template <class T>
 __device__ inline T scan_wave(T v) {
@@ -108,6 +120,9 @@ __device__ inline T scan_wave(T v) {
 __device__ inline uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
 __device__ inline unsigned long long last_lane(unsigned long long v) {
   return (unsigned long long)last_lane((uint32_t)(v >> 32)) << 32 | last_lane((uint32_t)v);
+}
+__device__ inline u128 last_lane(u128 v) {
+  return (u128)last_lane((unsigned long long)(v >> 64)) << 64 | last_lane((unsigned long long)v);
 }
 template <class T>
 __device__ inline T sum_wave(T v) {
@@ -141,45 +156,71 @@ __device__ const double kExp2[64] = {
     0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
-// 2^(z/64) as a whole number of 2^-bits, bits <= 49: 2^(j/64) from a table, a polynomial of degree 4 over a 64th of an
-// octave (off by 4e-14 of it at most); the sums with large constants round to whole numbers.  *n: z rounded.  (With rint,
-// ldexp and conversions in place of the constants the 12.6 million weights of 48 rows took 20 us more.)
+// 2^((k + r)/64) as a whole number, |r| <= 1/2 or little more: 2^(j/64) from a table, a polynomial of degree 4 over a 64th of
+// an octave (off by 4e-14 of it at most); sums with large constants round to whole numbers.  (With rint, ldexp and
+// conversions in place of the constants the 12.6 million weights of 48 rows took 20 us more.)
 struct Exp2 {
   const double *table;  // LDS, [64]
-  __device__ unsigned long long operator()(double z, int bits, int *n) const {
+  // times 2^e in place of 2^(k/64 rounded down), e <= 49
+  __device__ unsigned long long whole(int k, double r, int e) const {
     constexpr double L = 0.010830424696249145;  // ln(2) / 64
-    z = __builtin_fmax(z, -3840.0);             // (2^-60: none)
-    const double m = z + 0x1.8p52, r = z - (m - 0x1.8p52);
-    const int k = (int)__double_as_longlong(m);
     double p = __builtin_fma(r, L * L * L * L / 24, L * L * L / 6);
     p = __builtin_fma(r, p, L * L / 2);
     p = __builtin_fma(r, p, L);
     p = __builtin_fma(r, p, 1.0);
-    const long long t = __double_as_longlong(table[k & 63]) + ((long long)((k >> 6) + bits) << 52);
-    *n = k;
+    const long long t = __double_as_longlong(table[k & 63]) + ((long long)e << 52);
     return (unsigned long long)__double_as_longlong(__builtin_fma(p, __longlong_as_double(t), 0x1p52)) & 0xFFFFFFFFFFFFFull;
+  }
+  // 2^(z/64) as a whole number of 2^-bits
+  __device__ unsigned long long operator()(double z, int bits) const {
+    z = __builtin_fmax(z, -3840.0);  // (2^-60: none)
+    const double m = z + 0x1.8p52, r = z - (m - 0x1.8p52);
+    const int k = (int)__double_as_longlong(m);
+    return whole(k, r, (k >> 6) + bits);
   }
 };
 __device__ inline void exp2_table(double *t) {
   if (threadIdx.x < 64) t[threadIdx.x] = kExp2[threadIdx.x];
 }
-// A logit's weight by sums: the same instructions in every kernel, which count on the same number.  *n: 64ths of an
-// octave below the reference.
-__device__ inline unsigned long long weight_of(const Exp2 &exp2, float x, double c64, int ref, int bits, int *n) {
-  return exp2(__builtin_fma((double)x, c64, -64.0 * ref), bits, n);
+// By sums a logit's place is x c64, k + r of it in 64ths of an octave, k its nearest whole number: the same whatever the
+// logit is compared with, and so is the bucket of 1/32 of an octave that it lies in, k / 2 rounded down.
+struct Place {
+  int k;
+  double r;
+};
+// (least: logits below it, none of which weighs anything, are taken as that)
+__device__ inline Place place_of(float x, double least, double c64) {
+  const double y = __builtin_fmax((double)x, least), m = __builtin_fma(y, c64, 0x1.8p52);
+  return {(int)__double_as_longlong(m), __builtin_fma(y, c64, -(m - 0x1.8p52))};
 }
-// The reference of a largest logit: a whole octave that rounds above it.  Logits by sums have buckets of 1/32 of an octave,
-// 32 ref - 1 - b for bucket b from the reference down; 2^17 octaves are the most.
+// The reference of a largest logit: the end of its octave; a row's largest is at most 2^17 octaves from 0.
 __device__ inline bool in_range(float top, double c64) { return fabs((double)top * c64) < 0x1p23; }
-__device__ inline int ref_of(float top, double c64) { return ((int)rint((double)top * c64) >> 6) + 1; }
+__device__ inline int ref_of(float top, double c64) { return (place_of(top, -INFINITY, c64).k >> 6) + 1; }
+// 66 octaves below it.
+__device__ inline double least_of(int ref, const RowSet &set) { return (64.0 * ref - 4224.0) * set.by; }
+// The weight by its own octave, and in the row's unit.
+__device__ inline unsigned long long weight_of_octave(const Exp2 &exp2, Place p, int bits) { return exp2.whole(p.k, p.r, bits); }
+__device__ inline unsigned long long weight_of(const Exp2 &exp2, Place p, int ref, int bits) {
+  return exp2.whole(p.k, p.r, (p.k >> 6) - ref + bits);
+}
 // By counts: a bucket is the exponent and eight bits of the mantissa, whatever the logits' size.
 __device__ inline int bucket_of(float x) { return (int)(key_of(x) >> 15); }
-// The least number whose product with c64 is at least z.  (by: 1 / c64, by which the first guess is off by one place at most)
-__device__ inline float least_float(double z, double c64, double by) {
-  const float x = fmaxf((float)(z * by), -MAX32);
-  auto ok = [&](float y) { return (double)y * c64 >= z; };
-  const float below = of_key(key_of(x) - 1);
+// The least number that is `ok`, as all larger ones are; z: its place, to a few roundings.  (by: 1 / c64, by which the first
+// guess is off by one number at most)
+template <class F>
+__device__ inline float least_float(double z, double by, const F &ok) {
+  const float x = fmaxf((float)(z * by), -MAX32), below = of_key(key_of(x) - 1);
   return !ok(x) ? of_key(key_of(x) + 1) : ok(below) ? below : x;
+}
+// The first logit of bucket b.
+__device__ inline float least_of_bucket(int b, const RowSet &set) {
+  return least_float(2.0 * b - 0.5, set.by, [&](float y) { return place_of(y, -INFINITY, set.c64).k >= 2 * b; });
+}
+// By sums min_p leaves the logits from this one on.
+__device__ inline float least_of_min_p(float top, const RowSet &set) {
+  if (!(set.min_p > 0.f)) return -MAX32;
+  const double z = __builtin_fma((double)top, set.c64, set.min64);
+  return fminf(top, least_float(z, set.by, [&](float y) { return (double)y * set.c64 >= z; }));
 }
 
 template <int PER, bool VEC>
@@ -215,10 +256,31 @@ __device__ inline unsigned long long share_of(float p, unsigned long long total)
   const unsigned long long t = (unsigned long long)ceil((double)p * (double)total);
   return t ? t : 1;
 }
+// The least whole number of p of the total, p < 1, rounded nowhere: a number of equal weights may be just that.  (Below 2^-32:
+// 1, which the largest weight reaches as well.)
+__device__ inline u128 share_of(float p, u128 total) {
+  if (p < 0x1p-32f) return 1;
+  const uint32_t b = __float_as_uint(p), s = 150 - (b >> 23), f = (b & 0x7FFFFFu) | 0x800000u;  // p = f 2^-s, 24 <= s <= 55
+  const u128 low = (u128)(unsigned long long)total * f, high = (total >> 64) * f + (low >> 64);
+  const unsigned long long lo = (unsigned long long)low;
+  return (high << (64 - s)) + (lo >> s) + ((lo & ((1ull << s) - 1)) != 0);
+}
+// By one wave, lane g holding the weight of the row's octave g (from the top, by that octave): the octave in which the running
+// weight reaches p of the whole, and of that octave's what it has to reach.
+__device__ inline int octave_of_share(float p, unsigned long long weight, unsigned long long *want) {
+  const int lane = threadIdx.x & 63;
+  const u128 w = (u128)weight << (63 - lane), upto = scan_wave(w), goal = share_of(p, last_lane(upto));
+  const unsigned long long hit = __ballot(upto >= goal);
+  const int g = __ffsll(hit) - 1;  // (the last octave's reaches the whole)
+  const u128 rest = goal - (upto - w);
+  const unsigned long long mine = (unsigned long long)((rest + (((u128)1 << (63 - lane)) - 1)) >> (63 - lane));
+  *want = __shfl(mine, g, 64);
+  return g;
+}
 
 struct CutLds {
   unsigned long long part[kNT / 64][64];
-  unsigned long long goal, before;
+  unsigned long long goal;
   int group;
   RowInfo info;
 };
@@ -239,18 +301,9 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
   const bool all = SUMS && set.top_p >= 1.f;
   const int group0 = in.state == kSum || in.state == kBest ? group_of<SUMS>(top, set.c64) : 0;
   if (in.state == kSum) in.ref = group0;
-  // the bounds that start z64 = lo and hi, and min_p's (the largest logit stays), each by a lane
-  auto bounds = [&](double lo, double hi) {
-    const bool least = set.min_p > 0.f;
-    const double z = lane == 0 ? lo : lane == 1 ? hi : __builtin_fma((double)top, set.c64, set.min64);
-    const float x = least_float(z, set.c64, set.by);
-    const float m = least ? fminf(top, __shfl(x, 2, 64)) : -MAX32;
-    in.lo = fmaxf(__shfl(x, 0, 64), m);
-    in.hi = fmaxf(__shfl(x, 1, 64), m);
-  };
   if (in.state == kNone || in.state == kSlow || all) {
     if (wave == 0) {
-      if (SUMS && in.state == kSum && set.min_p > 0.f) bounds(-INFINITY, -INFINITY);
+      if (in.state == kSum) in.lo = in.hi = least_of_min_p(top, set);
       if (lane == 0) lds.info = in;
     }
     __syncthreads();
@@ -259,12 +312,6 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
   // groups that a slice's buckets begin below the row's
   const bool has = mine > -INFINITY && (!SUMS || in_range(mine, set.c64));
   const int down = has ? group0 - group_of<SUMS>(mine, set.c64) : kBins;
-  // a slice's weights in the row's unit, rounded
-  auto in_unit = [&](unsigned long long w, int down) {
-    if constexpr (!SUMS) return w;
-    const int sh = min(kSliceBits - a.bits + down, 63);  // (2^63 at most: that and more leave 0 or 1)
-    return (w >> sh) + (sh ? w >> (sh - 1) & 1 : 0);
-  };
   unsigned long long h[Q], s = 0;
   int d[Q];
 #pragma unroll
@@ -277,7 +324,7 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
 #pragma unroll
   for (int e = 0; e < Q; ++e) {
     if (W * e >= a.slices) break;
-    s += wave + W * e < a.slices && lane >= d[e] ? in_unit(h[e], d[e]) : 0;
+    s += wave + W * e < a.slices && lane >= d[e] ? h[e] : 0;
   }
   lds.part[wave][lane] = s;
   __syncthreads();
@@ -285,21 +332,23 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
     s = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) s += lds.part[w][lane];
-    const unsigned long long upto = scan_wave(s);
-    unsigned long long goal = (unsigned long long)set.k;
-    if (SUMS) goal = share_of(set.top_p, last_lane(upto));
-    const unsigned long long hit = __ballot(upto >= goal);
-    const int group = hit ? __ffsll(hit) - 1 : -1;
-    const unsigned long long before = __shfl(upto - s, max(group, 0), 64);
+    unsigned long long goal;
+    int group;
+    if constexpr (SUMS) {
+      group = octave_of_share(set.top_p, s, &goal);
+    } else {
+      const unsigned long long upto = scan_wave(s), hit = __ballot(upto >= (unsigned long long)set.k);
+      group = hit ? __ffsll(hit) - 1 : -1;
+      goal = set.k - __shfl(upto - s, max(group, 0), 64);
+    }
     if (lane == 0) {
       // (top-k, whose buckets end eight octaves below the largest logit: all that can be drawn is in the list, if it holds
       // that, and nothing is `want`ed of a bucket)
-      if (group < 0 && (SUMS || real > kList)) in.state = kSlow;
+      if (group < 0 && real > kList) in.state = kSlow;
       if (!SUMS) in.hi = INFINITY;
       lds.info = in;
       lds.group = group;
       lds.goal = goal;
-      lds.before = before;
     }
   }
   __syncthreads();
@@ -322,7 +371,7 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
 #pragma unroll
   for (int e = 0; e < Q / 2; ++e) {
     if (2 * W * e >= a.slices) break;
-    s += 2 * (wave + W * e) + (lane >> 5) < a.slices && group >= d[e] ? in_unit(h[e], d[e]) : 0;
+    s += 2 * (wave + W * e) + (lane >> 5) < a.slices && group >= d[e] ? h[e] : 0;
   }
   lds.part[wave][lane] = s;
   __syncthreads();
@@ -331,18 +380,19 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
 #pragma unroll
     for (int w = 0; w < W; ++w) s += lds.part[w][lane & 31] + lds.part[w][32 + (lane & 31)];
     if (lane >= 32) s = 0;
-    const unsigned long long goal = lds.goal, upto = lds.before + scan_wave(s), hit = __ballot(upto >= goal && lane < 32);
-    // (buckets are rounded one by one: the group's last, should they stay below the goal)
-    const int bin = hit ? __ffsll(hit) - 1 : 31;
-    const unsigned long long under = __shfl(upto - s, bin, 64);
+    const unsigned long long goal = lds.goal, upto = scan_wave(s), hit = __ballot(upto >= goal && lane < 32);
+    const int bin = __ffsll(hit) - 1;
+    in.want = goal - __shfl(upto - s, bin, 64);
     const int bucket = 32 * (group0 - group) - 1 - bin;
     if constexpr (SUMS) {
-      bounds(2.0 * bucket - 0.5, 2.0 * bucket + 1.5);
+      // (the first lane's and the others' bound)
+      const float x = least_of_bucket(bucket + (lane > 0), set), least = least_of_min_p(top, set);
+      in.lo = fmaxf(__shfl(x, 0, 64), least);
+      in.hi = fmaxf(__shfl(x, 1, 64), least);
     } else {
       in.lo = of_key((uint32_t)bucket << 15);
       in.hi = INFINITY;
     }
-    in.want = goal > under ? goal - under : 1;
     if (lane == 0) lds.info = in;
   }
   __syncthreads();
@@ -394,12 +444,12 @@ __global__ __launch_bounds__(kNT) void k_rows_scan(SampleRowsArgs a) {
     if (sums) {
       const Exp2 exp2{table};
       const int ref = ref_of(top, set.c64);
+      const double least = least_of(ref, set);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        int n;
-        const unsigned long long w = weight_of(exp2, v[j], set.c64, ref, kSliceBits, &n);
-        // (n is below 0, and above -64 50 where there is any weight)
-        if (w) atomicAdd(&hist[max(-1 - (n >> 1), 0) & (kBins - 1)], w);
+        const Place p = place_of(v[j], least, set.c64);
+        const uint32_t d = 32 * ref - 1 - (p.k >> 1);
+        if (d < kBins) atomicAdd(&hist[d], weight_of_octave(exp2, p, a.bits));
       }
     } else {
       const int base = bucket_of(top) | 31;
@@ -449,6 +499,7 @@ __global__ __launch_bounds__(kNT) void k_rows_pick(SampleRowsArgs a) {
   if (blockIdx.x == 0 && tid == 0) a.info[row] = in;
   if (in.state == kNone || in.state == kSlow) return;
   const Exp2 exp2{table};
+  const double least = least_of(in.ref, set);
   unsigned long long sum = 0;
   uint32_t num = 0, listed = 0;  // bit j: logit j goes to the list
   float v[PER];
@@ -457,9 +508,8 @@ __global__ __launch_bounds__(kNT) void k_rows_pick(SampleRowsArgs a) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       listed |= (uint32_t)(v[j] >= in.lo && v[j] < in.hi) << j;
-      int n;
       if (v[j] >= in.hi) {
-        sum += weight_of(exp2, v[j], set.c64, in.ref, a.bits, &n);
+        sum += weight_of(exp2, place_of(v[j], least, set.c64), in.ref, a.bits);
         ++num;
       }
     }
@@ -665,17 +715,19 @@ __device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, 
   top = (uint32_t)lds.before;
   least = ~(uint32_t)lds.cut;
   const double vmax = of_key(top);
+  // (whether the lists hold a row depends on how it was cut into slices: what is done to it here does not)
+  const bool sums = set.k == 0 && in_range((float)vmax, set.c64);
+  const int ref = sums ? ref_of((float)vmax, set.c64) : 0;
+  const double from = least_of(ref, set);
   auto place = [&](float v) { return v == (float)vmax ? 0.0 : ((double)v - vmax) * set.c64; };
-  auto weight = [&](float v) {
-    int k;
-    return exp2(place(v), a.bits, &k);
-  };
+  auto weight = [&](float v) { return sums ? weight_of(exp2, place_of(v, from, set.c64), ref, a.bits) : exp2(place(v), a.bits); };
 
-  // Where the count (or weight) from the top reaches `want`, of what lies at or above `floor` (of those equal
+  // Where the count (or weight) from the top, `hi`, reaches `want`, of what lies at or above `floor` (of those equal
   // to it, floor_n): the key; what lies above it.
+  enum By { kCount, kWeight, kOctave };
   unsigned long long above;
-  auto find = [&](bool by_weight, unsigned long long want, uint32_t floor, uint32_t floor_n) {
-    uint32_t hi = top, lo = floor;
+  auto find = [&](By by, unsigned long long want, uint32_t hi, uint32_t floor, uint32_t floor_n) {
+    uint32_t lo = floor;
     above = 0;
     for (;;) {
       const int shift = hi - lo < kBins ? 0 : 21 - __clz(hi - lo);
@@ -684,9 +736,11 @@ __device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, 
       __syncthreads();
       each(tid, n, kNT, [&](float v, int) {
         const uint32_t k = key_of(v);
-        if (k >= lo && k <= hi && (!by_weight || k > floor)) atomicAdd(&lds.bin[(hi - k) >> shift], by_weight ? weight(v) : 1ull);
+        if (k >= lo && k <= hi && (by != kWeight || k > floor))
+          atomicAdd(&lds.bin[(hi - k) >> shift],
+                    by == kCount ? 1ull : by == kWeight ? weight(v) : weight_of_octave(exp2, place_of(v, from, set.c64), a.bits));
       });
-      if (by_weight && tid == 0 && lo == floor) atomicAdd(&lds.bin[(hi - floor) >> shift], floor_n * weight(of_key(floor)));
+      if (by == kWeight && tid == 0 && lo == floor) atomicAdd(&lds.bin[(hi - floor) >> shift], floor_n * weight(of_key(floor)));
       __syncthreads();
       find_bin(lds, above, want);
       above = lds.before;
@@ -703,10 +757,40 @@ __device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, 
 
   uint32_t key = least, eq = 0xFFFFFFFFu;  // of the logits equal to the cut, the first eq are left
   if (set.k > 0 && (uint32_t)set.k < real) {
-    key = find(false, set.k, least, 0);
+    key = find(kCount, set.k, top, least, 0);
     eq = (uint32_t)(set.k - above);
   }
-  if (set.temperature != 0.f && set.top_p < 1.f) {
+  if (sums && set.top_p < 1.f) {
+    // the octave, its bucket and the logit in which the cut lies
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kNT) lds.bin[i] = 0;
+    __syncthreads();
+    each(tid, n, kNT, [&](float v, int) {
+      const Place p = place_of(v > -INFINITY ? v : -INFINITY, from, set.c64);
+      const uint32_t d = 32 * ref - 1 - (p.k >> 1);
+      if (d < kBins) atomicAdd(&lds.bin[d], weight_of_octave(exp2, p, a.bits));
+    });
+    __syncthreads();
+    if (wave == 0) {
+      unsigned long long w = 0, want;
+      for (int i = 0; i < 32; ++i) w += lds.bin[32 * lane + i];
+      const int g = octave_of_share(set.top_p, w, &want);
+      const unsigned long long mine = lane < 32 ? lds.bin[32 * g + lane] : 0, upto = scan_wave(mine);
+      const int b = __ffsll((unsigned long long)__ballot(upto >= want)) - 1;
+      want -= __shfl(upto - mine, b, 64);
+      if (lane == 0) {
+        lds.found = 32 * g + b;
+        lds.cut = want;
+      }
+    }
+    __syncthreads();
+    const int bucket = 32 * ref - 1 - lds.found;
+    const unsigned long long want = lds.cut;
+    key = find(kOctave, want, min(top, key_of(least_of_bucket(bucket + 1, set)) - 1),
+               max(least, key_of(least_of_bucket(bucket, set))), 0);
+    const unsigned long long w = weight_of_octave(exp2, place_of(of_key(key), from, set.c64), a.bits);
+    eq = (uint32_t)min((want - above + w - 1) / w, 0xFFFFFFFFull);
+  } else if (set.temperature != 0.f && set.top_p < 1.f) {
     unsigned long long sum = 0;
     each(tid, n, kNT, [&](float v, int) {
       if (key_of(v) > key) sum += weight(v);
@@ -715,7 +799,7 @@ __device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, 
     sum = over_block(sum) + floor_n * weight(of_key(key));
     const unsigned long long want = share_of(set.top_p, sum);
     const uint32_t floor = key;
-    key = find(true, want, floor, floor_n);
+    key = find(kWeight, want, top, floor, floor_n);
     const unsigned long long w = weight(of_key(key)), take = (want - above + w - 1) / w;
     eq = (uint32_t)min(take, (unsigned long long)(key == floor ? floor_n : 0xFFFFFFFFu));
   }
@@ -734,9 +818,11 @@ __device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, 
     __syncthreads();
     last_eq = (uint32_t)lds.found;
   }
+  const float min_x = sums ? least_of_min_p((float)vmax, set) : 0.f;
   auto left = [&](float v, int i) {
     const uint32_t k = key_of(v);
-    return k > key || (k == key && (uint32_t)i <= last_eq) ? k == top || place(v) >= set.min64 : false;
+    if (k < key || (k == key && (uint32_t)i > last_eq)) return false;
+    return sums ? v >= min_x : k == top || place(v) >= set.min64;
   };
   // ---- the draw: the wave, then the sixteenth of its part, and so on, in which the running weight passes the target
   unsigned long long total = 0, target = 0, before = 0;
@@ -791,8 +877,7 @@ __device__ inline void draw_few(const SampleRowsArgs &a, const RowSet &set, int 
     const float v = logit_of(x);
     id[e] = id_of(x);
     const double z = v == top ? 0.0 : ((double)v - (double)top) * set.c64;
-    int n;
-    w[e] = in ? exp2(z, a.bits, &n) : 0;
+    w[e] = in ? exp2(z, a.bits) : 0;
     over += __popcll(__ballot(in && (v == top || z >= set.min64)));
     sum += w[e];
   }
@@ -911,8 +996,7 @@ __device__ inline void draw_many(const SampleRowsArgs &a, const RowSet &set, int
   for (int e = 0; e < E; ++e) {
     if (kNT * e >= n_list) break;
     const double z = logit_of(x[e]) == in.top ? 0.0 : ((double)logit_of(x[e]) - (double)in.top) * set.c64;
-    int n;
-    w[e] = x[e] ? exp2(z, a.bits, &n) : 0;
+    w[e] = x[e] ? exp2(z, a.bits) : 0;
     if (cut_p && w[e]) atomicAdd(&lds.bin[bin_of(x[e])], w[e]);
   }
   if (cut_p) {
@@ -931,8 +1015,7 @@ __device__ inline void draw_many(const SampleRowsArgs &a, const RowSet &set, int
       for (int i0 = 0; i0 < num && before < goal; i0 += 64) {
         const unsigned long long y = i0 + lane < num ? list[i0 + lane] : 0;
         const double z = logit_of(y) == in.top ? 0.0 : ((double)logit_of(y) - (double)in.top) * set.c64;
-        int n;
-        const unsigned long long v = y ? exp2(z, a.bits, &n) : 0, upto = before + scan_wave(v);
+        const unsigned long long v = y ? exp2(z, a.bits) : 0, upto = before + scan_wave(v);
         const unsigned long long m = __ballot(y && upto - v < goal);
         if (m) cut = __shfl(y, 63 - __clzll(m), 64);
         before = last_lane(upto);
@@ -972,8 +1055,7 @@ __device__ inline void draw_many(const SampleRowsArgs &a, const RowSet &set, int
     const unsigned long long y = i0 + lane < num ? list[i0 + lane] : 0;
     const float v = of_key((uint32_t)y);
     const double z = v == in.top ? 0.0 : ((double)v - (double)in.top) * set.c64;
-    int n;
-    const unsigned long long w = y ? exp2(z, a.bits, &n) : 0, upto = before + scan_wave(w);
+    const unsigned long long w = y ? exp2(z, a.bits) : 0, upto = before + scan_wave(w);
     if (upto > target && upto - w <= target)
       write_row(a, row, (int)(0xFFFFFFFFu - (uint32_t)(y >> 32)), (float)((double)w / (double)total), lds.kept);
     before = last_lane(upto);
@@ -1047,16 +1129,17 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   }
   if (wave != 0) return;
   if (n_list <= kWave) sort_by_wave(list, (int)n_list);
+  const double least = least_of(in.ref, set);
   unsigned long long before = 0, cut = ~0ull;
   uint32_t taken = 0;
   for (int i0 = 0; i0 < (int)n_list && before < in.want; i0 += 64) {
     const int i = i0 + lane;
     const unsigned long long x = i < (int)n_list ? list[i] : 0;
-    int n;
-    const unsigned long long w = i < (int)n_list ? weight_of(exp2, logit_of(x), set.c64, in.ref, a.bits, &n) : 0;
+    const Place p = place_of(logit_of(x), least, set.c64);
+    const unsigned long long w = i < (int)n_list ? weight_of_octave(exp2, p, a.bits) : 0;
     const unsigned long long upto = before + scan_wave(w);
     const bool take = i < (int)n_list && upto - w < in.want;
-    if (take) atomicAdd(&chunk[id_of(x) / chunk_len], w);
+    if (take) atomicAdd(&chunk[id_of(x) / chunk_len], weight_of(exp2, p, in.ref, a.bits));
     const unsigned long long m = __ballot(take);
     if (m) cut = __shfl(x, 63 - __clzll(m), 64);
     taken += __popcll(m);
@@ -1074,11 +1157,10 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   unsigned long long w[PER], sum = 0;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
-    int n;
     w[e] = 0;
     if (v[e] >= in.hi ||
         (v[e] >= in.lo && ((unsigned long long)key_of(v[e]) << 32 | (0xFFFFFFFFu - (uint32_t)(id0 + e))) >= cut))
-      w[e] = weight_of(exp2, v[e], set.c64, in.ref, a.bits, &n);
+      w[e] = weight_of(exp2, place_of(v[e], least, set.c64), in.ref, a.bits);
     sum += w[e];
   }
   unsigned long long upto = before + scan_wave(sum) - sum;
@@ -1140,7 +1222,7 @@ extern "C" int ms_sample_rows(const float *d_logits, size_t in_stride, int rows,
   SampleRowsArgs a{};
   a.ld = in_stride;
   a.n = vocab;
-  a.bits = kSliceBits;
+  a.bits = kMostBits;
   while (a.bits < 63 && (1 << (63 - a.bits)) < vocab) --a.bits;
   // Slices of 16384 logits where these are as many as compute units, else of 4096.
   const int m0 = rows < kRows ? rows : kRows;
