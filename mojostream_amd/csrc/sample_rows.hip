@@ -193,8 +193,10 @@ __device__ inline Place place_of(float x, double least, double c64) {
   const double y = __builtin_fmax((double)x, least), m = __builtin_fma(y, c64, 0x1.8p52);
   return {(int)__double_as_longlong(m), __builtin_fma(y, c64, -(m - 0x1.8p52))};
 }
-// The reference of a largest logit: the end of its octave; a row's largest is at most 2^17 octaves from 0.
+// The reference of a largest logit: the end of its octave; a row's largest is at most 2^17 octaves from 0.  (A slice's at most
+// 2^18: of a row in the range the slices past that weigh nothing, those between do.)
 __device__ inline bool in_range(float top, double c64) { return fabs((double)top * c64) < 0x1p23; }
+__device__ inline bool slice_in_range(float top, double c64) { return fabs((double)top * c64) < 0x1p24; }
 __device__ inline int ref_of(float top, double c64) { return (place_of(top, -INFINITY, c64).k >> 6) + 1; }
 // 66 octaves below it.
 __device__ inline double least_of(int ref, const RowSet &set) { return (64.0 * ref - 4224.0) * set.by; }
@@ -310,7 +312,7 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
     return;
   }
   // groups that a slice's buckets begin below the row's
-  const bool has = mine > -INFINITY && (!SUMS || in_range(mine, set.c64));
+  const bool has = mine > -INFINITY && (!SUMS || slice_in_range(mine, set.c64));
   const int down = has ? group0 - group_of<SUMS>(mine, set.c64) : kBins;
   unsigned long long h[Q], s = 0;
   int d[Q];
@@ -440,7 +442,7 @@ __global__ __launch_bounds__(kNT) void k_rows_scan(SampleRowsArgs a) {
     a.top[at] = top;
     a.real[at] = real;
   }
-  if (bins && top > -INFINITY && top < INFINITY && (!sums || in_range(top, set.c64))) {
+  if (bins && top > -INFINITY && top < INFINITY && (!sums || slice_in_range(top, set.c64))) {
     if (sums) {
       const Exp2 exp2{table};
       const int ref = ref_of(top, set.c64);

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from tests.test_gpu_sample_rows import SETTINGS, draw, logits, say
+from tests.test_gpu_sample_rows import SETTINGS, check, draw, logits, say
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,19 @@ def test_alone_and_among_others(gpu, vocab):
     for r in range(0, R, 1 if vocab < 10000 else 4):
         one = draw(ms, x[r:r + 1], rows[r:r + 1], u[r:r + 1])
         assert all(np.array_equal(a.view(np.int32)[:1], b.view(np.int32)[r:r + 1]) for a, b in zip(one, many)), (r, settings[r])
+
+
+@pytest.mark.parametrize("size", [90850.0, -90850.0, 1453635.0 / 16, -1453635.0 / 16, 2e5, -2e5])
+def test_logits_far_from_zero(gpu, size):
+    """Rows some of whose slices lie past 2^17 octaves from 0 and some do not: these weigh as much."""
+    say(f"sample_rows: logits about {size}")
+    rng = np.random.default_rng(1)
+    V = 40000
+    settings = [dict(top_p=0.5), dict(top_p=0.9, min_p=0.01), dict(), dict(top_p=0.97), dict(top_k=300, top_p=0.6)] * 3
+    x = np.full((len(settings), V), -np.inf, np.float32)
+    for r in range(len(settings)):
+        x[r, rng.choice(np.arange(20000, 36000), 1000, replace=False)] = size - 3 - rng.integers(0, 3, 1000) * (r % 3)
+        x[r, rng.integers(0, 8000)] = size
+        if size == 2e5:
+            x[r, 38000:38100] = size - 0.5
+    check(gpu, x, settings, rng.random(len(settings)).astype(np.float32))
