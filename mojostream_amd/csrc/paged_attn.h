@@ -305,8 +305,8 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
 // as 0 or NaN.)
 // span(n, &low, &high): the keys that the lane's query of query tile n attends to.
 // ks, vs: an 8-bit pool's scales of keys 4 g .. 4 g + 3 of both half tiles; vtop: the power of two that the values' scales
-// are taken in, above all that the query has attended to.  CAP: the scores are capped.  l_far: 8-bit pools, the
-// sums of the tiles but for the last sixteen (fold).
+// are taken in, above all that the query has attended to.  CAP: the scores are capped.  l_far: 8-bit pools and
+// capped scores, the sums of the tiles but for the last sixteen (fold).
 template <int DT, bool CAP, int NQ, int ND, class Span>
 __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2][NQ], int kb, bool edge,
                                               const float (&scale)[NQ], const f4 (&ks)[2], const f4 (&vs)[2],
@@ -397,7 +397,7 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
       const float mn = fmaxf(m[n], max_groups(mx)), al = __builtin_amdgcn_exp2f(m[n] - mn);
       m[n] = mn;
       l[n] *= al;
-      if constexpr (E8) l_far[n] *= al;
+      if constexpr (E8 || CAP) l_far[n] *= al;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[n][d] *= al;
 #pragma unroll
@@ -444,10 +444,12 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
 }
 
 // Every sixteenth of a wave's tiles.  One key may weigh as much as all others: added one after the other to a sum of its
-// size the tiles lost up to half of its last place each (16,000 rows over 65,536 keys: 2.8e-6 of the result, so 0.7e-6).
-template <int DT, int NQ>
+// size the tiles lost up to half of its last place each (16,000 rows over 65,536 keys: 2.8e-6 of the result, so 0.7e-6; where
+// all keys but the first are alike 8e-5, so below 1e-5).  (The plain calls add them up as they come, and keep their results to
+// the last bit.)
+template <int DT, bool CAP, int NQ>
 __device__ __forceinline__ void fold(int nth, float (&l)[NQ], float (&l_far)[NQ]) {
-  if (!Form<DT>::E8 || (nth & 15) != 0) return;
+  if (!(Form<DT>::E8 || CAP) || (nth & 15) != 0) return;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     l_far[n] += l[n];
@@ -678,7 +680,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
     const int tile = step * NG + grp, kb = it.k0 + tile * kTile;
     const bool work = SP == 1 || tile < n_tiles, more = tile + NG < n_tiles;
     if (SP == 1 && tile >= n_tiles) break;
-    fold<DT, NQ>(step, l, l_far);
+    fold<DT, CAP, NQ>(step, l, l_far);
     f4 s[2][NQ] = {}, ks8[2] = {}, vs8[2] = {};
     if (work) {
       if (!AHEAD) {
@@ -797,7 +799,7 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   int bad = 0;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    l[n] = sum_groups(E8 ? l[n] + l_far[n] : l[n]);
+    l[n] = sum_groups(E8 || CAP ? l[n] + l_far[n] : l[n]);
     bad |= !(fabsf(l[n]) < INFINITY);
     if constexpr (E8)
 #pragma unroll
@@ -1045,7 +1047,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   for (int tile = 0; tile < n_tiles; ++tile) {
     const int kb = it.k0 + tile * kTile;
     if (B::ONE && tile) __syncthreads();
-    fold<DT, NQ>(tile, l, l_far);
+    fold<DT, CAP, NQ>(tile, l, l_far);
 #pragma unroll
     for (int u = 0; u < UK; ++u) {
       const int key = (tid + 64 * W * u) / D8, d8 = tid % D8;
@@ -1215,7 +1217,7 @@ __device__ __forceinline__ void item_by_block(const PagedAttnArgs &a, const Page
   int bad = 0;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    l[n] = sum_groups(E8 ? l[n] + l_far[n] : l[n]);
+    l[n] = sum_groups(E8 || CAP ? l[n] + l_far[n] : l[n]);
     bad |= !(fabsf(l[n]) < INFINITY);
     if constexpr (E8)
 #pragma unroll
