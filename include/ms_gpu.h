@@ -332,7 +332,7 @@ int ms_paged_append_ext(const ms_paged_layer_ext *layer, const ms_paged_batch *b
                         const float *d_sin, int n_pos);
 /* ms_paged_attention over any of the pools, with capped scores or not.  Over 8-bit pools the products take
  * the codes with all their bits, and 22 bits of q times the scores' scale (of these nothing below 2^-32 of a row's largest) and
- * of the probabilities times the values' scales (nothing below 2^-32 of the largest scale that the row attends to).  A cap holds for infinite scores too.
+ * of the probabilities times the values' scales (nothing below 2^-31 of the row's largest such product).  A cap holds for infinite scores too.
  * A row's q is brought to about 2^15 by a power of two before it meets the keys: 8-bit keys past 2^100 in size may
  * overflow. */
 int ms_paged_attention_ext(const ms_paged_layer_ext *layer, ms_paged_batch *b, const float *d_q,

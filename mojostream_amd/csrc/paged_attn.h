@@ -97,9 +97,9 @@ constexpr float kLag = 8.0f;
 //   fp16  q and p in two fp16 parts (22 bits): q scaled by a power of two to below 2^15, p by
 //         2^kLift, so that what falls below fp16's smallest step is below 2^-32 of the largest
 //   8-bit the codes, which fp16 holds exactly, and two fp16 parts of q and of p times the values'
-//         scales, in units of the smallest power of two above the scales that the row has attended to
-//         (a scale's head has a code of full size, so that what is lost is below 2^-32 of that too).  The keys' scales
-//         multiply the scores.  (Three bf16 parts of p times the scales as they are: the chunk of 4096 rows over 16384
+//         scales, in 2^-7 of a power of two that is at most twice the largest of these products so far
+//         (a scale's head has a code of full size, so that what is lost is below 2^-31 of that too; a large scale of a key
+//         that weighs nothing takes no bits from the others).  The keys' scales multiply the scores.  (Three bf16 parts of p times the scales as they are: the chunk of 4096 rows over 16384
 //         keys 2.60 ms, so 2.53, before its last spans were cut and its keys loaded earlier)
 template <int DT>
 struct Form {
@@ -110,6 +110,7 @@ struct Form {
   static constexpr int QP = F16 ? 2 : 3, KP = DT == MS_KV_F32 ? 3 : 1;
 };
 constexpr float kLift = 7.0f;
+constexpr float kRoom = 0x1p8f;  // 2^(7 + 8) is below fp16's largest
 
 template <bool F16>
 __device__ inline uint32_t pack2(float a, float b) {
@@ -304,8 +305,8 @@ __device__ __forceinline__ void item_by_key(const PagedAttnArgs &a, const PagedI
 // product in m and not in t it was off by up to half of m's last place: from 2^29 on rows came out
 // as 0 or NaN.)
 // span(n, &low, &high): the keys that the lane's query of query tile n attends to.
-// ks, vs: an 8-bit pool's scales of keys 4 g .. 4 g + 3 of both half tiles; vtop: the power of two that the values' scales
-// are taken in, above all that the query has attended to.  CAP: the scores are capped.  l_far: 8-bit pools and
+// ks, vs: an 8-bit pool's scales of keys 4 g .. 4 g + 3 of both half tiles; vtop: the power of two that the query's probabilities
+// times these are taken in; none is above kRoom of it.  CAP: the scores are capped.  l_far: 8-bit pools and
 // capped scores, the sums of the tiles but for the last sixteen (fold).
 template <int DT, bool CAP, int NQ, int ND, class Span>
 __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2][NQ], int kb, bool edge,
@@ -398,23 +399,39 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
       m[n] = mn;
       l[n] *= al;
       if constexpr (E8 || CAP) l_far[n] *= al;
+      float by = al;
+      if constexpr (E8) {  // (vtop falls with the products: what is left of al is 1 to 2)
+        const float now = vtop[n] * al;
+        const uint32_t u = __float_as_uint(now);
+        by = now < 0x1p-119f ? now * 0x1p119f : __uint_as_float((u & 0x7FFFFFu) | 0x3F800000u);
+        vtop[n] = fmaxf(0x1p-119f, __uint_as_float(u & 0x7F800000u));
+      }
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[n][d] *= al;
+      for (int d = 0; d < ND; ++d) o[n][d] *= by;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (t[n][j] != -INFINITY) t[n][j] = __builtin_fmaf(s[j >> 2][n][j & 3], sc[n], CAP ? from[n] - mn : -mn);
     }
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    float *p = t[n];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(Form<DT>::LIFT ? p[j] + kLift : p[j]);
+    l[n] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    if constexpr (E8)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] *= vs[j >> 2][j & 3];
   }
   if constexpr (E8) {
     float big[NQ];
     bool more = false;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      big[n] = 0.f;
+      big[n] = 0.f;  // (a key that is masked: 0, or NaN, which is no maximum)
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        big[n] = fmaxf(big[n], edge && t[n][j] == -INFINITY ? 0.f : vs[j >> 2][j & 3]);
-      more |= big[n] > vtop[n];
+      for (int j = 0; j < 8; ++j) big[n] = fmaxf(big[n], t[n][j]);
+      more |= big[n] > kRoom * vtop[n];
     }
     if (__any(more))
 #pragma unroll
@@ -425,22 +442,18 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[n][d] *= f;
       }
-  }
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    float *p = t[n];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(Form<DT>::LIFT ? p[j] + kLift : p[j]);
-    l[n] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-    if constexpr (E8) {
+    for (int n = 0; n < NQ; ++n) {
       const float by = __uint_as_float(((254u + (int)kLift) << 23) - __float_as_uint(vtop[n]));  // 2^kLift / vtop
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] *= vs[j >> 2][j & 3] * by;
+      for (int j = 0; j < 8; ++j) t[n][j] *= by;
     }
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      split2<F16, Form<DT>::QP>(p[2 * j], p[2 * j + 1], &pf[n][0][j], 4);
-  }
+      split2<F16, Form<DT>::QP>(t[n][2 * j], t[n][2 * j + 1], &pf[n][0][j], 4);
 }
 
 // Every sixteenth of a wave's tiles.  One key may weigh as much as all others: added one after the other to a sum of its

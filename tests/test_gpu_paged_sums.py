@@ -1,8 +1,8 @@
-"""Attention's sums over the pages where one key outweighs the others."""
+"""Attention's sums over the pages where one key outweighs the others: in the probabilities, or in its values' scale."""
 import numpy as np
 import pytest
 
-from tests.paged_ext_ref import SetupExt
+from tests.paged_ext_ref import VALUE, SetupExt
 from tests.paged_ref import encode
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +50,46 @@ def test_one_key_before_many(gpu, dtype):
     tol = (16 + 128 + 4 + (113 + 4) * others * want) * 2.0 ** -24
     off = np.abs(got / want[..., None] - 1).max(-1)
     assert np.all(off <= tol), (off.max(), (off > tol).mean())
+
+
+@pytest.mark.parametrize("cap", [0.0, 40.0])
+@pytest.mark.parametrize("dtype", ["e4m3", "i8"])
+@pytest.mark.parametrize("new,hd,heads,kv", [(1, 64, 4, 4), (1, 128, 8, 2), (3, 128, 8, 1), (1, 512, 8, 2), (6, 256, 4, 1),
+                                             (60, 64, 2, 1), (60, 128, 8, 2), (60, 256, 2, 1), (60, 512, 2, 1)])
+def test_large_scale_of_no_weight(gpu, new, hd, heads, kv, dtype, cap):
+    """A key of no weight whose values' scale is 2^8 to 2^40 times the others': what they weigh keeps its bits,
+    wherever the key lies and however the running maximum rises.
+
+    Probabilities times scales come in two fp16 parts: off by 2^-22 of themselves or by half of fp16's smallest step,
+    2^-25, in units of 2^-7 of at most twice the largest such product: 2^-31 of that for each key, times its code.
+    The other roundings as for any pool (Setup.attend; a score's scale and q's 22 bits are five more)."""
+    say(f"a large scale of no weight: {dtype} new={new} hd={hd} cap={cap}")
+    n = 300
+    st = SetupExt(gpu, [(new, n)], heads, kv, hd, dtype, 16, cap=cap, seed=hd + new)
+    rng = np.random.default_rng(7 * hd + new)
+    for at, ratio, best in ((1, 40, 0), (0, 16, 200), (37, 28, 5), (n - 61, 20, 100), (130, 12, 130 - 32), (210, 8, 0), (2, 30, 1)):
+        k, v = 0.25 * rng.standard_normal((n, kv, hd)), rng.standard_normal((n, kv, hd))
+        k[best], k[at] = 1.0, -1.0
+        k[20] = 0.4  # (the running maximum rises more than once)
+        v[at] *= 2.0 ** ratio
+        put(st, k, v)
+        q = (1 + 0.1 * rng.standard_normal((new, heads, hd))).astype(np.float32) * np.float32(45 / np.sqrt(hd))
+        got = st.run_attention(q.reshape(new, -1)).reshape(q.shape)
+        K, V = (st.pool[m][st.slots(0, 0, n)] for m in "kv")
+        code, scale = np.abs(VALUE[dtype][st.raw["v"][st.slots(0, 0, n)]]), st.scales["v"].transpose(0, 2, 1)[st.slots(0, 0, n)].astype(np.float64)
+        for r in range(new):
+            p = n - new + r + 1
+            for h in range(heads):
+                g = h * kv // heads
+                x = K[:p, g] @ q[r, h].astype(np.float64) / np.sqrt(hd)
+                d = (hd + 8) * 2.0 ** -24 * (np.abs(K[:p, g]) @ np.abs(q[r, h]).astype(np.float64)).max() / np.sqrt(hd) + 2.0 ** -22
+                if cap:
+                    x = cap * np.tanh(x / cap)
+                    d += 2.0 ** -20 * np.abs(x).max()
+                w = np.exp(x - x.max())
+                w /= w.sum()
+                assert w[at] * 2.0 ** ratio < 2.0 ** -30
+                want = w @ V[:p, g]
+                tol = 2 * (d + (p + 9) * 2.0 ** -24) * (w @ np.abs(V[:p, g])) + 2.0 ** -31 * (w * scale[:p, g]).max() * code[:p, g].sum(0) + 1e-30
+                off = np.abs(got[r, h] - want)
+                assert np.all(off <= tol), (at, ratio, r, h, (off / tol).max())
