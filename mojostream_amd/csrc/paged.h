@@ -57,6 +57,8 @@ struct PagedPlan {
   int G = 0, rows = 0, n_kv = 0, window = 0, blocks = 0, tile_cost = 0, merge_cost = 0;
   bool block = false;  // items of more than 16 pairs go to item_by_block
   bool tail = false;   // a last turn of whole spans that does not fill the blocks is cut
+  bool count = false;  // `shared` is asked for
+  bool shared = false;  // more than a third of the pages that rows attend to are other sequences' too
   bool valid = false;
   int n_items = 0, n_merge = 0, n_parts = 0;
   int most = 0, most_parts = 0;  // (row, head) pairs of the longest item; parts of one result
@@ -75,10 +77,13 @@ struct ms_paged_batch {
   std::vector<int32_t> held;                 // per sequence: first position whose page is there
   std::vector<int64_t> writer;               // per page: the last set() that writes it
   int64_t n_set = 0;
+  std::vector<int64_t> reader;               // per page: the last plan that has counted it
+  int64_t n_counted = 0;
   ms::Upload up;                             // PagedRow [rows], then pages [n_seqs][stride]
   size_t pages_at = 0;
   std::vector<ms::PagedPlan *> plans;
   const ms::PagedRow *d_rows() const { return reinterpret_cast<const ms::PagedRow *>(up.d); }
+  const int32_t *h_pages() const { return reinterpret_cast<const int32_t *>(up.h + pages_at); }
   const int32_t *d_pages() const { return reinterpret_cast<const int32_t *>(up.d + pages_at); }
 };
 

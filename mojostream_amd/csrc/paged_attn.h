@@ -52,9 +52,9 @@ struct PagedAttnArgs {
 };
 
 // The split of the batch's work for a shape of layers (made anew after each set).  tail: a last turn of whole spans that
-// does not fill the blocks is cut.
+// does not fill the blocks is cut; count: the plan says whether sequences share pages.
 int plan_for(ms_paged_batch *b, int G, int rows, bool block, int n_kv, int window, int blocks,
-             int tile_cost, int merge_cost, bool tail, PagedPlan **out);
+             int tile_cost, int merge_cost, bool tail, bool count, PagedPlan **out);
 
 // The launches of pools of 8 bits (dtype MS_KV_E4M3, MS_KV_I8; scores capped or not) and of the other pools
 // with capped scores: each in a source of its own.
@@ -618,7 +618,10 @@ __device__ __forceinline__ void item_by_tile(const PagedAttnArgs &a, const Paged
   };
   // 8-bit values that no other item reads are not kept in the caches, where those that are still to come are looked
   // for; 14B class, 48 tokens over up to 4096 and 16384 keys, e4m3, not in the caches before: 56 to 52 and 190 to 175 us (two
-  // heads of 256 dims that are: 28 to 30 us; the keys too: 56 and 185; rows of 64 bytes: 36 to 37).
+  // heads of 256 dims that are: 28 to 30 us; the keys too: 56 and 185; rows of 64 bytes: 36 to 37).  Where sequences share
+  // pages they are kept (PagedPlan::shared): 48 tokens over 4096 keys, the first of them the same pages for all, 29% of these
+  // read again 80 us past the caches and 83 kept, 49% 77 and 77, 73% 72 and 70, 93% 68 and 62; the first the same for two or
+  // four sequences, 25% 85 and 84, 45% 83 to 85 and 80; 15,000 shared by 48, 244 and 198.
   auto get_v = [&](const char *p) {
     if constexpr (ONCE)
       return __builtin_nontemporal_load(reinterpret_cast<const u2 *>(p));
@@ -1306,7 +1309,7 @@ __device__ inline BlockOf block_of(int block, int n_blocks, int heads) {
 
 // Items of at most 16 NQ pairs: single tokens, or a few of them.  (Two query tiles of three parts do
 // not fit the registers of two waves a SIMD: with spills 110 us where one wave takes 72 us.)
-template <int HD, int DT, int NQ, bool CAP, bool ONCE = Form<DT>::E8>
+template <int HD, int DT, int NQ, bool CAP, bool ONCE>
 __global__ __launch_bounds__(256, NQ == 2 && DT != MS_KV_F16 ? 1 : 2) void k_paged_tile(PagedAttnArgs a) {
   __shared__ __align__(16) char lds[tile_lds<HD, DT, NQ, 4>()];
   if constexpr (Form<DT>::E8) {
@@ -1317,7 +1320,9 @@ __global__ __launch_bounds__(256, NQ == 2 && DT != MS_KV_F16 ? 1 : 2) void k_pag
   }
 }
 
-// Items of longer chunks, and single tokens beside them.
+// Items of longer chunks, and single tokens beside them: 47 of these over 4096 keys and a chunk of 128 rows, e4m3, 114 us,
+// with their values kept in the caches 118.  (A chunk's last few rows, whose values its other items read: 129 rows of 8
+// heads of 512 dims, 20 times, 590 us either way.)
 template <int HD, int DT, bool CAP, int NT = 64 * Shape<HD, DT>::W>
 __global__ __launch_bounds__(NT, 2) void k_paged_block(PagedAttnArgs a) {
   constexpr int A = tile_lds<HD, DT, 1, Shape<HD, DT>::W>(), B = Shape<HD, DT>::LDS;
@@ -1476,8 +1481,11 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   const int merge = block ? 8 : DT == MS_KV_F32 ? 4 : HD == 64 ? 20 : HD == 128 ? 12 : 8;
   // (pools and scores that the plain calls take keep their split, and so their results to the last bit)
   const bool tail = block && (Form<DT>::E8 || CAP);
-  if (int rc = plan_for(b, a.G, rows, block, a.n_kv >> a.hp_log, a.window, 8 / w * ctx().n_cu, cost, merge, tail, &p))
+  constexpr bool ONCE = Form<DT>::E8 && v_dims<HD, DT>() == 8;
+  const bool count = ONCE && !block && (TWO || most <= 16);  // (of 17 to 32 pairs two items have the same keys)
+  if (int rc = plan_for(b, a.G, rows, block, a.n_kv >> a.hp_log, a.window, 8 / w * ctx().n_cu, cost, merge, tail, count, &p))
     return rc;
+  const bool once = count && !p->shared;
   a.part_rows = p->most;
   if (const size_t n = (size_t)p->n_parts * a.n_kv * a.part_rows) {
     void *buf = nullptr;
@@ -1492,12 +1500,18 @@ int launch(PagedAttnArgs &a, ms_paged_batch *b, int most, hipStream_t st) {
   const dim3 grid(p->n_items * (a.n_kv >> a.hp_log));
   if (block) {
     hipLaunchKernelGGL((k_paged_block<HD, DT, CAP>), grid, dim3(64 * B::W), 0, st, a);
-  } else if (Form<DT>::E8 && !TWO && most > 16) {  // (two items have the same keys)
-    if constexpr (!TWO) hipLaunchKernelGGL((k_paged_tile<HD, DT, 1, CAP, false>), grid, dim3(256), 0, st, a);
   } else if (rows == 16) {
-    hipLaunchKernelGGL((k_paged_tile<HD, DT, 1, CAP>), grid, dim3(256), 0, st, a);
+    if (once)
+      hipLaunchKernelGGL((k_paged_tile<HD, DT, 1, CAP, ONCE>), grid, dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((k_paged_tile<HD, DT, 1, CAP, false>), grid, dim3(256), 0, st, a);
   } else {
-    if constexpr (TWO) hipLaunchKernelGGL((k_paged_tile<HD, DT, 2, CAP>), grid, dim3(256), 0, st, a);
+    if constexpr (TWO) {
+      if (once)
+        hipLaunchKernelGGL((k_paged_tile<HD, DT, 2, CAP, ONCE>), grid, dim3(256), 0, st, a);
+      else
+        hipLaunchKernelGGL((k_paged_tile<HD, DT, 2, CAP, false>), grid, dim3(256), 0, st, a);
+    }
   }
   if (p->n_merge) {
     // about four parts a thread, more of them in a larger block

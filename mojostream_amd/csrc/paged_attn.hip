@@ -76,6 +76,24 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
     for (int i = 0; i < last; ++i)  // (16 tiles a part at least: the merge costs about two)
       cut_in[by_cost[i]] = std::max(1, std::min(std::min(4, places / last), spans[by_cost[i]].tiles / 16));
   }
+  // (every fourth page: a prefix that sequences share lies at the same places of theirs)
+  p->shared = false;
+  if (p->count) {
+    b->reader.resize(b->n_pages, 0);
+    const int64_t stamp = ++b->n_counted;
+    int64_t all = 0, again = 0;
+    for (int s = 0; s < b->n_seqs; ++s) {
+      if (!b->n_new[s]) continue;
+      const int lo = p->window ? std::max(0, b->len[s] - b->n_new[s] - p->window + 1) : 0;
+      const int32_t *pg = b->h_pages() + (size_t)s * b->stride;
+      for (int i = (lo / b->page_size + 3) / 4 * 4; i <= (b->len[s] - 1) / b->page_size; i += 4) {
+        ++all;
+        again += b->reader[pg[i]] == stamp;
+        b->reader[pg[i]] = stamp;
+      }
+    }
+    p->shared = 3 * again > all;
+  }
   std::vector<PagedItem> items;
   std::vector<PagedMerge> merge;
   std::vector<std::pair<int, int>> order;
@@ -111,11 +129,11 @@ int make_plan(ms_paged_batch *b, PagedPlan *p, int blocks) {
 }  // namespace
 
 int plan_for(ms_paged_batch *b, int G, int rows, bool block, int n_kv, int window, int blocks,
-             int tile_cost, int merge_cost, bool tail, PagedPlan **out) {
+             int tile_cost, int merge_cost, bool tail, bool count, PagedPlan **out) {
   PagedPlan *p = nullptr;
   for (PagedPlan *x : b->plans)
     if (x->G == G && x->rows == rows && x->block == block && x->n_kv == n_kv && x->window == window && x->blocks == blocks &&
-        x->tile_cost == tile_cost && x->merge_cost == merge_cost && x->tail == tail)
+        x->tile_cost == tile_cost && x->merge_cost == merge_cost && x->tail == tail && x->count == count)
       p = x;
   if (!p) {
     // (a model has a few shapes of layers; more than that reuse the oldest place)
@@ -134,6 +152,7 @@ int plan_for(ms_paged_batch *b, int G, int rows, bool block, int n_kv, int windo
     p->tile_cost = tile_cost;
     p->merge_cost = merge_cost;
     p->tail = tail;
+    p->count = count;
     p->n_kv = n_kv;
     p->window = window;
   }
