@@ -93,3 +93,35 @@ def test_large_scale_of_no_weight(gpu, new, hd, heads, kv, dtype, cap):
                 tol = 2 * (d + (p + 9) * 2.0 ** -24) * (w @ np.abs(V[:p, g])) + 2.0 ** -31 * (w * scale[:p, g]).max() * code[:p, g].sum(0) + 1e-30
                 off = np.abs(got[r, h] - want)
                 assert np.all(off <= tol), (at, ratio, r, h, (off / tol).max())
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "i8", "f32", "bf16", "f16"])
+@pytest.mark.parametrize("seqs,heads,kv,hd", [([(1, 40000), (1, 3)], 3, 1, 64), ([(2, 12000)], 6, 2, 128), ([(1, 9000)], 16, 1, 256),
+                                              ([(3, 5000), (1, 1)], 4, 1, 512), ([(1, 131065)], 4, 1, 128), ([(1, 20000)] * 3, 10, 2, 128)])
+def test_every_part_counts(gpu, seqs, heads, kv, hd, dtype):
+    """Few rows over many keys that all score 0, their values whole numbers of 0 to 16 that turn slowly along the keys: every
+    sum is a whole number below 2^24, and exact; a mean is off by its division, 2^-22 of it with room for one more rounding.
+    Were 32 keys or more side by side left out, some dim would be off by more."""
+    say(f"every part counts: {dtype} {seqs} hd={hd}")
+    st = SetupExt(gpu, seqs, heads, kv, hd, dtype, 32, cap=25.0, seed=22)
+    n = max(st.len)
+    v = ((np.arange(n)[:, None] // max(1, n // 16) + np.arange(hd)) % 17).astype(np.float64)
+    for s, length in enumerate(st.len):
+        g = st.slots(s, 0, length)
+        for name, x in (("k", np.zeros((length, kv, hd))), ("v", np.repeat(v[:length, None], kv, 1))):
+            if st.eight:
+                code = np.argsort(VALUE[dtype][:128], kind="stable")[np.searchsorted(np.sort(VALUE[dtype][:128]), x)]
+                st.raw[name][g] = code.astype(np.uint8)
+                st.scales[name].transpose(0, 2, 1)[g] = 1.0
+            else:
+                st.pool[name][g] = encode(x.astype(np.float32), dtype)
+    st.upload()
+    q = np.random.default_rng(1).standard_normal((st.rows, heads * hd)).astype(np.float32)
+    got = st.run_attention(q).reshape(st.rows, heads, hd)
+    upto = np.concatenate([np.zeros((1, hd)), np.cumsum(v, 0)])
+    for r, (s, p) in enumerate(st.row_of()):
+        want = upto[p + 1] / (p + 1)
+        assert np.all(np.abs(got[r] - want) <= 2.0 ** -22 * want)
+        at = np.arange(32, p - 63, 32)
+        less = (upto[p + 1] - upto[at + 32] + upto[at]) / (p + 1 - 32)
+        assert np.all(np.any(np.abs(less - want) > 2.0 ** -20 * want, axis=1))
