@@ -48,7 +48,8 @@ struct RowInfo {
   int ref;                  // weights are 2^(x log2(e) / T - ref)
   float top;                // the largest logit
   float lo, hi;             // the cut lies among the logits lo <= x < hi (the candidates); what lies above stays
-  unsigned long long want;  // top-p: weight (of its octave) that the candidates have to reach; top-k: ids of the cut's bucket
+  unsigned long long want;  // top-p: weight (of its octave) that the bucket has to reach; top-k: ids of the cut's bucket
+  int bucket;               // top-p: the one in which the cut lies, whatever min_p leaves of it
 };
 // A row's settings.
 struct RowSet {
@@ -298,7 +299,7 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
   uint32_t real = lane < a.slices ? ldg<uint32_t>(a.real + at + lane) : 0;
   const float top = of_key(max_wave(key_of(mine)));
   real = sum_wave(real);
-  RowInfo in{real == 0 ? kNone : top == INFINITY || set.k > kMostK ? kSlow : SUMS ? kSum : kBest, 0, top, -MAX32, -MAX32, 0};
+  RowInfo in{real == 0 ? kNone : top == INFINITY || set.k > kMostK ? kSlow : SUMS ? kSum : kBest, 0, top, -MAX32, -MAX32, 0, 0};
   if (in.state == kSum && !in_range(top, set.c64)) in.state = kSlow;
   const bool all = SUMS && set.top_p >= 1.f;
   const int group0 = in.state == kSum || in.state == kBest ? group_of<SUMS>(top, set.c64) : 0;
@@ -386,6 +387,7 @@ __device__ inline void find_cut(const SampleRowsArgs &a, const RowSet &set, size
     const int bin = __ffsll(hit) - 1;
     in.want = goal - __shfl(upto - s, bin, 64);
     const int bucket = 32 * (group0 - group) - 1 - bin;
+    in.bucket = bucket;
     if constexpr (SUMS) {
       // (the first lane's and the others' bound)
       const float x = least_of_bucket(bucket + (lane > 0), set), least = least_of_min_p(top, set);
@@ -668,10 +670,10 @@ __device__ inline void find_bin(RowLds &lds, unsigned long long before, unsigned
   __syncthreads();
 }
 
-// The whole of a row, by one block.  The cut's logit is found by histograms over the keys of a range,
+// The whole of a row, by one block (in: what is known of it, or null).  The cut's logit is found by histograms over the keys of a range,
 // by counts (top-k) or weights (top-p), the range then being the bin that the cut lies in.  (One row of 262144
 // logits that are all alike, about ten times over the row: 0.5 ms.)
-__device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, RowLds &lds) {
+__device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, RowLds &lds, const RowInfo *in) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n, row = blockIdx.x;
   const RowSet &set = a.rows[row];
   const float *x = a.x + row * a.ld;
@@ -762,32 +764,40 @@ __device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, 
     key = find(kCount, set.k, top, least, 0);
     eq = (uint32_t)(set.k - above);
   }
-  if (sums && set.top_p < 1.f) {
+  if (sums && set.top_p < 1.f && least == top) {
+    eq = (uint32_t)share_of(set.top_p, (u128)real);
+  } else if (sums && set.top_p < 1.f) {
     // the octave, its bucket and the logit in which the cut lies
-    __syncthreads();
-    for (int i = tid; i < kBins; i += kNT) lds.bin[i] = 0;
-    __syncthreads();
-    each(tid, n, kNT, [&](float v, int) {
-      const Place p = place_of(v > -INFINITY ? v : -INFINITY, from, set.c64);
-      const uint32_t d = 32 * ref - 1 - (p.k >> 1);
-      if (d < kBins) atomicAdd(&lds.bin[d], weight_of_octave(exp2, p, a.bits));
-    });
-    __syncthreads();
-    if (wave == 0) {
-      unsigned long long w = 0, want;
-      for (int i = 0; i < 32; ++i) w += lds.bin[32 * lane + i];
-      const int g = octave_of_share(set.top_p, w, &want);
-      const unsigned long long mine = lane < 32 ? lds.bin[32 * g + lane] : 0, upto = scan_wave(mine);
-      const int b = __ffsll((unsigned long long)__ballot(upto >= want)) - 1;
-      want -= __shfl(upto - mine, b, 64);
-      if (lane == 0) {
-        lds.found = 32 * g + b;
-        lds.cut = want;
+    int bucket;
+    unsigned long long want;
+    if (in) {
+      bucket = in->bucket;
+      want = in->want;
+    } else {
+      for (int i = tid; i < kBins; i += kNT) lds.bin[i] = 0;
+      __syncthreads();
+      each(tid, n, kNT, [&](float v, int) {
+        const Place p = place_of(v > -INFINITY ? v : -INFINITY, from, set.c64);
+        const uint32_t d = 32 * ref - 1 - (p.k >> 1);
+        if (d < kBins) atomicAdd(&lds.bin[d], weight_of_octave(exp2, p, a.bits));
+      });
+      __syncthreads();
+      if (wave == 0) {
+        unsigned long long w = 0, rest;
+        for (int i = 0; i < 32; ++i) w += lds.bin[32 * lane + i];
+        const int g = octave_of_share(set.top_p, w, &rest);
+        const unsigned long long mine = lane < 32 ? lds.bin[32 * g + lane] : 0, upto = scan_wave(mine);
+        const int b = __ffsll((unsigned long long)__ballot(upto >= rest)) - 1;
+        rest -= __shfl(upto - mine, b, 64);
+        if (lane == 0) {
+          lds.found = 32 * ref - 1 - (32 * g + b);
+          lds.cut = rest;
+        }
       }
+      __syncthreads();
+      bucket = lds.found;
+      want = lds.cut;
     }
-    __syncthreads();
-    const int bucket = 32 * ref - 1 - lds.found;
-    const unsigned long long want = lds.cut;
     key = find(kOctave, want, min(top, key_of(least_of_bucket(bucket + 1, set)) - 1),
                max(least, key_of(least_of_bucket(bucket, set))), 0);
     const unsigned long long w = weight_of_octave(exp2, place_of(of_key(key), from, set.c64), a.bits);
@@ -1089,7 +1099,7 @@ __global__ __launch_bounds__(kNT) void k_rows_draw(SampleRowsArgs a) {
   }
   if (in.state == kSlow || !fits || n_list > kList) {
     __syncthreads();  // (the table)
-    row_by_ranges(a, exp2, lds);
+    row_by_ranges(a, exp2, lds, in.state == kSum ? &in : nullptr);
     return;
   }
   const float u = ldg<float>(a.u + row);
@@ -1193,7 +1203,7 @@ __global__ __launch_bounds__(kNT) void k_rows_whole(SampleRowsArgs a) {
   __shared__ RowLds lds;
   exp2_table(table);
   __syncthreads();
-  row_by_ranges(a, Exp2{table}, lds);
+  row_by_ranges(a, Exp2{table}, lds, nullptr);
 }
 
 }  // namespace

@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("below", [-np.inf, -70.0])
-@pytest.mark.parametrize("vocab", [1000, 16385, 32003, 262144, 300001])
+@pytest.mark.parametrize("vocab", [1000, 16385, 32003, 262144, 300001, (1 << 20) + 3])
 @pytest.mark.parametrize("best", [2, 4, 8, 1000, 15000])
 def test_borders_among_equals(gpu, best, vocab, below):
     """`best` equal logits, the others masked or without any weight: a quarter, half or three quarters of the row's weight are
@@ -19,7 +19,7 @@ def test_borders_among_equals(gpu, best, vocab, below):
     if best > vocab:
         best = vocab
     rng = np.random.default_rng(best * vocab)
-    for rows in (6, 70):
+    for rows in (6, 70) if vocab < 1 << 20 else (3,):
         x = np.full((rows, vocab), -np.inf, np.float32)
         at, top_p = [], []
         for r in range(rows):
