@@ -9,13 +9,13 @@
 //                 (item_by_tile).  Bound by memory: 48 tokens over up to 4096 keys, 14B class, bf16,
 //                 458 MB in 92 to 97 us; 32 tokens over up to 4096 keys in fp32, 8 kv heads of 128
 //                 dims, 5.1 TB/s, 2 of 512 dims, 5.6 TB/s (a large copy: 4.6 TB/s).  8-bit pools: the 48 tokens'
-//                 237 MB in 44 us (5.4 TB/s); one token over 131065 keys, 2 kv heads of 128 dims, capped, 69 MB in 20 us.
+//                 237 MB in 44 us (5.4 TB/s); one token over 131065 keys, 2 kv heads of 128 dims, capped, 69 MB in 21 us.
 //  k_paged_block  longer chunks, and single tokens beside them (item_by_block, item_by_tile).
 //                 Bound by the matrix cores: 4096 rows over 16384 keys, 14B class, bf16 (three
 //                 products a multiplication): 2.7 to 2.9 ms among other calls (2.9 to 3.1 in ten
 //                 passes under the profiler), 1.3 PFLOP/s of bf16 products, MFMA busy 56% of the time
-//                 at 2.1 GHz (a large bf16 matrix product: 1.2 PFLOP/s).  8-bit pools (two products): 2.39 to 2.48 ms,
-//                 with a cap 3.2 to 3.4 ms; capped over bf16 3.0 to 3.15 ms.
+//                 at 2.1 GHz (a large bf16 matrix product: 1.2 PFLOP/s).  8-bit pools (two products): e4m3 2.29 to
+//                 2.33 ms, int8 2.36, with a cap 3.27 and 3.38 ms; capped over bf16 3.3 ms, fp16 2.45, fp32 5.6.
 //  k_paged_merge  the spans' results (k_paged_merge_cols: of many spans a row, over 8-bit pools or capped).
 #pragma once
 #include <cmath>
@@ -334,7 +334,7 @@ __device__ __forceinline__ void probabilities(const PagedAttnArgs &a, f4 (&s)[2]
   float from[NQ] = {};
   const int g = (threadIdx.x & 63) >> 4;
   // (both forms for each score of every tile: 4096 rows over 16384 keys, 14B class, i8, 3.5 ms; the near one alone
-  // where a tile's scores allow it, 3.2 ms; uncapped 2.5 ms)
+  // where a tile's scores allow it, 3.2 ms; uncapped 2.5 ms, all before the values' unit went by the products)
   if constexpr (CAP) {
     if (__any(z2 >= kNear)) {
 #pragma unroll

@@ -53,8 +53,8 @@ __device__ inline T max_over(T x, int lanes) {
 // and the N that turn with them, or 2 N side by side.  x / sqrt(mean x^2 + eps) * gamma, then the rotation; 8-bit heads
 // in 64 bits (their codes are then the nearest ones), the others in 32.  A head stays in its lanes' registers: sums and
 // the largest value over them by lane moves, one pass over the rows.
-// Bound by memory: 3001 rows of 40 + 8 + 8 heads of 128 dims, q and k normed, e4m3: 155 MB in 33.5 to 35 us (4.5 TB/s; a
-// large copy 4.6 to 5.1).  One row of 8 + 2 + 2 heads of 512 dims: 3.8 us, the launch and a chain of loads.
+// Bound by memory: 3001 rows of 40 + 8 + 8 heads of 128 dims, q and k normed, e4m3: 155 MB in 35 us (4.4 TB/s; a
+// large copy 4.6 to 5.1).  One row of 8 + 2 + 2 heads of 512 dims: 4.2 us, the launch and a chain of loads.
 template <int DT, int HD, int N, bool PAIRS>
 __global__ __launch_bounds__(kBlock) void k_append_ext(AppendExtArgs a) {
   constexpr bool E8 = DT == MS_KV_E4M3 || DT == MS_KV_I8;
@@ -251,9 +251,11 @@ __device__ inline f4 load4(const void *pool, size_t at) {
 }
 
 // A thread has four values of k and of v of one position: 16 bytes of each written.  Bound by memory: 20011 positions of 8
-// heads of 128 dims, int8, 206 MB, four fifths of them written, in 31 us (6.7 TB/s); 700 of 2 heads of 256 dims 2.9 us.
-// Rows that are more than half of the last cache (256 MB) are written past the caches: these 164 MB in 49 us without, and with a
-// sum over both behind it 90 against 83; 66 MB alone 14.3 us, past the caches 13.7, but with the sum 37 against 41.
+// heads of 128 dims, int8, 206 MB, four fifths of them written, in 31 us (6.6 TB/s); 700 of 2 heads of 256 dims 2.9 us.
+// Rows that are more than half of the last cache (256 MB) are written past the caches.  Of three layers in turn, int8, in the caches
+// and past them: 64 MB 17.8 and 17.0 us, 128 MB 44 and 29, 160 MB 52 and 35, 256 MB 80 and 52, 400 MB 120 and 112; what
+// reads them next pays for it where they would have been there: with a sum over both behind each 69 and 74, 105 and 112, 123
+// and 127, 170 and 175, 255 and 248 (a sum over the same rows again and again, 164 MB, 90 and 83).
 template <int DT, bool PAST>
 __global__ __launch_bounds__(kBlock) void k_paged_read(ReadArgs a) {
   constexpr bool E8 = DT == MS_KV_E4M3 || DT == MS_KV_I8;

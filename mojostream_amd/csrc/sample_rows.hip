@@ -18,7 +18,7 @@
 //  k_rows_draw  a block a row: sorts the candidates, finds the cut and draws.  Rows that this does not
 //               fit (more candidates than the list holds, a large top-k, infinite logits) it goes over as a whole.
 //
-// Three launches, each with a chain of loads behind the last one's results: 4.8 + 7.2 + 6.6 us for a row of 262144 ids; 48 such
+// Three launches, each with a chain of loads behind the last one's results: 4.8 + 7.6 + 7.2 us for a row of 262144 ids; 48 such
 // rows, 50 MB, 17 + 17 + 12 us (the first without its weights and sums 17 as well; in slices of 28672 ids, whose
 // blocks are all there at once, 20 + 16 + 14).
 #include <climits>
@@ -672,7 +672,7 @@ __device__ inline void find_bin(RowLds &lds, unsigned long long before, unsigned
 
 // The whole of a row, by one block (in: what is known of it, or null).  The cut's logit is found by histograms over the keys of a range,
 // by counts (top-k) or weights (top-p), the range then being the bin that the cut lies in.  (One row of 262144
-// logits that are all alike, about ten times over the row: 0.5 ms.)
+// logits that are all alike, about nine times over the row: 0.43 ms.)
 __device__ inline void row_by_ranges(const SampleRowsArgs &a, const Exp2 &exp2, RowLds &lds, const RowInfo *in) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n, row = blockIdx.x;
   const RowSet &set = a.rows[row];
